@@ -387,6 +387,131 @@ int skv_compact(const skv_pool_ref* pools, int32_t n_pools, int32_t* block_table
                 int64_t n_pages, int32_t* free_stack, int32_t* free_top, int32_t* workspace,
                 int32_t* info, void* stream);
 
+/* ---- pages that sequences share ---------------------------------------------
+ * A forked sequence shares the whole pages of its source.  refs: int32
+ * [n_pages], zero before the first fork: how many sequences hold a page beyond
+ * the first (0: one, or none).  Only whole pages are shared, and appends write
+ * behind them, so the appends, gathers and attentions above need not know of
+ * it; the sequences are released and compacted by the two calls below.  No
+ * reference counterpart (the reference copies its tensors).
+ *
+ * skv_fork: for each f < n_forks sequence dst[f] (empty) becomes a copy of
+ * src[f]: the whole pages are shared, the page that the last tokens have begun
+ * is copied, in every pool, into a page popped from the free stack (forks in
+ * order), the length is set.  src and dst are device arrays.  All-or-nothing:
+ * if the stack lacks pages (SKV_STATUS_NOSPC), or an index is outside the
+ * batch, a dst is not empty or is named twice, or a source's length or last
+ * page is not a valid one (SKV_STATUS_BADARG), nothing is written but *status,
+ * which may not be NULL here.  batch and n_forks <= 4096, up to 32 pools. */
+int skv_fork(int32_t* free_stack, int32_t* free_top, int64_t n_pages, int32_t* refs, int32_t* block_table,
+             int64_t bt_stride, int32_t* seq_lens, int64_t batch, int64_t block_size, const int32_t* src,
+             const int32_t* dst, int64_t n_forks, const skv_pool_ref* pools, int32_t n_pools, int32_t* status,
+             void* stream);
+
+/* What a sequence holds outside its pages (rings, pooling states, counts): for
+ * each f, slot dst[f] of every array becomes a copy of slot src[f]; slot i of
+ * an array is page_bytes bytes at base + i*page_bytes, of n_slots.  An index
+ * outside the slots copies nothing; a dst named twice, or as a src too, is left
+ * with either's bytes.  n_forks <= 65535. */
+int skv_copy_slots(const skv_pool_ref* arrays, int64_t n_arrays, int64_t n_slots, const int32_t* src,
+                   const int32_t* dst, int64_t n_forks, void* stream);
+
+/* skv_release over shared pages: a page goes on the stack when its last holder
+ * leaves (at the place of the last of those that leave together), otherwise its
+ * count goes down.  Refuses besides (SKV_STATUS_BADARG) what more sequences
+ * release than hold it. */
+int skv_release_shared(int32_t* free_stack, int32_t* free_top, int64_t n_pages, int32_t* refs, int32_t* block_table,
+                       int64_t bt_stride, int32_t* seq_lens, const uint8_t* release_mask, int64_t batch,
+                       int64_t block_size, int32_t* status, void* stream);
+
+/* skv_compact over shared pages: a page moves once, every table that holds it
+ * is rewritten, its count moves with it. */
+int skv_compact_shared(const skv_pool_ref* pools, int32_t n_pools, int32_t* block_table, int64_t bt_stride,
+                       const int32_t* seq_lens, int64_t batch, int64_t block_size, int64_t n_pages,
+                       int32_t* free_stack, int32_t* free_top, int32_t* refs, int32_t* workspace, int32_t* info,
+                       void* stream);
+
+/* ---- 4-bit token cache ----------------------------------------------------------
+ * Pages of raw keys and values, 17/32 of a byte per value: e2m1 codes (0, .5,
+ * 1, 1.5, 2, 3, 4, 6 and a sign), and a scale byte s = 2^(s - 127) per 32
+ * dims.  The keys and values of a token's n_kv_heads heads of head_dim dims
+ * (a multiple of 32, at most 512).  A page holds block_size tokens (a multiple
+ * of 16), per head
+ *   [block_size][head_dim / 2]      the keys' codes, dim 2i in byte i's low half,
+ *   [block_size][head_dim / 2]      the values' codes,
+ *   [block_size][2][head_dim / 32]  scale bytes, a token's key's then its value's;
+ * skv_fp4_page_bytes gives its size (-1: bad shape).  Pages come from
+ * skv_reserve, and skv_fork, skv_release(_shared) and skv_compact(_shared) move
+ * them like any other.  bt_stride * block_size <= 2^24, batch <= 65535.  The
+ * reference plans a mixed-precision cache without code
+ * (saint_llm_inference/__init__.py:9) and keeps raw rows (kv_cache.py:59-83). */
+typedef struct skv_fp4_cache {
+  void* pool;                 /* n_pages pages, 16-byte aligned */
+  int64_t block_size, n_pages, n_kv_heads, head_dim;
+  const int32_t* block_table; /* [batch, bt_stride] */
+  int64_t bt_stride, batch;
+} skv_fp4_cache;
+
+/* Rows outside the pages: token i, head h of sequence b at data + b*seq_stride
+ * + i*tok_stride + h*head_stride (bytes; multiples of 16), its dims contiguous. */
+typedef struct skv_fp4_rows {
+  void* data;
+  int64_t seq_stride, tok_stride, head_stride;
+} skv_fp4_rows;
+
+int64_t skv_fp4_page_bytes(int64_t block_size, int64_t n_kv_heads, int64_t head_dim);
+
+/* Quantize the n_new[b] newest tokens of each sequence (seq_lens counts them
+ * already) from the rows k and v (bf16, or fp32 with src_f32; src_len tokens per
+ * sequence) into the pages: per 32 dims the scale is the smallest power of two
+ * under which no value passes 6 (at least 2^-120; at most 2^125, where larger
+ * values become 6), and each value its nearest code (ties to the even one).  A
+ * block that holds a NaN or an infinity gets scale byte 255: it reads as NaN. */
+int skv_fp4_quant_append(const skv_fp4_cache* cache, const int32_t* seq_lens, const int32_t* n_new,
+                         int32_t n_new_uniform, const skv_fp4_rows* k, const skv_fp4_rows* v, int64_t src_len,
+                         int32_t src_f32, void* stream);
+
+/* The n_rows[b] newest tokens of each sequence as bf16 (exact) to the rows k and
+ * v (dst_len tokens per sequence; rows past n_rows[b] are left as they are);
+ * zeros for a token whose page is not mapped. */
+int skv_fp4_gather(const skv_fp4_cache* cache, const int32_t* seq_lens, const int32_t* n_rows,
+                   int32_t n_rows_uniform, const skv_fp4_rows* k, const skv_fp4_rows* v, int64_t dst_len,
+                   void* stream);
+
+/* Attention of the newest n_queries tokens of each sequence over its 4-bit
+ * pages: token t of sequence b is position p = seq_lens[b] - n_queries + t and
+ * sees positions [max(0, p - window + 1), p] (window 0: from 0); n_heads query
+ * heads, n_heads / n_kv_heads of them to a K/V head (head h reads K/V head
+ * h / (n_heads / n_kv_heads)):
+ *   s_j = scale * q . k_j            (scale 0: 1 / sqrt(head_dim))
+ *   s_j = softcap * tanh(s_j / softcap)                (softcap > 0)
+ *   out = sum_j exp(s_j) v_j / (sum_j exp(s_j) + exp(sink[h]))   (sink optional)
+ * A token that sees nothing (or only unmapped pages) gets 0; a NaN block makes
+ * NaN the outputs of the tokens that see it, and of no other.  q: bf16, token t, head h of
+ * sequence b at q + b*q_seq_stride + t*q_tok_stride + h*q_head_stride (bytes,
+ * multiples of 16); out: bf16 [batch, n_queries, n_heads, head_dim].  max_len
+ * bounds the lengths for the split of long sequences over workgroups (0: what
+ * the table holds; longer sequences are still right).  splits 0: chosen by the
+ * library.  skv_fp4_attention_workspace returns the bytes that a call needs
+ * (16-byte aligned; -1: bad descriptor).  The generalisation of the window
+ * branch of SWAttention.forward (swa.py:115-137) to several K/V heads and the
+ * whole history. */
+typedef struct skv_fp4_attention_desc {
+  skv_fp4_cache cache;
+  const int32_t* seq_lens;
+  int64_t n_queries, n_heads;
+  const void* q;
+  int64_t q_seq_stride, q_tok_stride, q_head_stride;
+  void* out;
+  const float* sink; /* [n_heads] or NULL */
+  int64_t window, max_len, splits;
+  float scale, softcap;
+} skv_fp4_attention_desc;
+
+int64_t skv_fp4_attention_desc_size(void);
+int64_t skv_fp4_attention_workspace(const skv_fp4_attention_desc* desc);
+int skv_fp4_attention(const skv_fp4_attention_desc* desc, void* workspace, int64_t ws_bytes, void* stream);
+
 /* ---- fused decode step ----------------------------------------------------
  * One decode step (one new token per sequence) of a stack of heterogeneous
  * layers in three launches, whatever the layer count:

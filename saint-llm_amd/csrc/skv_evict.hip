@@ -89,6 +89,102 @@ __global__ __launch_bounds__(kEvictThreads) void k_release(
   }
 }
 
+// k_release over shared pages (refs[p]: holders beyond the first).  Positions u of
+// the released pages in push order (ascending b, within b from the last logical
+// page) are dealt to the threads in runs.  A page whose holders all leave drops to
+// -1; the largest u among its releases, found by a minimum over -2 - u in the
+// count itself, pushes it, so that the stack does not depend on the order in
+// which the atomics run.
+__global__ __launch_bounds__(kEvictThreads) void k_release_shared(
+    int32_t* __restrict__ stack, int32_t* __restrict__ top_ptr, int64_t n_pages, int32_t* refs, int32_t* bt,
+    int64_t bt_stride, int32_t* __restrict__ lens, const uint8_t* __restrict__ mask, int batch, int bs,
+    int32_t* __restrict__ status) {
+  __shared__ int off[kEvictMaxBatch + 1];
+  __shared__ int cnt[kEvictMaxBatch];
+  __shared__ int scan_lds[17];
+  __shared__ int bad_all;
+  const int tid = threadIdx.x;
+  if (tid == 0) bad_all = 0;
+  int carry = 0;
+  for (int base = 0; base < batch; base += kEvictThreads) {
+    const int b = base + tid;
+    int c = 0;
+    if (b < batch && mask[b]) c = static_cast<int>(min<int64_t>(ceil_div(max(lens[b], 0), bs), bt_stride));
+    int tot;
+    const int ex = block_exclusive_scan(c, scan_lds, &tot);
+    if (b < batch) {
+      off[b] = carry + ex;
+      cnt[b] = c;
+    }
+    carry += tot;
+  }
+  if (tid == 0) off[batch] = carry;
+  __syncthreads();
+  const int top = *top_ptr;
+  const int per = (carry + kEvictThreads - 1) / kEvictThreads;
+  const int u0 = min(tid * per, carry), u1 = min(u0 + per, carry);
+  // f(u, page) for the thread's run of positions
+  const auto each = [&](auto&& f) {
+    int b = u0 < u1 ? owner_of(off, batch, u0) : 0;
+    for (int u = u0; u < u1; ++u) {
+      while (u >= off[b + 1]) ++b;
+      f(u, bt[static_cast<int64_t>(b) * bt_stride + (cnt[b] - 1 - (u - off[b]))]);
+    }
+  };
+  const auto refuse = [&](int bad) {  // the whole workgroup's answer
+    if (bad) atomicOr(&bad_all, bad);
+    __syncthreads();
+    if (bad_all && tid == 0 && status) *status = bad_all;
+    return bad_all != 0;
+  };
+  int bad = (top < 0 || top > n_pages) ? SKV_STATUS_STACK : 0;
+  each([&](int, int32_t page) {
+    if (page < 0 || page >= n_pages) bad = SKV_STATUS_BADARG;
+  });
+  if (refuse(bad)) return;
+  int freed = 0;
+  each([&](int, int32_t page) {
+    const int was = atomicSub(&refs[page], 1);
+    freed += was == 0 ? 1 : 0;
+    if (was < 0) bad = SKV_STATUS_BADARG;
+  });
+  const int pushes = block_reduce_sum(freed, scan_lds);
+  if (static_cast<int64_t>(top) + pushes > n_pages) bad |= SKV_STATUS_STACK;
+  if (refuse(bad)) {
+    each([&](int, int32_t page) { atomicAdd(&refs[page], 1); });
+    return;
+  }
+  const auto count_of = [&](int32_t page) {  // past the L1 cache, which holds what it was
+    return __hip_atomic_load(&refs[page], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  };
+  each([&](int u, int32_t page) {
+    if (count_of(page) < 0) atomicMin(&refs[page], -2 - u);
+  });
+  __syncthreads();
+  int mine = 0;
+  each([&](int u, int32_t page) { mine += count_of(page) == -2 - u ? 1 : 0; });
+  int tot;
+  int at = top + block_exclusive_scan(mine, scan_lds, &tot);
+  each([&](int u, int32_t page) {
+    if (count_of(page) == -2 - u) {
+      stack[at++] = page;
+      atomicExch(&refs[page], 0);
+    }
+  });
+  __syncthreads();  // every page id is read before the tables are cleared
+  for (int t = tid; t < carry; t += kEvictThreads) {
+    const int b = owner_of(off, batch, t);
+    bt[static_cast<int64_t>(b) * bt_stride + (t - off[b])] = -1;
+  }
+  for (int b = tid; b < batch; b += kEvictThreads) {
+    if (mask[b]) lens[b] = 0;
+  }
+  if (tid == 0) {
+    *top_ptr = top + pushes;
+    if (status) *status = 0;
+  }
+}
+
 // ---- compaction -------------------------------------------------------------
 struct PoolRefs {
   uint8_t* base[kMaxPools];
@@ -268,6 +364,9 @@ __device__ __forceinline__ void slice_ids(const CopySlices& cs, const int32_t* m
   }
 }
 
+// kShared: several tables may hold a page, so the rewrite leaves the marks to
+// k_compact_finish.
+template <bool kShared>
 __global__ __launch_bounds__(kCompactCopyThreads) void k_compact_copy(PoolRefs pools, CopySlices cs, TableRef tr,
                                                                      int32_t* __restrict__ ws, int64_t n,
                                                                      const int32_t* __restrict__ info) {
@@ -299,11 +398,13 @@ __global__ __launch_bounds__(kCompactCopyThreads) void k_compact_copy(PoolRefs p
       const int32_t p = tr.bt[t];
       if (p >= n_live && p < n) {
         tr.bt[t] = holes[remap[p]];
-        remap[p] = 0;
+        if constexpr (!kShared) remap[p] = 0;
       }
     }
   }
-  for (int i = gtid; i < n_live; i += gsize) remap[i] = 0;
+  if constexpr (!kShared) {
+    for (int i = gtid; i < n_live; i += gsize) remap[i] = 0;
+  }
   for (; s0 < total; s0 += gridDim.x * kCopySlices) {
     int q_of[kCopySlices], off[kCopySlices];
 #pragma unroll
@@ -347,6 +448,20 @@ __global__ __launch_bounds__(kCompactCopyThreads) void k_compact_copy(PoolRefs p
   }
 }
 
+// Clears the marks and moves the counts of the pages that moved.
+__global__ __launch_bounds__(kCompactCopyThreads) void k_compact_finish(int32_t* __restrict__ ws, int64_t n,
+                                                                       const int32_t* __restrict__ info,
+                                                                       int32_t* __restrict__ refs) {
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * kCompactCopyThreads + threadIdx.x;
+  if (i >= n) return;
+  ws[i] = 0;
+  if (i < info[1]) {
+    const int32_t hole = ws[n + i], mover = ws[2 * n + i];
+    refs[hole] = refs[mover];
+    refs[mover] = 0;
+  }
+}
+
 }  // namespace skv
 
 using namespace skv;
@@ -370,11 +485,32 @@ extern "C" int skv_release(int32_t* free_stack, int32_t* free_top, int64_t n_pag
   return check_launch("skv_release");
 }
 
-extern "C" int skv_compact(const skv_pool_ref* pools, int32_t n_pools, int32_t* block_table,
-                           int64_t bt_stride, const int32_t* seq_lens, int64_t batch,
-                           int64_t block_size, int64_t n_pages, int32_t* free_stack,
-                           int32_t* free_top, int32_t* workspace, int32_t* info, void* stream) {
-  const char* what = "skv_compact";
+extern "C" int skv_release_shared(int32_t* free_stack, int32_t* free_top, int64_t n_pages, int32_t* refs,
+                                  int32_t* block_table, int64_t bt_stride, int32_t* seq_lens,
+                                  const uint8_t* release_mask, int64_t batch, int64_t block_size, int32_t* status,
+                                  void* stream) {
+  const char* what = "skv_release_shared";
+  if (batch < 0 || batch > kEvictMaxBatch) {
+    return set_error(SKV_EINVAL, "%s: batch must be in [0, %d]; got %lld", what, kEvictMaxBatch, (long long)batch);
+  }
+  if (block_size <= 0 || block_size > INT32_MAX || bt_stride <= 0 || n_pages <= 0 || n_pages > INT32_MAX ||
+      batch * bt_stride > INT32_MAX - kEvictThreads) {
+    return set_error(SKV_EINVAL, "%s: bad block_size/bt_stride/n_pages", what);
+  }
+  if (!free_stack || !free_top || !refs || (batch > 0 && (!block_table || !seq_lens || !release_mask))) {
+    return set_error(SKV_EINVAL, "%s: NULL pointer", what);
+  }
+  if (batch == 0) return SKV_OK;
+  hipLaunchKernelGGL(k_release_shared, dim3(1), dim3(kEvictThreads), 0, static_cast<hipStream_t>(stream), free_stack,
+                     free_top, n_pages, refs, block_table, bt_stride, seq_lens, release_mask, static_cast<int>(batch),
+                     static_cast<int>(block_size), status);
+  return check_launch(what);
+}
+
+// The launches of skv_compact and, with refs, skv_compact_shared.
+static int compact(const char* what, const skv_pool_ref* pools, int32_t n_pools, int32_t* block_table, int64_t bt_stride,
+                   const int32_t* seq_lens, int64_t batch, int64_t block_size, int64_t n_pages, int32_t* free_stack,
+                   int32_t* free_top, int32_t* refs, int32_t* workspace, int32_t* info, void* stream) {
   if (n_pools < 1 || n_pools > kMaxPools || !pools) {
     return set_error(SKV_EINVAL, "%s: n_pools must be in [1, %d]; got %d", what, kMaxPools, n_pools);
   }
@@ -385,16 +521,16 @@ extern "C" int skv_compact(const skv_pool_ref* pools, int32_t n_pools, int32_t* 
   if (!workspace || !info || !free_stack || !free_top) {
     return set_error(SKV_EINVAL, "%s: NULL workspace/info/free list", what);
   }
-  PoolRefs refs{};
-  refs.n = n_pools;
+  PoolRefs pr{};
+  pr.n = n_pools;
   int64_t slices_per_mover = 0;
   for (int q = 0; q < n_pools; ++q) {
     if (!pools[q].base || pools[q].page_bytes <= 0 || (pools[q].page_bytes & 15) ||
         (reinterpret_cast<uintptr_t>(pools[q].base) & 15)) {
       return set_error(SKV_EINVAL, "%s: pool %d needs a 16-byte aligned base and page_bytes", what, q);
     }
-    refs.base[q] = static_cast<uint8_t*>(pools[q].base);
-    refs.page_bytes[q] = pools[q].page_bytes;
+    pr.base[q] = static_cast<uint8_t*>(pools[q].base);
+    pr.page_bytes[q] = pools[q].page_bytes;
     slices_per_mover += ceil_div(pools[q].page_bytes, kCopySlice);
   }
   if (n_pages >= (1 << 24) || n_pages * slices_per_mover >= (1 << 24)) {
@@ -419,11 +555,37 @@ extern "C" int skv_compact(const skv_pool_ref* pools, int32_t n_pools, int32_t* 
                      free_stack, free_top, info);
   if ((rc = check_launch(what))) return rc;
   CopySlices cs{};
-  for (int q = 0; q < n_pools; ++q) cs.first[q + 1] = cs.first[q] + static_cast<int32_t>(ceil_div(refs.page_bytes[q], kCopySlice));
+  for (int q = 0; q < n_pools; ++q) cs.first[q + 1] = cs.first[q] + static_cast<int32_t>(ceil_div(pr.page_bytes[q], kCopySlice));
   cs.per_mover = cs.first[n_pools];
   const TableRef tr{block_table, seq_lens, static_cast<int32_t>(bt_stride), static_cast<int32_t>(batch),
                     static_cast<int32_t>(block_size)};
-  hipLaunchKernelGGL(k_compact_copy, dim3(kPersistentBlocks), dim3(kCompactCopyThreads), 0, s, refs, cs, tr,
+  if (!refs) {
+    hipLaunchKernelGGL((k_compact_copy<false>), dim3(kPersistentBlocks), dim3(kCompactCopyThreads), 0, s, pr, cs, tr,
+                       workspace, n_pages, info);
+    return check_launch(what);
+  }
+  hipLaunchKernelGGL((k_compact_copy<true>), dim3(kPersistentBlocks), dim3(kCompactCopyThreads), 0, s, pr, cs, tr,
                      workspace, n_pages, info);
+  if ((rc = check_launch(what))) return rc;
+  hipLaunchKernelGGL(k_compact_finish, dim3(static_cast<unsigned>(ceil_div(n_pages, kCompactCopyThreads))),
+                     dim3(kCompactCopyThreads), 0, s, workspace, n_pages, info, refs);
   return check_launch(what);
+}
+
+extern "C" int skv_compact(const skv_pool_ref* pools, int32_t n_pools, int32_t* block_table,
+                           int64_t bt_stride, const int32_t* seq_lens, int64_t batch,
+                           int64_t block_size, int64_t n_pages, int32_t* free_stack,
+                           int32_t* free_top, int32_t* workspace, int32_t* info, void* stream) {
+  return compact("skv_compact", pools, n_pools, block_table, bt_stride, seq_lens, batch, block_size, n_pages, free_stack,
+                 free_top, nullptr, workspace, info, stream);
+}
+
+extern "C" int skv_compact_shared(const skv_pool_ref* pools, int32_t n_pools, int32_t* block_table, int64_t bt_stride,
+                                  const int32_t* seq_lens, int64_t batch, int64_t block_size, int64_t n_pages,
+                                  int32_t* free_stack, int32_t* free_top, int32_t* refs, int32_t* workspace,
+                                  int32_t* info, void* stream) {
+  const char* what = "skv_compact_shared";
+  if (!refs) return set_error(SKV_EINVAL, "%s: refs is NULL", what);
+  return compact(what, pools, n_pools, block_table, bt_stride, seq_lens, batch, block_size, n_pages, free_stack,
+                 free_top, refs, workspace, info, stream);
 }

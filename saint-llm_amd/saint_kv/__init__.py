@@ -11,18 +11,21 @@ C-ABI call.
 from saint_kv import ops
 from saint_kv.attention import cached_attention, decode_attention
 from saint_kv.decode import CapturedSteps, DecodeCache, LayerSpec
+from saint_kv.fp4 import Fp4TokenCache, fp4_attention
 from saint_kv.kv_cache import CSAKVCacheLayer, HCAKVCacheLayer, KVCacheBundle, SWAKVCacheLayer
 
 __all__ = [
     "CSAKVCacheLayer",
     "CapturedSteps",
     "DecodeCache",
+    "Fp4TokenCache",
     "HCAKVCacheLayer",
     "KVCacheBundle",
     "LayerSpec",
     "SWAKVCacheLayer",
     "cached_attention",
     "decode_attention",
+    "fp4_attention",
     "ops",
 ]
 __version__ = "0.1.0"

@@ -85,6 +85,16 @@ SIGNATURES: dict[str, list] = {
         _P, _P, _I64, _I64, _I64, _P, _I64, _P, _P, _I64, _I64, _I64, _P, _I64, _I32, _P,
     ],
     "skv_release": [_P, _P, _I64, _P, _I64, _P, _P, _I64, _I64, _P, _P],
+    "skv_fork": [_P, _P, _I64, _P, _P, _I64, _P, _I64, _I64, _P, _P, _I64, _P, _I32, _P, _P],
+    "skv_copy_slots": [_P, _I64, _I64, _P, _P, _I64, _P],
+    "skv_release_shared": [_P, _P, _I64, _P, _P, _I64, _P, _P, _I64, _I64, _P, _P],
+    "skv_compact_shared": [_P, _I32, _P, _I64, _P, _I64, _I64, _I64, _P, _P, _P, _P, _P, _P],
+    "skv_fp4_page_bytes": [_I64, _I64, _I64],
+    "skv_fp4_quant_append": [_P, _P, _P, _I32, _P, _P, _I64, _I32, _P],
+    "skv_fp4_gather": [_P, _P, _P, _I32, _P, _P, _I64, _P],
+    "skv_fp4_attention_desc_size": [],
+    "skv_fp4_attention_workspace": [_P],
+    "skv_fp4_attention": [_P, _P, _I64, _P],
     "skv_decode_step": [_P, _P, _P],
     "skv_decode_step_launches": [_P],
     "skv_decode_desc_sizes": [_P],
@@ -134,9 +144,25 @@ class RingLayer(ctypes.Structure):
     ]
 
 
+class Fp4Cache(ctypes.Structure):
+    """skv_fp4_cache: the pages of a 4-bit token cache and their block table."""
+
+    _fields_ = [
+        ("pool", _P), ("block_size", _I64), ("n_pages", _I64), ("n_kv_heads", _I64), ("head_dim", _I64),
+        ("block_table", _P), ("bt_stride", _I64), ("batch", _I64),
+    ]
+
+
+class Fp4Rows(ctypes.Structure):
+    """skv_fp4_rows: keys or values outside the pages."""
+
+    _fields_ = [("data", _P), ("seq_stride", _I64), ("tok_stride", _I64), ("head_stride", _I64)]
+
+
 # entry points returning a size rather than a status code
 INT64_RESULTS = {"skv_topk_workspace_words", "skv_attention_workspace", "skv_attention_desc_size",
-                 "skv_decode_step_attend_workspace"}
+                 "skv_decode_step_attend_workspace", "skv_fp4_page_bytes", "skv_fp4_attention_desc_size",
+                 "skv_fp4_attention_workspace"}
 
 _lib: ctypes.CDLL | None = None
 

@@ -99,6 +99,7 @@ class _Group:
     free_top: torch.Tensor
     block_table: torch.Tensor
     n_entries: torch.Tensor
+    refs: torch.Tensor | None = None  # int32 [n_pages] from the first fork on: a page's holders beyond the first
 
 
 class DecodeCache:
@@ -547,7 +548,47 @@ class DecodeCache:
 
         return state.load_sequence(self, b, path)
 
-    # -------------------------------------------------- eviction / compaction --
+    # ----------------------------------------- forks / eviction / compaction --
+    def _group_pools(self, gi: int) -> list[torch.Tensor]:
+        """The pools whose pages page group gi hands out."""
+        pools = []
+        for i, spec in enumerate(self.layers):
+            if spec.kind in ("csa", "hca") and self.group_of_rate[spec.m] == gi:
+                pools.append(self.pool[i])
+                if self.idx_pool[i] is not None:
+                    pools.append(self.idx_pool[i])
+        return pools
+
+    def fork(self, src, dst) -> None:
+        """Make the empty sequences dst[f] copies of src[f] (lists of sequences, or
+        one of each): they share src's whole pages; begun pages, rings and pooling
+        states are copied.  Raises RuntimeError, with every sequence and free list
+        as before, if a page group lacks pages for the begun ones."""
+        from saint_kv.fp4 import check_forks
+
+        src, dst = check_forks(src, dst, self.host_lens)
+        dev = self.device
+        idx = torch.as_tensor(np.stack([src, dst]).astype(np.int32), device=dev)
+        gst = self.group_status
+        for gi, g in enumerate(self.groups):
+            if g.refs is None:
+                g.refs = torch.zeros(g.n_pages, dtype=torch.int32, device=dev)
+            ops.fork(g.free_stack, g.free_top, g.refs, g.block_table, g.n_entries, idx[0], idx[1], self.block_size,
+                     self._group_pools(gi), gst[gi:gi + 1])
+        bad = gst[: len(self.groups)].cpu().tolist()
+        if any(bad):
+            mask = torch.zeros(self.batch, dtype=torch.uint8, device=dev)
+            mask[idx[1].long()] = 1
+            for gi, g in enumerate(self.groups):
+                if bad[gi] == 0:
+                    ops.release(g.free_stack, g.free_top, g.block_table, g.n_entries, mask, self.block_size,
+                                refs=g.refs)
+            raise RuntimeError("DecodeCache fork refused (" + "; ".join(
+                f"group m={g.m}: status bits {b}" for g, b in zip(self.groups, bad) if b) + ")")
+        slots = [t for t in (*self.ring, *self.state, *self.idx_state) if t is not None]
+        ops.copy_slots([self.tok_lens, *slots], idx[0], idx[1])
+        self.host_lens[dst] = self.host_lens[src]
+
     def release(self, mask: np.ndarray, mask_dev: torch.Tensor | None = None, check: bool = True) -> None:
         """Finish the sequences with mask[b]: their pages return to the free lists.
 
@@ -566,7 +607,7 @@ class DecodeCache:
         m_dev = torch.as_tensor(mask.astype(np.uint8), device=self.device) if mask_dev is None else mask_dev
         for gi, g in enumerate(self.groups):
             ops.release(g.free_stack, g.free_top, g.block_table, g.n_entries, m_dev,
-                        self.block_size, self.group_status[gi:gi + 1])
+                        self.block_size, self.group_status[gi:gi + 1], refs=g.refs)
         self.tok_lens.masked_fill_(m_dev.view(torch.bool), 0)  # 0/1 bytes read as bool, no conversion
         self.host_lens[mask] = 0
         if check:
@@ -598,16 +639,11 @@ class DecodeCache:
             raise ValueError(f"compaction workspace needs {self.compact_workspace_words()} int32")
         ws_off = 0
         for gi, g in enumerate(self.groups):
-            pools = []
-            for i, spec in enumerate(self.layers):
-                if spec.kind in ("csa", "hca") and self.group_of_rate[spec.m] == gi:
-                    pools.append(self.pool[i])
-                    if self.idx_pool[i] is not None:
-                        pools.append(self.idx_pool[i])
+            pools = self._group_pools(gi)
             ws = ws_all[ws_off: ws_off + 3 * g.n_pages]
             ws_off += 3 * g.n_pages
             ops.compact(pools, g.block_table, g.n_entries, self.block_size, g.free_stack,
-                        g.free_top, ws, info[gi])
+                        g.free_top, ws, info[gi], refs=g.refs)
         if not sync:
             return info
         return [tuple(int(v) for v in row) for row in info.cpu()]

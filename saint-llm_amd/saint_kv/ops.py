@@ -34,6 +34,23 @@ def _require_i32(t: torch.Tensor, name: str, shape: tuple[int, ...] | None = Non
         raise ValueError(f"{name} must have shape {shape}; got {tuple(t.shape)}")
 
 
+class _on_device:
+    """Makes the tensor's device the current one for a launch, where it is not."""
+
+    def __init__(self, t: torch.Tensor) -> None:
+        self.index, self.back = t.device.index, -1
+
+    def __enter__(self) -> None:
+        here = torch.cuda.current_device()
+        if self.index is not None and self.index != here:
+            self.back = here
+            torch.cuda.set_device(self.index)
+
+    def __exit__(self, *exc) -> None:
+        if self.back >= 0:
+            torch.cuda.set_device(self.back)
+
+
 def row_bytes_of(pool: torch.Tensor) -> int:
     """Bytes of one row of a pool shaped [n_pages, block_size, *row]."""
     if pool.dim() < 3:
@@ -647,12 +664,183 @@ def indexer_topk_chunk(q: torch.Tensor, w: torch.Tensor, keys: torch.Tensor, n_b
 
 
 # ---------------------------------------------------------------------------
-# Eviction and compaction
+# 4-bit token cache
 # ---------------------------------------------------------------------------
+FP4_MAX_DIM = 512
+
+
+def fp4_pool(n_pages: int, block_size: int, n_kv_heads: int, head_dim: int,
+             device: torch.device | str) -> torch.Tensor:
+    """An empty pool of the 4-bit token cache: uint8 [n_pages, block_size,
+    n_kv_heads, 17 * head_dim / 16] (a page's bytes are laid out by head and
+    plane, as skv_fp4_cache says; block_size is a multiple of 16, head_dim a
+    multiple of 32 up to 512)."""
+    size = int(_lib.load().skv_fp4_page_bytes(block_size, n_kv_heads, head_dim))
+    if size < 0:
+        _lib.check(_lib.SKV_EINVAL, "skv_fp4_page_bytes")
+    return torch.zeros(n_pages, block_size, n_kv_heads, size // (block_size * n_kv_heads), dtype=torch.uint8,
+                       device=device)
+
+
+def fp4_cache(pool: torch.Tensor, block_table: torch.Tensor) -> _lib.Fp4Cache:
+    """The checked skv_fp4_cache of a pool and a block table."""
+    _require_gpu(pool, "pool")
+    if pool.dtype != torch.uint8 or pool.dim() != 4 or not pool.is_contiguous():
+        raise ValueError("pool must be a contiguous uint8 [n_pages, block_size, n_kv_heads, 17 * head_dim / 16] tensor")
+    n_pages, bs, heads, row = pool.shape
+    if row % 34 or not row or row // 17 * 16 > FP4_MAX_DIM:
+        raise ValueError(f"pool rows of {row} bytes are not 17/16 of a head_dim that is a multiple of 32 up to "
+                         f"{FP4_MAX_DIM}")
+    _require_i32(block_table, "block_table")
+    if block_table.dim() != 2:
+        raise ValueError("block_table must be 2D [batch, max_pages]")
+    _same_device(pool, "pool", block_table=block_table)
+    batch, bt_stride = block_table.shape
+    return _lib.Fp4Cache(pool.data_ptr(), bs, n_pages, heads, row // 17 * 16, block_table.data_ptr(), bt_stride, batch)
+
+
+def _same_device(t: torch.Tensor, name: str, **others: torch.Tensor | None) -> None:
+    for other, x in others.items():
+        if x is not None and x.device != t.device:
+            raise ValueError(f"{other} is on {x.device}, {name} on {t.device}")
+
+
+def _fp4_rows(t: torch.Tensor, name: str, cache: _lib.Fp4Cache, dtypes: tuple[torch.dtype, ...]) -> _lib.Fp4Rows:
+    _require_gpu(t, name)
+    if t.dtype not in dtypes or t.dim() != 4 or t.shape[0] != cache.batch or \
+            tuple(t.shape[2:]) != (cache.n_kv_heads, cache.head_dim):
+        raise ValueError(f"{name} must be {' or '.join(str(d) for d in dtypes)} [{cache.batch}, T, {cache.n_kv_heads}, "
+                         f"{cache.head_dim}]; got {t.dtype} {tuple(t.shape)}")
+    es = t.element_size()
+    strides = [s * es if n > 1 else 0 for n, s in zip(t.shape[:3], t.stride()[:3])]
+    if t.stride(3) != 1 or t.data_ptr() % 16 or any(s % 16 for s in strides):
+        raise ValueError(f"{name} needs contiguous dims and 16-byte aligned rows")
+    return _lib.Fp4Rows(t.data_ptr(), *strides)
+
+
+def fp4_quant_append(pool: torch.Tensor, block_table: torch.Tensor, seq_lens: torch.Tensor, k: torch.Tensor,
+                     v: torch.Tensor, n_new: int | torch.Tensor) -> None:
+    """Quantize the ``n_new`` newest tokens of each sequence (``seq_lens`` counts
+    them already) into the 4-bit pages: token i of k, v (bf16 or fp32 [B, T,
+    n_kv_heads, head_dim], any strides that keep rows 16-byte aligned) becomes
+    position ``seq_lens - n_new + i``."""
+    c = fp4_cache(pool, block_table)
+    _require_i32(seq_lens, "seq_lens", (c.batch,))
+    rows = [_fp4_rows(t, name, c, (torch.bfloat16, torch.float32)) for t, name in ((k, "k"), (v, "v"))]
+    if k.dtype != v.dtype or k.shape != v.shape:
+        raise ValueError("k and v must have the same dtype and shape")
+    n_ptr, n_uni = _n_new_args(n_new, c.batch)
+    if n_ptr is None and n_uni > k.shape[1]:
+        raise ValueError(f"n_new={n_uni} exceeds the {k.shape[1]} tokens of k and v")
+    _same_device(pool, "pool", seq_lens=seq_lens, k=k, v=v, n_new=n_new if n_ptr is not None else None)
+    with _on_device(pool):
+        _lib.call("skv_fp4_quant_append", ctypes.byref(c), seq_lens.data_ptr(), n_ptr, n_uni, ctypes.byref(rows[0]),
+                  ctypes.byref(rows[1]), k.shape[1], int(k.dtype == torch.float32), _lib.stream_handle(pool.device))
+
+
+def fp4_gather(pool: torch.Tensor, block_table: torch.Tensor, seq_lens: torch.Tensor, out_k: torch.Tensor,
+               out_v: torch.Tensor, n: int | torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """The ``n`` newest tokens of each sequence as bf16 (exact): position
+    ``seq_lens - n + i`` goes to token i of out_k, out_v (bf16 [B, T, n_kv_heads,
+    head_dim]); later tokens of them are left as they are."""
+    c = fp4_cache(pool, block_table)
+    _require_i32(seq_lens, "seq_lens", (c.batch,))
+    rows = [_fp4_rows(t, name, c, (torch.bfloat16,)) for t, name in ((out_k, "out_k"), (out_v, "out_v"))]
+    if out_k.shape != out_v.shape:
+        raise ValueError("out_k and out_v must have the same shape")
+    n_ptr, n_uni = _n_new_args(n, c.batch)
+    if n_ptr is None and n_uni > out_k.shape[1]:
+        raise ValueError(f"n={n_uni} exceeds the {out_k.shape[1]} tokens of out_k and out_v")
+    _same_device(pool, "pool", seq_lens=seq_lens, out_k=out_k, out_v=out_v, n=n if n_ptr is not None else None)
+    with _on_device(pool):
+        _lib.call("skv_fp4_gather", ctypes.byref(c), seq_lens.data_ptr(), n_ptr, n_uni, ctypes.byref(rows[0]),
+                  ctypes.byref(rows[1]), out_k.shape[1], _lib.stream_handle(pool.device))
+    return out_k, out_v
+
+
+# ---------------------------------------------------------------------------
+# Eviction, forks and compaction
+# ---------------------------------------------------------------------------
+def _pool_refs(pools: list[torch.Tensor], n_pages: int, block_size: int) -> ctypes.Array:
+    """skv_pool_refs of pools of n_pages pages of block_size rows."""
+    refs = (_lib.PoolRef * len(pools))()
+    for i, p in enumerate(pools):
+        _require_gpu(p, "pool")
+        if not p.is_contiguous():
+            raise ValueError("pool must be contiguous")
+        rb = row_bytes_of(p)
+        if p.shape[0] != n_pages or p.shape[1] != block_size:
+            raise ValueError("every pool must have n_pages pages of block_size rows")
+        if (block_size * rb) % 16:
+            raise ValueError(f"a pool's page must be a multiple of 16 bytes; got {block_size * rb}")
+        refs[i].base = p.data_ptr()
+        refs[i].page_bytes = block_size * rb
+    return refs
+
+
+def fork(free_stack: torch.Tensor, free_top: torch.Tensor, refs: torch.Tensor, block_table: torch.Tensor,
+         seq_lens: torch.Tensor, src: torch.Tensor, dst: torch.Tensor, block_size: int, pools: list[torch.Tensor],
+         status: torch.Tensor) -> None:
+    """Make the empty sequences ``dst[f]`` copies of ``src[f]`` (int32 [n]): whole
+    pages are shared, the last, begun page is copied in every pool.
+
+    ``refs`` (int32 [n_pages], zero before the first fork) counts a page's
+    holders beyond the first; ``release`` and ``compact`` of such a cache take
+    it too.  All-or-nothing: a refusal sets ``status`` and writes nothing else
+    (see skv_fork)."""
+    n_pages = free_stack.numel()
+    _require_i32(free_stack, "free_stack")
+    _require_i32(free_top, "free_top", (1,))
+    _require_i32(refs, "refs", (n_pages,))
+    _require_i32(block_table, "block_table")
+    if block_table.dim() != 2:
+        raise ValueError("block_table must be 2D [batch, max_pages]")
+    batch, bt_stride = block_table.shape
+    _require_i32(seq_lens, "seq_lens", (batch,))
+    _require_i32(src, "src")
+    if src.dim() != 1:
+        raise ValueError(f"src must be int32 [n]; got {tuple(src.shape)}")
+    _require_i32(dst, "dst", tuple(src.shape))
+    _require_i32(status, "status", (1,))
+    _same_device(block_table, "block_table", free_stack=free_stack, free_top=free_top, refs=refs, seq_lens=seq_lens,
+                 src=src, dst=dst, status=status, **{f"pools[{i}]": p for i, p in enumerate(pools)})
+    arr = _pool_refs(pools, n_pages, block_size)
+    with _on_device(block_table):
+        _lib.call("skv_fork", free_stack.data_ptr(), free_top.data_ptr(), n_pages, refs.data_ptr(),
+                  block_table.data_ptr(), bt_stride, seq_lens.data_ptr(), batch, block_size, src.data_ptr(),
+                  dst.data_ptr(), src.shape[0], ctypes.cast(arr, ctypes.c_void_p), len(pools), status.data_ptr(),
+                  _lib.stream_handle(block_table.device))
+
+
+def copy_slots(arrays: list[torch.Tensor], src: torch.Tensor, dst: torch.Tensor) -> None:
+    """``t[dst[f]] = t[src[f]]`` for every tensor t [n_slots, ...] of ``arrays`` and
+    every f (int32 [n]): what forked sequences hold outside their pages."""
+    if not arrays:
+        return
+    _require_i32(src, "src")
+    if src.dim() != 1:
+        raise ValueError(f"src must be int32 [n]; got {tuple(src.shape)}")
+    _require_i32(dst, "dst", tuple(src.shape))
+    n = arrays[0].shape[0]
+    refs = (_lib.PoolRef * len(arrays))()
+    for i, t in enumerate(arrays):
+        _require_gpu(t, f"arrays[{i}]")
+        if t.dim() < 1 or t.shape[0] != n or not t.is_contiguous():
+            raise ValueError(f"arrays[{i}] must be contiguous with {n} slots; got {tuple(t.shape)}")
+        refs[i].base = t.data_ptr()
+        refs[i].page_bytes = t[0].numel() * t.element_size() if n else 0
+    _same_device(src, "src", dst=dst, **{f"arrays[{i}]": t for i, t in enumerate(arrays)})
+    if n:
+        with _on_device(src):
+            _lib.call("skv_copy_slots", ctypes.cast(refs, ctypes.c_void_p), len(arrays), n, src.data_ptr(),
+                      dst.data_ptr(), src.shape[0], _lib.stream_handle(src.device))
+
+
 def release(free_stack: torch.Tensor, free_top: torch.Tensor, block_table: torch.Tensor,
             seq_lens: torch.Tensor, mask: torch.Tensor, block_size: int,
-            status: torch.Tensor | None = None) -> None:
-    """Return every page of the sequences with mask[b] to the free stack."""
+            status: torch.Tensor | None = None, refs: torch.Tensor | None = None) -> None:
+    """Return every page of the sequences with mask[b] to the free stack; with
+    ``refs`` (a cache that forks, see ``fork``) those that no other holds."""
     _require_i32(free_stack, "free_stack")
     _require_i32(free_top, "free_top", (1,))
     _require_i32(block_table, "block_table")
@@ -663,6 +851,14 @@ def release(free_stack: torch.Tensor, free_top: torch.Tensor, block_table: torch
         raise ValueError("mask must be uint8/bool [batch]")
     if status is not None:
         _require_i32(status, "status", (1,))
+    if refs is not None:
+        _require_i32(refs, "refs", (free_stack.numel(),))
+        with _on_device(block_table):
+            _lib.call("skv_release_shared", free_stack.data_ptr(), free_top.data_ptr(), free_stack.numel(),
+                      refs.data_ptr(), block_table.data_ptr(), bt_stride, seq_lens.data_ptr(),
+                      mask.contiguous().data_ptr(), batch, block_size, _lib.ptr(status),
+                      _lib.stream_handle(block_table.device))
+        return
     _lib.call("skv_release", free_stack.data_ptr(), free_top.data_ptr(), free_stack.numel(),
               block_table.data_ptr(), bt_stride, seq_lens.data_ptr(), mask.contiguous().data_ptr(),
               batch, block_size, _lib.ptr(status), _lib.stream_handle(block_table.device))
@@ -670,20 +866,16 @@ def release(free_stack: torch.Tensor, free_top: torch.Tensor, block_table: torch
 
 def compact(pools: list[torch.Tensor], block_table: torch.Tensor, seq_lens: torch.Tensor,
             block_size: int, free_stack: torch.Tensor, free_top: torch.Tensor,
-            workspace: torch.Tensor, info: torch.Tensor) -> None:
+            workspace: torch.Tensor, info: torch.Tensor, refs: torch.Tensor | None = None) -> None:
     """Defragment ``pools`` (sharing ``block_table``) so live pages occupy [0, n_live).
 
     ``workspace`` (int32 [3 * n_pages]): its first n_pages words must be zero
     before the first call; every call leaves them zero (the rest is scratch).
+    ``refs``: the counts of a cache that forks (see ``fork``), which move with
+    their pages.
     """
     n_pages = free_stack.numel()
-    refs = (_lib.PoolRef * len(pools))()
-    for i, p in enumerate(pools):
-        pn, pbs, rb = _check_pool(p)
-        if pn != n_pages or pbs != block_size:
-            raise ValueError("every pool must have n_pages pages of block_size rows")
-        refs[i].base = p.data_ptr()
-        refs[i].page_bytes = pbs * rb
+    arr = _pool_refs(pools, n_pages, block_size)
     _require_i32(block_table, "block_table")
     batch, bt_stride = block_table.shape
     _require_i32(seq_lens, "seq_lens", (batch,))
@@ -691,7 +883,12 @@ def compact(pools: list[torch.Tensor], block_table: torch.Tensor, seq_lens: torc
     _require_i32(free_top, "free_top", (1,))
     _require_i32(workspace, "workspace", (3 * n_pages,))
     _require_i32(info, "info", (2,))
-    _lib.call("skv_compact", ctypes.cast(refs, ctypes.c_void_p), len(pools), block_table.data_ptr(), bt_stride,
-              seq_lens.data_ptr(), batch, block_size, n_pages, free_stack.data_ptr(),
-              free_top.data_ptr(), workspace.data_ptr(), info.data_ptr(),
-              _lib.stream_handle(block_table.device))
+    args = (ctypes.cast(arr, ctypes.c_void_p), len(pools), block_table.data_ptr(), bt_stride,
+            seq_lens.data_ptr(), batch, block_size, n_pages, free_stack.data_ptr(), free_top.data_ptr())
+    if refs is not None:
+        _require_i32(refs, "refs", (n_pages,))
+        with _on_device(block_table):
+            _lib.call("skv_compact_shared", *args, refs.data_ptr(), workspace.data_ptr(), info.data_ptr(),
+                      _lib.stream_handle(block_table.device))
+        return
+    _lib.call("skv_compact", *args, workspace.data_ptr(), info.data_ptr(), _lib.stream_handle(block_table.device))
