@@ -8,21 +8,28 @@
 // by exp2(m_old - m_new) where the maximum moves.
 //
 // A K/V head's query rows (its query heads times the query tokens) are cut into
-// blocks of 16 MT rows, the positions into chunks; a workgroup takes a row block over a
-// chunk, its four waves tiles of 32 positions in turn, each with a softmax of
-// its own, joined at the end.  No wave waits for another on the way:
-//   * S^T = K Q^T: lane (key, g) of a 16-key tile reads D / 4 consecutive dims of
-//     its key, g's quarter, from the page straight into the registers of the
-//     products' A operand (the order of the dims within a product is free as
-//     long as the query's is the same: step s takes dims g D / 4 + 8 s ..+7);
-//     for 128 dims that is 16 bytes and one scale byte a lane, a tile 1 KB in one run.
+// blocks of 16 MT rows.  A workgroup takes a row block over a run of positions, its four
+// waves tiles of 32 positions in turn, each with a softmax of its own, joined at the
+// end.  No wave waits for another on the way:
+//   * S^T = K Q^T by the scaled products of gfx950 (v_mfma_scale_f32_16x16x128_f8f6f4),
+//     which take e2m1 codes and their scale bytes as they lie in the page: lane
+//     (key, g) of 16 keys reads g's quarter of its key's codes straight into the operand
+//     registers, 16 bytes of 128 dims a step.  The query goes in as two e4m3 parts,
+//     q = hi 2^a + lo 2^(a - 5) with 2^a by 32 dims: a bf16 value's 8 bits are 4 and 4, so
+//     the parts are exact (but for values below 2^-13 of their 32's largest, which are
+//     exact to 2^-23 of it).
 //   * the values go through the wave's own part of LDS as bf16, rows of D in
 //     swizzled chunks, and come back transposed (ds_read_b64_tr_b16) as the A
 //     operand of O^T = V^T P^T, whose B operand is P^T as the scores' accumulators
 //     hold it.  O^T keeps a row's output in the lanes that hold its m and l.
-// The codes of the next tile are in flight while one is multiplied, the page
-// ids of 32 tiles sit in the lanes of a register.  Chunks of long sequences are
-// joined by a second launch.
+// The codes of the next two tiles are in flight while one is multiplied, the page
+// ids of 32 tiles sit in the lanes of a register.
+//
+// Work: the tiles of all (sequence, row block, head) items, one after another, are
+// dealt to as many workgroups as the device holds at once, in equal runs that may
+// cut a long item; the lengths are on the device, so every workgroup works the
+// runs out for itself from their prefix sum.  A cut item's pieces are joined by a
+// second launch.
 #include <algorithm>
 
 #include "skv_fp4.h"
@@ -32,12 +39,14 @@ namespace skv {
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef short short4v __attribute__((ext_vector_type(4)));
+typedef int i32x8 __attribute__((ext_vector_type(8)));
 
 constexpr int kF4Threads = 256;
 constexpr int kF4Waves = kF4Threads / kWave;
 constexpr int kF4Tile = 32;        // positions per tile
 constexpr float kF4Log2e = 1.4426950408889634f;
 constexpr float kF4Move = 8.f;     // log2: the reference maximum moves when a tile's passes it by more
+constexpr float kF4None = -3e38f;  // the reference maximum before the first key: exp2(-inf - kF4None) is 0, not NaN
 
 struct Fp4AttnArgs {
   const uint8_t* q;
@@ -52,7 +61,9 @@ struct Fp4AttnArgs {
   int32_t B, T, H, Hkv, G, D;
   int32_t window;  // 0: none
   float scale, softcap;
-  int32_t row_blocks, chunks, chunk_tiles;
+  int32_t row_blocks;
+  int32_t* sched;   // [items + 1]: tiles before every (sequence, row block), for the join
+  int32_t max_groups, small;  // see fp4_groups; items of at most `small` tiles are not cut
 };
 
 // The positions that the rows [r0, r0 + n) of a K/V head see.
@@ -61,6 +72,7 @@ struct Fp4Span {
   int first, last;       // [first, last): some row sees them
   int all_lo, all_hi;    // [all_lo, all_hi): every row sees them
   int tile0, tiles;
+  __device__ __forceinline__ int units() const { return max(tiles, 1); }  // an item that sees nothing is one, too
 };
 
 __device__ __forceinline__ Fp4Span fp4_span(const Fp4AttnArgs& a, int b, int r0, int n) {
@@ -78,11 +90,18 @@ __device__ __forceinline__ Fp4Span fp4_span(const Fp4AttnArgs& a, int b, int r0,
   return s;
 }
 
-// Chunks that hold positions of a span: the last takes what is past the bound
-// that the chunks were made for.
-__device__ __forceinline__ int fp4_chunks(const Fp4AttnArgs& a, const Fp4Span& s) {
-  return min((s.tiles + a.chunk_tiles - 1) / a.chunk_tiles, a.chunks);
+// Workgroups that share the units: a run of fewer than 8 tiles, 2 a wave, is not
+// worth a workgroup, but an item is.  Workgroup i takes [i total / n, (i + 1) total / n).
+constexpr int kF4RunTiles = 8;
+constexpr int kF4SmallTiles = 16;
+constexpr int kF4MaxItems = 2048;  // (sequence, row block)s whose prefix sum LDS holds
+
+__device__ __forceinline__ int fp4_groups(const Fp4AttnArgs& a, int total) {
+  return min(a.max_groups, max((total + kF4RunTiles - 1) / kF4RunTiles, a.B * a.row_blocks * a.Hkv));
 }
+__device__ __forceinline__ int fp4_run_start(int64_t i, int total, int n) { return static_cast<int>(i * total / n); }
+// The workgroup whose run holds unit x.
+__device__ __forceinline__ int fp4_owner(int64_t x, int total, int n) { return static_cast<int>(((x + 1) * n - 1) / total); }
 
 __device__ __forceinline__ bf16x8 fp4_bf16x8(u32x4 v) { return __builtin_bit_cast(bf16x8, v); }
 
@@ -117,9 +136,21 @@ template <int DP>
 struct Fp4Raw {
   static constexpr int kWords = DP / 32;                    // of a lane's quarter of a row
   static constexpr int kScales = DP >= 128 ? DP / 128 : 1;  // 32-dim blocks it reaches into
-  uint32_t k[2][kWords], v[2][kWords];
-  uint8_t ks[2][kScales], vs[2][kScales];
-  bool mapped[2];  // uniform
+  static constexpr int kKeyWords = DP >= 128 ? kWords : 4;  // of 64 dims a whole block, each in two lanes
+  uint32_t k[2][kKeyWords], v[2][kWords];
+  uint32_t ks[2][kScales], vs[2][kScales];
+  uint32_t packed[2];  // scale bytes as loaded, of heads of 64 and 128 dims
+  int page[2];  // uniform; -1: not mapped
+};
+
+// A tile's scores, and what their masks need (uniform): every row sees every
+// key; the halves that are mapped; keys with a NaN block among their values.
+template <int MT>
+struct Fp4Tile {
+  f32x4 st[MT][2];  // row 16 mt + col, keys 16 h + 4 grp + i
+  int page[2];
+  bool masked;
+  uint32_t nan_keys;
 };
 
 template <int DP>
@@ -127,6 +158,8 @@ struct Fp4Smem {
   // per wave: 32 value rows of DP bf16; at the end 16 output rows of DP fp32
   alignas(16) uint8_t tile[kF4Waves][64 * DP];
   float m[kF4Waves][64], l[kF4Waves][64];
+  int pre[kF4MaxItems + 1];
+  int scan[17];
 };
 
 // DP: the head's dims padded to 64, 128, 256 or 512 (kExact: D == DP).
@@ -134,24 +167,31 @@ template <int DP, int MT, bool kExact>
 struct Fp4Wave {
   using Raw = Fp4Raw<DP>;
   static constexpr int kWords = Raw::kWords, kScales = Raw::kScales;
+  static constexpr int kSteps = DP >= 128 ? DP / 128 : 1;  // products of 128 dims, or of the two parts of 64
   static constexpr int kBlocks = DP / 16;  // 16-dim blocks of the output
+  static constexpr bool kPacked = kExact && DP <= 128;
+  static constexpr bool kOnce = DP * MT <= 256 && MT * 16 < 64;  // all of a head's rows in a workgroup: no page is read twice
 
   const Fp4AttnArgs& a;
   const Fp4Span& sp;
   const Fp4Page pg;
-  int lane, col, grp;
+  int col, grp;
   const uint8_t* head;  // the K/V head's block in page 0
-  u32x4 q[MT][kWords];
+  uint32_t code_at, scale_at;  // the lane's place in 16 keys' codes and scale bytes
+  i32x8 q[MT][kSteps][DP >= 128 ? 2 : 1];  // the two parts of the query (64 dims: both in one)
+  int q_scale[MT][kSteps];                 // scale byte of k-block g: byte 0 of the first part, byte 1 of the second
   int hi[MT], lo[MT];   // the positions that row 16 mt + col sees
   float m[MT], l[MT];
   f32x4 acc[MT][kBlocks];
 
-  __device__ __forceinline__ Fp4Wave(const Fp4AttnArgs& a_, const Fp4Span& sp_, int b, int hk, int r0)
+  __device__ __forceinline__ Fp4Wave(const Fp4AttnArgs& a_, const Fp4Span& sp_, int b, int hk, int r0, int lane)
       : a(a_), sp(sp_), pg(fp4_page(a_.bs, a_.Hkv, kExact ? DP : a_.D)) {
-    lane = threadIdx.x % kWave;
     col = lane & 15;
     grp = lane >> 4;
     head = a.pool + hk * pg.head;
+    const int nb = dims() / kFp4Block;
+    code_at = col * (dims() / 2) + grp * (DP / 8);
+    scale_at = col * 2 * nb + grp * kScales;
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
       const int r = r0 + 16 * mt + col;
@@ -161,17 +201,77 @@ struct Fp4Wave {
       lo[mt] = a.window > 0 ? hi[mt] - a.window : 0;
       const uint8_t* row = a.q + b * a.q_seq + t * a.q_tok + (hk * a.G + g) * a.q_head;
 #pragma unroll
-      for (int w = 0; w < kWords; ++w) {
-        const int d = grp * (DP / 4) + 8 * w;
-        q[mt][w] = u32x4{0u, 0u, 0u, 0u};
-        if (in && (kExact || d < a.D)) q[mt][w] = *reinterpret_cast<const u32x4*>(row + 2 * d);
-      }
-      m[mt] = -__builtin_huge_valf();
+      for (int s = 0; s < kSteps; ++s) load_query(mt, s, row, in);
+      m[mt] = kF4None;
       l[mt] = 0.f;
 #pragma unroll
       for (int x = 0; x < kBlocks; ++x) acc[mt][x] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
   }
+
+  // 16 dims of a query row from `d` on as e4m3 parts: words of the first and the
+  // second part, and the scale byte of the 32 dims that this lane and the one 16 away
+  // hold the halves of.
+  __device__ __forceinline__ uint32_t split16(const uint8_t* row, int d, bool in, uint32_t* hi, uint32_t* lo) const {
+    uint32_t x[8];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const bool live = in && (kExact || d + 8 * i < a.D);
+      const u32x4 v = *reinterpret_cast<const u32x4*>(live ? row + 2 * (d + 8 * i) : a.q);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) x[4 * i + j] = live ? v[j] : 0u;
+    }
+    uint32_t big = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) big = max(big, max((x[j] << 16) & 0x7fffffffu, x[j] & 0x7fff0000u));
+    big = max(big, static_cast<uint32_t>(__shfl_xor(static_cast<int>(big), 16)));
+    const int byte = max(static_cast<int>(big >> 23) - 7, 6);  // the largest lands in [2^7, 2^8)
+    const float f = __uint_as_float(static_cast<uint32_t>(254 - byte) << 23);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float v[4] = {__uint_as_float(x[2 * j] << 16) * f, __uint_as_float(x[2 * j] & 0xffff0000u) * f,
+                          __uint_as_float(x[2 * j + 1] << 16) * f, __uint_as_float(x[2 * j + 1] & 0xffff0000u) * f};
+      hi[j] = e4m3fn_pack2<true>(v[2], v[3], e4m3fn_pack2<false>(v[0], v[1], 0u));
+      float h[4];
+      e4m3fn_x4_to_f32(hi[j], h);
+      lo[j] = e4m3fn_pack2<true>((v[2] - h[2]) * 32.f, (v[3] - h[3]) * 32.f,
+                                 e4m3fn_pack2<false>((v[0] - h[0]) * 32.f, (v[1] - h[1]) * 32.f, 0u));
+    }
+    return static_cast<uint32_t>(byte);
+  }
+
+  // The query of row 16 mt + col for step s.  The second operand's lane g holds
+  // k = 16 g .. + 15 and 64 + 16 g .. + 15 of the 128, and the scale of k-block g (k = 32 g ..);
+  // k-block j is dims 32 (j kScales + s) .. as the keys' lanes have them.
+  __device__ __forceinline__ void load_query(int mt, int s, const uint8_t* row, bool in) {
+    const int half = 16 * (grp & 1);
+    uint32_t hi[8], lo[8];
+    if constexpr (DP >= 128) {
+      const uint32_t b0 = split16(row, 32 * ((grp >> 1) * kScales + s) + half, in, hi, lo);
+      const uint32_t b1 = split16(row, 32 * ((2 + (grp >> 1)) * kScales + s) + half, in, hi + 4, lo + 4);
+      const int from = col + 32 * (grp & 1);  // k-blocks 0, 1 (2, 3) are the first (second) 16 of lanes 0 and 32
+      const int a0 = __shfl(static_cast<int>(b0), from), a1 = __shfl(static_cast<int>(b1), from);
+      const int own = grp < 2 ? a0 : a1;
+      q_scale[mt][s] = own | (own - 5) << 8;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        q[mt][s][0][i] = static_cast<int>(hi[i]);
+        q[mt][s][DP >= 128 ? 1 : 0][i] = static_cast<int>(lo[i]);
+      }
+    } else {
+      // k-blocks 0, 1: the first part of dims 0 .. 63; 2, 3: the second part of the same
+      const uint32_t b = split16(row, 16 * grp, in, hi, lo);
+      const int own = __shfl(static_cast<int>(b), col + 32 * (grp & 1));
+      q_scale[mt][s] = grp < 2 ? own : own - 5;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        q[mt][s][0][i] = static_cast<int>(hi[i]);
+        q[mt][s][0][i + 4] = static_cast<int>(lo[i]);
+      }
+    }
+  }
+
+  __device__ __forceinline__ int dims() const { return kExact ? DP : a.D; }
 
   // page id (-1: not mapped) and first slot of the 16 positions from `pos` on
   __device__ __forceinline__ void lookup(int b, int pos, int& page, int& slot) const {
@@ -181,71 +281,164 @@ struct Fp4Wave {
     if (page >= a.n_pages) page = -1;
   }
 
-  __device__ __forceinline__ void load(Raw& r, int half, int page, int slot) const {
-    r.mapped[half] = page >= 0;
-    const uint8_t* base = head + (page >= 0 ? page : 0) * pg.page;  // uniform
-    const int D = kExact ? DP : a.D;
-    const int nb = D / kFp4Block;
-    const int row = (slot + col) * (D / 2) + grp * (DP / 8);
-    const int sc = pg.scales + 2 * (slot + col) * nb;
-    if constexpr (kExact && DP >= 128) {
-#pragma unroll
-      for (int w = 0; w < kWords; w += 4) {
-        const u32x4 x = *reinterpret_cast<const u32x4*>(base + row + 4 * w);
-        const u32x4 y = *reinterpret_cast<const u32x4*>(base + pg.v_codes + row + 4 * w);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          r.k[half][w + i] = x[i];
-          r.v[half][w + i] = y[i];
-        }
+  // The codes of half h of a tile, 16 keys from slot `slot` of a page (all uniform).
+  __device__ __forceinline__ void load_codes(Raw& r, int h, int page, int slot) const {
+    r.page[h] = page;
+    // scalar bases, and a lane's offset that the loads add themselves
+    const uint8_t* kc = head + max(page, 0) * pg.page + slot * (dims() / 2);
+    const uint8_t* vc = kc + pg.v_codes;
+    uint32_t lane_at = code_at;
+    asm("" : "+v"(lane_at));
+    constexpr int kRun = DP >= 128 ? 4 : 2;  // words of one load
+    typedef uint32_t run_t __attribute__((ext_vector_type(kRun)));
+    const auto get = [&](auto* p) {
+      if constexpr (kOnce) {
+        return __builtin_nontemporal_load(p);
+      } else {
+        return *p;
       }
-    } else {
+    };
+    if constexpr (DP == 64) {  // lanes g and g + 2: block g of the key
+      const bool in = kExact || 32 * (grp & 1) < a.D;
+      uint32_t key_at = col * (dims() / 2) + 16 * (grp & 1);
+      asm("" : "+v"(key_at));
+      const u32x4 x = get(reinterpret_cast<const u32x4*>(kc + (in ? key_at : 0u)));
 #pragma unroll
-      for (int w = 0; w < kWords; w += 2) {
-        const bool in = kExact || grp * (DP / 4) + 8 * w < D;
-        const int o = in ? row + 4 * w : 0;
-        const u32x2 x = *reinterpret_cast<const u32x2*>(base + o);
-        const u32x2 y = *reinterpret_cast<const u32x2*>(base + pg.v_codes + o);
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          r.k[half][w + i] = in ? x[i] : 0u;
-          r.v[half][w + i] = in ? y[i] : 0u;
-        }
-      }
+      for (int i = 0; i < 4; ++i) r.k[h][i] = in ? x[i] : 0u;
     }
 #pragma unroll
-    for (int i = 0; i < kScales; ++i) {
-      const int blk = DP >= 128 ? grp * kScales + i : grp >> 1;
-      const int o = kExact || blk < nb ? blk : 0;
-      r.ks[half][i] = base[sc + o];
-      r.vs[half][i] = base[sc + nb + o];
+    for (int w = 0; w < kWords; w += kRun) {
+      const bool in = kExact || grp * (DP / 4) + 8 * w < a.D;
+      const uint32_t at = in ? lane_at + 4 * w : 0u;
+      if constexpr (DP >= 128) {
+        const run_t x = get(reinterpret_cast<const run_t*>(kc + at));
+#pragma unroll
+        for (int i = 0; i < kRun; ++i) r.k[h][w + i] = in ? x[i] : 0u;
+      }
+      const run_t y = get(reinterpret_cast<const run_t*>(vc + at));
+#pragma unroll
+      for (int i = 0; i < kRun; ++i) r.v[h][w + i] = in ? y[i] : 0u;
     }
   }
 
-  // One tile: positions pos .. pos + 31.
-  __device__ __forceinline__ void tile(Raw& r, int pos, uint16_t* vt) {
-    // keys that no row sees hold stale bytes: their values become zeros (their
-    // weights are); a NaN block among the values too, and its key's scores NaN
-    const bool whole = pos >= sp.all_lo && pos + kF4Tile <= sp.all_hi && r.mapped[0] && r.mapped[1];  // uniform
+  // Both halves' scale bytes.  Heads of 64 and 128 dims: a token's (4 or 8, its
+  // key's and its value's) in one load, half h's by the lanes of odd or even g = h, which
+  // then hand them to the rest; others a lane's own.
+  __device__ __forceinline__ const uint8_t* scales_of(int page, int slot) const {
+    return head + max(page, 0) * pg.page + pg.scales + slot * 2 * (dims() / kFp4Block);
+  }
+  __device__ __forceinline__ void load_scales(Raw& r, int page0, int slot0, int page1, int slot1) const {
+    const int nb = dims() / kFp4Block;
+    if constexpr (kPacked) {
+      typedef uint32_t run_t __attribute__((ext_vector_type(kPacked ? DP / 64 : 1)));
+      const uint8_t *sc0 = scales_of(page0, slot0), *sc1 = scales_of(page1, slot1);
+      asm("" : "+s"(sc0), "+s"(sc1));  // made in scalar registers, then chosen
+      const uint8_t* sc = (grp & 1) ? sc1 : sc0;
+      const run_t x = *reinterpret_cast<const run_t*>(sc + col * (DP / 16));
+#pragma unroll
+      for (int i = 0; i < DP / 64; ++i) r.packed[i] = x[i];
+    } else {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const uint8_t* sc = scales_of(h ? page1 : page0, h ? slot1 : slot0);
+        if constexpr (kExact && kScales > 1) {
+          typedef uint8_t run_t __attribute__((ext_vector_type(kScales)));
+          const run_t x = *reinterpret_cast<const run_t*>(sc + scale_at), y = *reinterpret_cast<const run_t*>(sc + nb + scale_at);
+#pragma unroll
+          for (int i = 0; i < kScales; ++i) {
+            r.ks[h][i] = x[i];
+            r.vs[h][i] = y[i];
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < kScales; ++i) {
+            const int kb = DP >= 128 ? grp * kScales + i : grp & 1, vb = DP >= 128 ? kb : grp >> 1;
+            const uint32_t ks = sc[col * 2 * nb + (kb < nb ? kb : 0)], vs = sc[col * 2 * nb + nb + (vb < nb ? vb : 0)];
+            r.ks[h][i] = kb < nb ? ks : 127u;
+            r.vs[h][i] = vb < nb ? vs : 127u;
+          }
+        }
+      }
+    }
+  }
+  __device__ __forceinline__ void unpack_scales(Raw& r) const {
+    if constexpr (kPacked) {
+      // 64 dims: a word K0 K1 V0 V1; 128: a word of K's, one of V's, g's block g
+#pragma unroll
+      for (int i = 0; i < DP / 64; ++i) {
+        const auto x = __builtin_amdgcn_permlane16_swap(r.packed[i], r.packed[i], false, false);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          if constexpr (DP == 64) {  // g's key block is g % 2, its values' block g / 2
+            r.ks[h][0] = x[h] >> (8 * (grp & 1));
+            r.vs[h][0] = (x[h] >> (16 + 8 * (grp >> 1))) & 0xff;
+          } else if (i == 0) {
+            r.ks[h][0] = x[h] >> (8 * grp);  // the products take byte 0
+          } else {
+            r.vs[h][0] = (x[h] >> (8 * grp)) & 0xff;
+          }
+        }
+      }
+    }
+  }
+
+  // Where not every row sees every key, or a value's block is NaN: the values of
+  // keys that no row sees (stale bytes, whose weights are zero) and of NaN blocks
+  // become zeros.  Returns the keys with a NaN block, whose scores will be NaN.
+  __device__ __forceinline__ uint32_t clean(Raw& r, int pos) const {
     uint32_t nan_keys = 0;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       bool nan = false;
 #pragma unroll
       for (int i = 0; i < kScales; ++i) nan |= r.vs[h][i] == kFp4NaN;
-      if constexpr (!kExact) nan &= grp * (DP / 4) < a.D;
-      bool dead = nan;
-      if (!whole) dead |= pos + 16 * h + col >= sp.last || pos + 16 * h + col < sp.first || !r.mapped[h];
-      if (__ballot(dead)) {
-        const uint64_t n = __ballot(nan);
-        nan_keys |= static_cast<uint32_t>((n | n >> 16 | n >> 32 | n >> 48) & 0xffff) << (16 * h);
-        if (dead) {
+      const int at = pos + 16 * h + col;
+      if (nan || at >= sp.last || at < sp.first || r.page[h] < 0) {
 #pragma unroll
-          for (int w = 0; w < kWords; ++w) r.v[h][w] = 0u;
+        for (int w = 0; w < kWords; ++w) r.v[h][w] = 0u;
 #pragma unroll
-          for (int i = 0; i < kScales; ++i) r.vs[h][i] = 127;
+        for (int i = 0; i < kScales; ++i) r.vs[h][i] = 127u;
+      }
+      const uint64_t n = __ballot(nan);
+      nan_keys |= static_cast<uint32_t>((n | n >> 16 | n >> 32 | n >> 48) & 0xffff) << (16 * h);
+    }
+    return nan_keys;
+  }
+
+  // One tile, positions pos .. pos + 31: its values to LDS and its scores.
+  __device__ __forceinline__ Fp4Tile<MT> scores(Raw& r, int pos, uint16_t* vt) const {
+    unpack_scales(r);
+    Fp4Tile<MT> tl;
+    bool nan = false;
+#pragma unroll
+    for (int i = 0; i < kScales; ++i) nan |= r.vs[0][i] == kFp4NaN || r.vs[1][i] == kFp4NaN;
+    tl.page[0] = r.page[0];
+    tl.page[1] = r.page[1];
+    tl.masked = pos < sp.all_lo || pos + kF4Tile > sp.all_hi || (r.page[0] | r.page[1]) < 0 || __ballot(nan) != 0;
+    tl.nan_keys = 0;
+    if (tl.masked) tl.nan_keys = clean(r, pos);  // uniform
+    auto& st = tl.st;
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) st[mt][0] = st[mt][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        i32x8 k = {0, 0, 0, 0, 0, 0, 0, 0};  // of e2m1 operands the first half counts
+#pragma unroll
+        for (int i = 0; i < 4; ++i) k[i] = static_cast<int>(r.k[h][4 * s + i]);
+        const int ks = static_cast<int>(r.ks[h][s]);
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+          st[mt][h] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(k, q[mt][s][0], st[mt][h], 4, 0, 0, ks, 0, q_scale[mt][s]);
+          if constexpr (DP >= 128) {
+            st[mt][h] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(k, q[mt][s][1], st[mt][h], 4, 0, 0, ks, 1, q_scale[mt][s]);
+          }
         }
       }
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
       uint16_t* dst = vt + (16 * h + col) * DP;
 #pragma unroll
       for (int w = 0; w < kWords; ++w) {
@@ -253,65 +446,71 @@ struct Fp4Wave {
             fp4_decode8(r.v[h][w], fp4_scale(r.vs[h][w / 4 < kScales ? w / 4 : 0]));
       }
     }
-    f32x4 st[MT][2];
-#pragma unroll
-    for (int mt = 0; mt < MT; ++mt) st[mt][0] = st[mt][1] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int w = 0; w < kWords; ++w) {
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const u32x4 k = fp4_decode8(r.k[h][w], fp4_scale(r.ks[h][w / 4 < kScales ? w / 4 : 0]));
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
-          st[mt][h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fp4_bf16x8(k), fp4_bf16x8(q[mt][w]), st[mt][h], 0, 0, 0);
-        }
-      }
-    }
+    return tl;
+  }
+
+  // The tile's weights, and its values times them onto the output.
+  __device__ __forceinline__ void output(Fp4Tile<MT>& tl, int pos, const uint16_t* vt) {
+    auto& st = tl.st;
     const bool capped = a.softcap > 0.f;
-    const float mult = capped ? 1.f : a.scale * kF4Log2e;
-    u32x4 p[MT];
+    const float mult = capped ? 2.f * kF4Log2e * a.scale / a.softcap : a.scale * kF4Log2e;
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
-      // scores of positions pos + 16 h + 4 grp + i for row 16 mt + col
-      if (capped) {
-        const float to = 2.f * kF4Log2e * a.scale / a.softcap, cap = a.softcap * kF4Log2e;
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
+      for (int h = 0; h < 2; ++h) st[mt][h] *= mult;  // to the log2 domain, or what the cap's tanh takes
+    }
+    if (capped || tl.masked) {  // uniform
+      const float cap = a.softcap * kF4Log2e;
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {  // tanh(x) = 1 - 2 / (exp(2x) + 1)
-            st[mt][h][i] = cap * (1.f - 2.f * __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(st[mt][h][i] * to) + 1.f));
-          }
-        }
-      }
-      if (!whole || nan_keys) {
+      for (int mt = 0; mt < MT; ++mt) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const int key = 16 * h + 4 * grp + i;
-            float v = (nan_keys >> key) & 1 ? __builtin_nanf("") : st[mt][h][i];
-            const bool seen = pos + key < hi[mt] && pos + key >= lo[mt] && r.mapped[h];
-            st[mt][h][i] = seen ? v : -__builtin_huge_valf();
+            float v = st[mt][h][i];
+            // tanh(x) = 1 - 2 / (exp(2x) + 1)
+            if (capped) v = cap * (1.f - 2.f * __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(v) + 1.f));
+            if (tl.masked) {
+              if ((tl.nan_keys >> key) & 1) v = __builtin_nanf("");
+              const bool seen = pos + key < hi[mt] && pos + key >= lo[mt] && tl.page[h] >= 0;
+              v = seen ? v : -__builtin_huge_valf();
+            }
+            st[mt][h][i] = v;
           }
         }
       }
-      float mx = fmaxf(fmaxf(fmaxf(st[mt][0][0], st[mt][0][1]), fmaxf(st[mt][0][2], st[mt][0][3])),
-                       fmaxf(fmaxf(st[mt][1][0], st[mt][1][1]), fmaxf(st[mt][1][2], st[mt][1][3])));
-      mx = fp4_max_groups(mx) * mult;
-      const bool move = mx > m[mt] + kF4Move;
-      if (__ballot(move)) {
-        const float alpha = move ? __builtin_amdgcn_exp2f(m[mt] - mx) : 1.f;
-        if (move) m[mt] = mx;
+    }
+    // the reference maximum is one for the four lanes of a row, and so is "no score of
+    // mine passes it by kF4Move": the row's own maximum is needed where one does
+    float mx[MT];
+    bool any = false;
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+      const f32x4 x = st[mt][0], y = st[mt][1];
+      mx[mt] = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3])));
+      any |= mx[mt] > m[mt] + kF4Move;
+    }
+    if (__ballot(any)) {
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) {
+        const float top = fp4_max_groups(mx[mt]);
+        const bool move = top > m[mt] + kF4Move;
+        const float alpha = move ? __builtin_amdgcn_exp2f(m[mt] - top) : 1.f;
+        if (move) m[mt] = top;
         l[mt] *= alpha;
 #pragma unroll
         for (int x = 0; x < kBlocks; ++x) acc[mt][x] *= alpha;
       }
-      const float ref = m[mt] == -__builtin_huge_valf() ? 0.f : m[mt];
+    }
+    u32x4 p[MT];
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
       float e[8];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) e[4 * h + i] = __builtin_amdgcn_exp2f(fmaf(st[mt][h][i], mult, -ref));
+        for (int i = 0; i < 4; ++i) e[4 * h + i] = __builtin_amdgcn_exp2f(st[mt][h][i] - m[mt]);
       }
       l[mt] += ((e[0] + e[1]) + (e[2] + e[3])) + ((e[4] + e[5]) + (e[6] + e[7]));
 #pragma unroll
@@ -333,163 +532,272 @@ struct Fp4Wave {
   }
 };
 
+// The thread's index, worked out where it is asked for: what is derived from it for
+// the end of a segment would otherwise be made ahead of the tiles and held through them.
+__device__ __forceinline__ int fp4_fresh_tid() {
+  int t = threadIdx.x;
+  asm volatile("" : "+v"(t));
+  return t;
+}
+
+// A segment: tiles [t_from, t_to) of an item; its rows' outputs, or where the
+// segment is a piece of the item, slot `slot` of the partial ones.
 template <int DP, int MT, bool kExact>
-__global__ __launch_bounds__(kF4Threads) void k_fp4_attn(Fp4AttnArgs a) {
+__device__ __forceinline__ void fp4_segment(Fp4Smem<DP>& sm, const Fp4AttnArgs& a, int b, int rb, int hk, const Fp4Span& sp,
+                                            int t_from, int t_to, int slot_of_part) {
   using Wave = Fp4Wave<DP, MT, kExact>;
-  __shared__ Fp4Smem<DP> sm;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x) / kWave, lane = threadIdx.x % kWave;
-  // block -> (chunk unit, row block): a unit's row blocks, which read the same
-  // pages, follow one another on one XCD (block i runs on XCD i % 8)
-  const int n_units = a.B * a.Hkv * a.chunks;
-  const int turn = blockIdx.x >> 3, in_turn = turn % a.row_blocks;
-  const int unit = (turn / a.row_blocks) * 8 + (blockIdx.x & 7);
-  if (unit >= n_units) return;  // uniform
-  const int rb = a.row_blocks - 1 - in_turn;
-  const int chunk = unit % a.chunks, bh = unit / a.chunks;
-  const int b = bh / a.Hkv, hk = bh - b * a.Hkv;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x) / kWave, lane = fp4_fresh_tid() % kWave;
   const int r0 = rb * 16 * MT;
-  const Fp4Span sp = fp4_span(a, b, r0, 16 * MT);
-  const int n_chunks = fp4_chunks(a, sp);
-  if (chunk >= max(n_chunks, 1)) return;  // uniform
-  const int t_lo = sp.tile0 + chunk * a.chunk_tiles;
-  const int t_hi = chunk == a.chunks - 1 ? sp.tile0 + sp.tiles : min(t_lo + a.chunk_tiles, sp.tile0 + sp.tiles);
-  Wave w(a, sp, b, hk, r0);
+  const int t_lo = sp.tile0 + t_from, t_hi = sp.tile0 + min(t_to, sp.tiles);
+  Wave w(a, sp, b, hk, r0, lane);
   uint16_t* vt = reinterpret_cast<uint16_t*>(sm.tile[wave]);
   // this wave's tiles t_lo + wave, + 4, ...; the page ids of 32 of them at a time
-  typename Wave::Raw raw;
   int page = -1, slot = 0;
   const int n = t_hi > t_lo + wave ? (t_hi - t_lo - wave + kF4Waves - 1) / kF4Waves : 0;
-  const auto ids = [&](int i) {  // lane 2 j + h: half h of tile i + j
-    const int t = t_lo + wave + (i + (lane >> 1)) * kF4Waves;
-    w.lookup(b, min(t, t_hi) * kF4Tile + 16 * (lane & 1), page, slot);
-  };
-  const auto fetch = [&](int i) {
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int at = 2 * (i & 31) + h;
-      w.load(raw, h, __builtin_amdgcn_readlane(page, at), __builtin_amdgcn_readlane(slot, at));
+  const auto fetch = [&](typename Wave::Raw& raw, int i) {
+    if (i >= n) return;  // uniform
+    if ((i & 31) == 0) {   // lane 2 j + h: half h of tile i + j
+      const int t = t_lo + wave + (i + (lane >> 1)) * kF4Waves;
+      w.lookup(b, min(t, t_hi) * kF4Tile + 16 * (lane & 1), page, slot);
     }
+    const int at = 2 * (i & 31);
+    const int p0 = __builtin_amdgcn_readlane(page, at), p1 = __builtin_amdgcn_readlane(page, at + 1);
+    const int s0 = __builtin_amdgcn_readlane(slot, at), s1 = __builtin_amdgcn_readlane(slot, at + 1);
+    w.load_scales(raw, p0, s0, p1, s1);
+    w.load_codes(raw, 0, p0, s0);
+    w.load_codes(raw, 1, p1, s1);
   };
-  if (n > 0) {
-    ids(0);
-    fetch(0);
-  }
-  for (int i = 0; i < n; ++i) {
-    typename Wave::Raw cur = raw;
-    if (i + 1 < n) {
-      if (((i + 1) & 31) == 0) ids(i + 1);
-      fetch(i + 1);
-    }
-    w.tile(cur, (t_lo + wave + i * kF4Waves) * kF4Tile, vt);
+  // the tile's registers take the tile after the next as soon as its scores are made
+  const auto step = [&](typename Wave::Raw& raw, int i) {
+    const int pos = (t_lo + wave + i * kF4Waves) * kF4Tile;
+    auto tl = w.scores(raw, pos, vt);
+    fetch(raw, i + 2);
+    w.output(tl, pos, vt);
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  };
+  typename Wave::Raw raw0, raw1;
+  fetch(raw0, 0);
+  fetch(raw1, 1);
+  for (int i = 0; i < n; i += 2) {
+    step(raw0, i);
+    if (i + 1 < n) step(raw1, i + 1);
   }
   // join the waves: maxima and sums of every row, then the outputs, a row tile at a time
+  const int tid = fp4_fresh_tid(), col = tid & 15, grp = (tid >> 4) & 3;
 #pragma unroll
   for (int mt = 0; mt < MT; ++mt) {
     const float l = fp4_sum_groups(w.l[mt]);
-    if (w.grp == 0) {
-      sm.m[wave][16 * mt + w.col] = w.m[mt];
-      sm.l[wave][16 * mt + w.col] = l;
+    if (grp == 0) {
+      sm.m[wave][16 * mt + col] = w.m[mt];
+      sm.l[wave][16 * mt + col] = l;
     }
   }
   const float ninf = -__builtin_huge_valf();
-  const int64_t part_row = (static_cast<int64_t>(unit) * a.row_blocks + rb) * (16 * MT);
-  const int64_t part_rows = static_cast<int64_t>(n_units) * a.row_blocks * (16 * MT);
+  const bool whole = slot_of_part < 0;
+  const int D = kExact ? DP : a.D;
 #pragma unroll
   for (int mt = 0; mt < MT; ++mt) {
     __syncthreads();  // the tiles (or the last row tile's outputs) have been read, the maxima are written
     f32x4* o = reinterpret_cast<f32x4*>(sm.tile[wave]);
 #pragma unroll
-    for (int x = 0; x < Wave::kBlocks; ++x) o[w.col * (DP / 4) + ((4 * x + w.grp) ^ (w.col & 7))] = w.acc[mt][x];
+    for (int x = 0; x < Wave::kBlocks; ++x) o[col * (DP / 4) + ((4 * x + grp) ^ (col & 7))] = w.acc[mt][x];
     __syncthreads();
-    for (int i = threadIdx.x; i < 16 * (DP / 4); i += kF4Threads) {
+    for (int i = tid; i < 16 * (DP / 4); i += kF4Threads) {
       const int row = i / (DP / 4), c = i % (DP / 4), r = r0 + 16 * mt + row;
       const int d = 4 * c;
-      if (r >= sp.r_end || (!kExact && d >= a.D)) continue;
+      if (r >= sp.r_end || (!kExact && d >= D)) continue;
       const int t = r / a.G, h = hk * a.G + r - t * a.G;
-      float top = ninf;
+      float top = kF4None;
 #pragma unroll
       for (int k = 0; k < kF4Waves; ++k) top = fmaxf(top, sm.m[k][16 * mt + row]);
-      const bool one = a.chunks == 1;
-      const float sink = one && a.sink ? a.sink[h] * kF4Log2e : ninf;
-      const float ref = fmaxf(top, sink) == ninf ? 0.f : fmaxf(top, sink);
+      const float sink = whole && a.sink ? a.sink[h] * kF4Log2e : ninf;
+      const float ref = fmaxf(top, sink) == kF4None ? 0.f : fmaxf(top, sink);
       float den = 0.f;
       f32x4 v = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int k = 0; k < kF4Waves; ++k) {
         const float f = __builtin_amdgcn_exp2f(sm.m[k][16 * mt + row] - ref);
         const float lk = sm.l[k][16 * mt + row];
-        den += f == 0.f && lk == 0.f ? 0.f : f * lk;
-        if (lk != lk) den = lk;  // NaN keys alone: no maximum
+        den += lk != lk ? lk : f == 0.f ? 0.f : f * lk;  // NaN keys alone leave no maximum
         v += reinterpret_cast<const f32x4*>(sm.tile[k])[row * (DP / 4) + (c ^ (row & 7))] * f;
       }
-      if (one) {
+      if (whole) {
         if (sink != ninf) den += __builtin_amdgcn_exp2f(sink - ref);
         const float inv = den == 0.f ? 0.f : 1.f / den;
         u32x2 y;
         y[0] = bf16_pack2(v[0] * inv, v[1] * inv);
         y[1] = bf16_pack2(v[2] * inv, v[3] * inv);
-        *reinterpret_cast<u32x2*>(a.out + ((static_cast<int64_t>(b) * a.T + t) * a.H + h) * (kExact ? DP : a.D) + d) = y;
+        *reinterpret_cast<u32x2*>(a.out + ((static_cast<int64_t>(b) * a.T + t) * a.H + h) * D + d) = y;
       } else {
-        const int64_t pr = part_row + 16 * mt + row;
+        const int64_t pr = static_cast<int64_t>(slot_of_part) * (16 * MT) + 16 * mt + row;
+        float* part = a.part + pr * (D + 4);
         if (c == 0) {
-          a.part[2 * pr] = top;
-          a.part[2 * pr + 1] = den;
+          part[0] = top;
+          part[1] = den;
         }
-        reinterpret_cast<f32x4*>(a.part + 2 * part_rows)[pr * ((kExact ? DP : a.D) / 4) + c] = v;
+        reinterpret_cast<f32x4*>(part + 4)[c] = v;
       }
     }
   }
 }
 
-// Joins the chunks of every row: one wave per row, four rows a workgroup.
-__global__ __launch_bounds__(kF4Threads) void k_fp4_attn_join(Fp4AttnArgs a, int rows_per_block) {
-  const int lane = threadIdx.x % kWave;
-  const int64_t item = static_cast<int64_t>(blockIdx.x) * kF4Waves + threadIdx.x / kWave;
-  const int R = a.T * a.G;
-  const int bh = static_cast<int>(item / R), r = static_cast<int>(item - static_cast<int64_t>(bh) * R);
-  if (bh >= a.B * a.Hkv) return;
-  const int b = bh / a.Hkv, hk = bh - b * a.Hkv;
-  const int t = r / a.G, h = hk * a.G + r - t * a.G;
-  const int rb = r / rows_per_block;
-  const Fp4Span sp = fp4_span(a, b, rb * rows_per_block, rows_per_block);
-  const int n = fp4_chunks(a, sp);
-  const int64_t part_rows = static_cast<int64_t>(a.B) * a.Hkv * a.chunks * a.row_blocks * rows_per_block;
-  const auto row_of = [&](int c) {
-    return ((static_cast<int64_t>(bh) * a.chunks + c) * a.row_blocks + rb) * rows_per_block + (r - rb * rows_per_block);
+template <int DP, int MT, bool kExact>
+__global__ __launch_bounds__(kF4Threads, DP * MT <= 256 ? 2 : 1) void k_fp4_attn(Fp4AttnArgs a) {
+  __shared__ Fp4Smem<DP> sm;
+  const int tid = threadIdx.x;
+  const int items = a.B * a.row_blocks;
+  const auto span_of = [&](int item, int& b, int& rb) {
+    b = item / a.row_blocks;
+    rb = item - b * a.row_blocks;
+    return fp4_span(a, b, rb * 16 * MT, 16 * MT);
   };
-  const float ninf = -__builtin_huge_valf();
-  float top = ninf;
-  for (int c = lane; c < n; c += kWave) top = fmaxf(top, a.part[2 * row_of(c)]);
-  for (int off = 32; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor(top, off));
-  const float sink = a.sink ? a.sink[h] * kF4Log2e : ninf;
-  const float ref = fmaxf(top, sink) == ninf ? 0.f : fmaxf(top, sink);
-  float den = 0.f;
-  for (int c = lane; c < n; c += kWave) {
-    const float f = __builtin_amdgcn_exp2f(a.part[2 * row_of(c)] - ref), l = a.part[2 * row_of(c) + 1];
-    den += l != l ? l : f == 0.f ? 0.f : f * l;
-  }
-  for (int off = 32; off > 0; off >>= 1) den += __shfl_xor(den, off);
-  if (sink != ninf) den += __builtin_amdgcn_exp2f(sink - ref);
-  const float inv = den == 0.f ? 0.f : 1.f / den;
-  const f32x4* o = reinterpret_cast<const f32x4*>(a.part + 2 * part_rows);
-  for (int d = lane; d < a.D / 4; d += kWave) {
-    f32x4 v = f32x4{0.f, 0.f, 0.f, 0.f};
-    for (int c = 0; c < n; ++c) {
-      const int64_t pr = row_of(c);
-      v += o[pr * (a.D / 4) + d] * __builtin_amdgcn_exp2f(a.part[2 * pr] - ref);
+  // values worked out in LDS are the same in every lane: scalar registers hold them
+  const auto uniform = [](int v) { return __builtin_amdgcn_readfirstlane(v); };
+  const bool each = a.max_groups == 0;  // more items than LDS holds: none is cut, a workgroup each
+  const int g = blockIdx.x;
+  int x = g, end = g + 1, total = 0, b, rb;
+  const auto item_of = [&](int u) {  // u < total: pre[item] <= u < pre[item + 1]
+    int lo = 0, hi = items;
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (sm.pre[mid] <= u) lo = mid; else hi = mid;
     }
-    u32x2 y;
-    y[0] = bf16_pack2(v[0] * inv, v[1] * inv);
-    y[1] = bf16_pack2(v[2] * inv, v[3] * inv);
-    *reinterpret_cast<u32x2*>(a.out + ((static_cast<int64_t>(b) * a.T + t) * a.H + h) * a.D + 4 * d) = y;
+    return lo;
+  };
+  if (!each) {
+    for (int base = 0; base < items; base += kF4Threads) {
+      const int item = base + tid;
+      const int n = item < items ? span_of(item, b, rb).units() * a.Hkv : 0;
+      int tot;
+      const int ex = block_exclusive_scan(n, sm.scan, &tot);
+      if (item < items) sm.pre[item] = total + ex;
+      total += tot;
+    }
+    if (tid == 0) sm.pre[items] = total;
+    __syncthreads();
+    total = uniform(total);
+    if (g == 0 && a.sched) {
+      for (int i = tid; i <= items; i += kF4Threads) a.sched[i] = sm.pre[i];
+    }
+    const int groups = fp4_groups(a, total);
+    if (g >= groups) return;  // uniform
+    // a run's end inside a small item moves to the item's end
+    const auto run_start = [&](int i) {
+      const int u = fp4_run_start(i, total, groups);
+      if (u <= 0 || u >= total) return u;
+      const int item = item_of(u), n = (sm.pre[item + 1] - sm.pre[item]) / a.Hkv;
+      const int over = (u - sm.pre[item]) % n;
+      return over > 0 && n <= a.small ? u - over + n : u;
+    };
+    x = uniform(run_start(g));
+    end = uniform(run_start(g + 1));
   }
+  while (x < end) {
+    const int item = each ? x / a.Hkv : uniform(item_of(x));
+    const Fp4Span sp = span_of(item, b, rb);
+    const int n = sp.units();
+    const int in = each ? 0 : x - uniform(sm.pre[item]);
+    const int hk = each ? x - item * a.Hkv : in / n;
+    const int from = each ? 0 : in - hk * n, to = each ? n : min(n, from + end - x);
+    const int part = from == 0 && to == n ? -1 : from == 0 ? 2 * g + 1 : 2 * g;
+    fp4_segment<DP, MT, kExact>(sm, a, b, rb, hk, sp, from, to, part);
+    x += each ? 1 : to - from;
+    __syncthreads();  // the segment's LDS has been read
+  }
+}
+
+// Joins the pieces of a cut item's row: the pieces' weights, then the weighted sum
+// of their outputs with D / 4 threads to a piece, as many pieces at a time as the
+// row's kThreads threads have room for.  (256 threads a row where there are few rows,
+// a wave where there are many.)
+template <int kThreads>
+__global__ __launch_bounds__(kF4Threads) void k_fp4_attn_join(Fp4AttnArgs a, int rows_per_block, int rows_per_group) {
+  constexpr int kRows = kF4Threads / kThreads;
+  __shared__ alignas(16) f32x4 sum[kF4Threads];
+  const int items = a.B * a.row_blocks;
+  const int item = blockIdx.x / a.Hkv, hk = blockIdx.x - item * a.Hkv;
+  const int b = item / a.row_blocks, rb = item - b * a.row_blocks;
+  const int total = a.sched[items], p0 = a.sched[item], n = (a.sched[item + 1] - p0) / a.Hkv;
+  if (n <= a.small) return;  // uniform
+  const int groups = fp4_groups(a, total);
+  const int64_t x0 = p0 + static_cast<int64_t>(hk) * n;
+  const int w0 = fp4_owner(x0, total, groups), pieces = fp4_owner(x0 + n - 1, total, groups) - w0 + 1;
+  if (pieces == 1) return;  // uniform
+  const int tid = threadIdx.x % kThreads, mine = threadIdx.x / kThreads, lane = threadIdx.x % kWave;
+  const int64_t pitch = a.D + 4;
+  const int quads = a.D / 4;
+  const int lanes = min(quads, kThreads), sets = kThreads / lanes;
+  const int set = tid / lanes, d0 = tid - set * lanes;
+  const float ninf = -__builtin_huge_valf();
+  for (int r1 = 0; r1 < rows_per_group; r1 += kRows) {  // uniform
+    const int at = blockIdx.y * rows_per_group + r1 + mine, r = rb * rows_per_block + at;
+    const bool live = r1 + mine < rows_per_group && at < rows_per_block && r < a.T * a.G;
+    const int t = live ? r / a.G : 0, h = live ? hk * a.G + r - t * a.G : 0;
+    const auto piece = [&](int k) {
+      return a.part + ((k == 0 ? 2 * static_cast<int64_t>(w0) + 1 : 2 * static_cast<int64_t>(w0 + k)) * rows_per_block + (live ? at : 0)) * pitch;
+    };
+    // every wave of the row works the weights' sum out for itself
+    float top = kF4None;
+    for (int k = lane; k < pieces; k += kWave) top = fmaxf(top, piece(k)[0]);
+    for (int off = 32; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor(top, off));
+    const float sink = a.sink ? a.sink[h] * kF4Log2e : ninf;
+    const float ref = fmaxf(top, sink) == kF4None ? 0.f : fmaxf(top, sink);
+    float den = 0.f;
+    for (int k = lane; k < pieces; k += kWave) {
+      const float f = __builtin_amdgcn_exp2f(piece(k)[0] - ref), l = piece(k)[1];
+      den += l != l ? l : f == 0.f ? 0.f : f * l;
+    }
+    for (int off = 32; off > 0; off >>= 1) den += __shfl_xor(den, off);
+    if (sink != ninf) den += __builtin_amdgcn_exp2f(sink - ref);
+    const float inv = den == 0.f ? 0.f : 1.f / den;
+    for (int d1 = 0; d1 < quads; d1 += lanes) {  // once, but for wide heads on a wave
+      const int d = d1 + d0;
+      f32x4 v = f32x4{0.f, 0.f, 0.f, 0.f};
+      if (set < sets && d < quads) {
+        constexpr int kAhead = 4;
+        for (int k0 = set; k0 < pieces; k0 += kAhead * sets) {
+          f32x4 x[kAhead];
+          float m[kAhead];
+#pragma unroll
+          for (int k = 0; k < kAhead; ++k) {
+            const float* p = piece(min(k0 + k * sets, pieces - 1));
+            m[k] = p[0];
+            x[k] = reinterpret_cast<const f32x4*>(p + 4)[d];
+          }
+#pragma unroll
+          for (int k = 0; k < kAhead; ++k) {
+            if (k0 + k * sets < pieces) v += x[k] * __builtin_amdgcn_exp2f(m[k] - ref);
+          }
+        }
+      }
+      __syncthreads();
+      sum[threadIdx.x] = v;
+      __syncthreads();
+      if (live && set == 0 && d < quads) {
+        for (int k = 1; k < min(sets, pieces); ++k) v += sum[mine * kThreads + k * lanes + d0];
+        u32x2 y;
+        y[0] = bf16_pack2(v[0] * inv, v[1] * inv);
+        y[1] = bf16_pack2(v[2] * inv, v[3] * inv);
+        *reinterpret_cast<u32x2*>(a.out + ((static_cast<int64_t>(b) * a.T + t) * a.H + h) * a.D + 4 * d) = y;
+      }
+    }
+  }
+}
+
+// Workgroups that a CU holds at once, by the kernels' registers (four waves of at
+// most 512 / n) and LDS.
+int64_t fp4_resident(int dims, int mt) {
+  if (dims == 64) return mt == 1 ? 4 : mt == 2 ? 3 : 2;
+  if (dims == 128) return mt == 1 ? 3 : mt == 2 ? 2 : 1;
+  return dims == 256 && mt == 1 ? 2 : 1;
 }
 
 struct Fp4AttnPlan {
   int dims, mt;  // padded dims, row tiles of a workgroup
-  int64_t row_blocks, chunks, chunk_tiles;
-  int64_t ws_bytes;
+  int64_t row_blocks, items;
+  int64_t groups;  // workgroups; of cut items where `cut` allows for it
+  bool cut;
+  int64_t sched_bytes, ws_bytes;
 };
 
 int fp4_attn_plan(const skv_fp4_attention_desc* d, Fp4AttnPlan& p) {
@@ -511,38 +819,35 @@ int fp4_attn_plan(const skv_fp4_attention_desc* d, Fp4AttnPlan& p) {
   }
   const int64_t D = d->cache.head_dim, rows = d->n_queries * (d->n_heads / hkv);
   p.dims = D <= 64 ? 64 : D <= 128 ? 128 : D <= 256 ? 256 : 512;
-  const int most = p.dims <= 128 ? 4 : p.dims == 256 ? 2 : 1;
-  p.mt = std::min(most, rows <= 16 ? 1 : rows <= 32 ? 2 : 4);
+  const int most = p.dims <= 256 ? 2 : 1;
+  p.mt = std::min(most, rows <= 16 ? 1 : 2);
   p.row_blocks = ceil_div(rows, 16 * p.mt);
-  // positions that a row block may see, in tiles (two may be cut at the ends)
+  p.items = d->cache.batch * p.row_blocks;
+  // the most tiles that a row block may see
   const int64_t capacity = d->cache.bt_stride * d->cache.block_size;
   int64_t len = d->max_len > 0 ? std::min(d->max_len, capacity) : capacity;
   if (d->window > 0) len = std::min(len, d->window + ceil_div(16 * p.mt, d->n_heads / hkv));
-  const int64_t tiles = ceil_div(len, kF4Tile) + 1;
-  const int64_t blocks = std::max<int64_t>(1, d->cache.batch * hkv * p.row_blocks);
-  int64_t chunks = d->splits;
-  if (chunks == 0) {
-    chunks = std::max<int64_t>(1, ceil_div(16 * device_cus(), blocks));
-    chunks = std::min(chunks, ceil_div(tiles, 2 * kF4Waves));
+  const int64_t tiles = ceil_div(len, kF4Tile) + 1, units = std::max<int64_t>(p.items * hkv, 1);
+  p.cut = tiles > kF4SmallTiles || d->splits > 0;
+  p.groups = fp4_resident(p.dims, p.mt) * device_cus();
+  if (d->splits > 0) p.groups = d->splits * units;
+  if (p.items > kF4MaxItems || units > INT32_MAX / (ceil_div(capacity, kF4Tile) + 1)) {
+    p.cut = false;
+    p.groups = 0;
   }
-  chunks = std::min<int64_t>(std::min(chunks, tiles), 1024);
-  p.chunk_tiles = ceil_div(tiles, chunks);
-  p.chunks = ceil_div(tiles, p.chunk_tiles);
-  if (blocks * p.chunks >= (1 << 28)) return set_error(SKV_EINVAL, "%s: too many workgroups", what);
-  p.ws_bytes = p.chunks > 1 ? blocks * p.chunks * 16 * p.mt * (D + 2) * 4 : 0;
+  if (units >= (1 << 24) || p.groups >= (1 << 24)) return set_error(SKV_EINVAL, "%s: too many workgroups", what);
+  p.sched_bytes = p.cut ? ceil_div((p.items + 1) * 4, 16) * 16 : 0;
+  p.ws_bytes = p.cut ? p.sched_bytes + 2 * p.groups * 16 * p.mt * (D + 4) * 4 : 0;
   return SKV_OK;
 }
 
 // The part launch for padded dims DP and mt row tiles (at most those that plan gives).
 template <int DP, bool kExact>
 void launch_rows(const Fp4AttnArgs& a, int mt, hipStream_t s) {
-  const dim3 grid(static_cast<unsigned>(ceil_div(static_cast<int64_t>(a.B) * a.Hkv * a.chunks, 8) * 8 * a.row_blocks));
+  const dim3 grid(static_cast<unsigned>(a.max_groups > 0 ? a.max_groups : static_cast<int64_t>(a.B) * a.row_blocks * a.Hkv));
   if (mt == 1) hipLaunchKernelGGL((k_fp4_attn<DP, 1, kExact>), grid, dim3(kF4Threads), 0, s, a);
   if constexpr (DP <= 256) {
     if (mt == 2) hipLaunchKernelGGL((k_fp4_attn<DP, 2, kExact>), grid, dim3(kF4Threads), 0, s, a);
-  }
-  if constexpr (DP <= 128) {
-    if (mt == 4) hipLaunchKernelGGL((k_fp4_attn<DP, 4, kExact>), grid, dim3(kF4Threads), 0, s, a);
   }
 }
 
@@ -592,10 +897,11 @@ extern "C" int skv_fp4_attention(const skv_fp4_attention_desc* d, void* workspac
   a.scale = d->scale > 0.f ? d->scale : 1.f / sqrtf(static_cast<float>(a.D));
   a.softcap = d->softcap;
   a.B = static_cast<int32_t>(d->cache.batch);
-  a.part = static_cast<float*>(workspace);
+  a.sched = p.cut ? static_cast<int32_t*>(workspace) : nullptr;
+  a.part = p.cut ? reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + p.sched_bytes) : nullptr;
   a.row_blocks = static_cast<int32_t>(p.row_blocks);
-  a.chunks = static_cast<int32_t>(p.chunks);
-  a.chunk_tiles = static_cast<int32_t>(p.chunk_tiles);
+  a.max_groups = static_cast<int32_t>(p.groups);
+  a.small = !p.cut ? INT32_MAX : d->splits > 0 ? 0 : kF4SmallTiles;
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (a.D != p.dims) {
     if (p.dims == 64) launch_rows<64, false>(a, p.mt, s);
@@ -609,9 +915,15 @@ extern "C" int skv_fp4_attention(const skv_fp4_attention_desc* d, void* workspac
     if (p.dims == 512) launch_rows<512, true>(a, p.mt, s);
   }
   if (const int rc = check_launch(what)) return rc;
-  if (p.chunks == 1) return SKV_OK;
-  const int64_t rows = static_cast<int64_t>(a.B) * a.Hkv * a.T * a.G;
-  hipLaunchKernelGGL(k_fp4_attn_join, dim3(static_cast<unsigned>(ceil_div(rows, kF4Waves))), dim3(kF4Threads), 0, s, a,
-                     16 * p.mt);
+  if (!p.cut) return SKV_OK;
+  // about 2,048 workgroups, a row each where there are fewer rows
+  const int64_t units = p.items * a.Hkv, block_rows = std::min<int64_t>(16 * p.mt, static_cast<int64_t>(a.T) * a.G);
+  const int64_t per = std::min(block_rows, ceil_div(units * block_rows, 2048));
+  const dim3 grid(static_cast<unsigned>(units), static_cast<unsigned>(ceil_div(block_rows, per)));
+  if (per == 1) {
+    hipLaunchKernelGGL((k_fp4_attn_join<kF4Threads>), grid, dim3(kF4Threads), 0, s, a, 16 * p.mt, static_cast<int>(per));
+  } else {
+    hipLaunchKernelGGL((k_fp4_attn_join<kWave>), grid, dim3(kF4Threads), 0, s, a, 16 * p.mt, static_cast<int>(per));
+  }
   return check_launch(what);
 }
