@@ -48,6 +48,12 @@ constexpr float kF4Log2e = 1.4426950408889634f;
 constexpr float kF4Move = 8.f;     // log2: the reference maximum moves when a tile's passes it by more
 constexpr float kF4None = -3e38f;  // the reference maximum before the first key: exp2(-inf - kF4None) is 0, not NaN
 
+// Workgroups that a CU holds at once: their four waves share its 4 x 512 registers
+// a lane.
+constexpr int fp4_resident(int dims, int mt) {
+  return dims == 64 ? (mt == 1 ? 4 : 3) : dims == 128 ? (mt == 1 ? 3 : 2) : dims == 256 && mt == 1 ? 2 : 1;
+}
+
 struct Fp4AttnArgs {
   const uint8_t* q;
   int64_t q_seq, q_tok, q_head;
@@ -331,10 +337,9 @@ struct Fp4Wave {
     const int nb = dims() / kFp4Block;
     if constexpr (kPacked) {
       typedef uint32_t run_t __attribute__((ext_vector_type(kPacked ? DP / 64 : 1)));
-      const uint8_t *sc0 = scales_of(page0, slot0), *sc1 = scales_of(page1, slot1);
+      uintptr_t sc0 = reinterpret_cast<uintptr_t>(scales_of(page0, slot0)), sc1 = reinterpret_cast<uintptr_t>(scales_of(page1, slot1));
       asm("" : "+s"(sc0), "+s"(sc1));  // made in scalar registers, then chosen
-      const uint8_t* sc = (grp & 1) ? sc1 : sc0;
-      const run_t x = *reinterpret_cast<const run_t*>(sc + col * (DP / 16));
+      const run_t x = *global_from_bits<const run_t>(((grp & 1) ? sc1 : sc0) + col * (DP / 16));
 #pragma unroll
       for (int i = 0; i < DP / 64; ++i) r.packed[i] = x[i];
     } else {
@@ -555,14 +560,20 @@ __device__ __forceinline__ void fp4_segment(Fp4Smem<DP>& sm, const Fp4AttnArgs& 
   int page = -1, slot = 0;
   const int n = t_hi > t_lo + wave ? (t_hi - t_lo - wave + kF4Waves - 1) / kF4Waves : 0;
   const auto fetch = [&](typename Wave::Raw& raw, int i) {
-    if (i >= n) return;  // uniform
-    if ((i & 31) == 0) {   // lane 2 j + h: half h of tile i + j
+    // past the last tile page 0 is read, so that the loads in flight are the same
+    // number whatever the path: a wait for a tile's then leaves the next one's alone
+    const bool in = i < n;  // uniform
+    if ((i & 31) == 0 && in) {   // lane 2 j + h: half h of tile i + j
       const int t = t_lo + wave + (i + (lane >> 1)) * kF4Waves;
       w.lookup(b, min(t, t_hi) * kF4Tile + 16 * (lane & 1), page, slot);
     }
     const int at = 2 * (i & 31);
-    const int p0 = __builtin_amdgcn_readlane(page, at), p1 = __builtin_amdgcn_readlane(page, at + 1);
-    const int s0 = __builtin_amdgcn_readlane(slot, at), s1 = __builtin_amdgcn_readlane(slot, at + 1);
+    int p0 = __builtin_amdgcn_readlane(page, at), p1 = __builtin_amdgcn_readlane(page, at + 1);
+    int s0 = __builtin_amdgcn_readlane(slot, at), s1 = __builtin_amdgcn_readlane(slot, at + 1);
+    p0 = in ? p0 : -1;
+    p1 = in ? p1 : -1;
+    s0 = in ? s0 : 0;
+    s1 = in ? s1 : 0;
     w.load_scales(raw, p0, s0, p1, s1);
     w.load_codes(raw, 0, p0, s0);
     w.load_codes(raw, 1, p1, s1);
@@ -578,10 +589,12 @@ __device__ __forceinline__ void fp4_segment(Fp4Smem<DP>& sm, const Fp4AttnArgs& 
   typename Wave::Raw raw0, raw1;
   fetch(raw0, 0);
   fetch(raw1, 1);
-  for (int i = 0; i < n; i += 2) {
+  int i = 0;
+  for (; i + 1 < n; i += 2) {
     step(raw0, i);
-    if (i + 1 < n) step(raw1, i + 1);
+    step(raw1, i + 1);
   }
+  if (i < n) step(raw0, i);
   // join the waves: maxima and sums of every row, then the outputs, a row tile at a time
   const int tid = fp4_fresh_tid(), col = tid & 15, grp = (tid >> 4) & 3;
 #pragma unroll
@@ -642,7 +655,7 @@ __device__ __forceinline__ void fp4_segment(Fp4Smem<DP>& sm, const Fp4AttnArgs& 
 }
 
 template <int DP, int MT, bool kExact>
-__global__ __launch_bounds__(kF4Threads, DP * MT <= 256 ? 2 : 1) void k_fp4_attn(Fp4AttnArgs a) {
+__global__ __launch_bounds__(kF4Threads, fp4_resident(DP, MT)) void k_fp4_attn(Fp4AttnArgs a) {
   __shared__ Fp4Smem<DP> sm;
   const int tid = threadIdx.x;
   const int items = a.B * a.row_blocks;
@@ -784,14 +797,6 @@ __global__ __launch_bounds__(kF4Threads) void k_fp4_attn_join(Fp4AttnArgs a, int
   }
 }
 
-// Workgroups that a CU holds at once, by the kernels' registers (four waves of at
-// most 512 / n) and LDS.
-int64_t fp4_resident(int dims, int mt) {
-  if (dims == 64) return mt == 1 ? 4 : mt == 2 ? 3 : 2;
-  if (dims == 128) return mt == 1 ? 3 : mt == 2 ? 2 : 1;
-  return dims == 256 && mt == 1 ? 2 : 1;
-}
-
 struct Fp4AttnPlan {
   int dims, mt;  // padded dims, row tiles of a workgroup
   int64_t row_blocks, items;
@@ -829,7 +834,7 @@ int fp4_attn_plan(const skv_fp4_attention_desc* d, Fp4AttnPlan& p) {
   if (d->window > 0) len = std::min(len, d->window + ceil_div(16 * p.mt, d->n_heads / hkv));
   const int64_t tiles = ceil_div(len, kF4Tile) + 1, units = std::max<int64_t>(p.items * hkv, 1);
   p.cut = tiles > kF4SmallTiles || d->splits > 0;
-  p.groups = fp4_resident(p.dims, p.mt) * device_cus();
+  p.groups = static_cast<int64_t>(fp4_resident(p.dims, p.mt)) * device_cus();
   if (d->splits > 0) p.groups = d->splits * units;
   if (p.items > kF4MaxItems || units > INT32_MAX / (ceil_div(capacity, kF4Tile) + 1)) {
     p.cut = false;
