@@ -54,6 +54,9 @@ constexpr int fp4_resident(int dims, int mt) {
   return dims == 64 ? (mt == 1 ? 4 : 3) : dims == 128 ? (mt == 1 ? 3 : 2) : dims == 256 && mt == 1 ? 2 : 1;
 }
 
+// Row tiles of a wave that shares its tiles.
+constexpr int fp4_shared_mt(int dims) { return dims <= 128 ? 2 : 1; }
+
 struct Fp4AttnArgs {
   const uint8_t* q;
   int64_t q_seq, q_tok, q_head;
@@ -68,7 +71,7 @@ struct Fp4AttnArgs {
   int32_t window;  // 0: none
   float scale, softcap;
   int32_t row_blocks;
-  int32_t* sched;   // [items + 1]: tiles before every (sequence, row block), for the join
+  int32_t* sched;   // for the join: [items + 1] tiles before every (sequence, row block), and `small`
   int32_t max_groups, small;  // see fp4_groups; items of at most `small` tiles are not cut
 };
 
@@ -97,17 +100,28 @@ __device__ __forceinline__ Fp4Span fp4_span(const Fp4AttnArgs& a, int b, int r0,
 }
 
 // Workgroups that share the units: a run of fewer than 8 tiles, 2 a wave, is not
-// worth a workgroup, but an item is.  Workgroup i takes [i total / n, (i + 1) total / n).
+// worth a workgroup, but an item is.  Workgroup i of n takes total / n tiles,
+// the first total mod n one more.
 constexpr int kF4RunTiles = 8;
 constexpr int kF4SmallTiles = 16;
+// No (sequence, row block, head) is cut where a workgroup for each leaves less than an
+// eighth of the chip's time unused: there is nothing to join then.
+constexpr int kF4Idle = 8;
 constexpr int kF4MaxItems = 2048;  // (sequence, row block)s whose prefix sum LDS holds
 
 __device__ __forceinline__ int fp4_groups(const Fp4AttnArgs& a, int total) {
   return min(a.max_groups, max((total + kF4RunTiles - 1) / kF4RunTiles, a.B * a.row_blocks * a.Hkv));
 }
-__device__ __forceinline__ int fp4_run_start(int64_t i, int total, int n) { return static_cast<int>(i * total / n); }
+__device__ __forceinline__ int fp4_run_start(int i, int total, int n) {
+  const uint32_t each = static_cast<uint32_t>(total) / static_cast<uint32_t>(n);
+  return static_cast<int>(i * each) + min(i, static_cast<int>(total - n * each));
+}
 // The workgroup whose run holds unit x.
-__device__ __forceinline__ int fp4_owner(int64_t x, int total, int n) { return static_cast<int>(((x + 1) * n - 1) / total); }
+__device__ __forceinline__ int fp4_owner(int x, int total, int n) {
+  const uint32_t each = static_cast<uint32_t>(total) / static_cast<uint32_t>(n), more = total - n * each, longer = more * (each + 1);
+  const uint32_t u = x;
+  return static_cast<int>(u < longer ? u / (each + 1) : more + (u - longer) / each);
+}
 
 __device__ __forceinline__ bf16x8 fp4_bf16x8(u32x4 v) { return __builtin_bit_cast(bf16x8, v); }
 
@@ -146,7 +160,7 @@ struct Fp4Raw {
   uint32_t k[2][kKeyWords], v[2][kWords];
   uint32_t ks[2][kScales], vs[2][kScales];
   uint32_t packed[2];  // scale bytes as loaded, of heads of 64 and 128 dims
-  int page[2];  // uniform; -1: not mapped
+  int slot[2];  // uniform; -1: not mapped
 };
 
 // A tile's scores, and what their masks need (uniform): every row sees every
@@ -154,29 +168,39 @@ struct Fp4Raw {
 template <int MT>
 struct Fp4Tile {
   f32x4 st[MT][2];  // row 16 mt + col, keys 16 h + 4 grp + i
-  int page[2];
+  int slot[2];
   bool masked;
   uint32_t nan_keys;
 };
 
+template <int kBytes>
+struct Fp4Run { using type = uint32_t; };
+template <>
+struct Fp4Run<2> { using type = uint16_t; };
+template <>
+struct Fp4Run<8> { using type = u32x2; };
+
 template <int DP>
 struct Fp4Smem {
-  // per wave: 32 value rows of DP bf16; at the end 16 output rows of DP fp32
+  // per wave: 32 value rows of DP bf16; at the end 16 output rows of DP fp32 (private tiles)
   alignas(16) uint8_t tile[kF4Waves][64 * DP];
-  float m[kF4Waves][64], l[kF4Waves][64];
+  float m[kF4Waves][32], l[kF4Waves][32];
+  uint32_t nan_keys[kF4Waves];  // of shared tiles
   int pre[kF4MaxItems + 1];
   int scan[17];
+  int longest;
 };
 
 // DP: the head's dims padded to 64, 128, 256 or 512 (kExact: D == DP).
-template <int DP, int MT, bool kExact>
+template <int DP, int MT, bool kExact, bool kShared>
 struct Fp4Wave {
   using Raw = Fp4Raw<DP>;
   static constexpr int kWords = Raw::kWords, kScales = Raw::kScales;
   static constexpr int kSteps = DP >= 128 ? DP / 128 : 1;  // products of 128 dims, or of the two parts of 64
   static constexpr int kBlocks = DP / 16;  // 16-dim blocks of the output
   static constexpr bool kPacked = kExact && DP <= 128;
-  static constexpr bool kOnce = DP * MT <= 256 && MT * 16 < 64;  // all of a head's rows in a workgroup: no page is read twice
+  static constexpr bool kTwo = DP * MT <= 256;  // two tiles in flight; wider ones have registers for one
+  static constexpr bool kOnce = !kShared && DP * MT <= 256;  // all of a head's rows in a workgroup: no page is read twice
 
   const Fp4AttnArgs& a;
   const Fp4Span& sp;
@@ -279,19 +303,19 @@ struct Fp4Wave {
 
   __device__ __forceinline__ int dims() const { return kExact ? DP : a.D; }
 
-  // page id (-1: not mapped) and first slot of the 16 positions from `pos` on
-  __device__ __forceinline__ void lookup(int b, int pos, int& page, int& slot) const {
+  // Where the codes of the 16 positions from `pos` on begin, as an offset from the
+  // pool, and their first slot (-1 and page 0: not mapped).
+  __device__ __forceinline__ void lookup(int b, int pos, uint64_t& at, int& slot) const {
     const int p = static_cast<int>(udiv24(pos, a.bs));
-    slot = pos - p * a.bs;
-    page = pos < sp.last ? a.bt[static_cast<int64_t>(b) * a.bt_stride + p] : -1;
+    int page = pos < sp.last ? a.bt[static_cast<int64_t>(b) * a.bt_stride + p] : -1;
     if (page >= a.n_pages) page = -1;
+    slot = page < 0 ? -1 : pos - p * a.bs;
+    at = static_cast<uint64_t>(max(page, 0)) * static_cast<uint64_t>(pg.page) + static_cast<uint64_t>(max(slot, 0) * (dims() / 2));
   }
 
-  // The codes of half h of a tile, 16 keys from slot `slot` of a page (all uniform).
-  __device__ __forceinline__ void load_codes(Raw& r, int h, int page, int slot) const {
-    r.page[h] = page;
-    // scalar bases, and a lane's offset that the loads add themselves
-    const uint8_t* kc = head + max(page, 0) * pg.page + slot * (dims() / 2);
+  // The codes of half h of a tile, 16 keys from `kc` on (uniform).
+  template <bool kKeys, bool kValues>
+  __device__ __forceinline__ void load_codes(Raw& r, int h, const uint8_t* kc) const {
     const uint8_t* vc = kc + pg.v_codes;
     uint32_t lane_at = code_at;
     asm("" : "+v"(lane_at));
@@ -304,7 +328,7 @@ struct Fp4Wave {
         return *p;
       }
     };
-    if constexpr (DP == 64) {  // lanes g and g + 2: block g of the key
+    if constexpr (DP == 64 && kKeys) {  // lanes g and g + 2: block g of the key
       const bool in = kExact || 32 * (grp & 1) < a.D;
       uint32_t key_at = col * (dims() / 2) + 16 * (grp & 1);
       asm("" : "+v"(key_at));
@@ -316,68 +340,86 @@ struct Fp4Wave {
     for (int w = 0; w < kWords; w += kRun) {
       const bool in = kExact || grp * (DP / 4) + 8 * w < a.D;
       const uint32_t at = in ? lane_at + 4 * w : 0u;
-      if constexpr (DP >= 128) {
+      if constexpr (DP >= 128 && kKeys) {
         const run_t x = get(reinterpret_cast<const run_t*>(kc + at));
 #pragma unroll
         for (int i = 0; i < kRun; ++i) r.k[h][w + i] = in ? x[i] : 0u;
       }
-      const run_t y = get(reinterpret_cast<const run_t*>(vc + at));
+      if constexpr (kValues) {
+        const run_t y = get(reinterpret_cast<const run_t*>(vc + at));
 #pragma unroll
-      for (int i = 0; i < kRun; ++i) r.v[h][w + i] = in ? y[i] : 0u;
+        for (int i = 0; i < kRun; ++i) r.v[h][w + i] = in ? y[i] : 0u;
+      }
     }
   }
 
   // Both halves' scale bytes.  Heads of 64 and 128 dims: a token's (4 or 8, its
   // key's and its value's) in one load, half h's by the lanes of odd or even g = h, which
   // then hand them to the rest; others a lane's own.
-  __device__ __forceinline__ const uint8_t* scales_of(int page, int slot) const {
-    return head + max(page, 0) * pg.page + pg.scales + slot * 2 * (dims() / kFp4Block);
+  __device__ __forceinline__ const uint8_t* scales_of(const uint8_t* kc, int slot) const {
+    return kc + static_cast<uint32_t>(pg.scales - max(slot, 0) * (dims() / 2 - 2 * (dims() / kFp4Block)));
   }
-  __device__ __forceinline__ void load_scales(Raw& r, int page0, int slot0, int page1, int slot1) const {
+  template <bool kKeys, bool kValues>
+  __device__ __forceinline__ void load_scales(Raw& r, const uint8_t* kc0, int slot0, const uint8_t* kc1, int slot1) const {
     const int nb = dims() / kFp4Block;
     if constexpr (kPacked) {
-      typedef uint32_t run_t __attribute__((ext_vector_type(kPacked ? DP / 64 : 1)));
-      uintptr_t sc0 = reinterpret_cast<uintptr_t>(scales_of(page0, slot0)), sc1 = reinterpret_cast<uintptr_t>(scales_of(page1, slot1));
+      using run_t = typename Fp4Run<(kKeys && kValues ? DP / 16 : DP / 32)>::type;
+      uintptr_t sc0 = reinterpret_cast<uintptr_t>(scales_of(kc0, slot0)), sc1 = reinterpret_cast<uintptr_t>(scales_of(kc1, slot1));
       asm("" : "+s"(sc0), "+s"(sc1));  // made in scalar registers, then chosen
-      const run_t x = *global_from_bits<const run_t>(((grp & 1) ? sc1 : sc0) + col * (DP / 16));
-#pragma unroll
-      for (int i = 0; i < DP / 64; ++i) r.packed[i] = x[i];
+      const run_t x = *global_from_bits<const run_t>(((grp & 1) ? sc1 : sc0) + col * (DP / 16) + (kKeys ? 0 : DP / 32));
+      if constexpr (sizeof(run_t) == 8) {
+        r.packed[0] = x[0];
+        r.packed[1] = x[1];
+      } else {
+        r.packed[0] = x;
+      }
     } else {
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const uint8_t* sc = scales_of(h ? page1 : page0, h ? slot1 : slot0);
+        const uint8_t* sc = scales_of(h ? kc1 : kc0, h ? slot1 : slot0);
         if constexpr (kExact && kScales > 1) {
           typedef uint8_t run_t __attribute__((ext_vector_type(kScales)));
-          const run_t x = *reinterpret_cast<const run_t*>(sc + scale_at), y = *reinterpret_cast<const run_t*>(sc + nb + scale_at);
+          if constexpr (kKeys) {
+            const run_t x = *reinterpret_cast<const run_t*>(sc + scale_at);
 #pragma unroll
-          for (int i = 0; i < kScales; ++i) {
-            r.ks[h][i] = x[i];
-            r.vs[h][i] = y[i];
+            for (int i = 0; i < kScales; ++i) r.ks[h][i] = x[i];
+          }
+          if constexpr (kValues) {
+            const run_t y = *reinterpret_cast<const run_t*>(sc + nb + scale_at);
+#pragma unroll
+            for (int i = 0; i < kScales; ++i) r.vs[h][i] = y[i];
           }
         } else {
 #pragma unroll
           for (int i = 0; i < kScales; ++i) {
             const int kb = DP >= 128 ? grp * kScales + i : grp & 1, vb = DP >= 128 ? kb : grp >> 1;
-            const uint32_t ks = sc[col * 2 * nb + (kb < nb ? kb : 0)], vs = sc[col * 2 * nb + nb + (vb < nb ? vb : 0)];
-            r.ks[h][i] = kb < nb ? ks : 127u;
-            r.vs[h][i] = vb < nb ? vs : 127u;
+            if constexpr (kKeys) {
+              const uint32_t ks = sc[col * 2 * nb + (kb < nb ? kb : 0)];
+              r.ks[h][i] = kb < nb ? ks : 127u;
+            }
+            if constexpr (kValues) {
+              const uint32_t vs = sc[col * 2 * nb + nb + (vb < nb ? vb : 0)];
+              r.vs[h][i] = vb < nb ? vs : 127u;
+            }
           }
         }
       }
     }
   }
+  template <bool kKeys, bool kValues>
   __device__ __forceinline__ void unpack_scales(Raw& r) const {
     if constexpr (kPacked) {
-      // 64 dims: a word K0 K1 V0 V1; 128: a word of K's, one of V's, g's block g
+      // 64 dims: K0 K1 V0 V1; 128: a word of K's, one of V's, g's block g
+      constexpr int kWordsIn = kKeys && kValues ? DP / 64 : 1;
 #pragma unroll
-      for (int i = 0; i < DP / 64; ++i) {
+      for (int i = 0; i < kWordsIn; ++i) {
         const auto x = __builtin_amdgcn_permlane16_swap(r.packed[i], r.packed[i], false, false);
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           if constexpr (DP == 64) {  // g's key block is g % 2, its values' block g / 2
-            r.ks[h][0] = x[h] >> (8 * (grp & 1));
-            r.vs[h][0] = (x[h] >> (16 + 8 * (grp >> 1))) & 0xff;
-          } else if (i == 0) {
+            if constexpr (kKeys) r.ks[h][0] = x[h] >> (8 * (grp & 1));
+            if constexpr (kValues) r.vs[h][0] = (x[h] >> ((kKeys ? 16 : 0) + 8 * (grp >> 1))) & 0xff;
+          } else if (kKeys && i == 0) {
             r.ks[h][0] = x[h] >> (8 * grp);  // the products take byte 0
           } else {
             r.vs[h][0] = (x[h] >> (8 * grp)) & 0xff;
@@ -385,6 +427,22 @@ struct Fp4Wave {
         }
       }
     }
+  }
+
+  // A tile's loads, or those of its keys or its values alone.
+  template <bool kKeys, bool kValues>
+  __device__ __forceinline__ void fetch(Raw& r, uint64_t at, int slot, int from) const {
+    const uint8_t* kc[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const uint32_t lo = __builtin_amdgcn_readlane(static_cast<uint32_t>(at), from + h);
+      const uint32_t hi = __builtin_amdgcn_readlane(static_cast<uint32_t>(at >> 32), from + h);
+      kc[h] = head + (static_cast<uint64_t>(hi) << 32 | lo);
+      r.slot[h] = __builtin_amdgcn_readlane(slot, from + h);
+    }
+    load_scales<kKeys, kValues>(r, kc[0], r.slot[0], kc[1], r.slot[1]);
+    load_codes<kKeys, kValues>(r, 0, kc[0]);
+    load_codes<kKeys, kValues>(r, 1, kc[1]);
   }
 
   // Where not every row sees every key, or a value's block is NaN: the values of
@@ -398,7 +456,7 @@ struct Fp4Wave {
 #pragma unroll
       for (int i = 0; i < kScales; ++i) nan |= r.vs[h][i] == kFp4NaN;
       const int at = pos + 16 * h + col;
-      if (nan || at >= sp.last || at < sp.first || r.page[h] < 0) {
+      if (nan || at >= sp.last || at < sp.first || r.slot[h] < 0) {
 #pragma unroll
         for (int w = 0; w < kWords; ++w) r.v[h][w] = 0u;
 #pragma unroll
@@ -410,18 +468,19 @@ struct Fp4Wave {
     return nan_keys;
   }
 
-  // One tile, positions pos .. pos + 31: its values to LDS and its scores.
-  __device__ __forceinline__ Fp4Tile<MT> scores(Raw& r, int pos, uint16_t* vt) const {
-    unpack_scales(r);
-    Fp4Tile<MT> tl;
+  // Whether a row may not see a key of the tile at `pos`, or a key's values are NaN somewhere.
+  __device__ __forceinline__ bool uneven(const Raw& r, int pos) const {
+    return pos < sp.all_lo || pos + kF4Tile > sp.all_hi || (r.slot[0] | r.slot[1]) < 0;
+  }
+  __device__ __forceinline__ bool any_nan(const Raw& r) const {
     bool nan = false;
 #pragma unroll
     for (int i = 0; i < kScales; ++i) nan |= r.vs[0][i] == kFp4NaN || r.vs[1][i] == kFp4NaN;
-    tl.page[0] = r.page[0];
-    tl.page[1] = r.page[1];
-    tl.masked = pos < sp.all_lo || pos + kF4Tile > sp.all_hi || (r.page[0] | r.page[1]) < 0 || __ballot(nan) != 0;
-    tl.nan_keys = 0;
-    if (tl.masked) tl.nan_keys = clean(r, pos);  // uniform
+    return __ballot(nan) != 0;
+  }
+
+  // The scores of 32 keys.
+  __device__ __forceinline__ void scores(const Raw& r, Fp4Tile<MT>& tl) const {
     auto& st = tl.st;
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) st[mt][0] = st[mt][1] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -442,6 +501,10 @@ struct Fp4Wave {
         }
       }
     }
+  }
+
+  // 32 keys' values to LDS.
+  __device__ __forceinline__ void values(const Raw& r, uint16_t* vt) const {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       uint16_t* dst = vt + (16 * h + col) * DP;
@@ -451,37 +514,39 @@ struct Fp4Wave {
             fp4_decode8(r.v[h][w], fp4_scale(r.vs[h][w / 4 < kScales ? w / 4 : 0]));
       }
     }
-    return tl;
   }
 
   // The tile's weights, and its values times them onto the output.
   __device__ __forceinline__ void output(Fp4Tile<MT>& tl, int pos, const uint16_t* vt) {
     auto& st = tl.st;
     const bool capped = a.softcap > 0.f;
-    const float mult = capped ? 2.f * kF4Log2e * a.scale / a.softcap : a.scale * kF4Log2e;
-#pragma unroll
-    for (int mt = 0; mt < MT; ++mt) {
-#pragma unroll
-      for (int h = 0; h < 2; ++h) st[mt][h] *= mult;  // to the log2 domain, or what the cap's tanh takes
-    }
-    if (capped || tl.masked) {  // uniform
-      const float cap = a.softcap * kF4Log2e;
+    float mult = a.scale * kF4Log2e;  // to the log2 domain
+    if (capped) {  // uniform; tanh(x) = 1 - 2 / (exp(2x) + 1)
+      const float k = 2.f * kF4Log2e * a.scale / a.softcap, cap = a.softcap * kF4Log2e;
+      mult = 1.f;
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const int key = 16 * h + 4 * grp + i;
-            float v = st[mt][h][i];
-            // tanh(x) = 1 - 2 / (exp(2x) + 1)
-            if (capped) v = cap * (1.f - 2.f * __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(v) + 1.f));
-            if (tl.masked) {
-              if ((tl.nan_keys >> key) & 1) v = __builtin_nanf("");
-              const bool seen = pos + key < hi[mt] && pos + key >= lo[mt] && tl.page[h] >= 0;
-              v = seen ? v : -__builtin_huge_valf();
-            }
-            st[mt][h][i] = v;
+            st[mt][h][i] = cap * (1.f - 2.f * __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(st[mt][h][i] * k) + 1.f));
+          }
+        }
+      }
+    }
+    if (tl.masked) {  // uniform
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          // keys 4 grp + i of the half: the first that the row may see, and how many
+          const int from = lo[mt] - pos - 16 * h - 4 * grp, to = tl.slot[h] < 0 ? INT32_MIN : hi[mt] - pos - 16 * h - 4 * grp;
+          const uint32_t nan = tl.nan_keys >> (16 * h + 4 * grp);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float v = (nan >> i) & 1 ? __builtin_nanf("") : st[mt][h][i];
+            st[mt][h][i] = i >= from && i < to ? v : -__builtin_huge_valf();
           }
         }
       }
@@ -493,7 +558,9 @@ struct Fp4Wave {
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
       const f32x4 x = st[mt][0], y = st[mt][1];
-      mx[mt] = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3])));
+      // (a NaN score makes its row NaN, whatever the maximum)
+      const auto top3 = [](float u, float v, float w) { return __builtin_elementwise_maximum(__builtin_elementwise_maximum(u, v), w); };
+      mx[mt] = __builtin_elementwise_maximum(top3(top3(top3(x[0], x[1], x[2]), x[3], y[0]), y[1], y[2]), y[3]) * mult;
       any |= mx[mt] > m[mt] + kF4Move;
     }
     if (__ballot(any)) {
@@ -515,7 +582,7 @@ struct Fp4Wave {
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) e[4 * h + i] = __builtin_amdgcn_exp2f(st[mt][h][i] - m[mt]);
+        for (int i = 0; i < 4; ++i) e[4 * h + i] = __builtin_amdgcn_exp2f(__builtin_fmaf(st[mt][h][i], mult, -m[mt]));
       }
       l[mt] += ((e[0] + e[1]) + (e[2] + e[3])) + ((e[4] + e[5]) + (e[6] + e[7]));
 #pragma unroll
@@ -546,55 +613,62 @@ __device__ __forceinline__ int fp4_fresh_tid() {
 }
 
 // A segment: tiles [t_from, t_to) of an item; its rows' outputs, or where the
-// segment is a piece of the item, slot `slot` of the partial ones.
+// segment is a piece of the item, slot `slot_of_part` of the partial ones.  Every wave
+// takes tiles of its own for all of the item's rows.
 template <int DP, int MT, bool kExact>
 __device__ __forceinline__ void fp4_segment(Fp4Smem<DP>& sm, const Fp4AttnArgs& a, int b, int rb, int hk, const Fp4Span& sp,
                                             int t_from, int t_to, int slot_of_part) {
-  using Wave = Fp4Wave<DP, MT, kExact>;
+  using Wave = Fp4Wave<DP, MT, kExact, false>;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x) / kWave, lane = fp4_fresh_tid() % kWave;
   const int r0 = rb * 16 * MT;
   const int t_lo = sp.tile0 + t_from, t_hi = sp.tile0 + min(t_to, sp.tiles);
   Wave w(a, sp, b, hk, r0, lane);
   uint16_t* vt = reinterpret_cast<uint16_t*>(sm.tile[wave]);
-  // this wave's tiles t_lo + wave, + 4, ...; the page ids of 32 of them at a time
-  int page = -1, slot = 0;
+  // this wave's tiles t_lo + wave, + 4, ...; the places of 32 of them at a time
+  uint64_t at = 0;
+  int slot = -1;
   const int n = t_hi > t_lo + wave ? (t_hi - t_lo - wave + kF4Waves - 1) / kF4Waves : 0;
   const auto fetch = [&](typename Wave::Raw& raw, int i) {
-    // past the last tile page 0 is read, so that the loads in flight are the same
-    // number whatever the path: a wait for a tile's then leaves the next one's alone
-    const bool in = i < n;  // uniform
-    if ((i & 31) == 0 && in) {   // lane 2 j + h: half h of tile i + j
+    // past the last tile something mapped is read, so that the loads in flight are the
+    // same number whatever the path: a wait for a tile's then leaves the next one's alone
+    if ((i & 31) == 0 && i < n) {  // lane 2 j + h: half h of tile i + j
       const int t = t_lo + wave + (i + (lane >> 1)) * kF4Waves;
-      w.lookup(b, min(t, t_hi) * kF4Tile + 16 * (lane & 1), page, slot);
+      w.lookup(b, min(t, t_hi) * kF4Tile + 16 * (lane & 1), at, slot);
     }
-    const int at = 2 * (i & 31);
-    int p0 = __builtin_amdgcn_readlane(page, at), p1 = __builtin_amdgcn_readlane(page, at + 1);
-    int s0 = __builtin_amdgcn_readlane(slot, at), s1 = __builtin_amdgcn_readlane(slot, at + 1);
-    p0 = in ? p0 : -1;
-    p1 = in ? p1 : -1;
-    s0 = in ? s0 : 0;
-    s1 = in ? s1 : 0;
-    w.load_scales(raw, p0, s0, p1, s1);
-    w.load_codes(raw, 0, p0, s0);
-    w.load_codes(raw, 1, p1, s1);
+    w.template fetch<true, true>(raw, at, slot, 2 * (i & 31));
   };
-  // the tile's registers take the tile after the next as soon as its scores are made
+  // the tile's registers take the next tile (of two in flight, the one after) as soon
+  // as its scores are made
+  constexpr int kAhead = Wave::kTwo ? 2 : 1;
   const auto step = [&](typename Wave::Raw& raw, int i) {
     const int pos = (t_lo + wave + i * kF4Waves) * kF4Tile;
-    auto tl = w.scores(raw, pos, vt);
-    fetch(raw, i + 2);
+    w.template unpack_scales<true, true>(raw);
+    Fp4Tile<MT> tl;
+    tl.slot[0] = raw.slot[0];
+    tl.slot[1] = raw.slot[1];
+    tl.masked = w.uneven(raw, pos) || w.any_nan(raw);
+    tl.nan_keys = 0;
+    if (tl.masked) tl.nan_keys = w.clean(raw, pos);  // uniform
+    w.scores(raw, tl);
+    w.values(raw, vt);
+    fetch(raw, i + kAhead);
     w.output(tl, pos, vt);
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
   };
-  typename Wave::Raw raw0, raw1;
+  typename Wave::Raw raw0;
   fetch(raw0, 0);
-  fetch(raw1, 1);
-  int i = 0;
-  for (; i + 1 < n; i += 2) {
-    step(raw0, i);
-    step(raw1, i + 1);
+  if constexpr (Wave::kTwo) {
+    typename Wave::Raw raw1;
+    fetch(raw1, 1);
+    int i = 0;
+    for (; i + 1 < n; i += 2) {
+      step(raw0, i);
+      step(raw1, i + 1);
+    }
+    if (i < n) step(raw0, i);
+  } else {
+    for (int i = 0; i < n; ++i) step(raw0, i);
   }
-  if (i < n) step(raw0, i);
   // join the waves: maxima and sums of every row, then the outputs, a row tile at a time
   const int tid = fp4_fresh_tid(), col = tid & 15, grp = (tid >> 4) & 3;
 #pragma unroll
@@ -654,19 +728,121 @@ __device__ __forceinline__ void fp4_segment(Fp4Smem<DP>& sm, const Fp4AttnArgs& 
   }
 }
 
+// The same with tiles that the waves share: each has 16 MT of the item's rows and
+// decodes one in four tiles' values for all of them.
 template <int DP, int MT, bool kExact>
+__device__ __forceinline__ void fp4_segment_shared(Fp4Smem<DP>& sm, const Fp4AttnArgs& a, int b, int rb, int hk, const Fp4Span& sp,
+                                                   int t_from, int t_to, int slot_of_part) {
+  using Wave = Fp4Wave<DP, MT, kExact, true>;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x) / kWave, lane = fp4_fresh_tid() % kWave;
+  const int r0 = (rb * kF4Waves + wave) * 16 * MT;
+  const int t_lo = sp.tile0 + t_from, t_hi = sp.tile0 + min(t_to, sp.tiles);
+  Wave w(a, sp, b, hk, r0, lane);
+  const int n = t_hi - t_lo;
+  // lane 2 j + h, j < 4: half h of tile i + j (past the last something mapped)
+  const auto places = [&](int i, uint64_t& at, int& slot) {
+    w.lookup(b, min(t_lo + i + ((lane >> 1) & 3), t_hi) * kF4Tile + 16 * (lane & 1), at, slot);
+  };
+  constexpr int kKeys = Wave::kTwo ? 2 : 1;  // tiles' keys in registers
+  typename Wave::Raw keys[kKeys], vals;
+  uint64_t at, at_next;
+  int slot, slot_next;
+  places(0, at, slot);
+  w.template fetch<false, true>(vals, at, slot, 2 * wave);
+  w.template fetch<true, false>(keys[0], at, slot, 0);
+  for (int i = 0; i < n; i += kF4Waves) {
+    {
+      const int pos = (t_lo + i + wave) * kF4Tile;
+      w.template unpack_scales<false, true>(vals);
+      uint32_t nan_keys = 0;
+      if (w.uneven(vals, pos) || w.any_nan(vals)) nan_keys = w.clean(vals, pos);  // uniform
+      w.values(vals, reinterpret_cast<uint16_t*>(sm.tile[wave]));
+      if (lane == 0) sm.nan_keys[wave] = nan_keys;
+    }
+    places(i + kF4Waves, at_next, slot_next);
+    __syncthreads();  // the tiles are there
+#pragma unroll
+    for (int j = 0; j < kF4Waves; ++j) {
+      typename Wave::Raw& kr = keys[j % kKeys];
+      const auto next = [&] {
+        typename Wave::Raw& to = keys[(j + 1) % kKeys];
+        if (j < kF4Waves - 1) {
+          w.template fetch<true, false>(to, at, slot, 2 * (j + 1));
+        } else {
+          w.template fetch<true, false>(to, at_next, slot_next, 0);
+        }
+      };
+      const int pos = (t_lo + i + j) * kF4Tile;
+      Fp4Tile<MT> tl;
+      if constexpr (kKeys == 2) next();
+      if (j == 1) w.template fetch<false, true>(vals, at_next, slot_next, 2 * wave);
+      tl.slot[0] = kr.slot[0];
+      tl.slot[1] = kr.slot[1];
+      tl.nan_keys = __builtin_amdgcn_readfirstlane(sm.nan_keys[j]);
+      tl.masked = w.uneven(kr, pos) || tl.nan_keys != 0;
+      w.template unpack_scales<true, false>(kr);
+      w.scores(kr, tl);
+      if constexpr (kKeys == 1) next();
+      if (i + j < n) w.output(tl, pos, reinterpret_cast<const uint16_t*>(sm.tile[j]));  // uniform
+    }
+    at = at_next;
+    slot = slot_next;
+    __syncthreads();  // the tiles have been read
+  }
+  const int tid = fp4_fresh_tid(), col = tid & 15, grp = (tid >> 4) & 3;
+  const float ninf = -__builtin_huge_valf();
+  const bool whole = slot_of_part < 0;
+  const int D = kExact ? DP : a.D;
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt) {
+    const float l = fp4_sum_groups(w.l[mt]);
+    const int r = r0 + 16 * mt + col;
+    if (r >= sp.r_end) continue;
+    const int t = r / a.G, h = hk * a.G + r - t * a.G;
+    if (whole) {
+      const float sink = a.sink ? a.sink[h] * kF4Log2e : ninf;
+      const float ref = fmaxf(w.m[mt], sink) == kF4None ? 0.f : fmaxf(w.m[mt], sink);
+      const float f = __builtin_amdgcn_exp2f(w.m[mt] - ref);
+      float den = l != l ? l : f == 0.f ? 0.f : f * l;
+      if (sink != ninf) den += __builtin_amdgcn_exp2f(sink - ref);
+      const float inv = den == 0.f ? 0.f : f / den;
+      uint16_t* out = a.out + ((static_cast<int64_t>(b) * a.T + t) * a.H + h) * D;
+#pragma unroll
+      for (int x = 0; x < Wave::kBlocks; ++x) {
+        const int d = 16 * x + 4 * grp;
+        if (!kExact && d >= D) continue;
+        const f32x4 v = w.acc[mt][x] * inv;
+        *reinterpret_cast<u32x2*>(out + d) = u32x2{bf16_pack2(v[0], v[1]), bf16_pack2(v[2], v[3])};
+      }
+    } else {
+      float* part = a.part + (static_cast<int64_t>(slot_of_part) * kF4Waves + wave) * (16 * MT) * (D + 4) + (16 * mt + col) * (D + 4);
+      if (grp == 0) {
+        part[0] = w.m[mt];
+        part[1] = l;
+      }
+#pragma unroll
+      for (int x = 0; x < Wave::kBlocks; ++x) {
+        const int d = 16 * x + 4 * grp;
+        if (kExact || d < D) *reinterpret_cast<f32x4*>(part + 4 + d) = w.acc[mt][x];
+      }
+    }
+  }
+}
+
+template <int DP, int MT, bool kExact, bool kShared>
 __global__ __launch_bounds__(kF4Threads, fp4_resident(DP, MT)) void k_fp4_attn(Fp4AttnArgs a) {
+  constexpr int kRows = 16 * MT * (kShared ? kF4Waves : 1);
   __shared__ Fp4Smem<DP> sm;
   const int tid = threadIdx.x;
   const int items = a.B * a.row_blocks;
   const auto span_of = [&](int item, int& b, int& rb) {
     b = item / a.row_blocks;
     rb = item - b * a.row_blocks;
-    return fp4_span(a, b, rb * 16 * MT, 16 * MT);
+    return fp4_span(a, b, rb * kRows, kRows);
   };
   // values worked out in LDS are the same in every lane: scalar registers hold them
   const auto uniform = [](int v) { return __builtin_amdgcn_readfirstlane(v); };
-  const bool each = a.max_groups == 0;  // more items than LDS holds: none is cut, a workgroup each
+  const bool each = a.max_groups == 0;  // none is cut, a workgroup each
   const int g = blockIdx.x;
   int x = g, end = g + 1, total = 0, b, rb;
   const auto item_of = [&](int u) {  // u < total: pre[item] <= u < pre[item + 1]
@@ -678,24 +854,35 @@ __global__ __launch_bounds__(kF4Threads, fp4_resident(DP, MT)) void k_fp4_attn(F
     return lo;
   };
   if (!each) {
+    if (tid == 0) sm.longest = 0;
+    __syncthreads();
+    int longest = 0;
     for (int base = 0; base < items; base += kF4Threads) {
       const int item = base + tid;
-      const int n = item < items ? span_of(item, b, rb).units() * a.Hkv : 0;
+      const int own = item < items ? span_of(item, b, rb).units() : 0, n = own * a.Hkv;
+      longest = max(longest, own);
       int tot;
       const int ex = block_exclusive_scan(n, sm.scan, &tot);
       if (item < items) sm.pre[item] = total + ex;
       total += tot;
     }
     if (tid == 0) sm.pre[items] = total;
+    if (longest > 0) atomicMax(&sm.longest, longest);
     __syncthreads();
     total = uniform(total);
-    if (g == 0 && a.sched) {
+    int groups = fp4_groups(a, total);
+    const int units = items * a.Hkv;
+    const bool whole = a.small == kF4SmallTiles && units <= groups &&
+                       static_cast<int64_t>(uniform(sm.longest)) * groups * (kF4Idle - 1) <= static_cast<int64_t>(total) * kF4Idle;
+    if (g == 0) {
       for (int i = tid; i <= items; i += kF4Threads) a.sched[i] = sm.pre[i];
+      if (tid == 0) a.sched[items + 1] = whole ? INT32_MAX : a.small;
     }
-    const int groups = fp4_groups(a, total);
+    if (whole) groups = units;
     if (g >= groups) return;  // uniform
     // a run's end inside a small item moves to the item's end
     const auto run_start = [&](int i) {
+      if (whole) return i == units ? total : sm.pre[i / a.Hkv] + i % a.Hkv * ((sm.pre[i / a.Hkv + 1] - sm.pre[i / a.Hkv]) / a.Hkv);
       const int u = fp4_run_start(i, total, groups);
       if (u <= 0 || u >= total) return u;
       const int item = item_of(u), n = (sm.pre[item + 1] - sm.pre[item]) / a.Hkv;
@@ -713,7 +900,11 @@ __global__ __launch_bounds__(kF4Threads, fp4_resident(DP, MT)) void k_fp4_attn(F
     const int hk = each ? x - item * a.Hkv : in / n;
     const int from = each ? 0 : in - hk * n, to = each ? n : min(n, from + end - x);
     const int part = from == 0 && to == n ? -1 : from == 0 ? 2 * g + 1 : 2 * g;
-    fp4_segment<DP, MT, kExact>(sm, a, b, rb, hk, sp, from, to, part);
+    if constexpr (kShared) {
+      fp4_segment_shared<DP, MT, kExact>(sm, a, b, rb, hk, sp, from, to, part);
+    } else {
+      fp4_segment<DP, MT, kExact>(sm, a, b, rb, hk, sp, from, to, part);
+    }
     x += each ? 1 : to - from;
     __syncthreads();  // the segment's LDS has been read
   }
@@ -731,9 +922,9 @@ __global__ __launch_bounds__(kF4Threads) void k_fp4_attn_join(Fp4AttnArgs a, int
   const int item = blockIdx.x / a.Hkv, hk = blockIdx.x - item * a.Hkv;
   const int b = item / a.row_blocks, rb = item - b * a.row_blocks;
   const int total = a.sched[items], p0 = a.sched[item], n = (a.sched[item + 1] - p0) / a.Hkv;
-  if (n <= a.small) return;  // uniform
+  if (n <= a.sched[items + 1]) return;  // uniform
   const int groups = fp4_groups(a, total);
-  const int64_t x0 = p0 + static_cast<int64_t>(hk) * n;
+  const int x0 = p0 + hk * n;
   const int w0 = fp4_owner(x0, total, groups), pieces = fp4_owner(x0 + n - 1, total, groups) - w0 + 1;
   if (pieces == 1) return;  // uniform
   const int tid = threadIdx.x % kThreads, mine = threadIdx.x / kThreads, lane = threadIdx.x % kWave;
@@ -798,10 +989,12 @@ __global__ __launch_bounds__(kF4Threads) void k_fp4_attn_join(Fp4AttnArgs a, int
 }
 
 struct Fp4AttnPlan {
-  int dims, mt;  // padded dims, row tiles of a workgroup
+  int dims, mt;  // padded dims, row tiles of a wave
+  bool shared;   // the waves share the tiles, each with rows of its own
+  int rows;      // of a workgroup
   int64_t row_blocks, items;
-  int64_t groups;  // workgroups; of cut items where `cut` allows for it
-  bool cut;
+  bool cut;        // items may be cut
+  int64_t groups;  // then: the most workgroups
   int64_t sched_bytes, ws_bytes;
 };
 
@@ -824,36 +1017,51 @@ int fp4_attn_plan(const skv_fp4_attention_desc* d, Fp4AttnPlan& p) {
   }
   const int64_t D = d->cache.head_dim, rows = d->n_queries * (d->n_heads / hkv);
   p.dims = D <= 64 ? 64 : D <= 128 ? 128 : D <= 256 ? 256 : 512;
-  const int most = p.dims <= 256 ? 2 : 1;
-  p.mt = std::min(most, rows <= 16 ? 1 : 2);
-  p.row_blocks = ceil_div(rows, 16 * p.mt);
+  // A wave's tiles are its own, or all four waves' with rows of their own for each, once
+  // more than half of the rows of such a workgroup are there.
+  const int mt = fp4_shared_mt(p.dims);
+  p.shared = p.dims <= 256 && rows > 16 * mt * kF4Waves / 2;
+  p.mt = p.shared ? mt : rows <= 16 || p.dims > 256 ? 1 : 2;
+  p.rows = 16 * p.mt * (p.shared ? kF4Waves : 1);
+  p.row_blocks = ceil_div(rows, p.rows);
   p.items = d->cache.batch * p.row_blocks;
   // the most tiles that a row block may see
   const int64_t capacity = d->cache.bt_stride * d->cache.block_size;
   int64_t len = d->max_len > 0 ? std::min(d->max_len, capacity) : capacity;
-  if (d->window > 0) len = std::min(len, d->window + ceil_div(16 * p.mt, d->n_heads / hkv));
+  if (d->window > 0) len = std::min(len, d->window + ceil_div(p.rows, d->n_heads / hkv));
   const int64_t tiles = ceil_div(len, kF4Tile) + 1, units = std::max<int64_t>(p.items * hkv, 1);
   p.cut = tiles > kF4SmallTiles || d->splits > 0;
-  p.groups = static_cast<int64_t>(fp4_resident(p.dims, p.mt)) * device_cus();
-  if (d->splits > 0) p.groups = d->splits * units;
-  if (p.items > kF4MaxItems || units > INT32_MAX / (ceil_div(capacity, kF4Tile) + 1)) {
-    p.cut = false;
-    p.groups = 0;
-  }
+  if (p.items > kF4MaxItems || units > INT32_MAX / (ceil_div(capacity, kF4Tile) + 1)) p.cut = false;
+  p.groups = !p.cut ? 0 : d->splits > 0 ? d->splits * units : static_cast<int64_t>(fp4_resident(p.dims, p.mt)) * device_cus();
   if (units >= (1 << 24) || p.groups >= (1 << 24)) return set_error(SKV_EINVAL, "%s: too many workgroups", what);
-  p.sched_bytes = p.cut ? ceil_div((p.items + 1) * 4, 16) * 16 : 0;
-  p.ws_bytes = p.cut ? p.sched_bytes + 2 * p.groups * 16 * p.mt * (D + 4) * 4 : 0;
+  p.sched_bytes = p.cut ? ceil_div((p.items + 2) * 4, 16) * 16 : 0;
+  p.ws_bytes = p.cut ? p.sched_bytes + 2 * p.groups * p.rows * (D + 4) * 4 : 0;
   return SKV_OK;
 }
 
-// The part launch for padded dims DP and mt row tiles (at most those that plan gives).
-template <int DP, bool kExact>
+// The part launch for padded dims DP.
+template <int DP, bool kExact, bool kShared>
 void launch_rows(const Fp4AttnArgs& a, int mt, hipStream_t s) {
   const dim3 grid(static_cast<unsigned>(a.max_groups > 0 ? a.max_groups : static_cast<int64_t>(a.B) * a.row_blocks * a.Hkv));
-  if (mt == 1) hipLaunchKernelGGL((k_fp4_attn<DP, 1, kExact>), grid, dim3(kF4Threads), 0, s, a);
-  if constexpr (DP <= 256) {
-    if (mt == 2) hipLaunchKernelGGL((k_fp4_attn<DP, 2, kExact>), grid, dim3(kF4Threads), 0, s, a);
+  if constexpr (kShared) {
+    hipLaunchKernelGGL((k_fp4_attn<DP, fp4_shared_mt(DP), kExact, true>), grid, dim3(kF4Threads), 0, s, a);
+  } else {
+    if (mt == 1) hipLaunchKernelGGL((k_fp4_attn<DP, 1, kExact, false>), grid, dim3(kF4Threads), 0, s, a);
+    if constexpr (DP <= 256) {
+      if (mt == 2) hipLaunchKernelGGL((k_fp4_attn<DP, 2, kExact, false>), grid, dim3(kF4Threads), 0, s, a);
+    }
   }
+}
+template <bool kExact>
+void launch_dims(const Fp4AttnArgs& a, const Fp4AttnPlan& p, hipStream_t s) {
+  const auto go = [&](auto dims) {
+    constexpr int DP = decltype(dims)::value;
+    if (p.shared) launch_rows<DP, kExact, true>(a, p.mt, s); else launch_rows<DP, kExact, false>(a, p.mt, s);
+  };
+  if (p.dims == 64) go(std::integral_constant<int, 64>());
+  if (p.dims == 128) go(std::integral_constant<int, 128>());
+  if (p.dims == 256) go(std::integral_constant<int, 256>());
+  if (p.dims == 512) go(std::integral_constant<int, 512>());
 }
 
 }  // namespace skv
@@ -906,29 +1114,19 @@ extern "C" int skv_fp4_attention(const skv_fp4_attention_desc* d, void* workspac
   a.part = p.cut ? reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + p.sched_bytes) : nullptr;
   a.row_blocks = static_cast<int32_t>(p.row_blocks);
   a.max_groups = static_cast<int32_t>(p.groups);
-  a.small = !p.cut ? INT32_MAX : d->splits > 0 ? 0 : kF4SmallTiles;
+  a.small = d->splits > 0 ? 0 : kF4SmallTiles;
   hipStream_t s = static_cast<hipStream_t>(stream);
-  if (a.D != p.dims) {
-    if (p.dims == 64) launch_rows<64, false>(a, p.mt, s);
-    if (p.dims == 128) launch_rows<128, false>(a, p.mt, s);
-    if (p.dims == 256) launch_rows<256, false>(a, p.mt, s);
-    if (p.dims == 512) launch_rows<512, false>(a, p.mt, s);
-  } else {
-    if (p.dims == 64) launch_rows<64, true>(a, p.mt, s);
-    if (p.dims == 128) launch_rows<128, true>(a, p.mt, s);
-    if (p.dims == 256) launch_rows<256, true>(a, p.mt, s);
-    if (p.dims == 512) launch_rows<512, true>(a, p.mt, s);
-  }
+  if (a.D == p.dims) launch_dims<true>(a, p, s); else launch_dims<false>(a, p, s);
   if (const int rc = check_launch(what)) return rc;
   if (!p.cut) return SKV_OK;
   // about 2,048 workgroups, a row each where there are fewer rows
-  const int64_t units = p.items * a.Hkv, block_rows = std::min<int64_t>(16 * p.mt, static_cast<int64_t>(a.T) * a.G);
+  const int64_t units = p.items * a.Hkv, block_rows = std::min<int64_t>(p.rows, static_cast<int64_t>(a.T) * a.G);
   const int64_t per = std::min(block_rows, ceil_div(units * block_rows, 2048));
   const dim3 grid(static_cast<unsigned>(units), static_cast<unsigned>(ceil_div(block_rows, per)));
   if (per == 1) {
-    hipLaunchKernelGGL((k_fp4_attn_join<kF4Threads>), grid, dim3(kF4Threads), 0, s, a, 16 * p.mt, static_cast<int>(per));
+    hipLaunchKernelGGL((k_fp4_attn_join<kF4Threads>), grid, dim3(kF4Threads), 0, s, a, p.rows, static_cast<int>(per));
   } else {
-    hipLaunchKernelGGL((k_fp4_attn_join<kWave>), grid, dim3(kF4Threads), 0, s, a, 16 * p.mt, static_cast<int>(per));
+    hipLaunchKernelGGL((k_fp4_attn_join<kWave>), grid, dim3(kF4Threads), 0, s, a, p.rows, static_cast<int>(per));
   }
   return check_launch(what);
 }
