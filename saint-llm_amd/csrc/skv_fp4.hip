@@ -7,7 +7,9 @@
 //
 // Both move a token's K and V of all heads in items of 8 dims: 16 bytes of bf16
 // (32 of fp32) on one side, a word of codes on the other; the four lanes of a
-// 32-dim block find its largest magnitude by two quad permutes.
+// 32-dim block find its largest magnitude by two quad permutes.  A thread has the
+// same item of four tokens, whose loads it sends together: where an item lies in
+// a token is worked out once for the four.
 #include <algorithm>
 
 #include "skv_fp4.h"
@@ -30,38 +32,57 @@ struct Fp4RowsArgs {
   int64_t rows;   // tokens per sequence that x holds
   int bs, heads, dim;
   int items;      // of a token: 2 * heads * dim / 8
+  int together;   // tokens whose items a workgroup's threads take at once
+};
+constexpr int kFp4Tokens = 4;  // of a thread, a.together apart
+
+// Where the tokens of a thread lie: page 0 where the page is not mapped or there is no token.
+struct Fp4Places {
+  int64_t page[kFp4Tokens];  // in bytes
+  int slot[kFp4Tokens];
+  int i[kFp4Tokens];  // token of its sequence's new ones
+  bool in[kFp4Tokens], mapped[kFp4Tokens];
 };
 
-// An item: token i of sequence b's n, K or V, head, 8-dim group.
+__device__ __forceinline__ Fp4Places fp4_places(const Fp4RowsArgs& a, const Fp4Page& pg, int b, int64_t first, int i0, int n) {
+  Fp4Places at;
+#pragma unroll
+  for (int k = 0; k < kFp4Tokens; ++k) {
+    const int i = i0 + k * a.together;
+    at.in[k] = i < n;
+    at.i[k] = at.in[k] ? i : 0;
+    const int pos = static_cast<int>(first) + at.i[k];  // <= 2^24
+    const int p = static_cast<int>(udiv24(pos, a.bs));
+    at.slot[k] = pos - p * a.bs;
+    const int32_t page = at.in[k] && p < a.bt_stride ? a.bt[b * a.bt_stride + p] : -1;
+    at.mapped[k] = page >= 0 && page < a.n_pages;
+    at.page[k] = at.mapped[k] ? page * pg.page : 0;
+  }
+  return at;
+}
+
+// An item of a token: K or V, head, 8-dim group; its codes, its block's scale byte
+// in slot 0 of page 0, and its values' row of token 0.
 struct Fp4Item {
-  uint8_t* x;      // its values outside the pages (of token 0 past the last token)
-  uint8_t* codes;  // its word of codes
-  uint8_t* scale;  // its block's scale byte
-  int i, d0;
-  bool mapped;     // a token whose page is mapped
+  uint8_t* codes;
+  uint8_t* scale;
+  uint8_t* x;
+  int64_t tok_stride;
+  int d0;
 };
 
-__device__ __forceinline__ Fp4Item fp4_item(const Fp4RowsArgs& a, const Fp4Page& pg, int b, int64_t first, int i0, int n,
-                                            int q) {
+__device__ __forceinline__ Fp4Item fp4_item(const Fp4RowsArgs& a, const Fp4Page& pg, int b, int r) {
   Fp4Item it;
-  const int t = static_cast<int>(udiv24(q, a.items));
-  int r = q - t * a.items;
   const int kv = r >= a.items >> 1 ? 1 : 0;
   r -= kv * (a.items >> 1);
   const int groups = a.dim >> 3;
   const int head = static_cast<int>(udiv24(r, groups));
   it.d0 = (r - head * groups) * 8;
-  it.i = i0 + t;
-  const bool in = it.i < n;
-  const int pos = static_cast<int>(first) + (in ? it.i : 0);  // <= 2^24
-  const int p = static_cast<int>(udiv24(pos, a.bs));
-  const int slot = pos - p * a.bs;
-  const int32_t page = in && p < a.bt_stride ? a.bt[b * a.bt_stride + p] : -1;
-  it.mapped = page >= 0 && page < a.n_pages;
-  uint8_t* block = a.pool + (it.mapped ? page : 0) * pg.page + head * pg.head;
-  it.codes = block + (kv ? pg.v_codes : 0) + slot * (a.dim >> 1) + (it.d0 >> 1);
-  it.scale = block + pg.scales + (2 * slot + kv) * (a.dim >> 5) + (it.d0 >> 5);
-  it.x = a.x[kv] + b * a.seq_stride[kv] + (in ? it.i : 0) * a.tok_stride[kv] + head * a.head_stride[kv];
+  uint8_t* block = a.pool + head * pg.head;
+  it.codes = block + (kv ? pg.v_codes : 0) + (it.d0 >> 1);
+  it.scale = block + pg.scales + kv * (a.dim >> 5) + (it.d0 >> 5);
+  it.x = a.x[kv] + b * a.seq_stride[kv] + head * a.head_stride[kv];
+  it.tok_stride = a.tok_stride[kv];
   return it;
 }
 
@@ -74,60 +95,95 @@ __device__ __forceinline__ int fp4_new(const Fp4RowsArgs& a, int b, int64_t* fir
   return n > L || n < 0 || L > (1 << 24) ? 0 : static_cast<int>(min(n, a.rows));
 }
 
+// A thread's first item and token: of the a.together tokens that the threads take
+// at once (past them: no token).
+__device__ __forceinline__ int fp4_first(const Fp4RowsArgs& a, int* r) {
+  const int tid = threadIdx.x;
+  if (a.items >= kFp4Threads) {
+    *r = tid;
+    return 0;
+  }
+  const int t = static_cast<int>(udiv24(tid, a.items));
+  *r = tid - t * a.items;
+  return t;
+}
+
 // grid: (workgroups over a sequence's tokens, batch)
 template <bool kF32>
-__global__ __launch_bounds__(kFp4Threads) void k_fp4_quant_append(Fp4RowsArgs a, int tokens) {
+__global__ __launch_bounds__(kFp4Threads) void k_fp4_quant_append(Fp4RowsArgs a) {
   const int b = blockIdx.y;
   int64_t first;
   const int n = fp4_new(a, b, &first);
-  const int i0 = blockIdx.x * tokens;
+  const int i0 = blockIdx.x * kFp4Tokens * a.together;
   if (i0 >= n) return;  // uniform
+  int r;
+  const int t = fp4_first(a, &r);
+  if (t >= a.together) return;  // whole blocks of lanes: an item count is a multiple of 8
   const Fp4Page pg = fp4_page(a.bs, a.heads, a.dim);
-  const int end = min(tokens, n - i0) * a.items;
-  for (int q = threadIdx.x; q < end; q += kFp4Threads) {  // the four lanes of a block take the same turns
-    const Fp4Item it = fp4_item(a, pg, b, first, i0, n, q);
-    if (!it.mapped) continue;
-    float v[8];
-    if constexpr (kF32) {
-      const f32x4_t lo = *reinterpret_cast<const f32x4_t*>(it.x + it.d0 * 4);
-      const f32x4_t hi = *reinterpret_cast<const f32x4_t*>(it.x + it.d0 * 4 + 16);
+  const Fp4Places at = fp4_places(a, pg, b, first, i0 + t, n);
+  for (; r < a.items; r += kFp4Threads) {
+    const Fp4Item it = fp4_item(a, pg, b, r);
+    u32x4 raw[kFp4Tokens][kF32 ? 2 : 1];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        v[j] = lo[j];
-        v[j + 4] = hi[j];
+    for (int k = 0; k < kFp4Tokens; ++k) {
+      const uint8_t* x = it.x + at.i[k] * it.tok_stride + it.d0 * (kF32 ? 4 : 2);
+      raw[k][0] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(x));
+      if constexpr (kF32) raw[k][1] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(x + 16));
+    }
+#pragma unroll
+    for (int k = 0; k < kFp4Tokens; ++k) {
+      float v[8];
+      if constexpr (kF32) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = __uint_as_float(raw[k][j / 4][j % 4]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          v[2 * j] = __uint_as_float(raw[k][0][j] << 16);
+          v[2 * j + 1] = __uint_as_float(raw[k][0][j] & 0xffff0000u);
+        }
       }
-    } else {
-      const u32x4 w = *reinterpret_cast<const u32x4*>(it.x + it.d0 * 2);
+      uint32_t amax = 0;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        v[2 * j] = __uint_as_float(w[j] << 16);
-        v[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
+      for (int j = 0; j < 8; ++j) amax = max(amax, __float_as_uint(v[j]) & 0x7fffffffu);
+      amax = max(amax, static_cast<uint32_t>(__shfl_xor(static_cast<int>(amax), 1, 4)));
+      amax = max(amax, static_cast<uint32_t>(__shfl_xor(static_cast<int>(amax), 2, 4)));
+      const uint32_t byte = fp4_scale_byte(amax), codes = fp4_encode8(v, byte);
+      if (at.mapped[k]) {
+        *reinterpret_cast<uint32_t*>(it.codes + at.page[k] + at.slot[k] * (a.dim >> 1)) = codes;
+        if ((it.d0 & 31) == 0) it.scale[at.page[k] + at.slot[k] * (a.dim >> 4)] = static_cast<uint8_t>(byte);
       }
     }
-    uint32_t amax = 0;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) amax = max(amax, __float_as_uint(v[j]) & 0x7fffffffu);
-    amax = max(amax, static_cast<uint32_t>(__shfl_xor(static_cast<int>(amax), 1, 4)));
-    amax = max(amax, static_cast<uint32_t>(__shfl_xor(static_cast<int>(amax), 2, 4)));
-    const uint32_t byte = fp4_scale_byte(amax);
-    *reinterpret_cast<uint32_t*>(it.codes) = fp4_encode8(v, byte);
-    if ((it.d0 & 31) == 0) *it.scale = static_cast<uint8_t>(byte);
   }
 }
 
-__global__ __launch_bounds__(kFp4Threads) void k_fp4_gather(Fp4RowsArgs a, int tokens) {
+__global__ __launch_bounds__(kFp4Threads) void k_fp4_gather(Fp4RowsArgs a) {
   const int b = blockIdx.y;
   int64_t first;
   const int n = fp4_new(a, b, &first);
-  const int i0 = blockIdx.x * tokens;
+  const int i0 = blockIdx.x * kFp4Tokens * a.together;
   if (i0 >= n) return;  // uniform
+  int r;
+  const int t = fp4_first(a, &r);
+  if (t >= a.together) return;
   const Fp4Page pg = fp4_page(a.bs, a.heads, a.dim);
-  const int end = min(tokens, n - i0) * a.items;
-  for (int q = threadIdx.x; q < end; q += kFp4Threads) {
-    const Fp4Item it = fp4_item(a, pg, b, first, i0, n, q);
-    const uint32_t codes = *reinterpret_cast<const uint32_t*>(it.codes);
-    const u32x4 v = fp4_decode8(codes, fp4_scale(*it.scale));
-    *reinterpret_cast<u32x4*>(it.x + it.d0 * 2) = it.mapped ? v : u32x4{0u, 0u, 0u, 0u};
+  const Fp4Places at = fp4_places(a, pg, b, first, i0 + t, n);
+  for (; r < a.items; r += kFp4Threads) {
+    const Fp4Item it = fp4_item(a, pg, b, r);
+    uint32_t codes[kFp4Tokens], byte[kFp4Tokens];
+#pragma unroll
+    for (int k = 0; k < kFp4Tokens; ++k) {
+      codes[k] = *reinterpret_cast<const uint32_t*>(it.codes + at.page[k] + at.slot[k] * (a.dim >> 1));
+      byte[k] = it.scale[at.page[k] + at.slot[k] * (a.dim >> 4)];
+    }
+#pragma unroll
+    for (int k = 0; k < kFp4Tokens; ++k) {
+      const u32x4 v = fp4_decode8(codes[k], fp4_scale(byte[k]));
+      if (at.in[k]) {
+        u32x4* x = reinterpret_cast<u32x4*>(it.x + at.i[k] * it.tok_stride + it.d0 * 2);
+        __builtin_nontemporal_store(at.mapped[k] ? v : u32x4{0u, 0u, 0u, 0u}, x);
+      }
+    }
   }
 }
 
@@ -162,6 +218,7 @@ int fp4_rows_args(Fp4RowsArgs& a, const char* what, const skv_fp4_cache* c, cons
   a.heads = static_cast<int>(c->n_kv_heads);
   a.dim = static_cast<int>(c->head_dim);
   a.items = 2 * a.heads * (a.dim / 8);
+  a.together = std::max(1, kFp4Threads / a.items);
   return SKV_OK;
 }
 
@@ -185,13 +242,12 @@ extern "C" int skv_fp4_quant_append(const skv_fp4_cache* cache, const int32_t* s
   Fp4RowsArgs a{};
   if (const int rc = fp4_rows_args(a, what, cache, seq_lens, n_new, n_new_uniform, k, v, src_len)) return rc;
   if (cache->batch == 0 || src_len == 0) return SKV_OK;
-  const int tokens = static_cast<int>(std::max(1, 1024 / a.items));
-  const dim3 grid(static_cast<unsigned>(ceil_div(src_len, tokens)), static_cast<unsigned>(cache->batch));
+  const dim3 grid(static_cast<unsigned>(ceil_div(src_len, kFp4Tokens * a.together)), static_cast<unsigned>(cache->batch));
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (src_f32) {
-    hipLaunchKernelGGL((k_fp4_quant_append<true>), grid, dim3(kFp4Threads), 0, s, a, tokens);
+    hipLaunchKernelGGL((k_fp4_quant_append<true>), grid, dim3(kFp4Threads), 0, s, a);
   } else {
-    hipLaunchKernelGGL((k_fp4_quant_append<false>), grid, dim3(kFp4Threads), 0, s, a, tokens);
+    hipLaunchKernelGGL((k_fp4_quant_append<false>), grid, dim3(kFp4Threads), 0, s, a);
   }
   return check_launch(what);
 }
@@ -203,8 +259,7 @@ extern "C" int skv_fp4_gather(const skv_fp4_cache* cache, const int32_t* seq_len
   Fp4RowsArgs a{};
   if (const int rc = fp4_rows_args(a, what, cache, seq_lens, n_rows, n_rows_uniform, k, v, dst_len)) return rc;
   if (cache->batch == 0 || dst_len == 0) return SKV_OK;
-  const int tokens = static_cast<int>(std::max(1, 1024 / a.items));
-  const dim3 grid(static_cast<unsigned>(ceil_div(dst_len, tokens)), static_cast<unsigned>(cache->batch));
-  hipLaunchKernelGGL(k_fp4_gather, grid, dim3(kFp4Threads), 0, static_cast<hipStream_t>(stream), a, tokens);
+  const dim3 grid(static_cast<unsigned>(ceil_div(dst_len, kFp4Tokens * a.together)), static_cast<unsigned>(cache->batch));
+  hipLaunchKernelGGL(k_fp4_gather, grid, dim3(kFp4Threads), 0, static_cast<hipStream_t>(stream), a);
   return check_launch(what);
 }
