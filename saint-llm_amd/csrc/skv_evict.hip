@@ -89,46 +89,68 @@ __global__ __launch_bounds__(kEvictThreads) void k_release(
   }
 }
 
-// k_release over shared pages (refs[p]: holders beyond the first).  Positions u of
-// the released pages in push order (ascending b, within b from the last logical
-// page) are dealt to the threads in runs.  A page whose holders all leave drops to
-// -1; the largest u among its releases, found by a minimum over -2 - u in the
-// count itself, pushes it, so that the stack does not depend on the order in
-// which the atomics run.
+// k_release over shared pages (refs[p]: holders beyond the first).  Push order is
+// ascending b, within b from the last logical page; a wave takes 64 entries of one
+// sequence's table at a time (a unit) and sends kReleaseAhead of them out together,
+// which is what this launch's time, a few dependent memory latencies a step, asks for.
+// A page whose holders all leave drops to -1; the last place u among its releases,
+// found by a minimum over -2 - u in the count itself, pushes it, so that the stack
+// does not depend on the order in which the atomics run.
+constexpr int kReleaseAhead = 8;
+
 __global__ __launch_bounds__(kEvictThreads) void k_release_shared(
     int32_t* __restrict__ stack, int32_t* __restrict__ top_ptr, int64_t n_pages, int32_t* refs, int32_t* bt,
     int64_t bt_stride, int32_t* __restrict__ lens, const uint8_t* __restrict__ mask, int batch, int bs,
     int32_t* __restrict__ status) {
-  __shared__ int off[kEvictMaxBatch + 1];
-  __shared__ int cnt[kEvictMaxBatch];
+  __shared__ int off[kEvictMaxBatch + 1];  // units before each sequence
+  __shared__ int cnt[kEvictMaxBatch];      // its pages
   __shared__ int scan_lds[17];
   __shared__ int bad_all;
-  const int tid = threadIdx.x;
+  const int tid = threadIdx.x, lane = tid % kWave;
+  const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
   if (tid == 0) bad_all = 0;
-  int carry = 0;
+  int units = 0;
   for (int base = 0; base < batch; base += kEvictThreads) {
     const int b = base + tid;
     int c = 0;
     if (b < batch && mask[b]) c = static_cast<int>(min<int64_t>(ceil_div(max(lens[b], 0), bs), bt_stride));
     int tot;
-    const int ex = block_exclusive_scan(c, scan_lds, &tot);
+    const int ex = block_exclusive_scan((c + kWave - 1) / kWave, scan_lds, &tot);
     if (b < batch) {
-      off[b] = carry + ex;
+      off[b] = units + ex;
       cnt[b] = c;
     }
-    carry += tot;
+    units += tot;
   }
-  if (tid == 0) off[batch] = carry;
+  if (tid == 0) off[batch] = units;
   __syncthreads();
   const int top = *top_ptr;
-  const int per = (carry + kEvictThreads - 1) / kEvictThreads;
-  const int u0 = min(tid * per, carry), u1 = min(u0 + per, carry);
-  // f(u, page) for the thread's run of positions
-  const auto each = [&](auto&& f) {
-    int b = u0 < u1 ? owner_of(off, batch, u0) : 0;
-    for (int u = u0; u < u1; ++u) {
-      while (u >= off[b + 1]) ++b;
-      f(u, bt[static_cast<int64_t>(b) * bt_stride + (cnt[b] - 1 - (u - off[b]))]);
+  constexpr int kStep = kEvictThreads / kWave * kReleaseAhead;
+  // f(places u, table entries, page ids) for every step's kReleaseAhead entries of the
+  // thread; no entry: u < 0.  All threads take the same steps.
+  const auto steps = [&](auto&& f) {
+    for (int base = 0; base < units; base += kStep) {
+      const int first = base + wave * kReleaseAhead;
+      int b = first < units ? owner_of(off, batch, first) : 0;
+      int u[kReleaseAhead];
+      int32_t* entry[kReleaseAhead];
+      int32_t page[kReleaseAhead];
+#pragma unroll
+      for (int k = 0; k < kReleaseAhead; ++k) {
+        u[k] = -1;
+        entry[k] = bt;
+        if (first + k < units) {  // uniform
+          while (first + k >= off[b + 1]) ++b;
+          const int j = (first + k - off[b]) * kWave + lane;
+          if (j < cnt[b]) {
+            u[k] = (first + k) * kWave + lane;
+            entry[k] = bt + static_cast<int64_t>(b) * bt_stride + (cnt[b] - 1 - j);
+          }
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < kReleaseAhead; ++k) page[k] = *entry[k];
+      f(u, entry, page);
     }
   };
   const auto refuse = [&](int bad) {  // the whole workgroup's answer
@@ -137,45 +159,75 @@ __global__ __launch_bounds__(kEvictThreads) void k_release_shared(
     if (bad_all && tid == 0 && status) *status = bad_all;
     return bad_all != 0;
   };
+  const auto known = [&](int32_t page) { return page >= 0 && page < n_pages; };
   int bad = (top < 0 || top > n_pages) ? SKV_STATUS_STACK : 0;
-  each([&](int, int32_t page) {
-    if (page < 0 || page >= n_pages) bad = SKV_STATUS_BADARG;
-  });
-  if (refuse(bad)) return;
   int freed = 0;
-  each([&](int, int32_t page) {
-    const int was = atomicSub(&refs[page], 1);
-    freed += was == 0 ? 1 : 0;
-    if (was < 0) bad = SKV_STATUS_BADARG;
+  steps([&](const int* u, int32_t* const*, const int32_t* page) {
+    int was[kReleaseAhead];
+#pragma unroll
+    for (int k = 0; k < kReleaseAhead; ++k) {
+      was[k] = 1;
+      if (u[k] < 0) continue;
+      if (known(page[k])) was[k] = atomicSub(&refs[page[k]], 1); else bad = SKV_STATUS_BADARG;
+    }
+#pragma unroll
+    for (int k = 0; k < kReleaseAhead; ++k) {
+      freed += was[k] == 0 ? 1 : 0;
+      if (was[k] < 0) bad = SKV_STATUS_BADARG;
+    }
   });
   const int pushes = block_reduce_sum(freed, scan_lds);
   if (static_cast<int64_t>(top) + pushes > n_pages) bad |= SKV_STATUS_STACK;
-  if (refuse(bad)) {
-    each([&](int, int32_t page) { atomicAdd(&refs[page], 1); });
+  if (refuse(bad)) {  // the counts as they were
+    steps([&](const int* u, int32_t* const*, const int32_t* page) {
+#pragma unroll
+      for (int k = 0; k < kReleaseAhead; ++k) {
+        if (u[k] >= 0 && known(page[k])) atomicAdd(&refs[page[k]], 1);
+      }
+    });
     return;
   }
-  const auto count_of = [&](int32_t page) {  // past the L1 cache, which holds what it was
-    return __hip_atomic_load(&refs[page], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  // past the L1 cache, which may hold what a count was
+  const auto counts = [&](const int* u, const int32_t* page, int* count) {
+#pragma unroll
+    for (int k = 0; k < kReleaseAhead; ++k) {
+      count[k] = u[k] < 0 ? 0 : __hip_atomic_load(&refs[page[k]], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
   };
-  each([&](int u, int32_t page) {
-    if (count_of(page) < 0) atomicMin(&refs[page], -2 - u);
-  });
-  __syncthreads();
-  int mine = 0;
-  each([&](int u, int32_t page) { mine += count_of(page) == -2 - u ? 1 : 0; });
-  int tot;
-  int at = top + block_exclusive_scan(mine, scan_lds, &tot);
-  each([&](int u, int32_t page) {
-    if (count_of(page) == -2 - u) {
-      stack[at++] = page;
-      atomicExch(&refs[page], 0);
+  steps([&](const int* u, int32_t* const*, const int32_t* page) {
+    int count[kReleaseAhead];
+    counts(u, page, count);
+#pragma unroll
+    for (int k = 0; k < kReleaseAhead; ++k) {
+      if (count[k] < 0) atomicMin(&refs[page[k]], -2 - u[k]);
     }
   });
-  __syncthreads();  // every page id is read before the tables are cleared
-  for (int t = tid; t < carry; t += kEvictThreads) {
-    const int b = owner_of(off, batch, t);
-    bt[static_cast<int64_t>(b) * bt_stride + (t - off[b])] = -1;
-  }
+  __syncthreads();
+  int at = top;
+  steps([&](const int* u, int32_t* const* entry, const int32_t* page) {
+    int count[kReleaseAhead];
+    counts(u, page, count);
+    uint64_t push[kReleaseAhead];
+    int mine = 0;  // the wave's
+#pragma unroll
+    for (int k = 0; k < kReleaseAhead; ++k) {
+      push[k] = __ballot(u[k] >= 0 && count[k] == -2 - u[k]);
+      mine += __popcll(push[k]);
+    }
+    int tot;
+    const int ex = block_exclusive_scan(lane == 0 ? mine : 0, scan_lds, &tot);
+    int to = at + __builtin_amdgcn_readfirstlane(ex);
+#pragma unroll
+    for (int k = 0; k < kReleaseAhead; ++k) {
+      if ((push[k] >> lane) & 1) {
+        stack[to + __popcll(push[k] & ((uint64_t{1} << lane) - 1))] = page[k];
+        atomicExch(&refs[page[k]], 0);
+      }
+      to += __popcll(push[k]);
+      if (u[k] >= 0) *entry[k] = -1;  // read by this thread alone
+    }
+    at += tot;
+  });
   for (int b = tid; b < batch; b += kEvictThreads) {
     if (mask[b]) lens[b] = 0;
   }
@@ -494,7 +546,7 @@ extern "C" int skv_release_shared(int32_t* free_stack, int32_t* free_top, int64_
     return set_error(SKV_EINVAL, "%s: batch must be in [0, %d]; got %lld", what, kEvictMaxBatch, (long long)batch);
   }
   if (block_size <= 0 || block_size > INT32_MAX || bt_stride <= 0 || n_pages <= 0 || n_pages > INT32_MAX ||
-      batch * bt_stride > INT32_MAX - kEvictThreads) {
+      batch * (bt_stride + kWave) > INT32_MAX - kEvictThreads) {
     return set_error(SKV_EINVAL, "%s: bad block_size/bt_stride/n_pages", what);
   }
   if (!free_stack || !free_top || !refs || (batch > 0 && (!block_table || !seq_lens || !release_mask))) {
