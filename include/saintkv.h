@@ -478,27 +478,33 @@ int skv_fp4_gather(const skv_fp4_cache* cache, const int32_t* seq_lens, const in
                    int32_t n_rows_uniform, const skv_fp4_rows* k, const skv_fp4_rows* v, int64_t dst_len,
                    void* stream);
 
-/* Attention of the newest n_queries tokens of each sequence over its 4-bit
- * pages: token t of sequence b is position p = seq_lens[b] - n_queries + t and
- * sees positions [max(0, p - window + 1), p] (window 0: from 0); n_heads query
- * heads, n_heads / n_kv_heads of them to a K/V head (head h reads K/V head
+/* Attention of each sequence's newest tokens over its 4-bit pages: of the
+ * n_queries tokens in q the first n_new[b] (n_new NULL: all) are sequence b's;
+ * token t is position p = seq_lens[b] - n_new[b] + t and sees positions
+ * [max(0, p - window + 1), p] (window 0: from 0); n_heads query heads,
+ * n_heads / n_kv_heads of them to a K/V head (head h reads K/V head
  * h / (n_heads / n_kv_heads)):
  *   s_j = scale * q . k_j            (scale 0: 1 / sqrt(head_dim))
  *   s_j = softcap * tanh(s_j / softcap)                (softcap > 0)
  *   out = sum_j exp(s_j) v_j / (sum_j exp(s_j) + exp(sink[h]))   (sink optional)
- * A token that sees nothing (or only unmapped pages) gets 0; a NaN block makes
- * NaN the outputs of the tokens that see it, and of no other.  q: bf16, token t, head h of
- * sequence b at q + b*q_seq_stride + t*q_tok_stride + h*q_head_stride (bytes,
- * multiples of 16); out: bf16 [batch, n_queries, n_heads, head_dim].  max_len
- * bounds the lengths for the split of long sequences over workgroups (0: what
- * the table holds; longer sequences are still right).  splits 0: chosen by the
- * library.  skv_fp4_attention_workspace returns the bytes that a call needs
+ * A token that sees nothing (or only unmapped pages), or is past n_new[b], gets
+ * 0; a NaN block makes NaN the outputs of the tokens that see it, and of no
+ * other, as do a NaN or an infinity in q those of their token and head.  q: bf16, token t, head h of sequence b at q + b*q_seq_stride +
+ * t*q_tok_stride + h*q_head_stride (bytes, multiples of 16); out: bf16 [batch,
+ * n_queries, n_heads, head_dim].  Long sequences are cut into runs of about equal
+ * length for as many workgroups as the device holds, and joined by a second
+ * launch.  max_len bounds the lengths (0: what the table holds; longer ones are
+ * still right): where it, or the window, shows that no sequence is worth cutting,
+ * the call is one launch and needs no workspace.  splits > 0: that many runs per
+ * K/V head and row block on average, whatever the lengths (0: the library's
+ * choice).  skv_fp4_attention_workspace returns the bytes that a call needs
  * (16-byte aligned; -1: bad descriptor).  The generalisation of the window
  * branch of SWAttention.forward (swa.py:115-137) to several K/V heads and the
  * whole history. */
 typedef struct skv_fp4_attention_desc {
   skv_fp4_cache cache;
   const int32_t* seq_lens;
+  const int32_t* n_new; /* [batch] or NULL */
   int64_t n_queries, n_heads;
   const void* q;
   int64_t q_seq_stride, q_tok_stride, q_head_stride;

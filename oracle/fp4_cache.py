@@ -97,15 +97,17 @@ def rows(pool: np.ndarray, block_table: np.ndarray, b: int, positions: range) ->
 
 
 def attention(q: np.ndarray, pool: np.ndarray, block_table: np.ndarray, seq_lens: np.ndarray, window: int | None = None,
-              sink: np.ndarray | None = None, softcap: float | None = None, scale: float | None = None) -> np.ndarray:
-    """q [B, T, H, D] over the pages, one (token, head) at a time."""
+              sink: np.ndarray | None = None, softcap: float | None = None, scale: float | None = None,
+              n_new: np.ndarray | None = None) -> np.ndarray:
+    """q [B, T, H, D] over the pages, one (token, head) at a time; of sequence b the first n_new[b] tokens."""
     batch, t_new, heads, dim = q.shape
     out = np.zeros(q.shape)
     for b in range(batch):
         length = int(seq_lens[b])
         k, v, mapped = rows(pool, block_table, b, range(length))
-        for t in range(t_new):
-            end = length - t_new + t + 1
+        own = t_new if n_new is None else min(int(n_new[b]), t_new)
+        for t in range(own):
+            end = length - own + t + 1
             begin = max(0, end - window) if window else 0
             live = np.flatnonzero(mapped[begin:max(end, 0)]) + begin if end > 0 else np.zeros(0, dtype=np.int64)
             if live.size == 0:

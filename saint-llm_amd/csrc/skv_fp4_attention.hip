@@ -31,6 +31,7 @@
 // runs out for itself from their prefix sum.  A cut item's pieces are joined by a
 // second launch.
 #include <algorithm>
+#include <cmath>
 
 #include "skv_fp4.h"
 
@@ -63,6 +64,7 @@ struct Fp4AttnArgs {
   uint16_t* out;  // [B, T, H, D] bf16
   float* part;    // of chunk parts: (m, l) of every row, then the rows' outputs
   const int32_t* lens;
+  const int32_t* n_new;  // each sequence's tokens of the T in q, or null: all
   const uint8_t* pool;
   const int32_t* bt;
   const float* sink;
@@ -77,7 +79,7 @@ struct Fp4AttnArgs {
 
 // The positions that the rows [r0, r0 + n) of a K/V head see.
 struct Fp4Span {
-  int L, r_end;          // tokens of the sequence; rows of the head
+  int L, T, r_end;       // tokens of the sequence, and new ones among them; rows of the head
   int first, last;       // [first, last): some row sees them
   int all_lo, all_hi;    // [all_lo, all_hi): every row sees them
   int tile0, tiles;
@@ -87,11 +89,13 @@ struct Fp4Span {
 __device__ __forceinline__ Fp4Span fp4_span(const Fp4AttnArgs& a, int b, int r0, int n) {
   Fp4Span s;
   s.L = min(max(a.lens[b], 0), a.bt_stride * a.bs);
+  s.T = a.n_new ? min(max(a.n_new[b], 0), a.T) : a.T;
   s.r_end = a.T * a.G;
-  const int r1 = min(r0 + n, s.r_end) - 1;
-  const int end0 = s.L - a.T + r0 / a.G + 1, end1 = s.L - a.T + r1 / a.G + 1;  // one past the last position seen
-  s.last = max(end1, 0);
-  s.all_hi = end0;
+  const int t0 = r0 / a.G, t1 = (min(r0 + n, s.r_end) - 1) / a.G;
+  // one past the last position seen
+  const int end0 = s.L - s.T + t0 + 1, end1 = s.L - s.T + min(t1, s.T - 1) + 1;
+  s.last = t0 < s.T ? max(end1, 0) : 0;
+  s.all_hi = t1 < s.T ? end0 : 0;  // a row past the new tokens sees none
   s.first = a.window > 0 ? max(end0 - a.window, 0) : 0;
   s.all_lo = a.window > 0 ? end1 - a.window : 0;
   s.tile0 = s.first / kF4Tile;
@@ -227,7 +231,7 @@ struct Fp4Wave {
       const int r = r0 + 16 * mt + col;
       const bool in = r < sp.r_end;
       const int t = in ? r / a.G : 0, g = in ? r - t * a.G : 0;
-      hi[mt] = in ? sp.L - a.T + t + 1 : 0;
+      hi[mt] = in && t < sp.T ? sp.L - sp.T + t + 1 : 0;
       lo[mt] = a.window > 0 ? hi[mt] - a.window : 0;
       const uint8_t* row = a.q + b * a.q_seq + t * a.q_tok + (hk * a.G + g) * a.q_head;
 #pragma unroll
@@ -266,6 +270,7 @@ struct Fp4Wave {
       e4m3fn_x4_to_f32(hi[j], h);
       lo[j] = e4m3fn_pack2<true>((v[2] - h[2]) * 32.f, (v[3] - h[3]) * 32.f,
                                  e4m3fn_pack2<false>((v[0] - h[0]) * 32.f, (v[1] - h[1]) * 32.f, 0u));
+      if (big >= 0x7f800000u) hi[j] = 0x7f7f7f7fu;  // an infinity or a NaN: NaN scores
     }
     return static_cast<uint32_t>(byte);
   }
@@ -1015,6 +1020,11 @@ int fp4_attn_plan(const skv_fp4_attention_desc* d, Fp4AttnPlan& p) {
   if (!(d->scale >= 0.f) || d->scale > 3e38f || !(d->softcap >= 0.f) || d->softcap > 3e38f) {
     return set_error(SKV_EINVAL, "%s: scale and softcap must be finite and >= 0", what);
   }
+  const float scale = d->scale > 0.f ? d->scale : 1.f / sqrtf(static_cast<float>(d->cache.head_dim));
+  if (!std::isfinite(scale * kF4Log2e) || !std::isfinite(d->softcap * kF4Log2e) ||
+      (d->softcap > 0.f && !std::isfinite(2.f * kF4Log2e * scale / d->softcap))) {
+    return set_error(SKV_EINVAL, "%s: scale, softcap and scale / softcap must leave fp32 room for a factor of 3", what);
+  }
   const int64_t D = d->cache.head_dim, rows = d->n_queries * (d->n_heads / hkv);
   p.dims = D <= 64 ? 64 : D <= 128 ? 128 : D <= 256 ? 256 : 512;
   // A wave's tiles are its own, or all four waves' with rows of their own for each, once
@@ -1095,6 +1105,7 @@ extern "C" int skv_fp4_attention(const skv_fp4_attention_desc* d, void* workspac
   a.q_head = d->q_head_stride;
   a.out = static_cast<uint16_t*>(d->out);
   a.lens = d->seq_lens;
+  a.n_new = d->n_new;
   a.pool = static_cast<const uint8_t*>(d->cache.pool);
   a.bt = d->cache.block_table;
   a.sink = d->sink;

@@ -33,7 +33,7 @@ class Fp4AttentionDesc(ctypes.Structure):
     """Mirror of skv_fp4_attention_desc (include/saintkv.h)."""
 
     _fields_ = [
-        ("cache", _lib.Fp4Cache), ("seq_lens", _P), ("n_queries", _I64), ("n_heads", _I64),
+        ("cache", _lib.Fp4Cache), ("seq_lens", _P), ("n_new", _P), ("n_queries", _I64), ("n_heads", _I64),
         ("q", _P), ("q_seq_stride", _I64), ("q_tok_stride", _I64), ("q_head_stride", _I64),
         ("out", _P), ("sink", _P), ("window", _I64), ("max_len", _I64), ("splits", _I64),
         ("scale", ctypes.c_float), ("softcap", ctypes.c_float),
@@ -54,9 +54,9 @@ def _check_layout() -> None:
 
 
 def fp4_attention(q: torch.Tensor, pool: torch.Tensor, block_table: torch.Tensor, seq_lens: torch.Tensor, *,
-                  window: int | None = None, sink: torch.Tensor | None = None, softcap: float | None = None,
-                  scale: float | None = None, max_len: int = 0, splits: int = 0, out: torch.Tensor | None = None,
-                  workspace: torch.Tensor | None = None) -> torch.Tensor:
+                  n_new: torch.Tensor | None = None, window: int | None = None, sink: torch.Tensor | None = None,
+                  softcap: float | None = None, scale: float | None = None, max_len: int = 0, splits: int = 0,
+                  out: torch.Tensor | None = None, workspace: torch.Tensor | None = None) -> torch.Tensor:
     """Attention of each sequence's newest tokens over its 4-bit pages, bf16 of
     q's shape.
 
@@ -64,15 +64,19 @@ def fp4_attention(q: torch.Tensor, pool: torch.Tensor, block_table: torch.Tensor
     the call: token t is position seq_lens - T + t and sees the positions up to
     itself), roped and normed, of any strides that keep its rows 16-byte aligned;
     H a multiple of the pool's K/V heads (head h reads K/V head h // (H / Hkv)).
-    pool, block_table: as ``ops.fp4_quant_append`` wrote them; seq_lens: int32
-    [B].  window: only the newest ``window`` positions up to itself (None: all);
-    sink: fp32 [H] or None; softcap: c*tanh(s/c) of the scores, or None; scale: of
-    the scores (None: 1/sqrt(D)).  A token that sees nothing gets 0.  max_len: a
-    bound on seq_lens, by which long sequences are split over workgroups (0:
-    what the table holds); splits: 0, or that many parts of every sequence.
+    n_new: int32 [B], of a padded batch: the first n_new[b] tokens of q are
+    sequence b's newest, token t at position seq_lens - n_new + t, and later ones
+    get 0.  pool, block_table: as ``ops.fp4_quant_append`` wrote them; seq_lens:
+    int32 [B].  window: only the newest ``window`` positions up to itself (None:
+    all); sink: fp32 [H] or None; softcap: c*tanh(s/c) of the scores, or None;
+    scale: of the scores (None: 1/sqrt(D)).  A token that sees nothing gets 0.
+    max_len: a bound on seq_lens (0: what the table holds; longer ones are still
+    right), which saves short sequences the launch that joins parts of long ones;
+    splits: about that many workgroups for a K/V head of every sequence, instead
+    of as many as the device holds (0).
     workspace: a tensor of at least ``fp4_attention_workspace`` bytes (None: one
     is allocated for the call)."""
-    d, out = _desc(q, pool, block_table, seq_lens, window, sink, softcap, scale, max_len, splits, out)
+    d, out = _desc(q, pool, block_table, seq_lens, n_new, window, sink, softcap, scale, max_len, splits, out)
     need = int(_lib.load().skv_fp4_attention_workspace(ctypes.byref(d)))
     if need < 0:
         _lib.check(_lib.SKV_EINVAL, "skv_fp4_attention_workspace")
@@ -97,14 +101,14 @@ def fp4_attention_workspace(q: torch.Tensor, pool: torch.Tensor, block_table: to
                             window: int | None = None, max_len: int = 0, splits: int = 0) -> int:
     """Bytes of workspace that ``fp4_attention`` needs for these shapes (0: none)."""
     lens = torch.empty(q.shape[0], dtype=torch.int32, device=q.device)
-    d, _ = _desc(q, pool, block_table, lens, window, None, None, None, max_len, splits, None)
+    d, _ = _desc(q, pool, block_table, lens, None, window, None, None, None, max_len, splits, None)
     need = int(_lib.load().skv_fp4_attention_workspace(ctypes.byref(d)))
     if need < 0:
         _lib.check(_lib.SKV_EINVAL, "skv_fp4_attention_workspace")
     return need
 
 
-def _desc(q, pool, block_table, seq_lens, window, sink, softcap, scale, max_len, splits,
+def _desc(q, pool, block_table, seq_lens, n_new, window, sink, softcap, scale, max_len, splits,
           out) -> tuple[Fp4AttentionDesc, torch.Tensor]:
     _check_layout()
     _require_gpu(q, "q")
@@ -117,6 +121,8 @@ def _desc(q, pool, block_table, seq_lens, window, sink, softcap, scale, max_len,
     if heads < 1 or heads % cache.n_kv_heads:
         raise ValueError(f"q's {heads} heads are not a multiple of the pool's {cache.n_kv_heads}")
     _require_i32(seq_lens, "seq_lens", (batch,))
+    if n_new is not None:
+        _require_i32(n_new, "n_new", (batch,))
     if window is not None and window < 1:
         raise ValueError(f"window must be positive (or None); got {window}")
     if softcap is not None and not softcap > 0:
@@ -135,8 +141,8 @@ def _desc(q, pool, block_table, seq_lens, window, sink, softcap, scale, max_len,
         out = torch.empty(q.shape, dtype=torch.bfloat16, device=q.device)
     elif out.dtype != torch.bfloat16 or out.shape != q.shape or not out.is_contiguous() or out.data_ptr() % 16:
         raise ValueError(f"out must be a contiguous bf16 {list(q.shape)} tensor, 16-byte aligned")
-    _same_device(q, "q", pool=pool, seq_lens=seq_lens, sink=sink, out=out)
-    d = Fp4AttentionDesc(cache, seq_lens.data_ptr(), q4.shape[1], heads, q.data_ptr(), *strides, out.data_ptr(),
+    _same_device(q, "q", pool=pool, seq_lens=seq_lens, n_new=n_new, sink=sink, out=out)
+    d = Fp4AttentionDesc(cache, seq_lens.data_ptr(), _lib.ptr(n_new), q4.shape[1], heads, q.data_ptr(), *strides, out.data_ptr(),
                          _lib.ptr(sink), window or 0, int(max_len), int(splits), scale or 0.0, softcap or 0.0)
     return d, out
 
@@ -154,9 +160,9 @@ class Fp4TokenCache:
             out = cache.attention(i, q)          # bf16 [B, T, H, D]
 
     A prompt goes the same way with its tokens (``n_new`` per sequence where
-    they are ragged).  Capacity (``max_len``) is checked on the host, the pool's
-    pages on the device: ``check_status()`` raises where a reservation found too
-    few.
+    they are ragged).  Lengths and free pages are counted on the host, so that a
+    reservation or a fork that cannot be raises before it changes anything; steps
+    and forks need no synchronisation, a release reads back what it freed.
     """
 
     def __init__(self, layers: int, batch: int, max_len: int, n_kv_heads: int, head_dim: int, *, block_size: int = 64,
@@ -187,7 +193,7 @@ class Fp4TokenCache:
                                     device=dev)
         ops.free_stack_init(self.free_stack, self.free_top, order)
         self.status = torch.zeros(1, **i32)
-        self.host_lens = np.zeros(batch, dtype=np.int64)
+        self.host_lens, self.host_free = np.zeros(batch, dtype=np.int64), self.n_pages
         self._n_new: int | torch.Tensor = 0
         self._compact_ws = torch.zeros(3 * self.n_pages, **i32)
         self._compact_info = torch.zeros(2, **i32)
@@ -201,11 +207,19 @@ class Fp4TokenCache:
             raise ValueError("n_new must be >= 0")
         if (self.host_lens + counts > self.max_len).any():
             raise RuntimeError(f"Fp4TokenCache overflow: a sequence would exceed max_len={self.max_len}")
+        bs = self.block_size
+        need = int(((self.host_lens + counts + bs - 1) // bs - (self.host_lens + bs - 1) // bs).sum())
+        self._take_pages(need)
         self._n_new = int(n_new) if np.ndim(n_new) == 0 else torch.as_tensor(counts.astype(np.int32),
                                                                             device=self.device)
         ops.reserve(self.free_stack, self.free_top, self.block_table, self.seq_lens, self._n_new, self.block_size,
                     self.status)
         self.host_lens = self.host_lens + counts
+
+    def _take_pages(self, need: int) -> None:
+        if need > self.host_free:
+            raise RuntimeError(f"Fp4TokenCache out of pages: {need} needed, {self.host_free} free")
+        self.host_free -= need
 
     def append(self, i: int, k: torch.Tensor, v: torch.Tensor) -> None:
         """Layer i's keys and values [B, T, Hkv, D] of the tokens reserved last
@@ -215,16 +229,21 @@ class Fp4TokenCache:
     def attention(self, i: int, q: torch.Tensor, *, window: int | None = None, sink: torch.Tensor | None = None,
                   softcap: float | None = None, scale: float | None = None,
                   out: torch.Tensor | None = None) -> torch.Tensor:
-        """``fp4_attention`` of layer i for the newest tokens' queries."""
-        return fp4_attention(q, self.pool[i], self.block_table, self.seq_lens, window=window, sink=sink,
+        """``fp4_attention`` of layer i for the queries of the newest tokens; after a
+        ragged reservation of sequence b's first n_new[b] (the others get 0)."""
+        n_new = self._n_new if isinstance(self._n_new, torch.Tensor) else None
+        return fp4_attention(q, self.pool[i], self.block_table, self.seq_lens, n_new=n_new, window=window, sink=sink,
                              softcap=softcap, scale=scale, max_len=int(self.host_lens.max()), out=out)
 
     def check_status(self) -> None:
-        """Synchronise and raise if the last reservation, fork or release was refused
-        (it changed nothing; the host's lengths are read back)."""
+        """Synchronise and raise if the device refused the last reservation, fork or
+        release, as it does where the tables were changed behind the host's back (it
+        wrote nothing; the host's counts are read back)."""
         st = int(self.status.item())
         if st:
+            self.status.zero_()
             self.host_lens = self.seq_lens.cpu().numpy().astype(np.int64)
+            self.host_free = int(self.free_top.item())
             raise RuntimeError(f"Fp4TokenCache reservation, fork or release refused (status bits {st})")
 
     # ------------------------------------------------------ forks, eviction --
@@ -232,10 +251,10 @@ class Fp4TokenCache:
         """Make the empty sequences dst[f] copies of src[f], sharing their whole
         pages; raises (and changes nothing) if the pool lacks a page for a begun one."""
         src, dst = check_forks(src, dst, self.host_lens)
+        self._take_pages(int((self.host_lens[src] % self.block_size != 0).sum()))
         idx = torch.as_tensor(np.stack([src, dst]).astype(np.int32), device=self.device)
         ops.fork(self.free_stack, self.free_top, self.refs, self.block_table, self.seq_lens, idx[0], idx[1],
                  self.block_size, self.pool, self.status)
-        self.check_status()
         self.host_lens[dst] = self.host_lens[src]
 
     def release(self, mask: np.ndarray) -> None:
@@ -251,6 +270,7 @@ class Fp4TokenCache:
                     refs=self.refs)
         self.check_status()
         self.host_lens[mask] = 0
+        self.host_free = int(self.free_top.item())
 
     def compact(self) -> tuple[int, int]:
         """Defragment the pages; returns (n_live, n_moved)."""
