@@ -74,6 +74,7 @@ struct Fp4AttnArgs {
   float scale, softcap;
   int32_t row_blocks;
   int32_t* sched;   // for the join: [items + 1] tiles before every (sequence, row block), and `small`
+  int32_t lead;     // kF4Lead, or 0
   int32_t max_groups, small;  // see fp4_groups; items of at most `small` tiles are not cut
 };
 
@@ -108,14 +109,22 @@ __device__ __forceinline__ Fp4Span fp4_span(const Fp4AttnArgs& a, int b, int r0,
 // the first total mod n one more.
 constexpr int kF4RunTiles = 8;
 constexpr int kF4SmallTiles = 16;
+// What a segment costs beside its tiles, in tiles: the first loads' latencies and the
+// waves' join.  A step of 64 sequences of 1k - 32k, 8 K/V heads: 168 us without it (runs end
+// between 81 and 159 us), with 12, 16 and 20 tiles 146, 142 and 141 us.  Counted where there are about as many items
+// as workgroups or more; a run that would begin in this lead or just past it begins with the item.
+constexpr int kF4Lead = 20;
 // No (sequence, row block, head) is cut where a workgroup for each leaves less than an
 // eighth of the chip's time unused: there is nothing to join then.
 constexpr int kF4Idle = 8;
 constexpr int kF4MaxItems = 2048;  // (sequence, row block)s whose prefix sum LDS holds
 
 __device__ __forceinline__ int fp4_groups(const Fp4AttnArgs& a, int total) {
-  return min(a.max_groups, max((total + kF4RunTiles - 1) / kF4RunTiles, a.B * a.row_blocks * a.Hkv));
+  const int units = a.B * a.row_blocks * a.Hkv;
+  return min(a.max_groups, max((total - units * a.lead + kF4RunTiles - 1) / kF4RunTiles, units));
 }
+// A run that begins at most so far into an item begins with it.
+__device__ __forceinline__ int fp4_early(const Fp4AttnArgs& a) { return a.lead ? a.lead + kF4Waves : 0; }
 __device__ __forceinline__ int fp4_run_start(int i, int total, int n) {
   const uint32_t each = static_cast<uint32_t>(total) / static_cast<uint32_t>(n);
   return static_cast<int>(i * each) + min(i, static_cast<int>(total - n * each));
@@ -617,12 +626,36 @@ __device__ __forceinline__ int fp4_fresh_tid() {
   return t;
 }
 
+// Of the workgroups that share a CU the oldest is served first, so that of equal runs
+// its ends long before the youngest's (at 52, 58, 66 and 75 us where four share it),
+// and few are left to keep the memory busy.  A workgroup's priority therefore falls at a
+// half, three quarters and seven eighths of its run: those behind are served first (66,
+// 69, 71 and 73 us).
+struct Fp4Pace {
+  int next, rest, left;  // tiles of the run up to the next fall, and from there on; falls to come
+  __device__ __forceinline__ void start(int tiles) {
+    rest = tiles / 2;
+    next = rest;
+    left = 3;
+    __builtin_amdgcn_s_setprio(3);
+  }
+  __device__ __forceinline__ void at(int tile) {
+    if (tile < next || left == 0) return;  // uniform
+    if (left == 3) __builtin_amdgcn_s_setprio(2);
+    if (left == 2) __builtin_amdgcn_s_setprio(1);
+    if (left == 1) __builtin_amdgcn_s_setprio(0);
+    --left;
+    rest /= 2;
+    next += rest;
+  }
+};
+
 // A segment: tiles [t_from, t_to) of an item; its rows' outputs, or where the
 // segment is a piece of the item, slot `slot_of_part` of the partial ones.  Every wave
 // takes tiles of its own for all of the item's rows.
 template <int DP, int MT, bool kExact>
 __device__ __forceinline__ void fp4_segment(Fp4Smem<DP>& sm, const Fp4AttnArgs& a, int b, int rb, int hk, const Fp4Span& sp,
-                                            int t_from, int t_to, int slot_of_part) {
+                                            int t_from, int t_to, int slot_of_part, Fp4Pace& pace, int done) {
   using Wave = Fp4Wave<DP, MT, kExact, false>;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x) / kWave, lane = fp4_fresh_tid() % kWave;
   const int r0 = rb * 16 * MT;
@@ -667,12 +700,16 @@ __device__ __forceinline__ void fp4_segment(Fp4Smem<DP>& sm, const Fp4AttnArgs& 
     fetch(raw1, 1);
     int i = 0;
     for (; i + 1 < n; i += 2) {
+      pace.at(done + i * kF4Waves);
       step(raw0, i);
       step(raw1, i + 1);
     }
     if (i < n) step(raw0, i);
   } else {
-    for (int i = 0; i < n; ++i) step(raw0, i);
+    for (int i = 0; i < n; ++i) {
+      pace.at(done + i * kF4Waves);
+      step(raw0, i);
+    }
   }
   // join the waves: maxima and sums of every row, then the outputs, a row tile at a time
   const int tid = fp4_fresh_tid(), col = tid & 15, grp = (tid >> 4) & 3;
@@ -737,7 +774,7 @@ __device__ __forceinline__ void fp4_segment(Fp4Smem<DP>& sm, const Fp4AttnArgs& 
 // decodes one in four tiles' values for all of them.
 template <int DP, int MT, bool kExact>
 __device__ __forceinline__ void fp4_segment_shared(Fp4Smem<DP>& sm, const Fp4AttnArgs& a, int b, int rb, int hk, const Fp4Span& sp,
-                                                   int t_from, int t_to, int slot_of_part) {
+                                                   int t_from, int t_to, int slot_of_part, Fp4Pace& pace, int done) {
   using Wave = Fp4Wave<DP, MT, kExact, true>;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x) / kWave, lane = fp4_fresh_tid() % kWave;
   const int r0 = (rb * kF4Waves + wave) * 16 * MT;
@@ -756,6 +793,7 @@ __device__ __forceinline__ void fp4_segment_shared(Fp4Smem<DP>& sm, const Fp4Att
   w.template fetch<false, true>(vals, at, slot, 2 * wave);
   w.template fetch<true, false>(keys[0], at, slot, 0);
   for (int i = 0; i < n; i += kF4Waves) {
+    pace.at(done + i);
     {
       const int pos = (t_lo + i + wave) * kF4Tile;
       w.template unpack_scales<false, true>(vals);
@@ -850,13 +888,14 @@ __global__ __launch_bounds__(kF4Threads, fp4_resident(DP, MT)) void k_fp4_attn(F
   const bool each = a.max_groups == 0;  // none is cut, a workgroup each
   const int g = blockIdx.x;
   int x = g, end = g + 1, total = 0, b, rb;
-  const auto item_of = [&](int u) {  // u < total: pre[item] <= u < pre[item + 1]
-    int lo = 0, hi = items;
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (sm.pre[mid] <= u) lo = mid; else hi = mid;
-    }
-    return lo;
+  const auto item_of = [&](int u) {  // u < total: pre[item] <= u < pre[item + 1]; the wave looks in 64 places at a time
+    const int lane = tid % kWave, step = (items + kWave - 1) / kWave;
+    const auto last_of = [&](int first, int by, int n) {  // of pre[first + by i] <= u, i < n
+      const int at = first + by * lane;
+      return first + by * (__popcll(__ballot(lane < n && at < items && sm.pre[at] <= u)) - 1);
+    };
+    const int from = last_of(0, step, kWave);
+    return step == 1 ? from : last_of(from, 1, step);
   };
   if (!each) {
     if (tid == 0) sm.longest = 0;
@@ -864,7 +903,7 @@ __global__ __launch_bounds__(kF4Threads, fp4_resident(DP, MT)) void k_fp4_attn(F
     int longest = 0;
     for (int base = 0; base < items; base += kF4Threads) {
       const int item = base + tid;
-      const int own = item < items ? span_of(item, b, rb).units() : 0, n = own * a.Hkv;
+      const int own = item < items ? span_of(item, b, rb).units() + a.lead : 0, n = own * a.Hkv;
       longest = max(longest, own);
       int tot;
       const int ex = block_exclusive_scan(n, sm.scan, &tot);
@@ -885,32 +924,37 @@ __global__ __launch_bounds__(kF4Threads, fp4_resident(DP, MT)) void k_fp4_attn(F
     }
     if (whole) groups = units;
     if (g >= groups) return;  // uniform
-    // a run's end inside a small item moves to the item's end
+    // a run's end inside a small item moves to one of the item's
     const auto run_start = [&](int i) {
       if (whole) return i == units ? total : sm.pre[i / a.Hkv] + i % a.Hkv * ((sm.pre[i / a.Hkv + 1] - sm.pre[i / a.Hkv]) / a.Hkv);
       const int u = fp4_run_start(i, total, groups);
       if (u <= 0 || u >= total) return u;
       const int item = item_of(u), n = (sm.pre[item + 1] - sm.pre[item]) / a.Hkv;
       const int over = (u - sm.pre[item]) % n;
-      return over > 0 && n <= a.small ? u - over + n : u;
+      if (n - a.lead <= a.small) return 2 * over < n ? u - over : u - over + n;
+      return over <= fp4_early(a) ? u - over : u;
     };
     x = uniform(run_start(g));
     end = uniform(run_start(g + 1));
   }
+  Fp4Pace pace{0, 0, 0};
+  if (!each) pace.start(end - x);  // in a grid of more than the device holds the oldest may go first
+  const int x0 = x;
   while (x < end) {
     const int item = each ? x / a.Hkv : uniform(item_of(x));
     const Fp4Span sp = span_of(item, b, rb);
-    const int n = sp.units();
+    const int lead = each ? 0 : a.lead, n = sp.units() + lead;
     const int in = each ? 0 : x - uniform(sm.pre[item]);
     const int hk = each ? x - item * a.Hkv : in / n;
-    const int from = each ? 0 : in - hk * n, to = each ? n : min(n, from + end - x);
-    const int part = from == 0 && to == n ? -1 : from == 0 ? 2 * g + 1 : 2 * g;
+    const int x1 = each ? 0 : in - hk * n, x2 = each ? n : min(n, x1 + end - x);
+    const int from = max(x1 - lead, 0), to = x2 - lead;
+    const int part = x1 == 0 && x2 == n ? -1 : x1 == 0 ? 2 * g + 1 : 2 * g;
     if constexpr (kShared) {
-      fp4_segment_shared<DP, MT, kExact>(sm, a, b, rb, hk, sp, from, to, part);
+      fp4_segment_shared<DP, MT, kExact>(sm, a, b, rb, hk, sp, from, to, part, pace, x - x0);
     } else {
-      fp4_segment<DP, MT, kExact>(sm, a, b, rb, hk, sp, from, to, part);
+      fp4_segment<DP, MT, kExact>(sm, a, b, rb, hk, sp, from, to, part, pace, x - x0);
     }
-    x += each ? 1 : to - from;
+    x += each ? 1 : x2 - x1;
     __syncthreads();  // the segment's LDS has been read
   }
 }
@@ -927,10 +971,10 @@ __global__ __launch_bounds__(kF4Threads) void k_fp4_attn_join(Fp4AttnArgs a, int
   const int item = blockIdx.x / a.Hkv, hk = blockIdx.x - item * a.Hkv;
   const int b = item / a.row_blocks, rb = item - b * a.row_blocks;
   const int total = a.sched[items], p0 = a.sched[item], n = (a.sched[item + 1] - p0) / a.Hkv;
-  if (n <= a.sched[items + 1]) return;  // uniform
+  if (n - a.lead <= a.sched[items + 1]) return;  // uniform
   const int groups = fp4_groups(a, total);
   const int x0 = p0 + hk * n;
-  const int w0 = fp4_owner(x0, total, groups), pieces = fp4_owner(x0 + n - 1, total, groups) - w0 + 1;
+  const int w0 = fp4_owner(x0 + min(fp4_early(a), n - 1), total, groups), pieces = fp4_owner(x0 + n - 1, total, groups) - w0 + 1;
   if (pieces == 1) return;  // uniform
   const int tid = threadIdx.x % kThreads, mine = threadIdx.x / kThreads, lane = threadIdx.x % kWave;
   const int64_t pitch = a.D + 4;
@@ -1041,7 +1085,7 @@ int fp4_attn_plan(const skv_fp4_attention_desc* d, Fp4AttnPlan& p) {
   if (d->window > 0) len = std::min(len, d->window + ceil_div(p.rows, d->n_heads / hkv));
   const int64_t tiles = ceil_div(len, kF4Tile) + 1, units = std::max<int64_t>(p.items * hkv, 1);
   p.cut = tiles > kF4SmallTiles || d->splits > 0;
-  if (p.items > kF4MaxItems || units > INT32_MAX / (ceil_div(capacity, kF4Tile) + 1)) p.cut = false;
+  if (p.items > kF4MaxItems || units > INT32_MAX / (ceil_div(capacity, kF4Tile) + 1 + kF4Lead)) p.cut = false;
   p.groups = !p.cut ? 0 : d->splits > 0 ? d->splits * units : static_cast<int64_t>(fp4_resident(p.dims, p.mt)) * device_cus();
   if (units >= (1 << 24) || p.groups >= (1 << 24)) return set_error(SKV_EINVAL, "%s: too many workgroups", what);
   p.sched_bytes = p.cut ? ceil_div((p.items + 2) * 4, 16) * 16 : 0;
@@ -1126,6 +1170,7 @@ extern "C" int skv_fp4_attention(const skv_fp4_attention_desc* d, void* workspac
   a.row_blocks = static_cast<int32_t>(p.row_blocks);
   a.max_groups = static_cast<int32_t>(p.groups);
   a.small = d->splits > 0 ? 0 : kF4SmallTiles;
+  a.lead = d->splits == 0 && 2 * p.items * a.Hkv >= p.groups ? kF4Lead : 0;
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (a.D == p.dims) launch_dims<true>(a, p, s); else launch_dims<false>(a, p, s);
   if (const int rc = check_launch(what)) return rc;
