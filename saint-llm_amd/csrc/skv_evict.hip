@@ -89,14 +89,46 @@ __global__ __launch_bounds__(kEvictThreads) void k_release(
   }
 }
 
-// k_release over shared pages (refs[p]: holders beyond the first).  Push order is
-// ascending b, within b from the last logical page; a wave takes 64 entries of one
-// sequence's table at a time (a unit) and sends kReleaseAhead of them out together,
-// which is what this launch's time, a few dependent memory latencies a step, asks for.
-// A page whose holders all leave drops to -1; the last place u among its releases,
-// found by a minimum over -2 - u in the count itself, pushes it, so that the stack
-// does not depend on the order in which the atomics run.
+// k_release over shared pages (refs[p]: holders beyond the first), in two launches.
+//
+// k_release_drop takes every released entry's page a holder: scattered atomics, which
+// one CU does at 1.6 ns each and many do at once.  A page whose holders have all left
+// is then at -1, one released more often than it was held below that.
+//
+// k_release_shared, one workgroup, checks that, pushes the pages at -1 and clears the
+// tables, or gives the counts back.  Push order is ascending b, within b from the last
+// logical page; of a page's releases the last place u pushes it, found by a minimum over
+// -2 - u in the count itself, so that the stack does not depend on the order in which
+// the atomics run.  A wave takes 64 entries of one sequence's table (a unit) at a time,
+// kReleaseAhead of them together; a release of up to kReleaseStep units keeps its
+// entries in registers from pass to pass.  Which entries' pages have dropped is noted
+// for the first kReleaseNoted units, so that later passes touch those alone.  48 sequences
+// of 8k - 64k tokens, 22,000 entries: 142 us with every entry by a thread in turn, 66 with
+// units and all in one launch, 5 + 48 so; with 24 units together 36, but 27 instead of 13
+// for a release of 1,600 entries.
 constexpr int kReleaseAhead = 8;
+constexpr int kReleaseStep = kEvictThreads / kWave * kReleaseAhead;
+constexpr int kReleaseNoted = 1024;
+constexpr int kDropThreads = 256;
+constexpr int kDropEntries = 4 * kDropThreads;
+
+__device__ __forceinline__ int released_pages(const int32_t* lens, const uint8_t* mask, int64_t bt_stride, int b, int bs) {
+  return mask[b] ? static_cast<int>(min<int64_t>(ceil_div(max(lens[b], 0), bs), bt_stride)) : 0;
+}
+
+// grid: (parts of a table row, batch)
+__global__ __launch_bounds__(kDropThreads) void k_release_drop(int64_t n_pages, int32_t* refs, const int32_t* __restrict__ bt,
+                                                               int64_t bt_stride, const int32_t* __restrict__ lens,
+                                                               const uint8_t* __restrict__ mask, int bs) {
+  const int b = blockIdx.y, n = released_pages(lens, mask, bt_stride, b, bs);
+#pragma unroll
+  for (int k = 0; k < kDropEntries / kDropThreads; ++k) {
+    const int64_t j = static_cast<int64_t>(blockIdx.x) * kDropEntries + k * kDropThreads + static_cast<int>(threadIdx.x);
+    if (j >= n) return;
+    const int32_t page = bt[b * bt_stride + j];
+    if (page >= 0 && page < n_pages) atomicSub(&refs[page], 1);
+  }
+}
 
 __global__ __launch_bounds__(kEvictThreads) void k_release_shared(
     int32_t* __restrict__ stack, int32_t* __restrict__ top_ptr, int64_t n_pages, int32_t* refs, int32_t* bt,
@@ -104,6 +136,7 @@ __global__ __launch_bounds__(kEvictThreads) void k_release_shared(
     int32_t* __restrict__ status) {
   __shared__ int off[kEvictMaxBatch + 1];  // units before each sequence
   __shared__ int cnt[kEvictMaxBatch];      // its pages
+  __shared__ uint64_t noted[kReleaseNoted];
   __shared__ int scan_lds[17];
   __shared__ int bad_all;
   const int tid = threadIdx.x, lane = tid % kWave;
@@ -111,9 +144,7 @@ __global__ __launch_bounds__(kEvictThreads) void k_release_shared(
   if (tid == 0) bad_all = 0;
   int units = 0;
   for (int base = 0; base < batch; base += kEvictThreads) {
-    const int b = base + tid;
-    int c = 0;
-    if (b < batch && mask[b]) c = static_cast<int>(min<int64_t>(ceil_div(max(lens[b], 0), bs), bt_stride));
+    const int b = base + tid, c = b < batch ? released_pages(lens, mask, bt_stride, b, bs) : 0;
     int tot;
     const int ex = block_exclusive_scan((c + kWave - 1) / kWave, scan_lds, &tot);
     if (b < batch) {
@@ -125,108 +156,146 @@ __global__ __launch_bounds__(kEvictThreads) void k_release_shared(
   if (tid == 0) off[batch] = units;
   __syncthreads();
   const int top = *top_ptr;
-  constexpr int kStep = kEvictThreads / kWave * kReleaseAhead;
-  // f(places u, table entries, page ids) for every step's kReleaseAhead entries of the
-  // thread; no entry: u < 0.  All threads take the same steps.
-  const auto steps = [&](auto&& f) {
-    for (int base = 0; base < units; base += kStep) {
-      const int first = base + wave * kReleaseAhead;
-      int b = first < units ? owner_of(off, batch, first) : 0;
-      int u[kReleaseAhead];
-      int32_t* entry[kReleaseAhead];
-      int32_t page[kReleaseAhead];
+  // all of them loaded before any is used: else each load sinks into its use's branch
+  const auto together = [](int32_t* x) {
+    static_assert(kReleaseAhead % 8 == 0);
 #pragma unroll
-      for (int k = 0; k < kReleaseAhead; ++k) {
-        u[k] = -1;
-        entry[k] = bt;
-        if (first + k < units) {  // uniform
-          while (first + k >= off[b + 1]) ++b;
-          const int j = (first + k - off[b]) * kWave + lane;
-          if (j < cnt[b]) {
-            u[k] = (first + k) * kWave + lane;
-            entry[k] = bt + static_cast<int64_t>(b) * bt_stride + (cnt[b] - 1 - j);
+    for (int k = 0; k < kReleaseAhead; k += 8) {
+      asm volatile("" : "+v"(x[k]), "+v"(x[k + 1]), "+v"(x[k + 2]), "+v"(x[k + 3]), "+v"(x[k + 4]), "+v"(x[k + 5]),
+                        "+v"(x[k + 6]), "+v"(x[k + 7]));
+    }
+  };
+  // the thread's entries of the step from unit `at` on: places (-1: no entry), indices in the table, page ids
+  int at = -1, first = 0, u[kReleaseAhead];
+  int entry[kReleaseAhead];
+  int32_t page[kReleaseAhead];
+  // f() for every step; all threads take the same steps
+  const auto steps = [&](auto&& f) {
+    for (int base = 0; base < units; base += kReleaseStep) {
+      if (at != base) {
+        at = base;
+        first = base + wave * kReleaseAhead;
+        int b = first < units ? owner_of(off, batch, first) : 0;
+#pragma unroll
+        for (int k = 0; k < kReleaseAhead; ++k) {
+          u[k] = -1;
+          entry[k] = 0;
+          if (first + k < units) {  // uniform
+            while (first + k >= off[b + 1]) ++b;
+            const int j = (first + k - off[b]) * kWave + lane;
+            if (j < cnt[b]) {
+              u[k] = (first + k) * kWave + lane;
+              entry[k] = static_cast<int>(b * bt_stride) + cnt[b] - 1 - j;
+            }
           }
         }
-      }
 #pragma unroll
-      for (int k = 0; k < kReleaseAhead; ++k) page[k] = *entry[k];
-      f(u, entry, page);
+        for (int k = 0; k < kReleaseAhead; ++k) page[k] = bt[entry[k]];
+        together(page);
+      }
+      f();
     }
+  };
+  // of the k-th entries those that may have a noted property (past the noted units: any)
+  const auto may = [&](int k) {
+    return u[k] >= 0 && (first + k >= kReleaseNoted || ((noted[min(first + k, kReleaseNoted - 1)] >> lane) & 1));
+  };
+  const auto note = [&](int k, bool yes) {
+    const uint64_t lanes = __ballot(yes);
+    if (lane == 0 && first + k < kReleaseNoted) noted[first + k] = lanes;
+    return lanes;
+  };
+  const auto known = [&](int k) { return u[k] >= 0 && page[k] >= 0 && page[k] < n_pages; };
+  const auto counts = [&](const bool* ask, int32_t* count) {
+#pragma unroll
+    for (int k = 0; k < kReleaseAhead; ++k) count[k] = refs[ask[k] ? page[k] : 0];
+    together(count);
   };
   const auto refuse = [&](int bad) {  // the whole workgroup's answer
     if (bad) atomicOr(&bad_all, bad);
     __syncthreads();
-    if (bad_all && tid == 0 && status) *status = bad_all;
-    return bad_all != 0;
-  };
-  const auto known = [&](int32_t page) { return page >= 0 && page < n_pages; };
-  int bad = (top < 0 || top > n_pages) ? SKV_STATUS_STACK : 0;
-  int freed = 0;
-  steps([&](const int* u, int32_t* const*, const int32_t* page) {
-    int was[kReleaseAhead];
-#pragma unroll
-    for (int k = 0; k < kReleaseAhead; ++k) {
-      was[k] = 1;
-      if (u[k] < 0) continue;
-      if (known(page[k])) was[k] = atomicSub(&refs[page[k]], 1); else bad = SKV_STATUS_BADARG;
-    }
-#pragma unroll
-    for (int k = 0; k < kReleaseAhead; ++k) {
-      freed += was[k] == 0 ? 1 : 0;
-      if (was[k] < 0) bad = SKV_STATUS_BADARG;
-    }
-  });
-  const int pushes = block_reduce_sum(freed, scan_lds);
-  if (static_cast<int64_t>(top) + pushes > n_pages) bad |= SKV_STATUS_STACK;
-  if (refuse(bad)) {  // the counts as they were
-    steps([&](const int* u, int32_t* const*, const int32_t* page) {
+    if (!bad_all) return false;
+    if (tid == 0 && status) *status = bad_all;
+    steps([&] {  // the counts as they were
 #pragma unroll
       for (int k = 0; k < kReleaseAhead; ++k) {
-        if (u[k] >= 0 && known(page[k])) atomicAdd(&refs[page[k]], 1);
+        if (known(k)) atomicAdd(&refs[page[k]], 1);
       }
     });
-    return;
-  }
-  // past the L1 cache, which may hold what a count was
-  const auto counts = [&](const int* u, const int32_t* page, int* count) {
-#pragma unroll
-    for (int k = 0; k < kReleaseAhead; ++k) {
-      count[k] = u[k] < 0 ? 0 : __hip_atomic_load(&refs[page[k]], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    }
+    return true;
   };
-  steps([&](const int* u, int32_t* const*, const int32_t* page) {
-    int count[kReleaseAhead];
-    counts(u, page, count);
+  int bad = (top < 0 || top > n_pages) ? SKV_STATUS_STACK : 0;
+  steps([&] {
+    bool ask[kReleaseAhead];
+    int32_t count[kReleaseAhead];
+#pragma unroll
+    for (int k = 0; k < kReleaseAhead; ++k) ask[k] = known(k);
+    counts(ask, count);
 #pragma unroll
     for (int k = 0; k < kReleaseAhead; ++k) {
-      if (count[k] < 0) atomicMin(&refs[page[k]], -2 - u[k]);
+      if (u[k] >= 0 && (!ask[k] || count[k] < -1)) bad = SKV_STATUS_BADARG;
+      note(k, ask[k] && count[k] < 0);
     }
   });
-  __syncthreads();
-  int at = top;
-  steps([&](const int* u, int32_t* const* entry, const int32_t* page) {
-    int count[kReleaseAhead];
-    counts(u, page, count);
-    uint64_t push[kReleaseAhead];
-    int mine = 0;  // the wave's
+  if (refuse(bad)) return;
+  // between a pass that changes counts and one that reads them: the changes have been
+  // made, and the L1 cache holds no count
+  const auto fresh = [] {
+    __builtin_amdgcn_s_waitcnt(0);
+    __syncthreads();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
+  };
+  steps([&] {
 #pragma unroll
     for (int k = 0; k < kReleaseAhead; ++k) {
-      push[k] = __ballot(u[k] >= 0 && count[k] == -2 - u[k]);
-      mine += __popcll(push[k]);
+      if (may(k) && (first + k < kReleaseNoted || refs[page[k]] < 0)) atomicMin(&refs[page[k]], -2 - u[k]);
+    }
+  });
+  fresh();
+  int mine = 0;  // pages that the wave will push
+  steps([&] {
+    bool ask[kReleaseAhead];
+    int32_t count[kReleaseAhead];
+#pragma unroll
+    for (int k = 0; k < kReleaseAhead; ++k) ask[k] = may(k);
+    counts(ask, count);
+#pragma unroll
+    for (int k = 0; k < kReleaseAhead; ++k) mine += __popcll(note(k, ask[k] && count[k] == -2 - u[k]));
+  });
+  const int pushes = block_reduce_sum(lane == 0 ? mine : 0, scan_lds);
+  const bool full = static_cast<int64_t>(top) + pushes > n_pages;
+  if (full) {  // uniform: the places leave the counts again
+    steps([&] {
+#pragma unroll
+      for (int k = 0; k < kReleaseAhead; ++k) {
+        if (may(k) && refs[page[k]] == -2 - u[k]) refs[page[k]] = -1;
+      }
+    });
+    fresh();
+  }
+  if (refuse(full ? SKV_STATUS_STACK : 0)) return;
+  int to = top;
+  steps([&] {
+    uint64_t push[kReleaseAhead];
+    int n = 0;  // the wave's
+#pragma unroll
+    for (int k = 0; k < kReleaseAhead; ++k) {
+      push[k] = __ballot(may(k) && (first + k < kReleaseNoted || refs[page[k]] == -2 - u[k]));
+      n += __popcll(push[k]);
     }
     int tot;
-    const int ex = block_exclusive_scan(lane == 0 ? mine : 0, scan_lds, &tot);
-    int to = at + __builtin_amdgcn_readfirstlane(ex);
+    const int ex = block_exclusive_scan(lane == 0 ? n : 0, scan_lds, &tot);
+    int slot = to + __builtin_amdgcn_readfirstlane(ex);
 #pragma unroll
     for (int k = 0; k < kReleaseAhead; ++k) {
       if ((push[k] >> lane) & 1) {
-        stack[to + __popcll(push[k] & ((uint64_t{1} << lane) - 1))] = page[k];
-        atomicExch(&refs[page[k]], 0);
+        stack[slot + __popcll(push[k] & ((uint64_t{1} << lane) - 1))] = page[k];
+        refs[page[k]] = 0;
       }
-      to += __popcll(push[k]);
-      if (u[k] >= 0) *entry[k] = -1;  // read by this thread alone
+      slot += __popcll(push[k]);
+      if (u[k] >= 0) bt[entry[k]] = -1;  // read by this thread alone
     }
-    at += tot;
+    to += tot;
   });
   for (int b = tid; b < batch; b += kEvictThreads) {
     if (mask[b]) lens[b] = 0;
@@ -553,6 +622,10 @@ extern "C" int skv_release_shared(int32_t* free_stack, int32_t* free_top, int64_
     return set_error(SKV_EINVAL, "%s: NULL pointer", what);
   }
   if (batch == 0) return SKV_OK;
+  hipLaunchKernelGGL(k_release_drop, dim3(static_cast<unsigned>(ceil_div(bt_stride, kDropEntries)), static_cast<unsigned>(batch)),
+                     dim3(kDropThreads), 0, static_cast<hipStream_t>(stream), n_pages, refs, block_table, bt_stride, seq_lens,
+                     release_mask, static_cast<int>(block_size));
+  if (const int rc = check_launch(what)) return rc;
   hipLaunchKernelGGL(k_release_shared, dim3(1), dim3(kEvictThreads), 0, static_cast<hipStream_t>(stream), free_stack,
                      free_top, n_pages, refs, block_table, bt_stride, seq_lens, release_mask, static_cast<int>(batch),
                      static_cast<int>(block_size), status);
