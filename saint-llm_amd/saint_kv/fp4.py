@@ -72,10 +72,10 @@ def fp4_attention(q: torch.Tensor, pool: torch.Tensor, block_table: torch.Tensor
     scale: of the scores (None: 1/sqrt(D)).  A token that sees nothing gets 0.
     max_len: a bound on seq_lens (0: what the table holds; longer ones are still
     right), which saves short sequences the launch that joins parts of long ones;
-    splits: about that many workgroups for a K/V head of every sequence, instead
-    of as many as the device holds (0).
-    workspace: a tensor of at least ``fp4_attention_workspace`` bytes (None: one
-    is allocated for the call)."""
+    splits: at most about that many workgroups for a K/V head of every sequence,
+    instead of as many as the device holds (0).
+    workspace: a tensor of at least ``fp4_attention_workspace`` bytes, of no other
+    call that may run at the same time (None: one is allocated for the call)."""
     d, out = _desc(q, pool, block_table, seq_lens, n_new, window, sink, softcap, scale, max_len, splits, out)
     need = int(_lib.load().skv_fp4_attention_workspace(ctypes.byref(d)))
     if need < 0:

@@ -748,6 +748,8 @@ def fp4_gather(pool: torch.Tensor, block_table: torch.Tensor, seq_lens: torch.Te
     rows = [_fp4_rows(t, name, c, (torch.bfloat16,)) for t, name in ((out_k, "out_k"), (out_v, "out_v"))]
     if out_k.shape != out_v.shape:
         raise ValueError("out_k and out_v must have the same shape")
+    if any(s == 0 and n > 1 for t in (out_k, out_v) for n, s in zip(t.shape, t.stride())):
+        raise ValueError("out_k and out_v must not be expanded tensors")
     n_ptr, n_uni = _n_new_args(n, c.batch)
     if n_ptr is None and n_uni > out_k.shape[1]:
         raise ValueError(f"n={n_uni} exceeds the {out_k.shape[1]} tokens of out_k and out_v")

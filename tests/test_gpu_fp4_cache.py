@@ -276,6 +276,25 @@ def test_captured_steps(dev) -> None:
     assert int(caches[0].status) == 0
 
 
+def test_expanded_rows(dev) -> None:
+    """Rows that are one expanded token are written for every position; none can be read into such."""
+    from saint_kv import ops
+
+    lens = torch.tensor([20, 33], dtype=torch.int32, device=dev)
+    pool, bt, _ = make(dev, [20, 33], 16, 2, 64)
+    k, v = (queries(dev, 1, 1, 2, 64, seed=s).expand(2, 33, 2, 64) for s in (1, 2))
+    ops.fp4_quant_append(pool, bt, lens, k, v, lens)
+    out = [torch.zeros(2, 33, 2, 64, dtype=torch.bfloat16, device=dev) for _ in range(2)]
+    ops.fp4_gather(pool, bt, lens, *out, lens)
+    for x, y in zip(out, (k, v)):
+        codes, scales = ora.quantize(y[0, 0].double().cpu().numpy())
+        want = torch.as_tensor(ora.dequantize(codes, scales))
+        assert all(torch.equal(x[b, i].double().cpu(), want) for b, n in ((0, 20), (1, 33)) for i in range(n))
+        assert not x[0, 20:].any()
+    with pytest.raises(ValueError, match="expanded"):
+        ops.fp4_gather(pool, bt, lens, k, v, lens)
+
+
 def test_what_is_read_back_is_what_attention_sees(dev) -> None:
     """fp4_gather's rows, attended over in 64 bits, give fp4_attention's outputs."""
     from saint_kv import fp4_attention, ops
