@@ -785,8 +785,7 @@ __device__ __forceinline__ void fp4_segment_shared(Fp4Smem<DP>& sm, const Fp4Att
   const auto places = [&](int i, uint64_t& at, int& slot) {
     w.lookup(b, min(t_lo + i + ((lane >> 1) & 3), t_hi) * kF4Tile + 16 * (lane & 1), at, slot);
   };
-  constexpr int kKeys = Wave::kTwo ? 2 : 1;  // tiles' keys in registers
-  typename Wave::Raw keys[kKeys], vals;
+  typename Wave::Raw keys[2], vals;
   uint64_t at, at_next;
   int slot, slot_next;
   places(0, at, slot);
@@ -806,26 +805,21 @@ __device__ __forceinline__ void fp4_segment_shared(Fp4Smem<DP>& sm, const Fp4Att
     __syncthreads();  // the tiles are there
 #pragma unroll
     for (int j = 0; j < kF4Waves; ++j) {
-      typename Wave::Raw& kr = keys[j % kKeys];
-      const auto next = [&] {
-        typename Wave::Raw& to = keys[(j + 1) % kKeys];
-        if (j < kF4Waves - 1) {
-          w.template fetch<true, false>(to, at, slot, 2 * (j + 1));
-        } else {
-          w.template fetch<true, false>(to, at_next, slot_next, 0);
-        }
-      };
+      typename Wave::Raw &kr = keys[j & 1], &next = keys[(j + 1) & 1];
+      if (j < kF4Waves - 1) {
+        w.template fetch<true, false>(next, at, slot, 2 * (j + 1));
+      } else {
+        w.template fetch<true, false>(next, at_next, slot_next, 0);
+      }
+      if (j == 1) w.template fetch<false, true>(vals, at_next, slot_next, 2 * wave);
       const int pos = (t_lo + i + j) * kF4Tile;
       Fp4Tile<MT> tl;
-      if constexpr (kKeys == 2) next();
-      if (j == 1) w.template fetch<false, true>(vals, at_next, slot_next, 2 * wave);
       tl.slot[0] = kr.slot[0];
       tl.slot[1] = kr.slot[1];
       tl.nan_keys = __builtin_amdgcn_readfirstlane(sm.nan_keys[j]);
       tl.masked = w.uneven(kr, pos) || tl.nan_keys != 0;
       w.template unpack_scales<true, false>(kr);
       w.scores(kr, tl);
-      if constexpr (kKeys == 1) next();
       if (i + j < n) w.output(tl, pos, reinterpret_cast<const uint16_t*>(sm.tile[j]));  // uniform
     }
     at = at_next;
@@ -1094,28 +1088,22 @@ int fp4_attn_plan(const skv_fp4_attention_desc* d, Fp4AttnPlan& p) {
 }
 
 // The part launch for padded dims DP.
-template <int DP, bool kExact, bool kShared>
-void launch_rows(const Fp4AttnArgs& a, int mt, hipStream_t s) {
+template <int DP, bool kExact>
+void launch_rows(const Fp4AttnArgs& a, const Fp4AttnPlan& p, hipStream_t s) {
   const dim3 grid(static_cast<unsigned>(a.max_groups > 0 ? a.max_groups : static_cast<int64_t>(a.B) * a.row_blocks * a.Hkv));
-  if constexpr (kShared) {
-    hipLaunchKernelGGL((k_fp4_attn<DP, fp4_shared_mt(DP), kExact, true>), grid, dim3(kF4Threads), 0, s, a);
-  } else {
-    if (mt == 1) hipLaunchKernelGGL((k_fp4_attn<DP, 1, kExact, false>), grid, dim3(kF4Threads), 0, s, a);
-    if constexpr (DP <= 256) {
-      if (mt == 2) hipLaunchKernelGGL((k_fp4_attn<DP, 2, kExact, false>), grid, dim3(kF4Threads), 0, s, a);
-    }
+  const auto go = [&](auto* kernel) { hipLaunchKernelGGL(kernel, grid, dim3(kF4Threads), 0, s, a); };
+  if constexpr (DP <= 256) {
+    if (p.shared) return go(&k_fp4_attn<DP, fp4_shared_mt(DP), kExact, true>);
+    if (p.mt == 2) return go(&k_fp4_attn<DP, 2, kExact, false>);
   }
+  go(&k_fp4_attn<DP, 1, kExact, false>);
 }
 template <bool kExact>
 void launch_dims(const Fp4AttnArgs& a, const Fp4AttnPlan& p, hipStream_t s) {
-  const auto go = [&](auto dims) {
-    constexpr int DP = decltype(dims)::value;
-    if (p.shared) launch_rows<DP, kExact, true>(a, p.mt, s); else launch_rows<DP, kExact, false>(a, p.mt, s);
-  };
-  if (p.dims == 64) go(std::integral_constant<int, 64>());
-  if (p.dims == 128) go(std::integral_constant<int, 128>());
-  if (p.dims == 256) go(std::integral_constant<int, 256>());
-  if (p.dims == 512) go(std::integral_constant<int, 512>());
+  if (p.dims == 64) launch_rows<64, kExact>(a, p, s);
+  if (p.dims == 128) launch_rows<128, kExact>(a, p, s);
+  if (p.dims == 256) launch_rows<256, kExact>(a, p, s);
+  if (p.dims == 512) launch_rows<512, kExact>(a, p, s);
 }
 
 }  // namespace skv
