@@ -401,7 +401,8 @@ int skv_compact(const skv_pool_ref* pools, int32_t n_pools, int32_t* block_table
  * order), the length is set.  src and dst are device arrays.  All-or-nothing:
  * if the stack lacks pages (SKV_STATUS_NOSPC), or an index is outside the
  * batch, a dst is not empty or is named twice, or a source's length or last
- * page is not a valid one (SKV_STATUS_BADARG), nothing is written but *status,
+ * page is not a valid one (SKV_STATUS_BADARG), or a page on the stack is none
+ * (SKV_STATUS_STACK), nothing is written but *status,
  * which may not be NULL here.  batch and n_forks <= 4096, up to 32 pools. */
 int skv_fork(int32_t* free_stack, int32_t* free_top, int64_t n_pages, int32_t* refs, int32_t* block_table,
              int64_t bt_stride, int32_t* seq_lens, int64_t batch, int64_t block_size, const int32_t* src,

@@ -10,6 +10,11 @@
 // 32-dim block find its largest magnitude by two quad permutes.  A thread has the
 // same item of four tokens, whose loads it sends together: where an item lies in
 // a token is worked out once for the four.
+//
+// HBM bounds both: 8 prompts of 8192 tokens, 8 heads of 128 dims (339 MB) are written
+// in 65 us (5.2 TB/s) and read back in 51 us (6.6 TB/s, part of the codes from the
+// last-level cache); with one token's item at a time and its place worked out anew
+// 97 and 87 us.  A step of 64 single tokens takes 3.8 and 3.1 us, its launch's latency.
 #include <algorithm>
 
 #include "skv_fp4.h"

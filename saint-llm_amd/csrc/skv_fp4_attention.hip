@@ -8,9 +8,7 @@
 // by exp2(m_old - m_new) where the maximum moves.
 //
 // A K/V head's query rows (its query heads times the query tokens) are cut into
-// blocks of 16 MT rows.  A workgroup takes a row block over a run of positions, its four
-// waves tiles of 32 positions in turn, each with a softmax of its own, joined at the
-// end.  No wave waits for another on the way:
+// blocks of 16 MT rows a wave, over tiles of 32 positions:
 //   * S^T = K Q^T by the scaled products of gfx950 (v_mfma_scale_f32_16x16x128_f8f6f4),
 //     which take e2m1 codes and their scale bytes as they lie in the page: lane
 //     (key, g) of 16 keys reads g's quarter of its key's codes straight into the operand
@@ -18,18 +16,37 @@
 //     q = hi 2^a + lo 2^(a - 5) with 2^a by 32 dims: a bf16 value's 8 bits are 4 and 4, so
 //     the parts are exact (but for values below 2^-13 of their 32's largest, which are
 //     exact to 2^-23 of it).
-//   * the values go through the wave's own part of LDS as bf16, rows of D in
-//     swizzled chunks, and come back transposed (ds_read_b64_tr_b16) as the A
-//     operand of O^T = V^T P^T, whose B operand is P^T as the scores' accumulators
-//     hold it.  O^T keeps a row's output in the lanes that hold its m and l.
-// The codes of the next two tiles are in flight while one is multiplied, the page
-// ids of 32 tiles sit in the lanes of a register.
+//   * the values go through LDS as bf16, rows of D in swizzled chunks, and come back
+//     transposed (ds_read_b64_tr_b16) as the A operand of O^T = V^T P^T, whose B
+//     operand is P^T as the scores' accumulators hold it.  O^T keeps a row's output in
+//     the lanes that hold its m and l.  P is rounded to bf16 (2^-8 of each weight, the
+//     operand that the product with exact bf16 values needs); scores, m, l and O are fp32.
+// Few rows (fp4_segment): all of a workgroup's rows are every wave's, and each wave takes
+// tiles of its own, with a softmax of its own, joined at the end; no wave waits for
+// another on the way, and the codes of the next two tiles are in flight while one is
+// multiplied.  Memory bounds it.  Many (fp4_segment_shared): the waves have rows of their
+// own and share the tiles, each decoding the values of one in four; a tile is read and
+// decoded once for 128 rows (64 of 256 dims).  The softmax's vector work and the matrix
+// products bound it.
 //
 // Work: the tiles of all (sequence, row block, head) items, one after another, are
 // dealt to as many workgroups as the device holds at once, in equal runs that may
 // cut a long item; the lengths are on the device, so every workgroup works the
 // runs out for itself from their prefix sum.  A cut item's pieces are joined by a
-// second launch.
+// second launch.  (Twice as many workgroups of half the run, for the hardware to deal out
+// as others end: 139 -> 180 us for the step below.)
+//
+// Measured, us a call among others, with the time of the bytes at 6.1 TB/s (or of the
+// products at 1.2 PFLOP/s):
+//   64 sequences of 1k - 32k, 64 heads on 8 of 128 dims                    140 (117)
+//   4 of 256k - 1M, 4 tokens, 16 heads on 4 of 64                          91 (75)
+//   16 of 64k, 64 heads on 1 of 128                                        66 (29, products)
+//   2 prompts' 1000 tokens over 16k, 32 heads on 8 of 128                  580 (428, products)
+//   1 prompt's 512 tokens over 200k, the same heads                        1700 (1400, products)
+//   32 windows of 128, 64 heads on 1 of 512                                21 (1)
+// and dropped: two row groups of two waves with half the tiles each for 33 - 64 rows (68 ->
+// 74 us for the 64k sequences: a tile's latency is then seen by all four waves); the next
+// tile's scores ahead of a tile's weights (1%); a prologue that loads the queries last.
 #include <algorithm>
 #include <cmath>
 
@@ -1066,7 +1083,10 @@ int fp4_attn_plan(const skv_fp4_attention_desc* d, Fp4AttnPlan& p) {
   const int64_t D = d->cache.head_dim, rows = d->n_queries * (d->n_heads / hkv);
   p.dims = D <= 64 ? 64 : D <= 128 ? 128 : D <= 256 ? 256 : 512;
   // A wave's tiles are its own, or all four waves' with rows of their own for each, once
-  // more than half of the rows of such a workgroup are there.
+  // more than half of the rows of such a workgroup are there: 16 sequences of 32k on one
+  // head of 128 dims take 65 us either way with 96 rows, 44 - 46 us shared and 43 apart with
+  // 64, 55 and 33 with 32; of 256 dims 75 and 84 us with 64 rows, 54 and 51 with 32.
+  // Heads of 512 dims stay apart (rows of 64: 117 us, shared 148, whose registers spill).
   const int mt = fp4_shared_mt(p.dims);
   p.shared = p.dims <= 256 && rows > 16 * mt * kF4Waves / 2;
   p.mt = p.shared ? mt : rows <= 16 || p.dims > 256 ? 1 : 2;

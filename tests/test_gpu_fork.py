@@ -179,6 +179,23 @@ def test_a_free_list_past_its_end_is_refused(dev) -> None:
     g.check()
 
 
+def test_a_free_list_of_pages_that_are_none_is_refused(dev) -> None:
+    """A fork that would pop one writes nothing; one that needs no page goes on."""
+    from saint_kv._lib import SKV_STATUS_STACK
+
+    g = Both(dev, 4, 4, 8, 16)
+    g.reserve([40, 32, 0, 0])
+    for bad in (-1, 8, 2 ** 31 - 1):
+        g.d["stack"][g.top - 1] = bad
+        g.fork([1, 0], [2, 3], SKV_STATUS_STACK)
+        g.d["stack"][g.top - 1] = int(g.stack[g.top - 1])
+        g.check()
+    g.d["stack"][g.top - 1] = 8
+    g.fork([1], [2])
+    g.d["stack"][g.top - 1] = int(g.stack[g.top - 1])
+    g.check()
+
+
 def test_copy_slots(dev) -> None:
     from saint_kv import ops
 
