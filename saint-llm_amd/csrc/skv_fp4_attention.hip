@@ -19,8 +19,9 @@
 //   * the values go through LDS as bf16, rows of D in swizzled chunks, and come back
 //     transposed (ds_read_b64_tr_b16) as the A operand of O^T = V^T P^T, whose B
 //     operand is P^T as the scores' accumulators hold it.  O^T keeps a row's output in
-//     the lanes that hold its m and l.  P is rounded to bf16 (2^-8 of each weight, the
-//     operand that the product with exact bf16 values needs); scores, m, l and O are fp32.
+//     the lanes that hold its m and l.  The values are exact in bf16; a weight goes in as
+//     a bf16 and, with few rows, its rounding's rest (see kRest).  Scores, m, l and O are
+//     fp32.
 // Few rows (fp4_segment): all of a workgroup's rows are every wave's, and each wave takes
 // tiles of its own, with a softmax of its own, joined at the end; no wave waits for
 // another on the way, and the codes of the next two tiles are in flight while one is
@@ -40,7 +41,7 @@
 // products at 1.2 PFLOP/s):
 //   64 sequences of 1k - 32k, 64 heads on 8 of 128 dims                    140 (117)
 //   4 of 256k - 1M, 4 tokens, 16 heads on 4 of 64                          91 (75)
-//   16 of 64k, 64 heads on 1 of 128                                        66 (29, products)
+//   16 of 64k, 64 heads on 1 of 128                                        79 (29, products)
 //   2 prompts' 1000 tokens over 16k, 32 heads on 8 of 128                  580 (428, products)
 //   1 prompt's 512 tokens over 200k, the same heads                        1700 (1400, products)
 //   32 windows of 128, 64 heads on 1 of 512                                21 (1)
@@ -229,6 +230,12 @@ struct Fp4Wave {
   static constexpr int kSteps = DP >= 128 ? DP / 128 : 1;  // products of 128 dims, or of the two parts of 64
   static constexpr int kBlocks = DP / 16;  // 16-dim blocks of the output
   static constexpr bool kPacked = kExact && DP <= 128;
+  // A weight's bf16 rounding, 2^-9 of it on average over few keys as over many, is as
+  // large an error as the output's own.  Waves with tiles of their own carry its rest
+  // into a second product, 139 us either way for a step of 64 sequences (64 rows on one
+  // head: 66 -> 79); where the products bound the time (580 -> 720 us for a prompt's chunk)
+  // the rounded weight stands.
+  static constexpr bool kRest = !kShared;
   static constexpr bool kTwo = DP * MT <= 256;  // two tiles in flight; wider ones have registers for one
   static constexpr bool kOnce = !kShared && DP * MT <= 256;  // all of a head's rows in a workgroup: no page is read twice
 
@@ -606,7 +613,7 @@ struct Fp4Wave {
         for (int x = 0; x < kBlocks; ++x) acc[mt][x] *= alpha;
       }
     }
-    u32x4 p[MT];
+    u32x4 p[MT], rest[kRest ? MT : 1];
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
       float e[8];
@@ -617,7 +624,12 @@ struct Fp4Wave {
       }
       l[mt] += ((e[0] + e[1]) + (e[2] + e[3])) + ((e[4] + e[5]) + (e[6] + e[7]));
 #pragma unroll
-      for (int i = 0; i < 4; ++i) p[mt][i] = bf16_pack2(e[2 * i], e[2 * i + 1]);
+      for (int i = 0; i < 4; ++i) {
+        p[mt][i] = bf16_pack2(e[2 * i], e[2 * i + 1]);
+        if constexpr (kRest) {
+          rest[mt][i] = bf16_pack2(e[2 * i] - __uint_as_float(p[mt][i] << 16), e[2 * i + 1] - __uint_as_float(p[mt][i] & 0xffff0000u));
+        }
+      }
     }
     // O^T += V^T P^T: dims 16 x + 4 grp + i of the output, row 16 mt + col
     const int vr = 4 * grp + (col >> 2);
@@ -630,6 +642,9 @@ struct Fp4Wave {
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt) {
         acc[mt][x] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fp4_bf16x8(v), fp4_bf16x8(p[mt]), acc[mt][x], 0, 0, 0);
+        if constexpr (kRest) {
+          acc[mt][x] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fp4_bf16x8(v), fp4_bf16x8(rest[mt]), acc[mt][x], 0, 0, 0);
+        }
       }
     }
   }
