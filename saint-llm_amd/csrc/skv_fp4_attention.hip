@@ -1198,11 +1198,12 @@ extern "C" int skv_fp4_attention(const skv_fp4_attention_desc* d, void* workspac
   if (a.D == p.dims) launch_dims<true>(a, p, s); else launch_dims<false>(a, p, s);
   if (const int rc = check_launch(what)) return rc;
   if (!p.cut) return SKV_OK;
-  // about 2,048 workgroups, a row each where there are fewer rows
+  // a row to a workgroup where that makes few of them, else to a wave, up to about 8,192 workgroups
   const int64_t units = p.items * a.Hkv, block_rows = std::min<int64_t>(p.rows, static_cast<int64_t>(a.T) * a.G);
-  const int64_t per = std::min(block_rows, ceil_div(units * block_rows, 2048));
+  const bool few = units * block_rows <= 2048;
+  const int64_t per = few ? 1 : std::min(block_rows, std::max<int64_t>(kF4Waves, ceil_div(units * block_rows, 8192)));
   const dim3 grid(static_cast<unsigned>(units), static_cast<unsigned>(ceil_div(block_rows, per)));
-  if (per == 1) {
+  if (few) {
     hipLaunchKernelGGL((k_fp4_attn_join<kF4Threads>), grid, dim3(kF4Threads), 0, s, a, p.rows, static_cast<int>(per));
   } else {
     hipLaunchKernelGGL((k_fp4_attn_join<kWave>), grid, dim3(kF4Threads), 0, s, a, p.rows, static_cast<int>(per));
