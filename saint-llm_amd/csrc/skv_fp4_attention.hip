@@ -129,8 +129,9 @@ constexpr int kF4RunTiles = 8;
 constexpr int kF4SmallTiles = 16;
 // What a segment costs beside its tiles, in tiles: the first loads' latencies and the
 // waves' join.  A step of 64 sequences of 1k - 32k, 8 K/V heads: 168 us without it (runs end
-// between 81 and 159 us), with 12, 16 and 20 tiles 146, 142 and 141 us.  Counted where there are about as many items
-// as workgroups or more; a run that would begin in this lead or just past it begins with the item.
+// between 81 and 159 us), with 12, 16 and 20 tiles 146, 142 and 141 us.  Counted where
+// there are about as many items as workgroups or more; a run that would begin in this
+// lead or just past it begins with the item.
 constexpr int kF4Lead = 20;
 // No (sequence, row block, head) is cut where a workgroup for each leaves less than an
 // eighth of the chip's time unused: there is nothing to join then.
@@ -237,7 +238,9 @@ struct Fp4Wave {
   // the rounded weight stands.
   static constexpr bool kRest = !kShared;
   static constexpr bool kTwo = DP * MT <= 256;  // two tiles in flight; wider ones have registers for one
-  static constexpr bool kOnce = !kShared && DP * MT <= 256;  // all of a head's rows in a workgroup: no page is read twice
+  // A page is read by one workgroup, or by two: nontemporal loads (a step of 64 sequences 169 us,
+  // 187 with plain ones; 64 rows on one head 69 and 67).
+  static constexpr bool kOnce = !kShared && DP * MT <= 256;
 
   const Fp4AttnArgs& a;
   const Fp4Span& sp;
