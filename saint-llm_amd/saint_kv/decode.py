@@ -562,8 +562,9 @@ class DecodeCache:
     def fork(self, src, dst) -> None:
         """Make the empty sequences dst[f] copies of src[f] (lists of sequences, or
         one of each): they share src's whole pages; begun pages, rings and pooling
-        states are copied.  Raises RuntimeError, with every sequence and free list
-        as before, if a page group lacks pages for the begun ones."""
+        states are copied.  Raises RuntimeError, with every sequence as before and
+        every page back on its free list (in whatever order), if a page group lacks
+        pages for the begun ones."""
         from saint_kv.fp4 import check_forks
 
         src, dst = check_forks(src, dst, self.host_lens)

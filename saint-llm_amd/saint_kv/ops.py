@@ -766,17 +766,20 @@ def fp4_gather(pool: torch.Tensor, block_table: torch.Tensor, seq_lens: torch.Te
 def _pool_refs(pools: list[torch.Tensor], n_pages: int, block_size: int) -> ctypes.Array:
     """skv_pool_refs of pools of n_pages pages of block_size rows."""
     refs = (_lib.PoolRef * len(pools))()
-    for i, p in enumerate(pools):
+    for ref, p in zip(refs, pools):
         _require_gpu(p, "pool")
         if not p.is_contiguous():
             raise ValueError("pool must be contiguous")
-        rb = row_bytes_of(p)
-        if p.shape[0] != n_pages or p.shape[1] != block_size:
+        shape = p.shape
+        if len(shape) < 3:
+            raise ValueError(f"pool must be [n_pages, block_size, *row]; got {tuple(shape)}")
+        if shape[0] != n_pages or shape[1] != block_size:
             raise ValueError("every pool must have n_pages pages of block_size rows")
-        if (block_size * rb) % 16:
-            raise ValueError(f"a pool's page must be a multiple of 16 bytes; got {block_size * rb}")
-        refs[i].base = p.data_ptr()
-        refs[i].page_bytes = block_size * rb
+        page = p.numel() // max(n_pages, 1) * p.element_size()
+        if page % 16:
+            raise ValueError(f"a pool's page must be a multiple of 16 bytes; got {page}")
+        ref.base = p.data_ptr()
+        ref.page_bytes = page
     return refs
 
 
@@ -805,8 +808,11 @@ def fork(free_stack: torch.Tensor, free_top: torch.Tensor, refs: torch.Tensor, b
     _require_i32(dst, "dst", tuple(src.shape))
     _require_i32(status, "status", (1,))
     _same_device(block_table, "block_table", free_stack=free_stack, free_top=free_top, refs=refs, seq_lens=seq_lens,
-                 src=src, dst=dst, status=status, **{f"pools[{i}]": p for i, p in enumerate(pools)})
+                 src=src, dst=dst, status=status)
     arr = _pool_refs(pools, n_pages, block_size)
+    for i, p in enumerate(pools):
+        if p.device != block_table.device:
+            raise ValueError(f"pools[{i}] is on {p.device}, block_table on {block_table.device}")
     with _on_device(block_table):
         _lib.call("skv_fork", free_stack.data_ptr(), free_top.data_ptr(), n_pages, refs.data_ptr(),
                   block_table.data_ptr(), bt_stride, seq_lens.data_ptr(), batch, block_size, src.data_ptr(),
