@@ -85,6 +85,46 @@ def test_many_sequences(dev, batch, kv, lens) -> None:
     check(fp4_attention(q, pool, bt, lens_t), q, pool, bt, lens_t)
 
 
+def test_many_row_blocks(dev) -> None:
+    """Whole prompts: more row blocks than are dealt out in runs, against the rows read back."""
+    from saint_kv import fp4_attention, ops
+
+    batch, t, heads, dim = 9, 2048, 16, 32
+    lens = [2048 + 7 * b for b in range(batch)]
+    pool, bt, lens_t = make(dev, lens, 64, 1, dim)
+    q = queries(dev, batch, t, heads, dim)
+    got = fp4_attention(q, pool, bt, lens_t)
+    k, v = (torch.zeros(batch, lens[-1], 1, dim, dtype=torch.bfloat16, device=dev) for _ in range(2))
+    ops.fp4_gather(pool, bt, lens_t, k, v, lens_t)
+    for b, h in ((0, 0), (0, 15), (5, 7), (8, 3)):
+        n = lens[b]
+        s = (q[b, :, h].double() @ k[b, :n, 0].double().T.contiguous()) * dim ** -0.5
+        seen = torch.arange(n, device=dev)[None, :] <= torch.arange(n - t, n, device=dev)[:, None]
+        p = torch.softmax(s.masked_fill(~seen, float("-inf")), 1)
+        want, a = p @ v[b, :n, 0].double(), p @ v[b, :n, 0].double().abs()
+        assert ((got[b, :, h].double() - want).abs() <= 2.0 ** -8 * want.abs() + 1.25 * 2.0 ** -8 * a).all()
+
+
+def test_two_streams_at_once(dev) -> None:
+    """Calls in flight together, each with a workspace of its own."""
+    from saint_kv import fp4_attention
+
+    work = []
+    for n, (t, heads, dim) in enumerate(((1, 8, 128), (80, 4, 64))):
+        pool, bt, lens = make(dev, [9000, 3000, 50], 64, 2, dim, seed=n)
+        q = queries(dev, 3, t, heads, dim, seed=n)
+        work.append((q, pool, bt, lens, fp4_attention(q, pool, bt, lens), torch.cuda.Stream(dev)))
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(10):
+        for q, pool, bt, lens, _, stream in work:
+            with torch.cuda.stream(stream):
+                got.append(fp4_attention(q, pool, bt, lens))
+    torch.cuda.synchronize()
+    for i, y in enumerate(got):
+        assert torch.equal(y, work[i % 2][4])
+
+
 @pytest.mark.parametrize("bad", [float("inf"), float("-inf"), float("nan")])
 @pytest.mark.parametrize("t,heads", [(1, 3), (1, 40), (70, 2)])
 def test_a_query_that_is_not_finite(dev, t, heads, bad) -> None:
