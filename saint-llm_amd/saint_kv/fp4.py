@@ -21,7 +21,7 @@ import numpy as np
 import torch
 
 from saint_kv import _lib, ops
-from saint_kv.ops import _on_device, _require_gpu, _require_i32, _same_device
+from saint_kv.ops import _launch, _require_gpu, _require_i32, _same_device
 
 _P = ctypes.c_void_p
 _I64 = ctypes.c_int64
@@ -92,8 +92,7 @@ def fp4_attention(q: torch.Tensor, pool: torch.Tensor, block_table: torch.Tensor
         ws_bytes = need
     if workspace is not None:
         ws_ptr = workspace.data_ptr()
-    with _on_device(q):
-        _lib.call("skv_fp4_attention", ctypes.byref(d), ws_ptr, ws_bytes, _lib.stream_handle(q.device))
+    _launch(q.device, "skv_fp4_attention", ctypes.byref(d), ws_ptr, ws_bytes)
     return out
 
 
@@ -115,11 +114,12 @@ def _desc(q, pool, block_table, seq_lens, n_new, window, sink, softcap, scale, m
     if q.dtype != torch.bfloat16 or q.dim() not in (3, 4):
         raise ValueError(f"q must be bf16 [B, H, D] or [B, T, H, D]; got {q.dtype} {tuple(q.shape)}")
     cache = ops.fp4_cache(pool, block_table)
-    batch, heads, dim = q.shape[0], q.shape[-2], q.shape[-1]
-    if batch != cache.batch or dim != cache.head_dim:
-        raise ValueError(f"q must have {cache.batch} sequences of head_dim {cache.head_dim}; got {tuple(q.shape)}")
-    if heads < 1 or heads % cache.n_kv_heads:
-        raise ValueError(f"q's {heads} heads are not a multiple of the pool's {cache.n_kv_heads}")
+    kv_heads, shape = cache.n_kv_heads, q.shape
+    batch, heads, dim = shape[0], shape[-2], shape[-1]
+    if batch != block_table.shape[0] or dim != cache.head_dim:
+        raise ValueError(f"q must have {cache.batch} sequences of head_dim {cache.head_dim}; got {tuple(shape)}")
+    if heads < 1 or heads % kv_heads:
+        raise ValueError(f"q's {heads} heads are not a multiple of the pool's {kv_heads}")
     _require_i32(seq_lens, "seq_lens", (batch,))
     if n_new is not None:
         _require_i32(n_new, "n_new", (batch,))
@@ -133,16 +133,18 @@ def _desc(q, pool, block_table, seq_lens, n_new, window, sink, softcap, scale, m
         _require_gpu(sink, "sink")
         if sink.dtype != torch.float32 or tuple(sink.shape) != (heads,) or not sink.is_contiguous():
             raise ValueError(f"sink must be a contiguous fp32 [{heads}] tensor")
-    q4 = q if q.dim() == 4 else q.unsqueeze(1)
-    strides = [2 * s if n > 1 else 0 for n, s in zip(q4.shape[:3], q4.stride()[:3])]
-    if q4.shape[1] < 1 or q4.stride(3) != 1 or q.data_ptr() % 16 or any(s % 16 for s in strides):
+    strides, data, tokens = q.stride(), q.data_ptr(), shape[1] if len(shape) == 4 else 1
+    seq = 2 * strides[0] if batch > 1 else 0
+    tok = 2 * strides[1] if tokens > 1 else 0
+    head = 2 * strides[-2] if heads > 1 else 0
+    if tokens < 1 or strides[-1] != 1 or (data | seq | tok | head) & 15:
         raise ValueError("q needs at least one token, contiguous dims and 16-byte aligned rows")
     if out is None:
-        out = torch.empty(q.shape, dtype=torch.bfloat16, device=q.device)
-    elif out.dtype != torch.bfloat16 or out.shape != q.shape or not out.is_contiguous() or out.data_ptr() % 16:
-        raise ValueError(f"out must be a contiguous bf16 {list(q.shape)} tensor, 16-byte aligned")
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    elif out.dtype != torch.bfloat16 or out.shape != shape or not out.is_contiguous() or out.data_ptr() % 16:
+        raise ValueError(f"out must be a contiguous bf16 {list(shape)} tensor, 16-byte aligned")
     _same_device(q, "q", pool=pool, seq_lens=seq_lens, n_new=n_new, sink=sink, out=out)
-    d = Fp4AttentionDesc(cache, seq_lens.data_ptr(), _lib.ptr(n_new), q4.shape[1], heads, q.data_ptr(), *strides, out.data_ptr(),
+    d = Fp4AttentionDesc(cache, seq_lens.data_ptr(), _lib.ptr(n_new), tokens, heads, data, seq, tok, head, out.data_ptr(),
                          _lib.ptr(sink), window or 0, int(max_len), int(splits), scale or 0.0, softcap or 0.0)
     return d, out
 

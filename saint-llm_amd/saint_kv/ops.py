@@ -30,25 +30,21 @@ def _require_i32(t: torch.Tensor, name: str, shape: tuple[int, ...] | None = Non
     _require_gpu(t, name)
     if t.dtype != INT32 or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous int32 tensor; got {t.dtype}")
-    if shape is not None and tuple(t.shape) != shape:
+    if shape is not None and t.shape != shape:
         raise ValueError(f"{name} must have shape {shape}; got {tuple(t.shape)}")
 
 
-class _on_device:
-    """Makes the tensor's device the current one for a launch, where it is not."""
-
-    def __init__(self, t: torch.Tensor) -> None:
-        self.index, self.back = t.device.index, -1
-
-    def __enter__(self) -> None:
-        here = torch.cuda.current_device()
-        if self.index is not None and self.index != here:
-            self.back = here
-            torch.cuda.set_device(self.index)
-
-    def __exit__(self, *exc) -> None:
-        if self.back >= 0:
-            torch.cuda.set_device(self.back)
+def _launch(device: torch.device, name: str, *args) -> None:
+    """Call an entry point whose last argument is the stream, with ``device``
+    current for the call where it is not."""
+    index, here = device.index, torch.cuda.current_device()
+    if index is None or index == here:
+        return _lib.call(name, *args, _lib.stream_handle(device))
+    torch.cuda.set_device(index)
+    try:
+        _lib.call(name, *args, _lib.stream_handle(device))
+    finally:
+        torch.cuda.set_device(here)
 
 
 def row_bytes_of(pool: torch.Tensor) -> int:
@@ -667,6 +663,7 @@ def indexer_topk_chunk(q: torch.Tensor, w: torch.Tensor, keys: torch.Tensor, n_b
 # 4-bit token cache
 # ---------------------------------------------------------------------------
 FP4_MAX_DIM = 512
+_FP4_INPUTS = (torch.bfloat16, torch.float32)
 
 
 def fp4_pool(n_pages: int, block_size: int, n_kv_heads: int, head_dim: int,
@@ -694,28 +691,33 @@ def fp4_cache(pool: torch.Tensor, block_table: torch.Tensor) -> _lib.Fp4Cache:
     _require_i32(block_table, "block_table")
     if block_table.dim() != 2:
         raise ValueError("block_table must be 2D [batch, max_pages]")
-    _same_device(pool, "pool", block_table=block_table)
+    if block_table.device != pool.device:
+        raise ValueError(f"block_table is on {block_table.device}, pool on {pool.device}")
     batch, bt_stride = block_table.shape
     return _lib.Fp4Cache(pool.data_ptr(), bs, n_pages, heads, row // 17 * 16, block_table.data_ptr(), bt_stride, batch)
 
 
 def _same_device(t: torch.Tensor, name: str, **others: torch.Tensor | None) -> None:
+    device = t.device
     for other, x in others.items():
-        if x is not None and x.device != t.device:
-            raise ValueError(f"{other} is on {x.device}, {name} on {t.device}")
+        if x is not None and x.device != device:
+            raise ValueError(f"{other} is on {x.device}, {name} on {device}")
 
 
-def _fp4_rows(t: torch.Tensor, name: str, cache: _lib.Fp4Cache, dtypes: tuple[torch.dtype, ...]) -> _lib.Fp4Rows:
+def _fp4_rows(t: torch.Tensor, name: str, like: tuple[int, int, int], dtypes: tuple[torch.dtype, ...]) -> _lib.Fp4Rows:
+    """skv_fp4_rows of t [B, T, heads, dim], of B, heads and dim as in ``like``."""
     _require_gpu(t, name)
-    if t.dtype not in dtypes or t.dim() != 4 or t.shape[0] != cache.batch or \
-            tuple(t.shape[2:]) != (cache.n_kv_heads, cache.head_dim):
-        raise ValueError(f"{name} must be {' or '.join(str(d) for d in dtypes)} [{cache.batch}, T, {cache.n_kv_heads}, "
-                         f"{cache.head_dim}]; got {t.dtype} {tuple(t.shape)}")
-    es = t.element_size()
-    strides = [s * es if n > 1 else 0 for n, s in zip(t.shape[:3], t.stride()[:3])]
-    if t.stride(3) != 1 or t.data_ptr() % 16 or any(s % 16 for s in strides):
+    shape = t.shape
+    if t.dtype not in dtypes or len(shape) != 4 or (shape[0], shape[2], shape[3]) != like:
+        raise ValueError(f"{name} must be {' or '.join(str(d) for d in dtypes)} [{like[0]}, T, {like[1]}, {like[2]}]; "
+                         f"got {t.dtype} {tuple(shape)}")
+    size, data, strides = t.element_size(), t.data_ptr(), t.stride()
+    seq = strides[0] * size if shape[0] > 1 else 0
+    tok = strides[1] * size if shape[1] > 1 else 0
+    head = strides[2] * size if shape[2] > 1 else 0
+    if strides[3] != 1 or (data | seq | tok | head) & 15:
         raise ValueError(f"{name} needs contiguous dims and 16-byte aligned rows")
-    return _lib.Fp4Rows(t.data_ptr(), *strides)
+    return _lib.Fp4Rows(data, seq, tok, head)
 
 
 def fp4_quant_append(pool: torch.Tensor, block_table: torch.Tensor, seq_lens: torch.Tensor, k: torch.Tensor,
@@ -725,17 +727,17 @@ def fp4_quant_append(pool: torch.Tensor, block_table: torch.Tensor, seq_lens: to
     n_kv_heads, head_dim], any strides that keep rows 16-byte aligned) becomes
     position ``seq_lens - n_new + i``."""
     c = fp4_cache(pool, block_table)
-    _require_i32(seq_lens, "seq_lens", (c.batch,))
-    rows = [_fp4_rows(t, name, c, (torch.bfloat16, torch.float32)) for t, name in ((k, "k"), (v, "v"))]
+    like = (block_table.shape[0], c.n_kv_heads, c.head_dim)
+    _require_i32(seq_lens, "seq_lens", like[:1])
+    k_rows, v_rows = _fp4_rows(k, "k", like, _FP4_INPUTS), _fp4_rows(v, "v", like, _FP4_INPUTS)
     if k.dtype != v.dtype or k.shape != v.shape:
         raise ValueError("k and v must have the same dtype and shape")
-    n_ptr, n_uni = _n_new_args(n_new, c.batch)
+    n_ptr, n_uni = _n_new_args(n_new, like[0])
     if n_ptr is None and n_uni > k.shape[1]:
         raise ValueError(f"n_new={n_uni} exceeds the {k.shape[1]} tokens of k and v")
     _same_device(pool, "pool", seq_lens=seq_lens, k=k, v=v, n_new=n_new if n_ptr is not None else None)
-    with _on_device(pool):
-        _lib.call("skv_fp4_quant_append", ctypes.byref(c), seq_lens.data_ptr(), n_ptr, n_uni, ctypes.byref(rows[0]),
-                  ctypes.byref(rows[1]), k.shape[1], int(k.dtype == torch.float32), _lib.stream_handle(pool.device))
+    _launch(pool.device, "skv_fp4_quant_append", ctypes.byref(c), seq_lens.data_ptr(), n_ptr, n_uni,
+            ctypes.byref(k_rows), ctypes.byref(v_rows), k.shape[1], int(k.dtype == torch.float32))
 
 
 def fp4_gather(pool: torch.Tensor, block_table: torch.Tensor, seq_lens: torch.Tensor, out_k: torch.Tensor,
@@ -744,19 +746,20 @@ def fp4_gather(pool: torch.Tensor, block_table: torch.Tensor, seq_lens: torch.Te
     ``seq_lens - n + i`` goes to token i of out_k, out_v (bf16 [B, T, n_kv_heads,
     head_dim]); later tokens of them are left as they are."""
     c = fp4_cache(pool, block_table)
-    _require_i32(seq_lens, "seq_lens", (c.batch,))
-    rows = [_fp4_rows(t, name, c, (torch.bfloat16,)) for t, name in ((out_k, "out_k"), (out_v, "out_v"))]
+    like = (block_table.shape[0], c.n_kv_heads, c.head_dim)
+    _require_i32(seq_lens, "seq_lens", like[:1])
+    k_rows, v_rows = _fp4_rows(out_k, "out_k", like, _FP4_INPUTS[:1]), _fp4_rows(out_v, "out_v", like, _FP4_INPUTS[:1])
     if out_k.shape != out_v.shape:
         raise ValueError("out_k and out_v must have the same shape")
-    if any(s == 0 and n > 1 for t in (out_k, out_v) for n, s in zip(t.shape, t.stride())):
+    if 0 in out_k.stride() + out_v.stride() and \
+            any(s == 0 and n > 1 for t in (out_k, out_v) for n, s in zip(t.shape, t.stride())):
         raise ValueError("out_k and out_v must not be expanded tensors")
-    n_ptr, n_uni = _n_new_args(n, c.batch)
+    n_ptr, n_uni = _n_new_args(n, like[0])
     if n_ptr is None and n_uni > out_k.shape[1]:
         raise ValueError(f"n={n_uni} exceeds the {out_k.shape[1]} tokens of out_k and out_v")
     _same_device(pool, "pool", seq_lens=seq_lens, out_k=out_k, out_v=out_v, n=n if n_ptr is not None else None)
-    with _on_device(pool):
-        _lib.call("skv_fp4_gather", ctypes.byref(c), seq_lens.data_ptr(), n_ptr, n_uni, ctypes.byref(rows[0]),
-                  ctypes.byref(rows[1]), out_k.shape[1], _lib.stream_handle(pool.device))
+    _launch(pool.device, "skv_fp4_gather", ctypes.byref(c), seq_lens.data_ptr(), n_ptr, n_uni, ctypes.byref(k_rows),
+            ctypes.byref(v_rows), out_k.shape[1])
     return out_k, out_v
 
 
@@ -813,11 +816,9 @@ def fork(free_stack: torch.Tensor, free_top: torch.Tensor, refs: torch.Tensor, b
     for i, p in enumerate(pools):
         if p.device != block_table.device:
             raise ValueError(f"pools[{i}] is on {p.device}, block_table on {block_table.device}")
-    with _on_device(block_table):
-        _lib.call("skv_fork", free_stack.data_ptr(), free_top.data_ptr(), n_pages, refs.data_ptr(),
-                  block_table.data_ptr(), bt_stride, seq_lens.data_ptr(), batch, block_size, src.data_ptr(),
-                  dst.data_ptr(), src.shape[0], ctypes.cast(arr, ctypes.c_void_p), len(pools), status.data_ptr(),
-                  _lib.stream_handle(block_table.device))
+    _launch(block_table.device, "skv_fork", free_stack.data_ptr(), free_top.data_ptr(), n_pages, refs.data_ptr(),
+            block_table.data_ptr(), bt_stride, seq_lens.data_ptr(), batch, block_size, src.data_ptr(), dst.data_ptr(),
+            src.shape[0], ctypes.byref(arr), len(pools), status.data_ptr())
 
 
 def copy_slots(arrays: list[torch.Tensor], src: torch.Tensor, dst: torch.Tensor) -> None:
@@ -839,9 +840,8 @@ def copy_slots(arrays: list[torch.Tensor], src: torch.Tensor, dst: torch.Tensor)
         refs[i].page_bytes = t[0].numel() * t.element_size() if n else 0
     _same_device(src, "src", dst=dst, **{f"arrays[{i}]": t for i, t in enumerate(arrays)})
     if n:
-        with _on_device(src):
-            _lib.call("skv_copy_slots", ctypes.cast(refs, ctypes.c_void_p), len(arrays), n, src.data_ptr(),
-                      dst.data_ptr(), src.shape[0], _lib.stream_handle(src.device))
+        _launch(src.device, "skv_copy_slots", ctypes.byref(refs), len(arrays), n, src.data_ptr(), dst.data_ptr(),
+                src.shape[0])
 
 
 def release(free_stack: torch.Tensor, free_top: torch.Tensor, block_table: torch.Tensor,
@@ -861,12 +861,11 @@ def release(free_stack: torch.Tensor, free_top: torch.Tensor, block_table: torch
         _require_i32(status, "status", (1,))
     if refs is not None:
         _require_i32(refs, "refs", (free_stack.numel(),))
-        with _on_device(block_table):
-            _lib.call("skv_release_shared", free_stack.data_ptr(), free_top.data_ptr(), free_stack.numel(),
-                      refs.data_ptr(), block_table.data_ptr(), bt_stride, seq_lens.data_ptr(),
-                      mask.contiguous().data_ptr(), batch, block_size, _lib.ptr(status),
-                      _lib.stream_handle(block_table.device))
-        return
+        _same_device(block_table, "block_table", free_stack=free_stack, free_top=free_top, refs=refs,
+                     seq_lens=seq_lens, mask=mask, status=status)
+        return _launch(block_table.device, "skv_release_shared", free_stack.data_ptr(), free_top.data_ptr(),
+                       free_stack.numel(), refs.data_ptr(), block_table.data_ptr(), bt_stride, seq_lens.data_ptr(),
+                       mask.contiguous().data_ptr(), batch, block_size, _lib.ptr(status))
     _lib.call("skv_release", free_stack.data_ptr(), free_top.data_ptr(), free_stack.numel(),
               block_table.data_ptr(), bt_stride, seq_lens.data_ptr(), mask.contiguous().data_ptr(),
               batch, block_size, _lib.ptr(status), _lib.stream_handle(block_table.device))
@@ -895,8 +894,6 @@ def compact(pools: list[torch.Tensor], block_table: torch.Tensor, seq_lens: torc
             seq_lens.data_ptr(), batch, block_size, n_pages, free_stack.data_ptr(), free_top.data_ptr())
     if refs is not None:
         _require_i32(refs, "refs", (n_pages,))
-        with _on_device(block_table):
-            _lib.call("skv_compact_shared", *args, refs.data_ptr(), workspace.data_ptr(), info.data_ptr(),
-                      _lib.stream_handle(block_table.device))
-        return
+        return _launch(block_table.device, "skv_compact_shared", *args, refs.data_ptr(), workspace.data_ptr(),
+                       info.data_ptr())
     _lib.call("skv_compact", *args, workspace.data_ptr(), info.data_ptr(), _lib.stream_handle(block_table.device))
