@@ -497,8 +497,9 @@ int skv_fp4_gather(const skv_fp4_cache* cache, const int32_t* seq_lens, const in
  * launch.  max_len bounds the lengths (0: what the table holds; longer ones are
  * still right): where it, or the window, shows that no sequence is worth cutting,
  * the call is one launch and needs no workspace.  splits > 0: at most that many
- * runs per K/V head and row block on average (0: as many as the device holds).  skv_fp4_attention_workspace returns the bytes that a call needs
- * (16-byte aligned; -1: bad descriptor).  The generalisation of the window
+ * runs per K/V head and row block on average (0: as many as the device holds),
+ * fewer than 2^24 runs in all.  skv_fp4_attention_workspace returns the bytes
+ * that a call needs (16-byte aligned; -1: bad descriptor).  The generalisation of the window
  * branch of SWAttention.forward (swa.py:115-137) to several K/V heads and the
  * whole history. */
 typedef struct skv_fp4_attention_desc {

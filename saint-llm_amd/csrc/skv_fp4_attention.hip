@@ -1118,8 +1118,12 @@ int fp4_attn_plan(const skv_fp4_attention_desc* d, Fp4AttnPlan& p) {
   const int64_t tiles = ceil_div(len, kF4Tile) + 1, units = std::max<int64_t>(p.items * hkv, 1);
   p.cut = tiles > kF4SmallTiles || d->splits > 0;
   if (p.items > kF4MaxItems || units > INT32_MAX / (ceil_div(capacity, kF4Tile) + 1 + kF4Lead)) p.cut = false;
+  if (units >= (1 << 24)) return set_error(SKV_EINVAL, "%s: too many workgroups", what);
+  if (p.cut && d->splits > ((1 << 24) - 1) / units) {  // before it is multiplied: the product could wrap
+    return set_error(SKV_EINVAL, "%s: splits must leave fewer than 2^24 runs; got %lld of %lld rows and heads", what,
+                     (long long)d->splits, (long long)units);
+  }
   p.groups = !p.cut ? 0 : d->splits > 0 ? d->splits * units : static_cast<int64_t>(fp4_resident(p.dims, p.mt)) * device_cus();
-  if (units >= (1 << 24) || p.groups >= (1 << 24)) return set_error(SKV_EINVAL, "%s: too many workgroups", what);
   p.sched_bytes = p.cut ? ceil_div((p.items + 2) * 4, 16) * 16 : 0;
   p.ws_bytes = p.cut ? p.sched_bytes + 2 * p.groups * p.rows * (D + 4) * 4 : 0;
   return SKV_OK;

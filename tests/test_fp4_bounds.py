@@ -1,0 +1,39 @@
+"""Arguments of the 4-bit cache that 64 bits hold and the launches do not: refused before anything
+is worked out of them (no GPU; the pointers are placeholders that a refused call never reads)."""
+
+from __future__ import annotations
+
+import ctypes
+
+import pytest
+
+FAKE = 4096  # aligned, never dereferenced
+
+
+@pytest.mark.parametrize("batch,kv_heads", [(1, 1), (3, 2), (8, 2), (4, 1), (512, 16)])
+@pytest.mark.parametrize("splits", [1 << 24, (1 << 24) + 1, 1 << 32, 1 << 58, 1 << 59, 1 << 60, 1 << 62, (1 << 63) - 1])
+def test_splits_past_any_launch_are_refused(batch: int, kv_heads: int, splits: int) -> None:
+    """Their product with the batch's items wraps to a small, zero or negative number of workgroups."""
+    from saint_kv import _lib
+    from saint_kv.fp4 import Fp4AttentionDesc
+
+    lib = _lib.load()
+    cache = _lib.Fp4Cache(FAKE, 64, 4096, kv_heads, 128, FAKE, 2048, batch)
+    d = Fp4AttentionDesc(cache=cache, seq_lens=FAKE, n_queries=1, n_heads=kv_heads, q=FAKE, out=FAKE, splits=splits)
+    assert lib.skv_fp4_attention_workspace(ctypes.byref(d)) == -1
+    assert "splits" in _lib.last_error()
+    assert lib.skv_fp4_attention(ctypes.byref(d), FAKE, (1 << 63) - 1, None) == _lib.SKV_EINVAL
+    assert "splits" in _lib.last_error()
+
+
+def test_the_most_splits() -> None:
+    """Up to the bound the workspace holds two pieces of every run: [rows] of m, l and 128 dims, in fp32."""
+    from saint_kv import _lib
+    from saint_kv.fp4 import Fp4AttentionDesc
+
+    lib = _lib.load()
+    for batch, kv_heads, splits in ((1, 1, (1 << 24) - 1), (4, 2, (1 << 21) - 1), (8, 2, 3)):
+        cache = _lib.Fp4Cache(FAKE, 64, 4096, kv_heads, 128, FAKE, 2048, batch)
+        d = Fp4AttentionDesc(cache=cache, seq_lens=FAKE, n_queries=1, n_heads=kv_heads, q=FAKE, out=FAKE, splits=splits)
+        sched = -(-(batch + 2) * 4 // 16) * 16
+        assert lib.skv_fp4_attention_workspace(ctypes.byref(d)) == sched + 2 * splits * batch * kv_heads * 16 * 132 * 4
