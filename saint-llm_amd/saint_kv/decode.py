@@ -99,7 +99,7 @@ class _Group:
     free_top: torch.Tensor
     block_table: torch.Tensor
     n_entries: torch.Tensor
-    refs: torch.Tensor | None = None  # int32 [n_pages] from the first fork on: a page's holders beyond the first
+    refs: torch.Tensor | None = None  # int32 [n_pages], with forks=True or from the first fork on: holders beyond the first
 
 
 class DecodeCache:
@@ -120,6 +120,12 @@ class DecodeCache:
     CSA/HCA layers and ``out_window``): the step then writes the top-k
     indices, pools, states, rings and lengths only, which is all a consumer
     reading the cache in place (``attention``) needs.
+
+    ``forks=True`` counts the holders of every page from the start, which a
+    caller needs who records ``release`` or ``compact`` in a HIP graph and forks
+    sequences later: a graph keeps the calls that it recorded.  Without it the
+    counts begin with the first ``fork`` (releases and compactions of pages with
+    one owner are faster), and ``fork`` refuses once such a call was recorded.
     """
 
     def __init__(self, layers: list[LayerSpec], batch: int, max_len: int, *,
@@ -127,7 +133,7 @@ class DecodeCache:
                  block_size: int = 64, device: torch.device | str | None = None,
                  page_order_seed: int | None = 0, pages_per_group: dict[int, int] | None = None,
                  hca_out_rows: int | None = None, score_cols: int | None = None,
-                 input_sets: int = 1, materialize: bool = True) -> None:
+                 input_sets: int = 1, materialize: bool = True, forks: bool = False) -> None:
         if not 0 < len(layers) <= MAX_LAYERS:
             raise ValueError(f"1..{MAX_LAYERS} layers supported; got {len(layers)}")
         scored = [s.idx_heads > 0 for s in layers if s.kind == "csa"]
@@ -181,7 +187,9 @@ class DecodeCache:
             self.groups.append(_Group(
                 m=m, n_pages=n_pages, free_stack=stack, free_top=top,
                 block_table=torch.full((batch, bt_stride), -1, dtype=torch.int32, device=dev),
-                n_entries=torch.zeros(batch, dtype=torch.int32, device=dev)))
+                n_entries=torch.zeros(batch, dtype=torch.int32, device=dev),
+                refs=torch.zeros(n_pages, dtype=torch.int32, device=dev) if forks else None))
+        self._recorded_unshared = False  # a release or compaction without counts is in some graph
         # compaction buffers: zeroed once; each page group has its own slice of
         # the workspace, whose page marks the compaction leaves zero
         self._compact_info = torch.zeros(max(len(self.groups), 1), 2, dtype=torch.int32, device=dev)
@@ -564,10 +572,14 @@ class DecodeCache:
         one of each): they share src's whole pages; begun pages, rings and pooling
         states are copied.  Raises RuntimeError, with every sequence as before and
         every page back on its free list (in whatever order), if a page group lacks
-        pages for the begun ones."""
+        pages for the begun ones; and before it does anything if a release or a
+        compaction of this cache was recorded in a graph without ``forks=True``."""
         from saint_kv.fp4 import check_forks
 
         src, dst = check_forks(src, dst, self.host_lens)
+        if self._recorded_unshared:
+            raise RuntimeError("a graph holds a release or compaction of this cache that does not count a page's "
+                               "holders; build the cache with forks=True to record those before the first fork")
         dev = self.device
         idx = torch.as_tensor(np.stack([src, dst]).astype(np.int32), device=dev)
         gst = self.group_status
@@ -590,6 +602,10 @@ class DecodeCache:
         ops.copy_slots([self.tok_lens, *slots], idx[0], idx[1])
         self.host_lens[dst] = self.host_lens[src]
 
+    def _note_recording(self) -> None:
+        if any(g.refs is None for g in self.groups) and torch.cuda.is_current_stream_capturing():
+            self._recorded_unshared = True
+
     def release(self, mask: np.ndarray, mask_dev: torch.Tensor | None = None, check: bool = True) -> None:
         """Finish the sequences with mask[b]: their pages return to the free lists.
 
@@ -605,6 +621,7 @@ class DecodeCache:
             raise ValueError("mask must be [batch]")
         if (mask & (self.host_lens == 0)).any():
             raise RuntimeError("release of a sequence that holds no tokens (double free)")
+        self._note_recording()
         m_dev = torch.as_tensor(mask.astype(np.uint8), device=self.device) if mask_dev is None else mask_dev
         for gi, g in enumerate(self.groups):
             ops.release(g.free_stack, g.free_top, g.block_table, g.n_entries, m_dev,
@@ -638,6 +655,7 @@ class DecodeCache:
         ws_all = workspace if workspace is not None else self._compact_ws
         if ws_all.numel() < self.compact_workspace_words():
             raise ValueError(f"compaction workspace needs {self.compact_workspace_words()} int32")
+        self._note_recording()
         ws_off = 0
         for gi, g in enumerate(self.groups):
             pools = self._group_pools(gi)
