@@ -89,7 +89,8 @@ struct Fp4AttnArgs {
   int32_t n_pages, bt_stride, bs;
   int32_t B, T, H, Hkv, G, D;
   int32_t window;  // 0: none
-  float scale, softcap;
+  float scale;             // to the log2 domain
+  float cap, cap_k;        // the softcap in the log2 domain (0: none); 2 log2(e) scale / softcap
   int32_t row_blocks;
   int32_t* sched;   // for the join: [items + 1] tiles before every (sequence, row block), and `small`
   int32_t lead;     // kF4Lead, or 0
@@ -154,6 +155,34 @@ __device__ __forceinline__ int fp4_owner(int x, int total, int n) {
   const uint32_t u = x;
   return static_cast<int>(u < longer ? u / (each + 1) : more + (u - longer) / each);
 }
+
+// cap tanh(x) of a score s in the log2 domain: lin s is the score without the cap, k s = u is
+// 2x log2(e).  tanh(x) = 1 - 2 / (exp(2x) + 1) has an error of 2^-23 whatever x is, which a cap far above
+// the scores would make as large as they are; for |x| < 1/4 the series stands instead, as a factor of
+// the score itself (its first term left out is 2^-26 there).  On either side 2^-20 of the result.
+struct Fp4Cap {
+  float lin, k, cap;
+  float c[4], sq;  // the series' coefficients; x^2 = sq u^2
+  __device__ __forceinline__ Fp4Cap(float lin_, float k_, float cap_) : lin(lin_), k(k_), cap(cap_) {
+    c[0] = -1.f / 3.f;
+    c[1] = 2.f / 15.f;
+    c[2] = -17.f / 315.f;
+    c[3] = 62.f / 2835.f;
+    sq = 0.25f / (kF4Log2e * kF4Log2e);
+    // made here, in scalar registers: as vector registers held through the tiles they cost calls without a
+    // cap 1-2% (64 sequences of 1k - 32k 137.6 us for 136.0, 4 of 256k - 1M 93.7 for 92.1)
+    asm volatile("" : "+s"(c[0]), "+s"(c[1]), "+s"(c[2]), "+s"(c[3]), "+s"(sq));
+  }
+  __device__ __forceinline__ float operator()(float s) const {
+    const float u = s * k, x2 = u * u * sq;
+    float f = __builtin_fmaf(x2, c[3], c[2]);
+    f = __builtin_fmaf(x2, f, c[1]);
+    f = __builtin_fmaf(x2, f, c[0]);
+    f = __builtin_fmaf(x2, f, 1.f);
+    const float far = cap * (1.f - 2.f * __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(u) + 1.f));
+    return __builtin_fabsf(u) < 0.5f * kF4Log2e ? s * lin * f : far;
+  }
+};
 
 __device__ __forceinline__ bf16x8 fp4_bf16x8(u32x4 v) { return __builtin_bit_cast(bf16x8, v); }
 
@@ -560,19 +589,17 @@ struct Fp4Wave {
   // The tile's weights, and its values times them onto the output.
   __device__ __forceinline__ void output(Fp4Tile<MT>& tl, int pos, const uint16_t* vt) {
     auto& st = tl.st;
-    const bool capped = a.softcap > 0.f;
-    float mult = a.scale * kF4Log2e;  // to the log2 domain
-    if (capped) {  // uniform; tanh(x) = 1 - 2 / (exp(2x) + 1)
-      const float k = 2.f * kF4Log2e * a.scale / a.softcap, cap = a.softcap * kF4Log2e;
+    const bool capped = a.cap > 0.f;
+    float mult = a.scale;
+    if (capped) {  // uniform
       mult = 1.f;
+      const Fp4Cap capped_score(a.scale, a.cap_k, a.cap);
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            st[mt][h][i] = cap * (1.f - 2.f * __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(st[mt][h][i] * k) + 1.f));
-          }
+          for (int i = 0; i < 4; ++i) st[mt][h][i] = capped_score(st[mt][h][i]);
         }
       }
     }
@@ -1192,8 +1219,10 @@ extern "C" int skv_fp4_attention(const skv_fp4_attention_desc* d, void* workspac
   a.G = a.H / a.Hkv;
   a.D = static_cast<int32_t>(d->cache.head_dim);
   a.window = static_cast<int32_t>(d->window);
-  a.scale = d->scale > 0.f ? d->scale : 1.f / sqrtf(static_cast<float>(a.D));
-  a.softcap = d->softcap;
+  const float scale = d->scale > 0.f ? d->scale : 1.f / sqrtf(static_cast<float>(a.D));
+  a.scale = scale * kF4Log2e;
+  a.cap = d->softcap * kF4Log2e;
+  a.cap_k = d->softcap > 0.f ? 2.f * kF4Log2e * scale / d->softcap : 0.f;
   a.B = static_cast<int32_t>(d->cache.batch);
   a.sched = p.cut ? static_cast<int32_t*>(workspace) : nullptr;
   a.part = p.cut ? reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + p.sched_bytes) : nullptr;
