@@ -206,7 +206,7 @@ extern "C" int skv_fork(int32_t* free_stack, int32_t* free_top, int64_t n_pages,
   if (n_pools < 0 || n_pools > kForkPools || (n_pools > 0 && !pools)) {
     return set_error(SKV_EINVAL, "%s: n_pools must be in [0, %d]; got %d", what, kForkPools, n_pools);
   }
-  if (!free_stack || !free_top || !refs || !block_table || !seq_lens || !src || !dst || !status) {
+  if (!free_stack || !free_top || !refs || !block_table || !seq_lens || !status || (n_forks > 0 && (!src || !dst))) {
     return set_error(SKV_EINVAL, "%s: NULL pointer", what);
   }
   ForkPools fp{};

@@ -580,6 +580,8 @@ class DecodeCache:
         if self._recorded_unshared:
             raise RuntimeError("a graph holds a release or compaction of this cache that does not count a page's "
                                "holders; build the cache with forks=True to record those before the first fork")
+        if not len(src):
+            return
         dev = self.device
         idx = torch.as_tensor(np.stack([src, dst]).astype(np.int32), device=dev)
         gst = self.group_status

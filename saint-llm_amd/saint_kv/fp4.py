@@ -253,6 +253,8 @@ class Fp4TokenCache:
         """Make the empty sequences dst[f] copies of src[f], sharing their whole
         pages; raises (and changes nothing) if the pool lacks a page for a begun one."""
         src, dst = check_forks(src, dst, self.host_lens)
+        if not len(src):
+            return
         self._take_pages(int((self.host_lens[src] % self.block_size != 0).sum()))
         idx = torch.as_tensor(np.stack([src, dst]).astype(np.int32), device=self.device)
         ops.fork(self.free_stack, self.free_top, self.refs, self.block_table, self.seq_lens, idx[0], idx[1],

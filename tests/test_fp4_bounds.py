@@ -37,3 +37,17 @@ def test_the_most_splits() -> None:
         d = Fp4AttentionDesc(cache=cache, seq_lens=FAKE, n_queries=1, n_heads=kv_heads, q=FAKE, out=FAKE, splits=splits)
         sched = -(-(batch + 2) * 4 // 16) * 16
         assert lib.skv_fp4_attention_workspace(ctypes.byref(d)) == sched + 2 * splits * batch * kv_heads * 16 * 132 * 4
+
+
+def test_no_forks_need_no_indices() -> None:
+    """An empty device array has no address."""
+    from saint_kv import _lib
+
+    lib = _lib.load()
+
+    def fork(n, src, dst):
+        return lib.skv_fork(FAKE, FAKE, 8, FAKE, FAKE, 4, FAKE, 3, 16, src, dst, n, None, 0, FAKE, None)
+
+    assert fork(0, None, None) == 0
+    for src, dst in ((None, FAKE), (FAKE, None)):
+        assert fork(1, src, dst) == _lib.SKV_EINVAL and "NULL" in _lib.last_error()

@@ -105,3 +105,21 @@ def test_counts_from_the_start_change_nothing_else(dev) -> None:
         assert torch.equal(a.block_table, b.block_table) and torch.equal(a.n_entries, b.n_entries)
         top = int(a.free_top)
         assert top == int(b.free_top) and torch.equal(a.free_stack[:top], b.free_stack[:top])
+
+
+def test_no_forks(dev) -> None:
+    """Nothing named, nothing done: the decode cache, the 4-bit cache and the call below them."""
+    from saint_kv import Fp4TokenCache, ops
+
+    cache = _prefilled(dev, [203, 0, 77, 0, 20])
+    before = _state(cache)
+    cache.fork([], [])
+    assert all(torch.equal(a, b) for a, b in zip(_state(cache), before))
+    four = Fp4TokenCache(1, 2, 64, 1, 64, block_size=16, device=dev)
+    four.reserve(20)
+    four.fork([], [])
+    none = torch.zeros(0, dtype=torch.int32, device=dev)
+    ops.fork(four.free_stack, four.free_top, four.refs, four.block_table, four.seq_lens, none, none, 16, four.pool,
+             four.status)
+    ops.copy_slots([four.seq_lens], none, none)
+    assert four.seq_lens.tolist() == four.host_lens.tolist() == [20, 20] and four.host_free == int(four.free_top)
