@@ -285,7 +285,9 @@ class Fp4TokenCache:
 
 
 def check_forks(src, dst, host_lens: np.ndarray) -> tuple[np.ndarray, np.ndarray]:
-    """The sequences of a fork as arrays, or the error of forks that cannot be."""
+    """The sequences of a fork as arrays, or the error of forks that cannot be.  Copies of
+    an empty sequence are left out: a destination is empty already, and one that is
+    another fork's source too would be read while it is written."""
     src, dst = np.atleast_1d(np.asarray(src, dtype=np.int64)), np.atleast_1d(np.asarray(dst, dtype=np.int64))
     if src.ndim != 1 or src.shape != dst.shape:
         raise ValueError("src and dst must name as many sequences")
@@ -296,4 +298,5 @@ def check_forks(src, dst, host_lens: np.ndarray) -> tuple[np.ndarray, np.ndarray
         raise ValueError("a sequence cannot be forked to twice")
     if (host_lens[dst] != 0).any():
         raise RuntimeError("a fork needs empty sequences to go to; release them first")
-    return src, dst
+    held = host_lens[src] != 0
+    return src[held], dst[held]

@@ -1,10 +1,11 @@
-"""Arguments of the 4-bit cache that 64 bits hold and the launches do not: refused before anything
-is worked out of them (no GPU; the pointers are placeholders that a refused call never reads)."""
+"""Arguments of the 4-bit cache and of forks at the ends of what they may be, refused or sorted out on
+the host (no GPU; the pointers are placeholders that a refused call never reads)."""
 
 from __future__ import annotations
 
 import ctypes
 
+import numpy as np
 import pytest
 
 FAKE = 4096  # aligned, never dereferenced
@@ -51,3 +52,11 @@ def test_no_forks_need_no_indices() -> None:
     assert fork(0, None, None) == 0
     for src, dst in ((None, FAKE), (FAKE, None)):
         assert fork(1, src, dst) == _lib.SKV_EINVAL and "NULL" in _lib.last_error()
+
+
+def test_forks_of_empty_sequences_are_left_out() -> None:
+    """Also where the empty source is another fork's destination: all copies are of what was there before."""
+    from saint_kv.fp4 import check_forks
+
+    src, dst = check_forks([0, 1, 2, 3], [1, 4, 5, 2], np.array([5, 0, 0, 7, 0, 0]))
+    assert src.tolist() == [0, 3] and dst.tolist() == [1, 2]

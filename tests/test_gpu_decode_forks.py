@@ -123,3 +123,17 @@ def test_no_forks(dev) -> None:
              four.status)
     ops.copy_slots([four.seq_lens], none, none)
     assert four.seq_lens.tolist() == four.host_lens.tolist() == [20, 20] and four.host_free == int(four.free_top)
+
+
+def test_a_source_that_is_a_destination_too(dev) -> None:
+    """All copies are of what the sources were before the call: of an empty one, an empty sequence."""
+    cache = _prefilled(dev, [203, 0, 77, 0, 0])
+    cache.fork([0, 1, 3], [1, 3, 4])
+    assert cache.host_lens.tolist() == cache.tok_lens.tolist() == [203, 203, 77, 0, 0]
+    for g in cache.groups:
+        assert g.n_entries.tolist() == [n // g.m for n in (203, 203, 77, 0, 0)]
+    cache.fork([3], [4])
+    assert cache.tok_lens.tolist() == [203, 203, 77, 0, 0]
+    cache.release(np.array([1, 1, 1, 0, 0], dtype=bool))
+    for g in cache.groups:
+        assert int(g.free_top) == g.n_pages
