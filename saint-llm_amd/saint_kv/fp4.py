@@ -260,6 +260,8 @@ class Fp4TokenCache:
         ops.fork(self.free_stack, self.free_top, self.refs, self.block_table, self.seq_lens, idx[0], idx[1],
                  self.block_size, self.pool, self.status)
         self.host_lens[dst] = self.host_lens[src]
+        if isinstance(self._n_new, torch.Tensor):  # the newest tokens of a copy are its source's
+            ops.copy_slots([self._n_new], idx[0], idx[1])
 
     def release(self, mask: np.ndarray) -> None:
         """Finish the sequences with mask[b]: the pages that no other sequence holds
