@@ -197,6 +197,10 @@ class Fp4TokenCache:
         self.status = torch.zeros(1, **i32)
         self.host_lens, self.host_free = np.zeros(batch, dtype=np.int64), self.n_pages
         self._n_new: int | torch.Tensor = 0
+        self._host_new = np.zeros(batch, dtype=np.int64)  # each sequence's tokens reserved last
+        self._unwritten: set[int] = set()  # layers that these have not been appended to
+        self._recorded: set[int] = set()  # layers that a graph appends to
+        self._shared = False  # some of these lie in shared pages
         self._compact_ws = torch.zeros(3 * self.n_pages, **i32)
         self._compact_info = torch.zeros(2, **i32)
 
@@ -217,6 +221,8 @@ class Fp4TokenCache:
         ops.reserve(self.free_stack, self.free_top, self.block_table, self.seq_lens, self._n_new, self.block_size,
                     self.status)
         self.host_lens = self.host_lens + counts
+        self._host_new, self._shared = counts.copy(), False
+        self._unwritten = set(range(len(self.pool))) if counts.any() else set()
 
     def _take_pages(self, need: int) -> None:
         if need > self.host_free:
@@ -225,8 +231,15 @@ class Fp4TokenCache:
 
     def append(self, i: int, k: torch.Tensor, v: torch.Tensor) -> None:
         """Layer i's keys and values [B, T, Hkv, D] of the tokens reserved last
-        (of sequence b the first n_new[b])."""
+        (of sequence b the first n_new[b]); not after a fork of these, which lie in
+        shared pages then."""
+        if self._shared:
+            raise RuntimeError("the tokens reserved last are a fork's, too; reserve new ones to append")
         ops.fp4_quant_append(self.pool[i], self.block_table, self.seq_lens, k, v, self._n_new)
+        layer = range(len(self.pool))[i]
+        self._unwritten.discard(layer)
+        if torch.cuda.is_current_stream_capturing():
+            self._recorded.add(layer)
 
     def attention(self, i: int, q: torch.Tensor, *, window: int | None = None, sink: torch.Tensor | None = None,
                   softcap: float | None = None, scale: float | None = None,
@@ -251,10 +264,16 @@ class Fp4TokenCache:
     # ------------------------------------------------------ forks, eviction --
     def fork(self, src: list[int], dst: list[int]) -> None:
         """Make the empty sequences dst[f] copies of src[f], sharing their whole
-        pages; raises (and changes nothing) if the pool lacks a page for a begun one."""
+        pages; raises (and changes nothing) if the pool lacks a page for a begun one, or
+        a layer still has to append the tokens that a source reserved last (layers whose
+        append a graph replays are taken to have done so)."""
         src, dst = check_forks(src, dst, self.host_lens)
         if not len(src):
             return
+        newest = self._host_new[src]
+        missing = self._unwritten - self._recorded
+        if newest.any() and missing:
+            raise RuntimeError(f"a fork's source has reserved tokens that have not been appended to layers {sorted(missing)}")
         self._take_pages(int((self.host_lens[src] % self.block_size != 0).sum()))
         idx = torch.as_tensor(np.stack([src, dst]).astype(np.int32), device=self.device)
         ops.fork(self.free_stack, self.free_top, self.refs, self.block_table, self.seq_lens, idx[0], idx[1],
@@ -262,6 +281,8 @@ class Fp4TokenCache:
         self.host_lens[dst] = self.host_lens[src]
         if isinstance(self._n_new, torch.Tensor):  # the newest tokens of a copy are its source's
             ops.copy_slots([self._n_new], idx[0], idx[1])
+        self._host_new[dst] = newest
+        self._shared |= bool(newest.any())
 
     def release(self, mask: np.ndarray) -> None:
         """Finish the sequences with mask[b]: the pages that no other sequence holds
@@ -274,6 +295,7 @@ class Fp4TokenCache:
         ops.release(self.free_stack, self.free_top, self.block_table, self.seq_lens,
                     torch.as_tensor(mask.astype(np.uint8), device=self.device), self.block_size, self.status,
                     refs=self.refs)
+        self._host_new[mask] = 0
         self.check_status()
         self.host_lens[mask] = 0
         self.host_free = int(self.free_top.item())

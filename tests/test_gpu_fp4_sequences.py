@@ -11,6 +11,15 @@ from test_gpu_fp4_cache import DIM, HEADS, KV, LAYERS, Model, new_cache
 pytestmark = pytest.mark.gpu
 
 
+def _books(cache):
+    return [x.clone() for x in (cache.block_table, cache.seq_lens, cache.refs, cache.free_top, cache.free_stack)]
+
+
+def _same(cache, before, lens) -> None:
+    assert all(torch.equal(a, b) for a, b in zip(_books(cache), before))
+    assert cache.host_lens.tolist() == list(lens) and cache.host_free == int(cache.free_top)
+
+
 @pytest.mark.parametrize("counts", [[37, 20, 0, 0, 5], [1, 1, 0, 0, 1], [16, 32, 0, 0, 3]])
 def test_attention_right_after_a_fork(dev, counts) -> None:
     """A fork of a ragged prompt gives its source's outputs, and the others give what they gave."""
@@ -29,3 +38,72 @@ def test_attention_right_after_a_fork(dev, counts) -> None:
     m.q[4] = m.q[1]
     got = cache.attention(LAYERS - 1, m.q)
     assert torch.equal(got[4], got[1]) and torch.equal(got[0], want[-1][0])
+
+
+def _rows(dev, t, heads=KV):
+    return torch.ones(5, t, heads, DIM, dtype=torch.bfloat16, device=dev)
+
+
+def test_a_fork_of_tokens_to_be_written_is_refused(dev) -> None:
+    """Until every layer has them; forks of the other sequences go on, and the tokens still can be written."""
+    cache = new_cache(dev)
+    Model(dev, cache).step(np.array([20, 18, 0, 0, 0]))
+    cache.reserve(np.array([16, 0, 0, 0, 0]))
+    before = _books(cache)
+    for i in range(LAYERS):
+        with pytest.raises(RuntimeError, match="not been appended"):
+            cache.fork([1, 0], [2, 3])
+        _same(cache, before, [36, 18, 0, 0, 0])
+        if i == 1:
+            cache.fork([1], [2])
+            before = _books(cache)
+            cache.release(np.array([0, 0, 1, 0, 0]))
+            before = _books(cache)
+        cache.append(i, _rows(dev, 16), _rows(dev, 16))
+    cache.fork([1, 0], [2, 3])
+    assert cache.host_lens.tolist() == [36, 18, 18, 36, 0]
+
+
+def test_an_append_after_a_fork_needs_a_reservation(dev) -> None:
+    """The tokens reserved last lie in pages that are shared now."""
+    cache = new_cache(dev)
+    Model(dev, cache).step(np.array([32, 0, 0, 0, 0]))
+    cache.fork([0], [1])
+    before = [p.clone() for p in cache.pool]
+    with pytest.raises(RuntimeError, match="reserve"):
+        cache.append(0, _rows(dev, 32), _rows(dev, 32))
+    assert all(torch.equal(a, b) for a, b in zip(cache.pool, before))
+    Model(dev, cache).step(np.array([1, 1, 0, 0, 0]))
+
+
+def test_appends_that_a_graph_replays(dev) -> None:
+    """Steps of an eager reservation and a replayed append and attention, with forks between them."""
+    cache, eager = new_cache(dev), new_cache(dev)
+    for c in (cache, eager):
+        Model(dev, c).step(np.array([20, 33, 0, 0, 0]))
+    g = torch.Generator(device=dev).manual_seed(3)
+    k, v, q = (torch.randn(5, 1, h, DIM, generator=g, device=dev).to(torch.bfloat16) for h in (KV, KV, HEADS))
+
+    def layers(c):
+        for i in range(LAYERS):
+            c.append(i, k, v)
+        return [c.attention(i, q) for i in range(LAYERS)]
+
+    for c in (cache, eager):
+        c.reserve(1)
+        layers(c)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = layers(cache)
+    for n in range(3):
+        for c in (cache, eager):
+            c.release(np.array([0, 0, 1, 1, 0]))
+            c.fork([1, 0], [2, 3])
+            c.reserve(1)
+        for x in (k, v, q):
+            x.normal_(generator=g)
+        graph.replay()
+        want = layers(eager)
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, want)), n
