@@ -27,6 +27,7 @@ _P = ctypes.c_void_p
 _I64 = ctypes.c_int64
 MAX_LAYERS = 16
 MAX_BATCH = 4096
+STATUS_WORDS = 64
 
 
 class Fp4AttentionDesc(ctypes.Structure):
@@ -195,6 +196,11 @@ class Fp4TokenCache:
                                     device=dev)
         ops.free_stack_init(self.free_stack, self.free_top, order)
         self.status = torch.zeros(1, **i32)
+        # the calls' status words, in turn: a call that succeeds clears its word, which must not be
+        # that of one whose refusal nobody has read
+        self._words = torch.zeros(STATUS_WORDS, **i32)
+        self._word_views = list(self._words.split(1))
+        self._word, self._refusals = 0, torch.zeros(STATUS_WORDS, **i32)
         self.host_lens, self.host_free = np.zeros(batch, dtype=np.int64), self.n_pages
         self._n_new: int | torch.Tensor = 0
         self._host_new = np.zeros(batch, dtype=np.int64)  # each sequence's tokens reserved last
@@ -219,10 +225,17 @@ class Fp4TokenCache:
         self._n_new = int(n_new) if np.ndim(n_new) == 0 else torch.as_tensor(counts.astype(np.int32),
                                                                             device=self.device)
         ops.reserve(self.free_stack, self.free_top, self.block_table, self.seq_lens, self._n_new, self.block_size,
-                    self.status)
+                    self._status_word())
         self.host_lens = self.host_lens + counts
         self._host_new, self._shared = counts.copy(), False
         self._unwritten = set(range(len(self.pool))) if counts.any() else set()
+
+    def _status_word(self) -> torch.Tensor:
+        if self._word == STATUS_WORDS:  # all used: what they hold is kept aside
+            self._refusals.bitwise_or_(self._words)
+            self._word = 0
+        self._word += 1
+        return self._word_views[self._word - 1]
 
     def _take_pages(self, need: int) -> None:
         if need > self.host_free:
@@ -251,15 +264,16 @@ class Fp4TokenCache:
                              softcap=softcap, scale=scale, max_len=int(self.host_lens.max()), out=out)
 
     def check_status(self) -> None:
-        """Synchronise and raise if the device refused the last reservation, fork or
-        release, as it does where the tables were changed behind the host's back (it
-        wrote nothing; the host's counts are read back)."""
-        st = int(self.status.item())
-        if st:
-            self.status.zero_()
+        """Synchronise and raise if the device refused a reservation, fork or release
+        since the last check, as it does where the tables were changed behind the
+        host's back (it wrote nothing; the host's counts are read back)."""
+        bits = int(np.bitwise_or.reduce(torch.cat((self._refusals, self._words, self.status)).cpu().numpy()))
+        if bits:
+            for t in (self._refusals, self._words, self.status):
+                t.zero_()
             self.host_lens = self.seq_lens.cpu().numpy().astype(np.int64)
             self.host_free = int(self.free_top.item())
-            raise RuntimeError(f"Fp4TokenCache reservation, fork or release refused (status bits {st})")
+            raise RuntimeError(f"Fp4TokenCache reservation, fork or release refused (status bits {bits})")
 
     # ------------------------------------------------------ forks, eviction --
     def fork(self, src: list[int], dst: list[int]) -> None:
@@ -277,7 +291,7 @@ class Fp4TokenCache:
         self._take_pages(int((self.host_lens[src] % self.block_size != 0).sum()))
         idx = torch.as_tensor(np.stack([src, dst]).astype(np.int32), device=self.device)
         ops.fork(self.free_stack, self.free_top, self.refs, self.block_table, self.seq_lens, idx[0], idx[1],
-                 self.block_size, self.pool, self.status)
+                 self.block_size, self.pool, self._status_word())
         self.host_lens[dst] = self.host_lens[src]
         if isinstance(self._n_new, torch.Tensor):  # the newest tokens of a copy are its source's
             ops.copy_slots([self._n_new], idx[0], idx[1])
@@ -293,7 +307,7 @@ class Fp4TokenCache:
         if (mask & (self.host_lens == 0)).any():
             raise RuntimeError("release of a sequence that holds no tokens (double free)")
         ops.release(self.free_stack, self.free_top, self.block_table, self.seq_lens,
-                    torch.as_tensor(mask.astype(np.uint8), device=self.device), self.block_size, self.status,
+                    torch.as_tensor(mask.astype(np.uint8), device=self.device), self.block_size, self._status_word(),
                     refs=self.refs)
         self._host_new[mask] = 0
         self.check_status()

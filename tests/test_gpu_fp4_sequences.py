@@ -107,3 +107,31 @@ def test_appends_that_a_graph_replays(dev) -> None:
         want = layers(eager)
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(out, want)), n
+
+
+def test_a_refusal_is_reported_whatever_comes_after(dev) -> None:
+    """The device refuses where the free list was changed behind the host's back; later calls succeed."""
+    cache = new_cache(dev)
+    Model(dev, cache).step(np.array([20, 0, 0, 0, 0]))
+
+    def without_pages(call):
+        top = cache.free_top.clone()
+        cache.free_top.zero_()
+        call()
+        cache.free_top.copy_(top)
+
+    for later in (1, 200):
+        for refused in (lambda: cache.reserve(np.array([0, 17, 0, 0, 0])), lambda: cache.fork([0], [2])):
+            without_pages(refused)
+            for _ in range(later):
+                cache.reserve(0)
+            with pytest.raises(RuntimeError, match="refused"):
+                cache.check_status()
+            assert cache.host_lens.tolist() == cache.seq_lens.tolist() == [20, 0, 0, 0, 0]
+            assert cache.host_free == int(cache.free_top)
+            cache.check_status()  # reported once
+    without_pages(lambda: cache.reserve(np.array([0, 17, 0, 0, 0])))
+    cache.reserve(0)
+    with pytest.raises(RuntimeError, match="refused"):
+        cache.release(np.array([1, 0, 0, 0, 0]))
+    assert cache.host_lens.tolist() == cache.seq_lens.tolist() and cache.host_free == int(cache.free_top)
