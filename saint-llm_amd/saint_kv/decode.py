@@ -164,6 +164,8 @@ class DecodeCache:
         # one status word per page group for the host-driven reserve / release
         # calls (a later group's success must not hide an earlier refusal)
         self.group_status = torch.zeros(MAX_GROUPS, dtype=torch.int32, device=dev)
+        # and the forks' own: check_release() may not have read a release's yet
+        self.fork_status = torch.zeros(MAX_GROUPS, dtype=torch.int32, device=dev)
         self.host_lens = np.zeros(batch, dtype=np.int64)
         self._attn_ws: dict[int | str, torch.Tensor] = {}  # per layer, and "step" for step_attend
 
@@ -584,7 +586,7 @@ class DecodeCache:
             return
         dev = self.device
         idx = torch.as_tensor(np.stack([src, dst]).astype(np.int32), device=dev)
-        gst = self.group_status
+        gst = self.fork_status
         for gi, g in enumerate(self.groups):
             if g.refs is None:
                 g.refs = torch.zeros(g.n_pages, dtype=torch.int32, device=dev)

@@ -137,3 +137,23 @@ def test_a_source_that_is_a_destination_too(dev) -> None:
     cache.release(np.array([1, 1, 1, 0, 0], dtype=bool))
     for g in cache.groups:
         assert int(g.free_top) == g.n_pages
+
+
+def test_a_fork_keeps_the_word_of_a_release(dev) -> None:
+    cache = _prefilled(dev, [203, 0, 77, 0, 20])
+    g = cache.groups[0]
+    top = g.free_top.clone()
+    g.free_top.fill_(g.n_pages)  # the pages would not fit: refused
+    cache.release(np.array([0, 0, 0, 0, 1], dtype=bool), check=False)
+    g.free_top.copy_(top)
+    cache.fork(0, 1)
+    with pytest.raises(RuntimeError, match="release refused"):
+        cache.check_release()
+
+
+def test_a_refused_fork_is_no_refused_release(dev) -> None:
+    cache = _prefilled(dev, [101, 110, 0, 0, 0], pages_per_group={4: 30, 8: 8})
+    with pytest.raises(RuntimeError, match="fork refused"):
+        cache.fork([1, 1], [2, 3])
+    cache.check_release()
+    cache.release(np.array([1, 0, 0, 0, 0], dtype=bool))
