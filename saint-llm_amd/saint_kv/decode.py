@@ -571,8 +571,10 @@ class DecodeCache:
 
     def fork(self, src, dst) -> None:
         """Make the empty sequences dst[f] copies of src[f] (lists of sequences, or
-        one of each): they share src's whole pages; begun pages, rings and pooling
-        states are copied.  Raises RuntimeError, with every sequence as before and
+        one of each): they share src's whole pages; begun pages, rings, pooling states
+        and the last step's picks are copied, so that ``attention`` gives both the
+        same at once (a ``v_ring`` is the caller's to copy, as are the step's gathered
+        copies; see ``ops.copy_slots``).  Raises RuntimeError, with every sequence as before and
         every page back on its free list (in whatever order), if a page group lacks
         pages for the begun ones; and before it does anything if a release or a
         compaction of this cache was recorded in a graph without ``forks=True``."""
@@ -602,7 +604,7 @@ class DecodeCache:
                                 refs=g.refs)
             raise RuntimeError("DecodeCache fork refused (" + "; ".join(
                 f"group m={g.m}: status bits {b}" for g, b in zip(self.groups, bad) if b) + ")")
-        slots = [t for t in (*self.ring, *self.state, *self.idx_state) if t is not None]
+        slots = [t for t in (*self.ring, *self.state, *self.idx_state, *self.topk_idx) if t is not None]
         ops.copy_slots([self.tok_lens, *slots], idx[0], idx[1])
         self.host_lens[dst] = self.host_lens[src]
 

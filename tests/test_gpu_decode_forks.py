@@ -157,3 +157,30 @@ def test_a_refused_fork_is_no_refused_release(dev) -> None:
         cache.fork([1, 1], [2, 3])
     cache.check_release()
     cache.release(np.array([1, 0, 0, 0, 0], dtype=bool))
+
+
+def test_attention_of_a_fork_before_the_next_step(dev) -> None:
+    """The last step's picks are the source's."""
+    from saint_kv import DecodeCache, LayerSpec
+
+    layers = [LayerSpec("csa", m=4, top_k=32), LayerSpec("hca", m=128), LayerSpec("swa")]
+    cache = DecodeCache(layers, 3, 2048, window=32, block_size=16, device=dev)
+    g = torch.Generator(device=dev).manual_seed(0)
+    cache.prefill(np.array([1500, 300, 0]), generator=g)
+    for i in range(3):
+        for x in cache.inputs[i].values():
+            x.normal_(generator=g)
+    cache.scores[0].normal_(generator=g)
+    cache.step()
+    cache.check_status()
+    q = torch.randn(3, 16, cache.latent, generator=g, device=dev).to(torch.bfloat16)
+    knw = torch.ones(cache.latent, device=dev)
+    want = [cache.attention(i, q, None if layers[i].kind == "swa" else knw).clone() for i in range(3)]
+    cache.release(np.array([0, 1, 1], dtype=bool))
+    cache.fork([0, 0], [1, 2])
+    q[1] = q[2] = q[0]
+    for i in range(3):
+        got = cache.attention(i, q, None if layers[i].kind == "swa" else knw)
+        for b in range(3):
+            assert torch.equal(got[b], got[0])
+        assert torch.equal(got[0], want[i][0])
