@@ -13,6 +13,8 @@
 //             is exactly [0, n_live) and pops return n_live, n_live+1, ...
 //             Sources are all >= n_live and destinations all < n_live, so the
 //             page copies are independent and run fully in parallel.
+#include <algorithm>
+
 #include "skv_common.h"
 
 namespace skv {
@@ -307,9 +309,11 @@ __global__ __launch_bounds__(kEvictThreads) void k_release_shared(
 }
 
 // ---- compaction -------------------------------------------------------------
+// The pools of a copy launch, or the parts of their pages that it copies: page_bytes
+// from page to page, part_bytes of each from base on.
 struct PoolRefs {
   uint8_t* base[kMaxPools];
-  int64_t page_bytes[kMaxPools];
+  int64_t page_bytes[kMaxPools], part_bytes[kMaxPools];
   int n;
 };
 
@@ -465,7 +469,8 @@ struct CopySlices {
 // stores, so only the first iteration waits for them.  The same grid first
 // rewrites the block tables (every table entry of a live page at or above
 // n_live takes the hole of its rank, which it then clears) and clears the
-// plan's marks below n_live.
+// plan's marks below n_live.  Slices are counted below 2^24: more of them are
+// copied by more launches, which come with no table (batch 0).
 struct TableRef {
   int32_t* bt;
   const int32_t* lens;
@@ -510,9 +515,10 @@ __global__ __launch_bounds__(kCompactCopyThreads) void k_compact_copy(PoolRefs p
   int s0 = blockIdx.x * kCopySlices;
   int32_t src_id[kCopySlices], dst_id[kCopySlices];
   if (s0 < total) slice_ids(cs, movers, holes, s0, total, src_id, dst_id);  // in flight during the rewrite
-  const int entries = tr.batch * tr.bt_stride;  // < 2^24 (checked on the host)
+  const int entries = tr.batch * tr.bt_stride;  // <= 2^30 (checked on the host)
+  const bool far = entries >= 1 << 24;
   for (int t = gtid; t < entries; t += gsize) {
-    const int b = static_cast<int>(udiv24(t, tr.bt_stride));
+    const int b = far ? t / tr.bt_stride : static_cast<int>(udiv24(t, tr.bt_stride));
     const int j = t - b * tr.bt_stride;
     const int np = static_cast<int>(min<int64_t>(ceil_div24(max(tr.lens[b], 0), tr.block_size), tr.bt_stride));
     if (j < np) {
@@ -542,7 +548,7 @@ __global__ __launch_bounds__(kCompactCopyThreads) void k_compact_copy(PoolRefs p
 #pragma unroll
     for (int k = 0; k < kCopySlices; ++k) {
       const int64_t pb = pools.page_bytes[q_of[k]];
-      const bool live = s0 + k < total && off[k] < pb;
+      const bool live = s0 + k < total && off[k] < pools.part_bytes[q_of[k]];
       const uint8_t* src = pools.base[q_of[k]] + static_cast<int64_t>(src_id[k]) * pb + (live ? off[k] : 0);
       v[k] = ld_stream(reinterpret_cast<const u32x4*>(src));
     }
@@ -552,7 +558,7 @@ __global__ __launch_bounds__(kCompactCopyThreads) void k_compact_copy(PoolRefs p
 #pragma unroll
     for (int k = 0; k < kCopySlices; ++k) {
       const int64_t pb = pools.page_bytes[q_of[k]];
-      if (s0 + k < total && off[k] < pb) {
+      if (s0 + k < total && off[k] < pools.part_bytes[q_of[k]]) {
         u32x4* dst = reinterpret_cast<u32x4*>(pools.base[q_of[k]] + static_cast<int64_t>(dst_id[k]) * pb + off[k]);
         if (wb) {
           *dst = v[k];
@@ -646,23 +652,15 @@ static int compact(const char* what, const skv_pool_ref* pools, int32_t n_pools,
   if (!workspace || !info || !free_stack || !free_top) {
     return set_error(SKV_EINVAL, "%s: NULL workspace/info/free list", what);
   }
-  PoolRefs pr{};
-  pr.n = n_pools;
-  int64_t slices_per_mover = 0;
   for (int q = 0; q < n_pools; ++q) {
     if (!pools[q].base || pools[q].page_bytes <= 0 || (pools[q].page_bytes & 15) ||
         (reinterpret_cast<uintptr_t>(pools[q].base) & 15)) {
       return set_error(SKV_EINVAL, "%s: pool %d needs a 16-byte aligned base and page_bytes", what, q);
     }
-    pr.base[q] = static_cast<uint8_t*>(pools[q].base);
-    pr.page_bytes[q] = pools[q].page_bytes;
-    slices_per_mover += ceil_div(pools[q].page_bytes, kCopySlice);
   }
-  if (n_pages >= (1 << 24) || n_pages * slices_per_mover >= (1 << 24)) {
-    return set_error(SKV_EINVAL, "%s: n_pages x 4 KB slices per page must stay below 2^24", what);
-  }
-  if (batch * bt_stride >= (1 << 24)) {
-    return set_error(SKV_EINVAL, "%s: batch x bt_stride must stay below 2^24", what);
+  if (n_pages >= (1 << 24)) return set_error(SKV_EINVAL, "%s: n_pages must stay below 2^24", what);
+  if (bt_stride > (1 << 30) || batch * bt_stride > (1 << 30)) {
+    return set_error(SKV_EINVAL, "%s: batch x bt_stride must be at most 2^30", what);
   }
   hipStream_t s = static_cast<hipStream_t>(stream);
   int rc;
@@ -679,19 +677,40 @@ static int compact(const char* what, const skv_pool_ref* pools, int32_t n_pools,
   hipLaunchKernelGGL(k_compact_plan, pgrid, dim3(kEvictThreads), 0, s, workspace, n_pages,
                      free_stack, free_top, info);
   if ((rc = check_launch(what))) return rc;
-  CopySlices cs{};
-  for (int q = 0; q < n_pools; ++q) cs.first[q + 1] = cs.first[q] + static_cast<int32_t>(ceil_div(pr.page_bytes[q], kCopySlice));
-  cs.per_mover = cs.first[n_pools];
-  const TableRef tr{block_table, seq_lens, static_cast<int32_t>(bt_stride), static_cast<int32_t>(batch),
-                    static_cast<int32_t>(block_size)};
-  if (!refs) {
-    hipLaunchKernelGGL((k_compact_copy<false>), dim3(kPersistentBlocks), dim3(kCompactCopyThreads), 0, s, pr, cs, tr,
-                       workspace, n_pages, info);
-    return check_launch(what);
+  const TableRef tables{block_table, seq_lens, static_cast<int32_t>(bt_stride), static_cast<int32_t>(batch),
+                        static_cast<int32_t>(block_size)};
+  const int64_t per_launch = std::min<int64_t>(((1 << 24) - 1) / n_pages, 1 << 18);  // slices of a page: 1 GB at most
+  int64_t done = 0;  // bytes of pool q's page
+  for (int q = 0; q < n_pools;) {
+    const bool first = q == 0 && done == 0;
+    PoolRefs pr{};
+    CopySlices cs{};
+    for (; q < n_pools && cs.per_mover < per_launch; ++pr.n) {
+      const int64_t left = pools[q].page_bytes - done;
+      const int64_t slices = std::min<int64_t>(ceil_div(left, kCopySlice), per_launch - cs.per_mover);
+      pr.base[pr.n] = static_cast<uint8_t*>(pools[q].base) + done;
+      pr.page_bytes[pr.n] = pools[q].page_bytes;
+      pr.part_bytes[pr.n] = std::min(left, slices * kCopySlice);
+      cs.per_mover += static_cast<int32_t>(slices);
+      cs.first[pr.n + 1] = cs.per_mover;
+      done += pr.part_bytes[pr.n];
+      if (done == pools[q].page_bytes) {
+        done = 0;
+        ++q;
+      }
+    }
+    TableRef tr = tables;
+    if (!first) tr.batch = 0;
+    if (refs || !first) {
+      hipLaunchKernelGGL((k_compact_copy<true>), dim3(kPersistentBlocks), dim3(kCompactCopyThreads), 0, s, pr, cs, tr,
+                         workspace, n_pages, info);
+    } else {
+      hipLaunchKernelGGL((k_compact_copy<false>), dim3(kPersistentBlocks), dim3(kCompactCopyThreads), 0, s, pr, cs, tr,
+                         workspace, n_pages, info);
+    }
+    if ((rc = check_launch(what))) return rc;
   }
-  hipLaunchKernelGGL((k_compact_copy<true>), dim3(kPersistentBlocks), dim3(kCompactCopyThreads), 0, s, pr, cs, tr,
-                     workspace, n_pages, info);
-  if ((rc = check_launch(what))) return rc;
+  if (!refs) return SKV_OK;
   hipLaunchKernelGGL(k_compact_finish, dim3(static_cast<unsigned>(ceil_div(n_pages, kCompactCopyThreads))),
                      dim3(kCompactCopyThreads), 0, s, workspace, n_pages, info, refs);
   return check_launch(what);

@@ -177,13 +177,21 @@ class Fp4TokenCache:
             raise ValueError(f"batch must be in [1, {MAX_BATCH}]; got {batch}")
         if max_len <= 0:
             raise ValueError(f"max_len must be positive; got {max_len}")
+        width = -(-max_len // block_size) if block_size > 0 else 1
+        pages = batch * width if n_pages is None else n_pages
+        # what the calls on it take: tokens of a sequence, pages that a compaction counts, table entries
+        if width * block_size > 1 << 24:
+            raise ValueError(f"a sequence holds at most 2^24 tokens; got max_len={max_len}")
+        if not 0 < pages < 1 << 24:
+            raise ValueError(f"n_pages must be in [1, 2^24); got {pages}")
+        if batch * (width + 64) > 1 << 30:
+            raise ValueError(f"a table of {batch} x {width} pages is too large")
         dev = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
         if dev.type != "cuda":
             raise RuntimeError("Fp4TokenCache runs only on a ROCm GPU (no CPU fallback)")
         _lib.load()
         self.device, self.batch, self.max_len, self.block_size = dev, batch, max_len, block_size
-        width = -(-max_len // block_size) if block_size > 0 else 1
-        self.n_pages = batch * width if n_pages is None else n_pages
+        self.n_pages = pages
         self.pool = [ops.fp4_pool(self.n_pages, block_size, n_kv_heads, head_dim, dev) for _ in range(layers)]
         i32 = dict(dtype=torch.int32, device=dev)
         self.block_table = torch.full((batch, width), -1, **i32)

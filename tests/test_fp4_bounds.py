@@ -60,3 +60,19 @@ def test_forks_of_empty_sequences_are_left_out() -> None:
 
     src, dst = check_forks([0, 1, 2, 3], [1, 4, 5, 2], np.array([5, 0, 0, 7, 0, 0]))
     assert src.tolist() == [0, 3] and dst.tolist() == [1, 2]
+
+
+def test_a_cache_that_its_calls_would_refuse() -> None:
+    """Sizes that only a later append, release or compaction would refuse."""
+    from saint_kv import Fp4TokenCache
+
+    ok = dict(layers=1, batch=2, max_len=4096, n_kv_heads=1, head_dim=64, device="cpu")
+    for bad, text in ((dict(max_len=(1 << 24) + 1), "tokens"), (dict(max_len=(1 << 24) - 8, block_size=96), "tokens"),
+                      (dict(n_pages=0), "n_pages"), (dict(n_pages=1 << 24), "n_pages"), (dict(n_pages=-4), "n_pages"),
+                      (dict(batch=4096, max_len=1 << 18, block_size=16), "n_pages"),
+                      (dict(batch=4096, max_len=1 << 23, block_size=16, n_pages=1000), "table")):
+        with pytest.raises(ValueError, match=text):
+            Fp4TokenCache(**{**ok, **bad})
+    for good in (dict(max_len=1 << 24), dict(n_pages=(1 << 24) - 1), dict(batch=4096, max_len=1 << 20, n_pages=1000)):
+        with pytest.raises(RuntimeError, match="GPU"):  # what is left to refuse is the device
+            Fp4TokenCache(**{**ok, **good})
