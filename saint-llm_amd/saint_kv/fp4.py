@@ -130,6 +130,9 @@ def _desc(q, pool, block_table, seq_lens, n_new, window, sink, softcap, scale, m
         raise ValueError(f"softcap must be positive (or None); got {softcap}")
     if scale is not None and not scale > 0:
         raise ValueError(f"scale must be positive (or None); got {scale}")
+    for name, x in (("scale", scale), ("softcap", softcap)):
+        if x is not None and ctypes.c_float(x).value == 0:  # would stand for the default
+            raise ValueError(f"{name}={x} is zero in fp32")
     if sink is not None:
         _require_gpu(sink, "sink")
         if sink.dtype != torch.float32 or tuple(sink.shape) != (heads,) or not sink.is_contiguous():

@@ -135,3 +135,17 @@ def test_a_refusal_is_reported_whatever_comes_after(dev) -> None:
     with pytest.raises(RuntimeError, match="refused"):
         cache.release(np.array([1, 0, 0, 0, 0]))
     assert cache.host_lens.tolist() == cache.seq_lens.tolist() and cache.host_free == int(cache.free_top)
+
+
+def test_scales_that_fp32_takes_for_zero_are_refused(dev) -> None:
+    """Zero stands for the default scale and for no cap in the descriptor."""
+    from saint_kv import fp4_attention
+
+    cache = new_cache(dev)
+    Model(dev, cache).step(1)
+    q = _rows(dev, 1, HEADS)
+    for kw in (dict(scale=1e-50), dict(softcap=1e-50), dict(scale=1e-50, softcap=2.0)):
+        with pytest.raises(ValueError, match="fp32"):
+            fp4_attention(q, cache.pool[0], cache.block_table, cache.seq_lens, **kw)
+        with pytest.raises(ValueError, match="fp32"):
+            cache.attention(0, q, **kw)
