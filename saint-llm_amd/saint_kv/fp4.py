@@ -215,6 +215,7 @@ class Fp4TokenCache:
         self.host_lens, self.host_free = np.zeros(batch, dtype=np.int64), self.n_pages
         self._n_new: int | torch.Tensor = 0
         self._host_new = np.zeros(batch, dtype=np.int64)  # each sequence's tokens reserved last
+        self._most_new, self._padded = 0, False
         self._unwritten: set[int] = set()  # layers that these have not been appended to
         self._recorded: set[int] = set()  # layers that a graph appends to
         self._shared = False  # some of these lie in shared pages
@@ -238,7 +239,8 @@ class Fp4TokenCache:
         ops.reserve(self.free_stack, self.free_top, self.block_table, self.seq_lens, self._n_new, self.block_size,
                     self._status_word())
         self.host_lens = self.host_lens + counts
-        self._host_new, self._shared = counts.copy(), False
+        self._host_new, self._most_new = counts.copy(), int(counts.max())
+        self._shared = self._padded = False
         self._unwritten = set(range(len(self.pool))) if counts.any() else set()
 
     def _status_word(self) -> torch.Tensor:
@@ -255,11 +257,14 @@ class Fp4TokenCache:
 
     def append(self, i: int, k: torch.Tensor, v: torch.Tensor) -> None:
         """Layer i's keys and values [B, T, Hkv, D] of the tokens reserved last
-        (of sequence b the first n_new[b]); not after a fork of these, which lie in
-        shared pages then."""
+        (of sequence b the first n_new[b], T at least the largest of them); not after a
+        fork of these, which lie in shared pages then."""
+        if k.dim() == 4 and k.shape[1] < self._most_new:
+            raise ValueError(f"{self._most_new} tokens of a sequence were reserved, k has {k.shape[1]}")
         if self._shared:
             raise RuntimeError("the tokens reserved last are a fork's, too; reserve new ones to append")
         ops.fp4_quant_append(self.pool[i], self.block_table, self.seq_lens, k, v, self._n_new)
+        self._padded = k.shape[1] > self._most_new
         layer = range(len(self.pool))[i]
         self._unwritten.discard(layer)
         if torch.cuda.is_current_stream_capturing():
@@ -271,6 +276,10 @@ class Fp4TokenCache:
         """``fp4_attention`` of layer i for the queries of the newest tokens; after a
         ragged reservation of sequence b's first n_new[b] (the others get 0)."""
         n_new = self._n_new if isinstance(self._n_new, torch.Tensor) else None
+        if n_new is None and self._padded and q.dim() == 4 and q.shape[1] > self._n_new:
+            # the newest of several reservations, or a padded batch as k and v were
+            raise ValueError(f"{self._n_new} tokens were reserved, q has {q.shape[1]}: reserve a count for each sequence "
+                             "for a padded batch")
         return fp4_attention(q, self.pool[i], self.block_table, self.seq_lens, n_new=n_new, window=window, sink=sink,
                              softcap=softcap, scale=scale, max_len=int(self.host_lens.max()), out=out)
 

@@ -149,3 +149,25 @@ def test_scales_that_fp32_takes_for_zero_are_refused(dev) -> None:
             fp4_attention(q, cache.pool[0], cache.block_table, cache.seq_lens, **kw)
         with pytest.raises(ValueError, match="fp32"):
             cache.attention(0, q, **kw)
+
+
+def test_tokens_that_do_not_fit_the_reservation(dev) -> None:
+    """Queries or rows of more or fewer tokens than were reserved, where nothing says which they are."""
+    cache = new_cache(dev)
+    cache.reserve(5)
+    with pytest.raises(ValueError, match="5"):
+        cache.append(0, _rows(dev, 4), _rows(dev, 4))
+    cache.append(0, _rows(dev, 8), _rows(dev, 8))  # a padded batch: the first five
+    with pytest.raises(ValueError, match="5"):
+        cache.attention(0, _rows(dev, 8, HEADS))
+    cache.attention(0, _rows(dev, 5, HEADS))
+    cache.attention(0, _rows(dev, 1, HEADS))  # the newest
+    cache.reserve(np.array([5, 3, 0, 1, 1]))
+    with pytest.raises(ValueError, match="5"):
+        cache.append(0, _rows(dev, 4), _rows(dev, 4))
+    cache.append(0, _rows(dev, 8), _rows(dev, 8))
+    cache.attention(0, _rows(dev, 8, HEADS))
+    for _ in range(2):  # the newest of two reservations
+        cache.reserve(2)
+        cache.append(0, _rows(dev, 2), _rows(dev, 2))
+    cache.attention(0, _rows(dev, 4, HEADS))
