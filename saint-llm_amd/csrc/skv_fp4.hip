@@ -218,7 +218,7 @@ int fp4_rows_args(Fp4RowsArgs& a, const char* what, const skv_fp4_cache* c, cons
   a.lens = seq_lens;
   a.n_new = n_new;
   a.n_uni = n_uni;
-  a.rows = rows;
+  a.rows = std::min<int64_t>(rows, 1 << 24);  // a sequence has no more tokens
   a.bs = static_cast<int>(c->block_size);
   a.heads = static_cast<int>(c->n_kv_heads);
   a.dim = static_cast<int>(c->head_dim);
@@ -247,7 +247,7 @@ extern "C" int skv_fp4_quant_append(const skv_fp4_cache* cache, const int32_t* s
   Fp4RowsArgs a{};
   if (const int rc = fp4_rows_args(a, what, cache, seq_lens, n_new, n_new_uniform, k, v, src_len)) return rc;
   if (cache->batch == 0 || src_len == 0) return SKV_OK;
-  const dim3 grid(static_cast<unsigned>(ceil_div(src_len, kFp4Tokens * a.together)), static_cast<unsigned>(cache->batch));
+  const dim3 grid(static_cast<unsigned>(ceil_div(a.rows, kFp4Tokens * a.together)), static_cast<unsigned>(cache->batch));
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (src_f32) {
     hipLaunchKernelGGL((k_fp4_quant_append<true>), grid, dim3(kFp4Threads), 0, s, a);
@@ -264,7 +264,7 @@ extern "C" int skv_fp4_gather(const skv_fp4_cache* cache, const int32_t* seq_len
   Fp4RowsArgs a{};
   if (const int rc = fp4_rows_args(a, what, cache, seq_lens, n_rows, n_rows_uniform, k, v, dst_len)) return rc;
   if (cache->batch == 0 || dst_len == 0) return SKV_OK;
-  const dim3 grid(static_cast<unsigned>(ceil_div(dst_len, kFp4Tokens * a.together)), static_cast<unsigned>(cache->batch));
+  const dim3 grid(static_cast<unsigned>(ceil_div(a.rows, kFp4Tokens * a.together)), static_cast<unsigned>(cache->batch));
   hipLaunchKernelGGL(k_fp4_gather, grid, dim3(kFp4Threads), 0, static_cast<hipStream_t>(stream), a);
   return check_launch(what);
 }

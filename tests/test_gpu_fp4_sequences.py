@@ -171,3 +171,17 @@ def test_tokens_that_do_not_fit_the_reservation(dev) -> None:
         cache.reserve(2)
         cache.append(0, _rows(dev, 2), _rows(dev, 2))
     cache.attention(0, _rows(dev, 4, HEADS))
+
+
+def test_rows_for_more_tokens_than_a_sequence_has(dev) -> None:
+    """One expanded token as the rows of 2^28, of which a few are new: as many as a launch's grid cannot count."""
+    from saint_kv import ops
+
+    pool = ops.fp4_pool(4, 16, 1, 512, dev)
+    i32 = dict(dtype=torch.int32, device=dev)
+    bt, lens = torch.tensor([[2, 0], [3, 1]], **i32), torch.tensor([20, 3], **i32)
+    k, v = (torch.randn(2, 1, 1, 512, device=dev).to(torch.bfloat16) for _ in range(2))
+    ops.fp4_quant_append(pool, bt, lens, k.expand(2, 1 << 28, 1, 512), v.expand(2, 1 << 28, 1, 512), lens)
+    want = ops.fp4_pool(4, 16, 1, 512, dev)
+    ops.fp4_quant_append(want, bt, lens, k.expand(2, 20, 1, 512), v.expand(2, 20, 1, 512), lens)
+    assert torch.equal(pool, want)
