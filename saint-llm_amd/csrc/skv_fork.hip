@@ -244,8 +244,8 @@ extern "C" int skv_copy_slots(const skv_pool_ref* arrays, int64_t n_arrays, int6
   }
   if ((n_arrays > 0 && !arrays) || (n_forks > 0 && (!src || !dst))) return set_error(SKV_EINVAL, "%s: NULL pointer", what);
   for (int64_t i = 0; i < n_arrays; ++i) {
-    if (!arrays[i].base || arrays[i].page_bytes <= 0 || arrays[i].page_bytes > (int64_t{1} << 40)) {
-      return set_error(SKV_EINVAL, "%s: array %lld needs a base and a slot size", what, (long long)i);
+    if (!arrays[i].base || arrays[i].page_bytes <= 0 || arrays[i].page_bytes > (int64_t{1} << 37)) {
+      return set_error(SKV_EINVAL, "%s: array %lld needs a base and a slot size of at most 2^37", what, (long long)i);
     }
   }
   if (n_forks == 0 || n_slots == 0) return SKV_OK;

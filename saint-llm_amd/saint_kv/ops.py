@@ -831,16 +831,18 @@ def copy_slots(arrays: list[torch.Tensor], src: torch.Tensor, dst: torch.Tensor)
         raise ValueError(f"src must be int32 [n]; got {tuple(src.shape)}")
     _require_i32(dst, "dst", tuple(src.shape))
     n = arrays[0].shape[0]
-    refs = (_lib.PoolRef * len(arrays))()
     for i, t in enumerate(arrays):
         _require_gpu(t, f"arrays[{i}]")
         if t.dim() < 1 or t.shape[0] != n or not t.is_contiguous():
             raise ValueError(f"arrays[{i}] must be contiguous with {n} slots; got {tuple(t.shape)}")
-        refs[i].base = t.data_ptr()
-        refs[i].page_bytes = t[0].numel() * t.element_size() if n else 0
     _same_device(src, "src", dst=dst, **{f"arrays[{i}]": t for i, t in enumerate(arrays)})
-    if n:
-        _launch(src.device, "skv_copy_slots", ctypes.byref(refs), len(arrays), n, src.data_ptr(), dst.data_ptr(),
+    held = [t for t in arrays if t.numel()]
+    refs = (_lib.PoolRef * len(held))()
+    for ref, t in zip(refs, held):
+        ref.base = t.data_ptr()
+        ref.page_bytes = t.numel() // n * t.element_size()
+    if held:
+        _launch(src.device, "skv_copy_slots", ctypes.byref(refs), len(held), n, src.data_ptr(), dst.data_ptr(),
                 src.shape[0])
 
 

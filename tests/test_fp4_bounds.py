@@ -76,3 +76,12 @@ def test_a_cache_that_its_calls_would_refuse() -> None:
     for good in (dict(max_len=1 << 24), dict(n_pages=(1 << 24) - 1), dict(batch=4096, max_len=1 << 20, n_pages=1000)):
         with pytest.raises(RuntimeError, match="GPU"):  # what is left to refuse is the device
             Fp4TokenCache(**{**ok, **good})
+
+
+def test_slots_past_a_launch_are_refused() -> None:
+    from saint_kv import _lib
+
+    lib = _lib.load()
+    arr = (_lib.PoolRef * 1)(_lib.PoolRef(FAKE, (1 << 37) + 16))
+    assert lib.skv_copy_slots(ctypes.cast(arr, ctypes.c_void_p), 1, 4, FAKE, FAKE, 2, None) == _lib.SKV_EINVAL
+    assert "slot size" in _lib.last_error()

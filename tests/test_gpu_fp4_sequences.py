@@ -185,3 +185,15 @@ def test_rows_for_more_tokens_than_a_sequence_has(dev) -> None:
     want = ops.fp4_pool(4, 16, 1, 512, dev)
     ops.fp4_quant_append(want, bt, lens, k.expand(2, 20, 1, 512), v.expand(2, 20, 1, 512), lens)
     assert torch.equal(pool, want)
+
+
+def test_slots_of_nothing(dev) -> None:
+    """Arrays without bytes, or without slots, beside others."""
+    from saint_kv import ops
+
+    idx = torch.tensor([[0, 2], [1, 3]], dtype=torch.int32, device=dev)
+    full = torch.arange(12, device=dev).view(4, 3)
+    ops.copy_slots([torch.zeros(4, 0, device=dev), full, torch.zeros(4, 2, 0, device=dev)], idx[0], idx[1])
+    assert full.tolist() == [[0, 1, 2], [0, 1, 2], [6, 7, 8], [6, 7, 8]]
+    ops.copy_slots([torch.zeros(4, 0, device=dev)], idx[0], idx[1])
+    ops.copy_slots([torch.zeros(0, 3, device=dev)], idx[0], idx[1])
