@@ -220,9 +220,12 @@ extern "C" int skv_fork(int32_t* free_stack, int32_t* free_top, int64_t n_pages,
     fp.base[q] = static_cast<uint8_t*>(pools[q].base);
     fp.page_bytes[q] = pools[q].page_bytes;
     slices += ceil_div(pools[q].page_bytes, kForkSlice);
-    if (slices > (1 << 24)) return set_error(SKV_EINVAL, "%s: pages too large", what);
+    if (slices >= (1 << 24)) return set_error(SKV_EINVAL, "%s: pages too large", what);
     fp.first[q + 1] = static_cast<int32_t>(slices);
   }
+  // the copies' grid, which is counted before the plan has popped a page
+  const int64_t table_parts = ceil_div(bt_stride, kForkEntries);
+  if (table_parts + slices >= (1 << 24)) return set_error(SKV_EINVAL, "%s: pages and tables too large", what);
   if (batch == 0 && n_forks > 0) return set_error(SKV_EINVAL, "%s: forks in an empty batch", what);
   if (n_forks == 0) return SKV_OK;
   const ForkArgs a{free_stack, free_top, n_pages, refs, block_table, bt_stride, seq_lens, src, dst,
@@ -230,9 +233,8 @@ extern "C" int skv_fork(int32_t* free_stack, int32_t* free_top, int64_t n_pages,
   hipStream_t s = static_cast<hipStream_t>(stream);
   hipLaunchKernelGGL(k_fork_plan, dim3(1), dim3(kForkThreads), 0, s, a);
   if (const int rc = check_launch(what)) return rc;
-  const int table_parts = static_cast<int>(ceil_div(bt_stride, kForkEntries));
   hipLaunchKernelGGL(k_fork_copy, dim3(static_cast<unsigned>(table_parts + slices), static_cast<unsigned>(n_forks)),
-                     dim3(kForkCopyThreads), 0, s, a, fp, table_parts);
+                     dim3(kForkCopyThreads), 0, s, a, fp, static_cast<int>(table_parts));
   return check_launch(what);
 }
 

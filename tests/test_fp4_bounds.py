@@ -85,3 +85,15 @@ def test_slots_past_a_launch_are_refused() -> None:
     arr = (_lib.PoolRef * 1)(_lib.PoolRef(FAKE, (1 << 37) + 16))
     assert lib.skv_copy_slots(ctypes.cast(arr, ctypes.c_void_p), 1, 4, FAKE, FAKE, 2, None) == _lib.SKV_EINVAL
     assert "slot size" in _lib.last_error()
+
+
+@pytest.mark.parametrize("page_bytes,bt_stride,text", [(1 << 38, 4, "pages too large"), ((1 << 38) - (1 << 14), 4, "pages and"),
+                                                       ((1 << 38) - (1 << 34), (1 << 31) - 1, "pages and")])
+def test_forks_past_a_launch_are_refused(page_bytes: int, bt_stride: int, text: str) -> None:
+    """Before their pages are popped: a copy launch that then fails would leave them lost."""
+    from saint_kv import _lib
+
+    lib = _lib.load()
+    pool = ctypes.cast((_lib.PoolRef * 1)(_lib.PoolRef(FAKE, page_bytes)), ctypes.c_void_p)
+    rc = lib.skv_fork(FAKE, FAKE, 8, FAKE, FAKE, bt_stride, FAKE, 3, 16, FAKE, FAKE, 2, pool, 1, FAKE, None)
+    assert rc == _lib.SKV_EINVAL and text in _lib.last_error()
