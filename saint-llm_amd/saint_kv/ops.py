@@ -96,8 +96,7 @@ def free_stack_init(free_stack: torch.Tensor, free_top: torch.Tensor,
     _require_i32(free_top, "free_top", (1,))
     if order is not None:
         _require_i32(order, "order", (n,))
-    _lib.call("skv_free_stack_init", free_stack.data_ptr(), free_top.data_ptr(),
-              _lib.ptr(order), n, _lib.stream_handle(free_stack.device))
+    _launch(free_stack.device, "skv_free_stack_init", free_stack.data_ptr(), free_top.data_ptr(), _lib.ptr(order), n)
 
 
 def reserve(free_stack: torch.Tensor, free_top: torch.Tensor, block_table: torch.Tensor,
@@ -114,11 +113,9 @@ def reserve(free_stack: torch.Tensor, free_top: torch.Tensor, block_table: torch
     if status is not None:
         _require_i32(status, "status", (1,))
     n_ptr, n_uni = _n_new_args(n_new, batch)
-    _lib.call("skv_reserve", free_stack.data_ptr(), free_top.data_ptr(), free_stack.numel(),
-              block_table.data_ptr(),
-              bt_stride, bt_stride if max_pages is None else max_pages, seq_lens.data_ptr(),
-              n_ptr, n_uni, batch, block_size, _lib.ptr(status),
-              _lib.stream_handle(block_table.device))
+    _launch(block_table.device, "skv_reserve", free_stack.data_ptr(), free_top.data_ptr(), free_stack.numel(),
+            block_table.data_ptr(), bt_stride, bt_stride if max_pages is None else max_pages, seq_lens.data_ptr(),
+            n_ptr, n_uni, batch, block_size, _lib.ptr(status))
 
 
 def paged_append(pool: torch.Tensor, block_table: torch.Tensor, seq_lens: torch.Tensor,
@@ -896,6 +893,8 @@ def compact(pools: list[torch.Tensor], block_table: torch.Tensor, seq_lens: torc
             seq_lens.data_ptr(), batch, block_size, n_pages, free_stack.data_ptr(), free_top.data_ptr())
     if refs is not None:
         _require_i32(refs, "refs", (n_pages,))
+        _same_device(block_table, "block_table", seq_lens=seq_lens, free_stack=free_stack, free_top=free_top,
+                     workspace=workspace, info=info, refs=refs, **{f"pools[{i}]": p for i, p in enumerate(pools)})
         return _launch(block_table.device, "skv_compact_shared", *args, refs.data_ptr(), workspace.data_ptr(),
                        info.data_ptr())
     _lib.call("skv_compact", *args, workspace.data_ptr(), info.data_ptr(), _lib.stream_handle(block_table.device))

@@ -197,3 +197,24 @@ def test_slots_of_nothing(dev) -> None:
     assert full.tolist() == [[0, 1, 2], [0, 1, 2], [6, 7, 8], [6, 7, 8]]
     ops.copy_slots([torch.zeros(4, 0, device=dev)], idx[0], idx[1])
     ops.copy_slots([torch.zeros(0, 3, device=dev)], idx[0], idx[1])
+
+
+def test_a_cache_on_another_device_than_the_current_one(dev, monkeypatch) -> None:
+    """Every launch finds the cache's device current, and the caller's is current again behind it."""
+    from saint_kv import Fp4TokenCache, _lib
+
+    here, call, seen = [1], _lib.call, []
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: here[0])
+    monkeypatch.setattr(torch.cuda, "set_device", lambda i: here.__setitem__(0, i))
+    monkeypatch.setattr(_lib, "call", lambda name, *args: (seen.append((name, here[0])), call(name, *args))[1])
+    cache = Fp4TokenCache(LAYERS, 5, 160, KV, DIM, block_size=16, device=dev)
+    cache.reserve(np.array([37, 0, 5, 1, 0]))
+    for i in range(LAYERS):
+        cache.append(i, _rows(dev, 37), _rows(dev, 37))
+        cache.attention(i, _rows(dev, 37, HEADS))
+    cache.fork([0], [1])
+    cache.release(np.array([1, 0, 0, 0, 0]))
+    cache.compact()
+    assert here == [1] and {d for _, d in seen} == {0}
+    assert {n for n, _ in seen} == {"skv_free_stack_init", "skv_reserve", "skv_fp4_quant_append", "skv_fp4_attention",
+                                    "skv_fork", "skv_copy_slots", "skv_release_shared", "skv_compact_shared"}
