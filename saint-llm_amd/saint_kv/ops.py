@@ -894,7 +894,10 @@ def compact(pools: list[torch.Tensor], block_table: torch.Tensor, seq_lens: torc
     if refs is not None:
         _require_i32(refs, "refs", (n_pages,))
         _same_device(block_table, "block_table", seq_lens=seq_lens, free_stack=free_stack, free_top=free_top,
-                     workspace=workspace, info=info, refs=refs, **{f"pools[{i}]": p for i, p in enumerate(pools)})
+                     workspace=workspace, info=info, refs=refs)
+        for i, p in enumerate(pools):
+            if p.device != block_table.device:
+                raise ValueError(f"pools[{i}] is on {p.device}, block_table on {block_table.device}")
         return _launch(block_table.device, "skv_compact_shared", *args, refs.data_ptr(), workspace.data_ptr(),
                        info.data_ptr())
     _lib.call("skv_compact", *args, workspace.data_ptr(), info.data_ptr(), _lib.stream_handle(block_table.device))
