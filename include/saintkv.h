@@ -490,9 +490,11 @@ int skv_fp4_gather(const skv_fp4_cache* cache, const int32_t* seq_lens, const in
  *   out = sum_j exp(s_j) v_j / (sum_j exp(s_j) + exp(sink[h]))   (sink optional)
  * A token that sees nothing (or only unmapped pages), or is past n_new[b], gets
  * 0; a NaN block makes NaN the outputs of the tokens that see it, and of no
- * other, as do a NaN or an infinity in q those of their token and head.  q: bf16, token t, head h of sequence b at q + b*q_seq_stride +
- * t*q_tok_stride + h*q_head_stride (bytes, multiples of 16); out: bf16 [batch,
- * n_queries, n_heads, head_dim].  Long sequences are cut into runs of about equal
+ * other, as do a NaN or an infinity in q those of their token and head.  (A count
+ * n_new[b] past n_queries is n_queries: q holds the newest tokens.)  The softcap's
+ * score is right to 2^-20 of itself under every cap.  q: bf16, token t, head h of
+ * sequence b at q + b*q_seq_stride + t*q_tok_stride + h*q_head_stride (bytes,
+ * multiples of 16); out: bf16 [batch, n_queries, n_heads, head_dim].  Long sequences are cut into runs of about equal
  * length for as many workgroups as the device holds, and joined by a second
  * launch.  max_len bounds the lengths (0: what the table holds; longer ones are
  * still right): where it, or the window, shows that no sequence is worth cutting,

@@ -106,7 +106,7 @@ __global__ __launch_bounds__(kEvictThreads) void k_release(
 // entries in registers from pass to pass.  Which entries' pages have dropped is noted
 // for the first kReleaseNoted units, so that later passes touch those alone.  48 sequences
 // of 8k - 64k tokens, 22,000 entries: 142 us with every entry by a thread in turn, 66 with
-// units and all in one launch, 5 + 48 so; with 24 units together 36, but 27 instead of 13
+// units and all in one launch, 5 + 44 so; with 24 units together 36, but 27 instead of 13
 // for a release of 1,600 entries.
 constexpr int kReleaseAhead = 8;
 constexpr int kReleaseStep = kEvictThreads / kWave * kReleaseAhead;

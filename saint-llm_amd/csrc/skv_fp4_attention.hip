@@ -35,19 +35,20 @@
 // cut a long item; the lengths are on the device, so every workgroup works the
 // runs out for itself from their prefix sum.  A cut item's pieces are joined by a
 // second launch.  (Twice as many workgroups of half the run, for the hardware to deal out
-// as others end: 139 -> 180 us for the step below.)
+// as others end, took 1.3 times as long for the step below.)
 //
-// Measured, us a call among others, with the time of the bytes at 6.1 TB/s (or of the
-// products at 1.2 PFLOP/s):
-//   64 sequences of 1k - 32k, 64 heads on 8 of 128 dims                    140 (117)
-//   4 of 256k - 1M, 4 tokens, 16 heads on 4 of 64                          91 (75)
-//   16 of 64k, 64 heads on 1 of 128                                        79 (29, products)
-//   2 prompts' 1000 tokens over 16k, 32 heads on 8 of 128                  580 (428, products)
-//   1 prompt's 512 tokens over 200k, the same heads                        1700 (1400, products)
-//   32 windows of 128, 64 heads on 1 of 512                                21 (1)
+// Measured, us a call (both launches) in a graph of several, with the time of the bytes
+// at 6.1 TB/s (or of the products at 1.4 PFLOP/s, an 8192^3 library product's rate):
+//   64 sequences of 1k - 32k, 64 heads on 8 of 128 dims                    139 (117)
+//   4 of 256k - 1M, 4 tokens, 16 heads on 4 of 64                          91 (74)
+//   16 of 64k, 64 heads on 1 of 128                                        79 (25, products)
+//   2 prompts' 1000 tokens over 16k, 32 heads on 8 of 128                  557 (367, products)
+//   1 prompt's 512 tokens over 200k, the same heads                        1690 (1200, products)
+//   32 windows of 128, 64 heads on 1 of 512                                23 (1)
 // and dropped: two row groups of two waves with half the tiles each for 33 - 64 rows (68 ->
-// 74 us for the 64k sequences: a tile's latency is then seen by all four waves); the next
-// tile's scores ahead of a tile's weights (1%); a prologue that loads the queries last.
+// 74 us for the 64k sequences, before their weights had rests: a tile's latency is then seen by
+// all four waves); the next tile's scores ahead of a tile's weights (1%); a prologue that loads
+// the queries last.
 #include <algorithm>
 #include <cmath>
 
@@ -129,8 +130,8 @@ __device__ __forceinline__ Fp4Span fp4_span(const Fp4AttnArgs& a, int b, int r0,
 constexpr int kF4RunTiles = 8;
 constexpr int kF4SmallTiles = 16;
 // What a segment costs beside its tiles, in tiles: the first loads' latencies and the
-// waves' join.  A step of 64 sequences of 1k - 32k, 8 K/V heads: 168 us without it (runs end
-// between 81 and 159 us), with 12, 16 and 20 tiles 146, 142 and 141 us.  Counted where
+// waves' join.  A step of 64 sequences of 1k - 32k, 8 K/V heads: 165 us without it, with 12 tiles
+// 144 and with 20 139 us; the other cases above stay within 1%.  Counted where
 // there are about as many items as workgroups or more; a run that would begin in this
 // lead or just past it begins with the item.
 constexpr int kF4Lead = 20;
@@ -262,13 +263,13 @@ struct Fp4Wave {
   static constexpr bool kPacked = kExact && DP <= 128;
   // A weight's bf16 rounding, 2^-9 of it on average over few keys as over many, is as
   // large an error as the output's own.  Waves with tiles of their own carry its rest
-  // into a second product, 139 us either way for a step of 64 sequences (64 rows on one
-  // head: 66 -> 79); where the products bound the time (580 -> 720 us for a prompt's chunk)
+  // into a second product, 139 us for a step of 64 sequences and 138 without (64 rows on one
+  // head 79 and 67); where the products bound the time (a prompt's chunk 557, with rests 705 us)
   // the rounded weight stands.
   static constexpr bool kRest = !kShared;
   static constexpr bool kTwo = DP * MT <= 256;  // two tiles in flight; wider ones have registers for one
-  // A page is read by one workgroup, or by two: nontemporal loads (a step of 64 sequences 169 us,
-  // 187 with plain ones; 64 rows on one head 69 and 67).
+  // A page is read by one workgroup, or by two: nontemporal loads (a step of 64 sequences 139 us,
+  // 156 with plain ones; 4 of 256k - 1M 91 and 103; 64 rows on one head, read twice, 79 either way).
   static constexpr bool kOnce = !kShared && DP * MT <= 256;
 
   const Fp4AttnArgs& a;
@@ -1129,9 +1130,10 @@ int fp4_attn_plan(const skv_fp4_attention_desc* d, Fp4AttnPlan& p) {
   p.dims = D <= 64 ? 64 : D <= 128 ? 128 : D <= 256 ? 256 : 512;
   // A wave's tiles are its own, or all four waves' with rows of their own for each, once
   // more than half of the rows of such a workgroup are there: 16 sequences of 32k on one
-  // head of 128 dims take 65 us either way with 96 rows, 44 - 46 us shared and 43 apart with
-  // 64, 55 and 33 with 32; of 256 dims 75 and 84 us with 64 rows, 54 and 51 with 32.
-  // Heads of 512 dims stay apart (rows of 64: 117 us, shared 148, whose registers spill).
+  // head of 128 dims take 56 us shared and 48 apart with 64 rows, 56 and 71 with 65 (another row
+  // block), 53 and 36 with 32; of 64 dims 44 and 42 with 64 rows, 45 either way with 65, 49 and 60 with
+  // 128; of 256 dims 68 and 65 with 32 rows, 68 and 101 with 33.  Heads of 512 dims stay apart (16
+  // sequences of 4k: 57 us with 33 rows and 53 with 64, shared 61 and 64; their registers spill).
   const int mt = fp4_shared_mt(p.dims);
   p.shared = p.dims <= 256 && rows > 16 * mt * kF4Waves / 2;
   p.mt = p.shared ? mt : rows <= 16 || p.dims > 256 ? 1 : 2;

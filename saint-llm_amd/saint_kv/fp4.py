@@ -67,14 +67,17 @@ def fp4_attention(q: torch.Tensor, pool: torch.Tensor, block_table: torch.Tensor
     H a multiple of the pool's K/V heads (head h reads K/V head h // (H / Hkv)).
     n_new: int32 [B], of a padded batch: the first n_new[b] tokens of q are
     sequence b's newest, token t at position seq_lens - n_new + t, and later ones
-    get 0.  pool, block_table: as ``ops.fp4_quant_append`` wrote them; seq_lens:
+    get 0 (a count past T is T).  pool, block_table: as ``ops.fp4_quant_append`` wrote them; seq_lens:
     int32 [B].  window: only the newest ``window`` positions up to itself (None:
     all); sink: fp32 [H] or None; softcap: c*tanh(s/c) of the scores, or None;
     scale: of the scores (None: 1/sqrt(D)).  A token that sees nothing gets 0.
     max_len: a bound on seq_lens (0: what the table holds; longer ones are still
     right), which saves short sequences the launch that joins parts of long ones;
     splits: at most about that many workgroups for a K/V head of every sequence,
-    instead of as many as the device holds (0).
+    instead of as many as the device holds (0).  Up to 64 query rows of a K/V head
+    (its query heads times the query tokens; 32 of 129 to 256 dims, any number of
+    more dims) the softmax's weights keep 16 bits for the product with the values,
+    beyond them 8, as the output has.
     workspace: a tensor of at least ``fp4_attention_workspace`` bytes, of no other
     call that may run at the same time (None: one is allocated for the call)."""
     d, out = _desc(q, pool, block_table, seq_lens, n_new, window, sink, softcap, scale, max_len, splits, out)
@@ -168,7 +171,8 @@ class Fp4TokenCache:
     A prompt goes the same way with its tokens (``n_new`` per sequence where
     they are ragged).  Lengths and free pages are counted on the host, so that a
     reservation or a fork that cannot be raises before it changes anything; steps
-    and forks need no synchronisation, a release reads back what it freed.
+    and forks need no synchronisation, a release reads back what it freed.  Up to
+    16 layers: a model of more has a cache, with a table of its own, for every 16.
     """
 
     def __init__(self, layers: int, batch: int, max_len: int, n_kv_heads: int, head_dim: int, *, block_size: int = 64,
