@@ -173,6 +173,7 @@ class Fp4TokenCache:
     reservation or a fork that cannot be raises before it changes anything; steps
     and forks need no synchronisation, a release reads back what it freed.  Up to
     16 layers: a model of more has a cache, with a table of its own, for every 16.
+    The pages hold a sequence's whole history, a windowed layer's too.
     """
 
     def __init__(self, layers: int, batch: int, max_len: int, n_kv_heads: int, head_dim: int, *, block_size: int = 64,
