@@ -521,6 +521,28 @@ int64_t skv_fp4_attention_desc_size(void);
 int64_t skv_fp4_attention_workspace(const skv_fp4_attention_desc* desc);
 int skv_fp4_attention(const skv_fp4_attention_desc* desc, void* workspace, int64_t ws_bytes, void* stream);
 
+/* skv_fp4_attention with a view of the cache.  A token's history is the
+ * positions before the new tokens, then those of the new tokens that it sees, in
+ * their order: without a tree the ones up to itself; with one those whose bit is
+ * set in its mask, bit j of word j / 64 of tree[b][t] standing for the
+ * sequence's new token j <= t (later tokens' bits are not read; a token is seen
+ * by itself only if its own bit is set; skv_draft_tree makes the masks of a
+ * drafted tree).  It sees the history's last `window` positions (0: all of it)
+ * and its first `first` ones.  A token with an empty mask sees nothing and gets
+ * 0, and so do all of a sequence that is shorter than its new tokens, with a
+ * tree.  n_queries <= 1024 with a tree.  The reference's first tokens
+ * (model.py:267-276) fall out of its window layers' sight (swa.py:119-125); its
+ * drafted tokens are a chain (eagle3.py). */
+typedef struct skv_fp4_view {
+  const uint64_t* tree; /* [batch, n_queries, tree_words] or NULL */
+  int64_t tree_words;   /* ceil(n_queries / 64) */
+  int64_t first;
+} skv_fp4_view;
+
+int64_t skv_fp4_attention_view_workspace(const skv_fp4_attention_desc* desc, const skv_fp4_view* view);
+int skv_fp4_attention_view(const skv_fp4_attention_desc* desc, const skv_fp4_view* view, void* workspace,
+                           int64_t ws_bytes, void* stream);
+
 /* ---- fused decode step ----------------------------------------------------
  * One decode step (one new token per sequence) of a stack of heterogeneous
  * layers in three launches, whatever the layer count:

@@ -125,3 +125,77 @@ def attention(q: np.ndarray, pool: np.ndarray, block_table: np.ndarray, seq_lens
                 w = np.exp(s - top)
                 out[b, t, h] = w @ vv / (w.sum() + (0.0 if sink is None else np.exp(float(sink[h]) - top)))
     return out
+
+
+def ancestors(parents: list[int], t: int) -> list[int] | None:
+    """Node t's ancestors and itself, ascending, or None where a parent on the way up is not an earlier node (-1: none)."""
+    got = []
+    while t != -1:
+        got.append(t)
+        if not -1 <= parents[t] < t:
+            return None
+        t = parents[t]
+    return got[::-1]
+
+
+def tree_masks(parents: np.ndarray, n_new: np.ndarray) -> np.ndarray:
+    """bool [B, T, T]: node t sees node j (itself, its ancestors); none of a node past n_new[b] or with a bad parent."""
+    batch, t_max = parents.shape
+    seen = np.zeros((batch, t_max, t_max), dtype=bool)
+    for b in range(batch):
+        for t in range(min(int(n_new[b]), t_max)):
+            up = ancestors([int(p) for p in parents[b]], t)
+            if up is not None:
+                seen[b, t, up] = True
+    return seen
+
+
+def pack_masks(seen: np.ndarray) -> np.ndarray:
+    """bool [B, T, T] to int64 [B, T, ceil(T / 64)], bit j % 64 of word j / 64."""
+    t = seen.shape[2]
+    wide = np.zeros((*seen.shape[:2], -(-t // 64) * 64), dtype=np.uint64)
+    wide[..., :t] = seen
+    words = wide.reshape(*seen.shape[:2], -1, 64) << np.arange(64, dtype=np.uint64)
+    return np.bitwise_or.reduce(words, axis=-1).view(np.int64)
+
+
+def history(length: int, own: int, t: int, seen: np.ndarray | None) -> list[int]:
+    """The positions of token t's history: those before the `own` new tokens, then the new ones that it sees (`seen`, a
+    row of masks; None: those up to itself)."""
+    base = length - own
+    if seen is None:
+        return list(range(max(base + t + 1, 0)))
+    new = [j for j in range(t + 1) if seen[j]]
+    return list(range(base)) + [base + j for j in new] if new and base >= 0 else []
+
+
+def view_attention(q: np.ndarray, pool: np.ndarray, block_table: np.ndarray, seq_lens: np.ndarray, *, window: int | None = None,
+                   first: int = 0, seen: np.ndarray | None = None, sink: np.ndarray | None = None,
+                   softcap: float | None = None, scale: float | None = None, n_new: np.ndarray | None = None) -> np.ndarray:
+    """As ``attention`` where a token sees the last `window` and the first `first` positions of its history."""
+    batch, t_new, heads, dim = q.shape
+    out = np.zeros(q.shape)
+    for b in range(batch):
+        length = int(seq_lens[b])
+        k, v, mapped = rows(pool, block_table, b, range(length))
+        own = t_new if n_new is None else min(int(n_new[b]), t_new)
+        for t in range(own):
+            hist = history(length, own, t, None if seen is None else seen[b, t])
+            if window:
+                hist = [p for i, p in enumerate(hist) if i < first or i >= len(hist) - window]
+            live = np.array([p for p in hist if mapped[p]], dtype=np.int64)
+            if live.size == 0:
+                continue
+            for h in range(heads):
+                hk = h // (heads // k.shape[1])
+                kk, vv = k[live, hk], v[live, hk]
+                if np.isnan(vv).any():
+                    out[b, t, h] = np.nan
+                    continue
+                s = kk @ q[b, t, h].astype(np.float64) * (dim ** -0.5 if scale is None else scale)
+                if softcap:
+                    s = softcap * np.tanh(s / softcap)
+                top = s.max() if sink is None else max(s.max(), float(sink[h]))
+                w = np.exp(s - top)
+                out[b, t, h] = w @ vv / (w.sum() + (0.0 if sink is None else np.exp(float(sink[h]) - top)))
+    return out

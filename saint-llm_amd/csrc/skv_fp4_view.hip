@@ -1,0 +1,30 @@
+// Attention over the 4-bit cache's pages with a view of it: the newest tokens as a tree, of which a
+// token sees its ancestors, and windows whose first tokens stay visible.
+//
+// The formula, the tiles and the split of the work are those of skv_fp4_attention.hip; what
+// differs is which positions a row sees.  A token's history is the positions before the new
+// ones, then the new ones of its mask (without a tree: those up to itself); it sees the history's
+// last `window` and first `first` positions.  Of a row that is a few numbers, worked out once: the
+// end hi of what it sees of the old positions, the begin lo of its window, the end `keep` of its
+// first tokens (both as positions, found in the mask where they fall among the new ones).  A
+// tile is then masked by a word of 32 bits for a row,
+//   (below hi, or of the mask) and (not below lo, or below keep),
+// and only the tiles at these borders are: the old positions between them are seen by all rows.
+// A span's tiles are the first tokens' and the window's, numbered through, so that the ones
+// between are neither read nor dealt to a workgroup.  A row whose mask is empty is as the others
+// in the tiles that all see, and cleared at the end.
+#include "skv_fp4_attn.h"
+
+using namespace skv;
+
+extern "C" int64_t skv_fp4_attention_view_workspace(const skv_fp4_attention_desc* d, const skv_fp4_view* v) {
+  if (!v) return set_error(SKV_EINVAL, "skv_fp4_attention_view: NULL view"), -1;
+  Fp4AttnPlan p;
+  return fp4_attn_plan(d, v, p) == SKV_OK ? p.ws_bytes : -1;
+}
+
+extern "C" int skv_fp4_attention_view(const skv_fp4_attention_desc* d, const skv_fp4_view* v, void* workspace, int64_t ws_bytes,
+                                      void* stream) {
+  if (!v) return set_error(SKV_EINVAL, "skv_fp4_attention_view: NULL view");
+  return fp4_attn_call<true>(d, v, workspace, ws_bytes, stream);
+}

@@ -95,6 +95,8 @@ SIGNATURES: dict[str, list] = {
     "skv_fp4_attention_desc_size": [],
     "skv_fp4_attention_workspace": [_P],
     "skv_fp4_attention": [_P, _P, _I64, _P],
+    "skv_fp4_attention_view_workspace": [_P, _P],
+    "skv_fp4_attention_view": [_P, _P, _P, _I64, _P],
     "skv_decode_step": [_P, _P, _P],
     "skv_decode_step_launches": [_P],
     "skv_decode_desc_sizes": [_P],
@@ -159,10 +161,16 @@ class Fp4Rows(ctypes.Structure):
     _fields_ = [("data", _P), ("seq_stride", _I64), ("tok_stride", _I64), ("head_stride", _I64)]
 
 
+class Fp4View(ctypes.Structure):
+    """skv_fp4_view: which of a 4-bit token cache's positions the newest tokens see."""
+
+    _fields_ = [("tree", _P), ("tree_words", _I64), ("first", _I64)]
+
+
 # entry points returning a size rather than a status code
 INT64_RESULTS = {"skv_topk_workspace_words", "skv_attention_workspace", "skv_attention_desc_size",
                  "skv_decode_step_attend_workspace", "skv_fp4_page_bytes", "skv_fp4_attention_desc_size",
-                 "skv_fp4_attention_workspace"}
+                 "skv_fp4_attention_workspace", "skv_fp4_attention_view_workspace"}
 
 _lib: ctypes.CDLL | None = None
 

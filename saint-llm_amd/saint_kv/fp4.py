@@ -57,7 +57,8 @@ def _check_layout() -> None:
 def fp4_attention(q: torch.Tensor, pool: torch.Tensor, block_table: torch.Tensor, seq_lens: torch.Tensor, *,
                   n_new: torch.Tensor | None = None, window: int | None = None, sink: torch.Tensor | None = None,
                   softcap: float | None = None, scale: float | None = None, max_len: int = 0, splits: int = 0,
-                  out: torch.Tensor | None = None, workspace: torch.Tensor | None = None) -> torch.Tensor:
+                  first: int = 0, tree: torch.Tensor | None = None, out: torch.Tensor | None = None,
+                  workspace: torch.Tensor | None = None) -> torch.Tensor:
     """Attention of each sequence's newest tokens over its 4-bit pages, bf16 of
     q's shape.
 
@@ -69,8 +70,12 @@ def fp4_attention(q: torch.Tensor, pool: torch.Tensor, block_table: torch.Tensor
     sequence b's newest, token t at position seq_lens - n_new + t, and later ones
     get 0 (a count past T is T).  pool, block_table: as ``ops.fp4_quant_append`` wrote them; seq_lens:
     int32 [B].  window: only the newest ``window`` positions up to itself (None:
-    all); sink: fp32 [H] or None; softcap: c*tanh(s/c) of the scores, or None;
+    all); first: the sequence's first positions that stay visible behind a window; sink: fp32 [H] or None; softcap: c*tanh(s/c) of the scores, or None;
     scale: of the scores (None: 1/sqrt(D)).  A token that sees nothing gets 0.
+    tree: int64 [B, T, ceil(T / 64)], T <= 1024, where the new tokens are a drafted tree
+    (``ops.draft_tree`` makes it): bit j of token t's words says that it sees new token
+    j <= t.  ``window`` and ``first`` then count in a token's history, the positions before the
+    new tokens and those of its mask after them; a token with an empty mask sees nothing.
     max_len: a bound on seq_lens (0: what the table holds; longer ones are still
     right), which saves short sequences the launch that joins parts of long ones;
     splits: at most about that many workgroups for a K/V head of every sequence,
@@ -81,9 +86,8 @@ def fp4_attention(q: torch.Tensor, pool: torch.Tensor, block_table: torch.Tensor
     workspace: a tensor of at least ``fp4_attention_workspace`` bytes, of no other
     call that may run at the same time (None: one is allocated for the call)."""
     d, out = _desc(q, pool, block_table, seq_lens, n_new, window, sink, softcap, scale, max_len, splits, out)
-    need = int(_lib.load().skv_fp4_attention_workspace(ctypes.byref(d)))
-    if need < 0:
-        _lib.check(_lib.SKV_EINVAL, "skv_fp4_attention_workspace")
+    view = _view(q, first, tree)
+    need = _workspace(d, view)
     ws_ptr, ws_bytes = None, 0
     if workspace is not None:
         ws_bytes = workspace.numel() * workspace.element_size()
@@ -96,19 +100,47 @@ def fp4_attention(q: torch.Tensor, pool: torch.Tensor, block_table: torch.Tensor
         ws_bytes = need
     if workspace is not None:
         ws_ptr = workspace.data_ptr()
-    _launch(q.device, "skv_fp4_attention", ctypes.byref(d), ws_ptr, ws_bytes)
+    if view is None:
+        _launch(q.device, "skv_fp4_attention", ctypes.byref(d), ws_ptr, ws_bytes)
+    else:
+        _launch(q.device, "skv_fp4_attention_view", ctypes.byref(d), ctypes.byref(view), ws_ptr, ws_bytes)
     return out
 
 
 def fp4_attention_workspace(q: torch.Tensor, pool: torch.Tensor, block_table: torch.Tensor, *,
-                            window: int | None = None, max_len: int = 0, splits: int = 0) -> int:
+                            window: int | None = None, max_len: int = 0, splits: int = 0, first: int = 0,
+                            tree: torch.Tensor | None = None) -> int:
     """Bytes of workspace that ``fp4_attention`` needs for these shapes (0: none)."""
     lens = torch.empty(q.shape[0], dtype=torch.int32, device=q.device)
     d, _ = _desc(q, pool, block_table, lens, None, window, None, None, None, max_len, splits, None)
-    need = int(_lib.load().skv_fp4_attention_workspace(ctypes.byref(d)))
+    return _workspace(d, _view(q, first, tree))
+
+
+def _workspace(d: Fp4AttentionDesc, view: _lib.Fp4View | None) -> int:
+    lib = _lib.load()
+    if view is None:
+        need = int(lib.skv_fp4_attention_workspace(ctypes.byref(d)))
+    else:
+        need = int(lib.skv_fp4_attention_view_workspace(ctypes.byref(d), ctypes.byref(view)))
     if need < 0:
         _lib.check(_lib.SKV_EINVAL, "skv_fp4_attention_workspace")
     return need
+
+
+def _view(q: torch.Tensor, first: int, tree: torch.Tensor | None) -> _lib.Fp4View | None:
+    """What the newest tokens see of the cache where it is not simply all, or a window of it."""
+    if first < 0:
+        raise ValueError(f"first must be >= 0; got {first}")
+    if tree is None:
+        return _lib.Fp4View(None, 0, int(first)) if first else None
+    _require_gpu(tree, "tree")
+    tokens = q.shape[1] if q.dim() == 4 else 1
+    shape = (q.shape[0], tokens, -(-tokens // 64))
+    if tree.dtype != torch.int64 or tuple(tree.shape) != shape or not tree.is_contiguous():
+        raise ValueError(f"tree must be a contiguous int64 {list(shape)} tensor; got {tree.dtype} {list(tree.shape)}")
+    if tree.device != q.device:
+        raise ValueError(f"tree is on {tree.device}, q on {q.device}")
+    return _lib.Fp4View(tree.data_ptr(), shape[2], int(first))
 
 
 def _desc(q, pool, block_table, seq_lens, n_new, window, sink, softcap, scale, max_len, splits,
