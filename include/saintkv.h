@@ -543,6 +543,79 @@ int64_t skv_fp4_attention_view_workspace(const skv_fp4_attention_desc* desc, con
 int skv_fp4_attention_view(const skv_fp4_attention_desc* desc, const skv_fp4_view* view, void* workspace,
                            int64_t ws_bytes, void* stream);
 
+/* ---- drafted tokens -------------------------------------------------------------
+ * A step that checks several tokens at once: the n_new[b] newest tokens of
+ * sequence b (n_new NULL: n_nodes of each) are the nodes of a tree, node t
+ * following node parents[b][t] < t, or for -1 the tokens before the tree.
+ * parents: int32 [batch, n_nodes]; n_nodes <= 1024, batch <= 65535.  The
+ * generalisation to trees of the greedy check of the reference's drafts
+ * (inference/eagle3.py), whose cache keeps rejected tokens only by being
+ * filled anew.
+ *
+ * skv_draft_tree: the masks that skv_fp4_attention_view takes, tree: uint64
+ * [batch, n_nodes, ceil(n_nodes / 64)], each node's bit and its ancestors', and
+ * depths: int32 [batch, n_nodes], how many ancestors it has (its rotary position
+ * is that of the first new token plus its depth).  A node past n_new[b], and one
+ * whose parent (or an ancestor's) is not -1 or an earlier node, gets an empty
+ * mask and depth 0.
+ *
+ * skv_accept_drafts: from node 0, which is always accepted (the token that the
+ * step before picked), to the child whose token is the one picked after its
+ * parent, and so on: tokens[b][t] is node t's token, picks[b][t] the model's pick
+ * after it; of children with the same token the first.  path: int32 [batch,
+ * n_nodes], the accepted nodes (ascending), then -1; n_keep: int32 [batch], how
+ * many; next: of picks' type [batch], the pick after the last (no nodes: -1). */
+typedef struct skv_token_ids {
+  const void* data;               /* int32, or int64 where wide; token t of sequence b at b*seq_stride + t*tok_stride */
+  int64_t seq_stride, tok_stride; /* in ids */
+  int32_t wide, reserved;
+} skv_token_ids;
+
+int skv_draft_tree(const int32_t* parents, const int32_t* n_new, int64_t batch, int64_t n_nodes, uint64_t* tree,
+                   int32_t* depths, void* stream);
+int skv_accept_drafts(const int32_t* parents, const skv_token_ids* tokens, const skv_token_ids* picks,
+                      const int32_t* n_new, int64_t batch, int64_t n_nodes, int32_t* path, int32_t* n_keep, void* next,
+                      void* stream);
+
+/* Of the n_new[b] newest tokens of sequence b (n_new NULL: n_new_uniform) the
+ * n_keep[b] ones path[b][0] < path[b][1] < ... stay, as its newest: in every
+ * pool (skv_fp4_cache pages of the same geometry, cache->pool and
+ * ->block_table unused) their keys' and values' rows move together behind the
+ * tokens before, seq_lens[b] shrinks by n_new[b] - n_keep[b], and pages
+ * without a token return to the free stack (sequences ascending, a sequence's
+ * last page first), their table entries becoming -1.  n_keep 0 drops all of the
+ * new tokens.  refs: the counts of a cache that forks, or NULL.  All-or-nothing:
+ * where a count or a path is not as said, a page is not mapped, or one that is
+ * written or cut is shared (SKV_STATUS_BADARG), or the stack would overflow
+ * (SKV_STATUS_STACK), nothing is written but *status (not NULL) and the
+ * workspace.  path: int32, rows of path_stride <= 1024; batch <= 4096, up to 32
+ * pools.  Calls that share a workspace must not overlap. */
+int64_t skv_keep_tokens_workspace(int64_t batch, int64_t path_stride);
+int skv_keep_tokens(int32_t* free_stack, int32_t* free_top, const int32_t* refs, const skv_fp4_cache* cache,
+                    int32_t* block_table, int32_t* seq_lens, const int32_t* n_new, int32_t n_new_uniform,
+                    const int32_t* path, int64_t path_stride, const int32_t* n_keep, void* const* pools,
+                    int32_t n_pools, int32_t* status, void* workspace, int64_t ws_bytes, void* stream);
+
+/* ---- token probabilities ----------------------------------------------------------
+ * For each of `rows` rows x of `vocab` logits (format SKV_LOGITS_*, row r at
+ * logits + r*row_stride elements, the logits of a row contiguous; aligned to
+ * their size): with m = max x, l = sum exp(x - m)
+ *   logprobs[r] = x[token] - m - ln l        (0 for a negative token, NaN past the vocabulary)
+ *   entropy[r]  = ln l - sum exp(x - m) (x - m) / l
+ *   top_ids[r], top_logprobs[r]: the `top` largest (0..64, at most vocab) in
+ *     descending order, of equal ones the lowest id first, a NaN before all
+ * in fp32 (int32 ids).  Logits of -inf have probability 0; a row whose largest
+ * logit is infinite or a NaN has NaN for all of its numbers.  tokens: rows ids with
+ * tok_stride (seq_stride unused), or NULL: logprobs is not written.  The bytes that
+ * a call needs: skv_token_logprobs_workspace (-1: bad sizes). */
+#define SKV_LOGITS_BF16 0
+#define SKV_LOGITS_F16 1
+#define SKV_LOGITS_F32 2
+int64_t skv_token_logprobs_workspace(int64_t rows, int64_t vocab, int32_t format, int64_t top);
+int skv_token_logprobs(const void* logits, int64_t rows, int64_t vocab, int64_t row_stride, int32_t format,
+                       const skv_token_ids* tokens, int64_t top, float* logprobs, float* entropy, int32_t* top_ids,
+                       float* top_logprobs, void* workspace, int64_t ws_bytes, void* stream);
+
 /* ---- fused decode step ----------------------------------------------------
  * One decode step (one new token per sequence) of a stack of heterogeneous
  * layers in three launches, whatever the layer count:

@@ -97,6 +97,12 @@ SIGNATURES: dict[str, list] = {
     "skv_fp4_attention": [_P, _P, _I64, _P],
     "skv_fp4_attention_view_workspace": [_P, _P],
     "skv_fp4_attention_view": [_P, _P, _P, _I64, _P],
+    "skv_draft_tree": [_P, _P, _I64, _I64, _P, _P, _P],
+    "skv_accept_drafts": [_P, _P, _P, _P, _I64, _I64, _P, _P, _P, _P],
+    "skv_keep_tokens_workspace": [_I64, _I64],
+    "skv_keep_tokens": [_P, _P, _P, _P, _P, _P, _P, _I32, _P, _I64, _P, _P, _I32, _P, _P, _I64, _P],
+    "skv_token_logprobs_workspace": [_I64, _I64, _I32, _I64],
+    "skv_token_logprobs": [_P, _I64, _I64, _I64, _I32, _P, _I64, _P, _P, _P, _P, _P, _I64, _P],
     "skv_decode_step": [_P, _P, _P],
     "skv_decode_step_launches": [_P],
     "skv_decode_desc_sizes": [_P],
@@ -167,10 +173,17 @@ class Fp4View(ctypes.Structure):
     _fields_ = [("tree", _P), ("tree_words", _I64), ("first", _I64)]
 
 
+class TokenIds(ctypes.Structure):
+    """skv_token_ids: int32 or int64 token ids of any strides."""
+
+    _fields_ = [("data", _P), ("seq_stride", _I64), ("tok_stride", _I64), ("wide", _I32), ("reserved", _I32)]
+
+
 # entry points returning a size rather than a status code
 INT64_RESULTS = {"skv_topk_workspace_words", "skv_attention_workspace", "skv_attention_desc_size",
                  "skv_decode_step_attend_workspace", "skv_fp4_page_bytes", "skv_fp4_attention_desc_size",
-                 "skv_fp4_attention_workspace", "skv_fp4_attention_view_workspace"}
+                 "skv_fp4_attention_workspace", "skv_fp4_attention_view_workspace",
+                 "skv_keep_tokens_workspace", "skv_token_logprobs_workspace"}
 
 _lib: ctypes.CDLL | None = None
 

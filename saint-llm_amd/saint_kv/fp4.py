@@ -308,17 +308,41 @@ class Fp4TokenCache:
             self._recorded.add(layer)
 
     def attention(self, i: int, q: torch.Tensor, *, window: int | None = None, sink: torch.Tensor | None = None,
-                  softcap: float | None = None, scale: float | None = None,
-                  out: torch.Tensor | None = None) -> torch.Tensor:
+                  softcap: float | None = None, scale: float | None = None, first: int = 0,
+                  tree: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
         """``fp4_attention`` of layer i for the queries of the newest tokens; after a
-        ragged reservation of sequence b's first n_new[b] (the others get 0)."""
+        ragged reservation of sequence b's first n_new[b] (the others get 0).  tree: the
+        masks of drafted tokens (``ops.draft_tree``)."""
         n_new = self._n_new if isinstance(self._n_new, torch.Tensor) else None
         if n_new is None and self._padded and q.dim() == 4 and q.shape[1] > self._n_new:
             # the newest of several reservations, or a padded batch as k and v were
             raise ValueError(f"{self._n_new} tokens were reserved, q has {q.shape[1]}: reserve a count for each sequence "
                              "for a padded batch")
         return fp4_attention(q, self.pool[i], self.block_table, self.seq_lens, n_new=n_new, window=window, sink=sink,
-                             softcap=softcap, scale=scale, max_len=int(self.host_lens.max()), out=out)
+                             softcap=softcap, scale=scale, max_len=int(self.host_lens.max()), first=first, tree=tree,
+                             out=out)
+
+    def keep(self, path: torch.Tensor, n_keep: torch.Tensor) -> np.ndarray:
+        """Of each sequence's tokens reserved last only ``path[b, :n_keep[b]]`` stay (int32 [B, P] and [B], as
+        ``ops.accept_drafts`` gives them): the others leave the lengths and every layer, and
+        pages behind return to the free list.  They are the tokens reserved last from then on.  Reads back, and returns,
+        how many stayed; raises if a layer still has to append them, or a fork shares them."""
+        missing = self._unwritten - self._recorded
+        if missing:
+            raise RuntimeError(f"the tokens reserved last have not been appended to layers {sorted(missing)}")
+        if self._shared:
+            raise RuntimeError("the tokens reserved last are a fork's, too: they lie in shared pages")
+        n_new = torch.as_tensor(self._host_new.astype(np.int32), device=self.device)  # none of a released sequence
+        ops.keep_tokens(self.free_stack, self.free_top, self.block_table, self.seq_lens, n_new, path, n_keep, self.pool,
+                        self._status_word(), refs=self.refs)
+        kept = n_keep.clone()
+        counts = kept.cpu().numpy().astype(np.int64)
+        self.check_status()
+        bs, before = self.block_size, self.host_lens
+        self.host_lens = before - self._host_new + counts
+        self.host_free += int(((before + bs - 1) // bs - (self.host_lens + bs - 1) // bs).sum())
+        self._n_new, self._host_new, self._most_new = kept, counts, int(counts.max())
+        return counts
 
     def check_status(self) -> None:
         """Synchronise and raise if the device refused a reservation, fork or release
@@ -330,7 +354,7 @@ class Fp4TokenCache:
                 t.zero_()
             self.host_lens = self.seq_lens.cpu().numpy().astype(np.int64)
             self.host_free = int(self.free_top.item())
-            raise RuntimeError(f"Fp4TokenCache reservation, fork or release refused (status bits {bits})")
+            raise RuntimeError(f"Fp4TokenCache reservation, fork or release refused, or a keep (status bits {bits})")
 
     # ------------------------------------------------------ forks, eviction --
     def fork(self, src: list[int], dst: list[int]) -> None:

@@ -9,12 +9,15 @@ from __future__ import annotations
 
 import ctypes
 import math
+from typing import NamedTuple
 
 import torch
 
 from saint_kv import _lib
 
 INT32 = torch.int32
+MAX_NODES = 1024  # of a drafted tree
+MAX_TOP = 64  # alternatives of token_logprobs
 
 
 def _require_gpu(t: torch.Tensor, name: str) -> None:
@@ -758,6 +761,194 @@ def fp4_gather(pool: torch.Tensor, block_table: torch.Tensor, seq_lens: torch.Te
     _launch(pool.device, "skv_fp4_gather", ctypes.byref(c), seq_lens.data_ptr(), n_ptr, n_uni, ctypes.byref(k_rows),
             ctypes.byref(v_rows), out_k.shape[1])
     return out_k, out_v
+
+
+# ---------------------------------------------------------------------------
+# Drafted tokens
+# ---------------------------------------------------------------------------
+def _tree_shape(parents: torch.Tensor, n_new: torch.Tensor | None) -> tuple[int, int]:
+    _require_i32(parents, "parents")
+    if parents.dim() != 2 or not 1 <= parents.shape[1] <= MAX_NODES:
+        raise ValueError(f"parents must be int32 [batch, 1..{MAX_NODES}]; got {tuple(parents.shape)}")
+    if n_new is not None:
+        _require_i32(n_new, "n_new", tuple(parents.shape[:1]))
+        _same_device(parents, "parents", n_new=n_new)
+    return parents.shape[0], parents.shape[1]
+
+
+def draft_tree(parents: torch.Tensor, n_new: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """What the nodes of drafted trees see, and how deep they are: (tree, depths).
+
+    parents: int32 [B, T], T <= 1024: node t of sequence b, its t-th newest token, follows node
+    ``parents[b, t]`` < t, or for -1 the tokens before the tree; n_new: int32 [B], the nodes of
+    each tree (None: T).  tree: int64 [B, T, ceil(T / 64)], the masks that ``fp4_attention`` takes (one call
+    a step, for all layers); depths: int32 [B, T], a node's rotary position less that of the first new
+    token.  Past ``n_new[b]``, and where a parent is not an earlier node, a mask is empty and the depth 0."""
+    batch, nodes = _tree_shape(parents, n_new)
+    tree = torch.empty(batch, nodes, -(-nodes // 64), dtype=torch.int64, device=parents.device)
+    depths = torch.empty(batch, nodes, dtype=INT32, device=parents.device)
+    _launch(parents.device, "skv_draft_tree", parents.data_ptr(), _lib.ptr(n_new), batch, nodes, tree.data_ptr(),
+            depths.data_ptr())
+    return tree, depths
+
+
+def _token_ids(t: torch.Tensor, name: str, shape: tuple[int, ...]) -> _lib.TokenIds:
+    """skv_token_ids of t, int32 or int64 of one or two dims and any strides."""
+    _require_gpu(t, name)
+    if t.dtype not in (INT32, torch.int64) or tuple(t.shape) != shape:
+        raise ValueError(f"{name} must be int32 or int64 {list(shape)}; got {t.dtype} {list(t.shape)}")
+    return _lib.TokenIds(t.data_ptr(), t.stride(0), t.stride(-1), t.dtype == torch.int64)
+
+
+def accept_drafts(parents: torch.Tensor, tokens: torch.Tensor, picks: torch.Tensor,
+                  n_new: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """The nodes of drafted trees that the model's own picks bear out: (path, n_keep, next).
+
+    parents, n_new: as in ``draft_tree``; tokens, picks: int32 or int64 [B, T] of any strides, node t's
+    token and the model's pick after it (its most likely token, or one drawn from its distribution).
+    Node 0 is accepted; after a node the child (the first of them) whose token is the node's pick.  path:
+    int32 [B, T], the accepted nodes, then -1; n_keep: int32 [B], their number; next: [B] of picks'
+    type, the pick after the last of them (-1 where a tree has no nodes).  ``keep_tokens`` takes path and n_keep."""
+    batch, nodes = _tree_shape(parents, n_new)
+    ids, wanted = _token_ids(tokens, "tokens", (batch, nodes)), _token_ids(picks, "picks", (batch, nodes))
+    _same_device(parents, "parents", tokens=tokens, picks=picks)
+    path = torch.empty(batch, nodes, dtype=INT32, device=parents.device)
+    n_keep = torch.empty(batch, dtype=INT32, device=parents.device)
+    following = torch.empty(batch, dtype=picks.dtype, device=parents.device)
+    _launch(parents.device, "skv_accept_drafts", parents.data_ptr(), ctypes.byref(ids), ctypes.byref(wanted),
+            _lib.ptr(n_new), batch, nodes, path.data_ptr(), n_keep.data_ptr(), following.data_ptr())
+    return path, n_keep, following
+
+
+def keep_tokens(free_stack: torch.Tensor, free_top: torch.Tensor, block_table: torch.Tensor, seq_lens: torch.Tensor,
+                n_new: int | torch.Tensor, path: torch.Tensor, n_keep: torch.Tensor, pools: list[torch.Tensor],
+                status: torch.Tensor, refs: torch.Tensor | None = None, workspace: torch.Tensor | None = None) -> None:
+    """Of each sequence's ``n_new`` newest tokens only ``path[b, :n_keep[b]]`` (int32 [B, P], P <= 1024,
+    ascending; n_keep int32 [B]) stay: in every 4-bit pool their rows move together, ``seq_lens``
+    shrinks, and the pages behind return to the free stack.
+
+    pools: up to 32 of ``fp4_pool``'s, of one shape; refs: the counts of a cache that forks (see ``fork``);
+    workspace: 16 bytes for each entry of path, of no other call that may run at the same time (None: one is
+    allocated for the call).  All-or-nothing: a refusal sets ``status`` and writes nothing else (see
+    skv_keep_tokens)."""
+    n_pages = free_stack.numel()
+    _require_i32(free_stack, "free_stack")
+    _require_i32(free_top, "free_top", (1,))
+    if not 1 <= len(pools) <= 32:
+        raise ValueError(f"keep_tokens takes 1 to 32 pools; got {len(pools)}")
+    cache = fp4_cache(pools[0], block_table)
+    batch = block_table.shape[0]
+    shape, bases = pools[0].shape, (ctypes.c_void_p * len(pools))()
+    if shape[0] != n_pages:
+        raise ValueError(f"free_stack is of {n_pages} pages, the pools of {shape[0]}")
+    for i, p in enumerate(pools):
+        _require_gpu(p, f"pools[{i}]")
+        if p.dtype != torch.uint8 or p.shape != shape or not p.is_contiguous():
+            raise ValueError(f"pools[{i}] must be a contiguous uint8 {list(shape)} tensor; got {p.dtype} {list(p.shape)}")
+        if p.device != block_table.device:
+            raise ValueError(f"pools[{i}] is on {p.device}, block_table on {block_table.device}")
+        bases[i] = p.data_ptr()
+    _require_i32(seq_lens, "seq_lens", (batch,))
+    _require_i32(path, "path")
+    if path.dim() != 2 or path.shape[0] != batch or not 1 <= path.shape[1] <= MAX_NODES:
+        raise ValueError(f"path must be int32 [{batch}, 1..{MAX_NODES}]; got {tuple(path.shape)}")
+    _require_i32(n_keep, "n_keep", (batch,))
+    _require_i32(status, "status", (1,))
+    if refs is not None:
+        _require_i32(refs, "refs", (n_pages,))
+    n_ptr, n_uni = _n_new_args(n_new, batch)
+    _same_device(block_table, "block_table", free_stack=free_stack, free_top=free_top, seq_lens=seq_lens, path=path,
+                 n_keep=n_keep, status=status, refs=refs, n_new=n_new if n_ptr is not None else None)
+    need = path.numel() * 16
+    if workspace is None:
+        workspace = torch.empty(need, dtype=torch.uint8, device=path.device)
+    elif (workspace.device != path.device or workspace.numel() * workspace.element_size() < need
+          or not workspace.is_contiguous() or workspace.data_ptr() % 16):
+        raise ValueError(f"workspace must hold {need} contiguous bytes on {path.device}, 16-byte aligned")
+    _launch(block_table.device, "skv_keep_tokens", free_stack.data_ptr(), free_top.data_ptr(), _lib.ptr(refs),
+            ctypes.byref(cache), block_table.data_ptr(), seq_lens.data_ptr(), n_ptr, n_uni, path.data_ptr(),
+            path.shape[1], n_keep.data_ptr(), ctypes.cast(bases, ctypes.c_void_p), len(pools), status.data_ptr(),
+            workspace.data_ptr(), workspace.numel() * workspace.element_size())
+
+
+# ---------------------------------------------------------------------------
+# Token probabilities
+# ---------------------------------------------------------------------------
+class TokenLogprobs(NamedTuple):
+    """What ``token_logprobs`` gives for each row of logits."""
+
+    logprobs: torch.Tensor | None
+    entropy: torch.Tensor
+    top_ids: torch.Tensor
+    top_logprobs: torch.Tensor
+
+
+_LOGITS = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}  # SKV_LOGITS_*
+
+
+def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor | None = None, *, top: int = 0,
+                   workspace: torch.Tensor | None = None) -> TokenLogprobs:
+    """Log probabilities of given tokens, the entropy and the most likely tokens of each row of logits, in one
+    pass over them: (logprobs, entropy, top_ids, top_logprobs).
+
+    logits: bf16, fp16 or fp32 [..., V] (rows contiguous, one stride between them); tokens: int32 or int64 [...]
+    or None.  logprobs: fp32 [...], 0 where a token is negative, NaN where it is past the vocabulary (None
+    without tokens); entropy: fp32 [...], in nats; top_ids, top_logprobs: int32 and fp32 [..., top], top <= 64, the
+    largest first, of equal ones the lowest id.  Logits of -inf have probability 0; a row whose largest is infinite or
+    a NaN gives NaN.  workspace: of at least ``token_logprobs_workspace`` bytes, of no other call that may run at the
+    same time (None: one is allocated where the call needs it)."""
+    rows, stride, lead = _logit_rows(logits, top)
+    vocab, device = logits.shape[-1], logits.device
+    f32 = dict(dtype=torch.float32, device=device)
+    ids = None
+    if tokens is not None:
+        if tuple(tokens.shape) != lead:
+            raise ValueError(f"tokens must be int32 or int64 {list(lead)}; got {tokens.dtype} {list(tokens.shape)}")
+        flat = tokens.reshape(-1)
+        ids = _token_ids(flat, "tokens", (rows,))
+        _same_device(logits, "logits", tokens=flat)
+    out = TokenLogprobs(None if tokens is None else torch.empty(lead, **f32), torch.empty(lead, **f32),
+                        torch.empty(*lead, top, dtype=INT32, device=device), torch.empty(*lead, top, **f32))
+    need = int(_lib.load().skv_token_logprobs_workspace(rows, vocab, _LOGITS[logits.dtype], top))
+    if need < 0:
+        _lib.check(_lib.SKV_EINVAL, "skv_token_logprobs_workspace")
+    if workspace is not None:
+        if (workspace.device != device or workspace.numel() * workspace.element_size() < need
+                or not workspace.is_contiguous() or workspace.data_ptr() % 16):
+            raise ValueError(f"workspace must hold {need} contiguous bytes on {device}, 16-byte aligned")
+    elif need:
+        workspace = torch.empty(need, dtype=torch.uint8, device=device)
+    _launch(device, "skv_token_logprobs", logits.data_ptr(), rows, vocab, stride, _LOGITS[logits.dtype],
+            None if ids is None else ctypes.byref(ids), top, _lib.ptr(out.logprobs), out.entropy.data_ptr(),
+            out.top_ids.data_ptr(), out.top_logprobs.data_ptr(), _lib.ptr(workspace),
+            0 if workspace is None else workspace.numel() * workspace.element_size())
+    return out
+
+
+def token_logprobs_workspace(logits: torch.Tensor, top: int = 0) -> int:
+    """Bytes of workspace that ``token_logprobs`` needs for these shapes (0: none)."""
+    rows, _, _ = _logit_rows(logits, top)
+    need = int(_lib.load().skv_token_logprobs_workspace(rows, logits.shape[-1], _LOGITS[logits.dtype], top))
+    if need < 0:
+        _lib.check(_lib.SKV_EINVAL, "skv_token_logprobs_workspace")
+    return need
+
+
+def _logit_rows(logits: torch.Tensor, top: int) -> tuple[int, int, tuple[int, ...]]:
+    """Rows, elements between them, and their shape."""
+    _require_gpu(logits, "logits")
+    if logits.dtype not in _LOGITS or logits.dim() < 1 or logits.shape[-1] < 1:
+        raise ValueError(f"logits must be bf16, fp16 or fp32 [..., V]; got {logits.dtype} {tuple(logits.shape)}")
+    lead, vocab = tuple(logits.shape[:-1]), logits.shape[-1]
+    if not 0 <= top <= min(MAX_TOP, vocab):
+        raise ValueError(f"top must be in [0, {min(MAX_TOP, vocab)}]; got {top}")
+    if vocab > 1 and logits.stride(-1) != 1:
+        raise ValueError("a row's logits must be contiguous")
+    sizes = [(n, s) for n, s in zip(lead, logits.stride()[:-1]) if n != 1]
+    for (_, outer), (n, inner) in zip(sizes, sizes[1:]):
+        if outer != n * inner:
+            raise ValueError(f"logits of strides {logits.stride()} have no one stride between their rows")
+    return math.prod(lead), sizes[-1][1] if sizes else vocab, lead
 
 
 # ---------------------------------------------------------------------------
