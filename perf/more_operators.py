@@ -44,9 +44,8 @@ def _dev() -> torch.device:
 
 
 def _api():
-    pkg = str(Path(__file__).resolve().parents[1] / "saint-llm_amd")
-    if pkg not in sys.path:
-        sys.path.insert(0, pkg)
+    if "saint_kv" not in sys.modules:  # a program finds and imports it once
+        sys.path.insert(0, str(Path(__file__).resolve().parents[1] / "saint-llm_amd"))
     import saint_kv
 
     return saint_kv
