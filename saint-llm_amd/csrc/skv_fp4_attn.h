@@ -128,7 +128,7 @@ constexpr int kF4RunTiles = 8;
 constexpr int kF4SmallTiles = 16;
 // What a segment costs beside its tiles, in tiles: the first loads' latencies and the
 // waves' join.  A step of 64 sequences of 1k - 32k, 8 K/V heads: 165 us without it, with 12 tiles
-// 144 and with 20 139 us; the other cases above stay within 1%.  Counted where
+// 144 and with 20 139 us; the other cases of skv_fp4_attention.hip stay within 1%.  Counted where
 // there are about as many items as workgroups or more; a run that would begin in this
 // lead or just past it begins with the item.
 constexpr int kF4Lead = 20;
@@ -239,7 +239,7 @@ struct Fp4Run<2> { using type = uint16_t; };
 template <>
 struct Fp4Run<8> { using type = u32x2; };
 
-template <int DP>
+template <int DP, bool kShared>
 struct Fp4Smem {
   // per wave: 32 value rows of DP bf16; at the end 16 output rows of DP fp32 (private tiles)
   alignas(16) uint8_t tile[kF4Waves][64 * DP];
@@ -248,7 +248,16 @@ struct Fp4Smem {
   int pre[kF4MaxItems + 1];
   int scan[17];
   int longest;
+  // of shared tiles the keys' codes and scale bytes, as the lanes hold them: this round's and the next one's
+  static constexpr bool kKeys = kShared && DP <= 128;
+  alignas(16) uint32_t keys[2][kKeys ? kF4Waves : 1][2][kKeys ? (Fp4Raw<DP>::kKeyWords + Fp4Raw<DP>::kScales) * kWave : 4];
 };
+
+// Four words of an operand register's eight.
+__device__ __forceinline__ u32x4 fp4_quarter(i32x8 v, int half) {
+  return half ? u32x4{static_cast<uint32_t>(v[4]), static_cast<uint32_t>(v[5]), static_cast<uint32_t>(v[6]), static_cast<uint32_t>(v[7])}
+              : u32x4{static_cast<uint32_t>(v[0]), static_cast<uint32_t>(v[1]), static_cast<uint32_t>(v[2]), static_cast<uint32_t>(v[3])};
+}
 
 // DP: the head's dims padded to 64, 128, 256 or 512 (kExact: D == DP).
 template <int DP, int MT, bool kExact, bool kShared, bool kView>
@@ -264,6 +273,10 @@ struct Fp4Wave {
   // head 79 and 67); where the products bound the time (a prompt's chunk 557, with rests 705 us)
   // the rounded weight stands.
   static constexpr bool kRest = !kShared;
+  // Waves of the same rows split a wide query's steps among them (a step is about 1,100 instructions;
+  // 32 windows of 128, 64 rows of 512 dims: 21 us a call, 23 with every wave splitting all four steps).
+  static constexpr bool kSplit = !kShared && kSteps > 1;
+  static constexpr int kSplitWords = 17 * kWave;
   static constexpr bool kTwo = DP * MT <= 256;  // two tiles in flight; wider ones have registers for one
   // A page is read by one workgroup, or by two: nontemporal loads (a step of 64 sequences 139 us,
   // 156 with plain ones; 4 of 256k - 1M 91 and 103; 64 rows on one head, read twice, 79 either way).
@@ -284,7 +297,8 @@ struct Fp4Wave {
   float m[MT], l[MT];
   f32x4 acc[MT][kBlocks];
 
-  __device__ __forceinline__ Fp4Wave(const Fp4Args<kView>& a_, const Fp4Span& sp_, int b, int hk, int r0, int lane)
+  // `split`: LDS where waves of the same rows share the query's split (kSplit), else unused.
+  __device__ __forceinline__ Fp4Wave(const Fp4Args<kView>& a_, const Fp4Span& sp_, int b, int hk, int r0, int lane, uint32_t* split = nullptr)
       : a(a_), sp(sp_), pg(fp4_page(a_.bs, a_.Hkv, kExact ? DP : a_.D)) {
     col = lane & 15;
     grp = lane >> 4;
@@ -301,12 +315,42 @@ struct Fp4Wave {
       lo[mt] = a.window > 0 ? hi[mt] - a.window : 0;
       if constexpr (kView) look(mt, b, in ? t : a.T);
       const uint8_t* row = a.q + b * a.q_seq + t * a.q_tok + (hk * a.G + g) * a.q_head;
+      if constexpr (!kSplit) {
 #pragma unroll
-      for (int s = 0; s < kSteps; ++s) load_query(mt, s, row, in);
+        for (int s = 0; s < kSteps; ++s) q_scale[mt][s] = load_query(s, row, in, q[mt][s]);
+      } else {
+        const int s = __builtin_amdgcn_readfirstlane(threadIdx.x) / kWave - mt * kSteps % kF4Waves;  // of these rows this wave's step
+        if (s >= 0 && s < kSteps) {
+          i32x8 part[2];
+          const int scale = load_query(s, row, in, part);
+          uint32_t* to = split + (mt * kSteps + s) * kSplitWords;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) reinterpret_cast<u32x4*>(to)[i * kWave + lane] = fp4_quarter(part[i >> 1], i & 1);
+          to[16 * kWave + lane] = scale;
+        }
+      }
       m[mt] = kF4None;
       l[mt] = 0.f;
 #pragma unroll
       for (int x = 0; x < kBlocks; ++x) acc[mt][x] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    if constexpr (kSplit) {
+      lds_barrier();  // the steps are there
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) {
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) {
+          const uint32_t* from = split + (mt * kSteps + s) * kSplitWords;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const u32x4 x = reinterpret_cast<const u32x4*>(from)[i * kWave + lane];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) q[mt][s][i >> 1][4 * (i & 1) + k] = static_cast<int>(x[k]);
+          }
+          q_scale[mt][s] = static_cast<int>(from[16 * kWave + lane]);
+        }
+      }
+      lds_barrier();  // and have been read
     }
   }
 
@@ -411,7 +455,7 @@ struct Fp4Wave {
   // The query of row 16 mt + col for step s.  The second operand's lane g holds
   // k = 16 g .. + 15 and 64 + 16 g .. + 15 of the 128, and the scale of k-block g (k = 32 g ..);
   // k-block j is dims 32 (j kScales + s) .. as the keys' lanes have them.
-  __device__ __forceinline__ void load_query(int mt, int s, const uint8_t* row, bool in) {
+  __device__ __forceinline__ int load_query(int s, const uint8_t* row, bool in, i32x8* parts) const {
     const int half = 16 * (grp & 1);
     uint32_t hi[8], lo[8];
     if constexpr (DP >= 128) {
@@ -420,22 +464,22 @@ struct Fp4Wave {
       const int from = col + 32 * (grp & 1);  // k-blocks 0, 1 (2, 3) are the first (second) 16 of lanes 0 and 32
       const int a0 = __shfl(static_cast<int>(b0), from), a1 = __shfl(static_cast<int>(b1), from);
       const int own = grp < 2 ? a0 : a1;
-      q_scale[mt][s] = own | (own - 5) << 8;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        q[mt][s][0][i] = static_cast<int>(hi[i]);
-        q[mt][s][DP >= 128 ? 1 : 0][i] = static_cast<int>(lo[i]);
+        parts[0][i] = static_cast<int>(hi[i]);
+        parts[DP >= 128 ? 1 : 0][i] = static_cast<int>(lo[i]);
       }
+      return own | (own - 5) << 8;
     } else {
       // k-blocks 0, 1: the first part of dims 0 .. 63; 2, 3: the second part of the same
       const uint32_t b = split16(row, 16 * grp, in, hi, lo);
       const int own = __shfl(static_cast<int>(b), col + 32 * (grp & 1));
-      q_scale[mt][s] = grp < 2 ? own : own - 5;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        q[mt][s][0][i] = static_cast<int>(hi[i]);
-        q[mt][s][0][i + 4] = static_cast<int>(lo[i]);
+        parts[0][i] = static_cast<int>(hi[i]);
+        parts[0][i + 4] = static_cast<int>(lo[i]);
       }
+      return grp < 2 ? own : own - 5;
     }
   }
 
@@ -617,6 +661,32 @@ struct Fp4Wave {
     return __ballot(nan) != 0;
   }
 
+  // A tile's keys to LDS and from there: words of 16 bytes by lane, then the scales'.
+  __device__ __forceinline__ void keep_keys(const Raw& r, uint32_t (*to)[(Raw::kKeyWords + kScales) * kWave], int lane) const {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+#pragma unroll
+      for (int w = 0; w < Raw::kKeyWords; w += 4) {
+        reinterpret_cast<u32x4*>(to[h])[(w / 4) * kWave + lane] = u32x4{r.k[h][w], r.k[h][w + 1], r.k[h][w + 2], r.k[h][w + 3]};
+      }
+#pragma unroll
+      for (int s = 0; s < kScales; ++s) to[h][(Raw::kKeyWords + s) * kWave + lane] = r.ks[h][s];
+    }
+  }
+  __device__ __forceinline__ void take_keys(Raw& r, const uint32_t (*from)[(Raw::kKeyWords + kScales) * kWave], int lane) const {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+#pragma unroll
+      for (int w = 0; w < Raw::kKeyWords; w += 4) {
+        const u32x4 x = reinterpret_cast<const u32x4*>(from[h])[(w / 4) * kWave + lane];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) r.k[h][w + i] = x[i];
+      }
+#pragma unroll
+      for (int s = 0; s < kScales; ++s) r.ks[h][s] = from[h][(Raw::kKeyWords + s) * kWave + lane];
+    }
+  }
+
   // The scores of 32 keys.
   __device__ __forceinline__ void scores(const Raw& r, Fp4Tile<MT>& tl) const {
     auto& st = tl.st;
@@ -654,8 +724,9 @@ struct Fp4Wave {
     }
   }
 
-  // The tile's weights, and its values times them onto the output.
-  __device__ __forceinline__ void output(Fp4Tile<MT>& tl, int pos, const uint16_t* vt) {
+  // The tile's scores under their cap and masks, and the rows' maxima with them.  Returns what the
+  // scores are multiplied by on the way to the log2 domain.
+  __device__ __forceinline__ float settle(Fp4Tile<MT>& tl, int pos) {
     auto& st = tl.st;
     const bool capped = a.cap > 0.f;
     float mult = a.scale;
@@ -726,7 +797,16 @@ struct Fp4Wave {
         for (int x = 0; x < kBlocks; ++x) acc[mt][x] *= alpha;
       }
     }
+    return mult;
+  }
+
+  struct Weights {
     u32x4 p[MT], rest[kRest ? MT : 1];
+  };
+
+  // The tile's weights as bf16 pairs.
+  __device__ __forceinline__ void weigh(const Fp4Tile<MT>& tl, float mult, Weights& w) {
+    const auto& st = tl.st;
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
       float e[8];
@@ -738,13 +818,17 @@ struct Fp4Wave {
       l[mt] += ((e[0] + e[1]) + (e[2] + e[3])) + ((e[4] + e[5]) + (e[6] + e[7]));
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        p[mt][i] = bf16_pack2(e[2 * i], e[2 * i + 1]);
+        const uint32_t p = bf16_pack2(e[2 * i], e[2 * i + 1]);
+        w.p[mt][i] = p;
         if constexpr (kRest) {
-          rest[mt][i] = bf16_pack2(e[2 * i] - __uint_as_float(p[mt][i] << 16), e[2 * i + 1] - __uint_as_float(p[mt][i] & 0xffff0000u));
+          w.rest[mt][i] = bf16_pack2(e[2 * i] - __uint_as_float(p << 16), e[2 * i + 1] - __uint_as_float(p & 0xffff0000u));
         }
       }
     }
-    // O^T += V^T P^T: dims 16 x + 4 grp + i of the output, row 16 mt + col
+  }
+
+  // O^T += V^T P^T: dims 16 x + 4 grp + i of the output, row 16 mt + col.
+  __device__ __forceinline__ void product(const Weights& w, const uint16_t* vt) {
     const int vr = 4 * grp + (col >> 2);
     const uint16_t* v0 = vt + vr * DP + 4 * (col & 1);
 #pragma unroll
@@ -754,12 +838,19 @@ struct Fp4Wave {
       const u32x4 v = u32x4{lo2[0], lo2[1], hi2[0], hi2[1]};
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt) {
-        acc[mt][x] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fp4_bf16x8(v), fp4_bf16x8(p[mt]), acc[mt][x], 0, 0, 0);
+        acc[mt][x] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fp4_bf16x8(v), fp4_bf16x8(w.p[mt]), acc[mt][x], 0, 0, 0);
         if constexpr (kRest) {
-          acc[mt][x] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fp4_bf16x8(v), fp4_bf16x8(rest[mt]), acc[mt][x], 0, 0, 0);
+          acc[mt][x] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fp4_bf16x8(v), fp4_bf16x8(w.rest[mt]), acc[mt][x], 0, 0, 0);
         }
       }
     }
+  }
+
+  __device__ __forceinline__ void output(Fp4Tile<MT>& tl, int pos, const uint16_t* vt) {
+    const float mult = settle(tl, pos);
+    Weights w;
+    weigh(tl, mult, w);
+    product(w, vt);
   }
 };
 
@@ -799,13 +890,13 @@ struct Fp4Pace {
 // segment is a piece of the item, slot `slot_of_part` of the partial ones.  Every wave
 // takes tiles of its own for all of the item's rows.
 template <int DP, int MT, bool kExact, bool kView>
-__device__ __forceinline__ void fp4_segment(Fp4Smem<DP>& sm, const Fp4Args<kView>& a, int b, int rb, int hk, const Fp4Span& sp,
+__device__ __forceinline__ void fp4_segment(Fp4Smem<DP, false>& sm, const Fp4Args<kView>& a, int b, int rb, int hk, const Fp4Span& sp,
                                             int t_from, int t_to, int slot_of_part, Fp4Pace& pace, int done) {
   using Wave = Fp4Wave<DP, MT, kExact, false, kView>;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x) / kWave, lane = fp4_fresh_tid() % kWave;
   const int r0 = rb * 16 * MT;
   const int t_lo = fp4_tile_base<kView>(sp) + t_from, t_hi = fp4_tile_base<kView>(sp) + min(t_to, sp.tiles);
-  Wave w(a, sp, b, hk, r0, lane);
+  Wave w(a, sp, b, hk, r0, lane, reinterpret_cast<uint32_t*>(sm.tile));
   uint16_t* vt = reinterpret_cast<uint16_t*>(sm.tile[wave]);
   // this wave's tiles t_lo + wave, + 4, ...; the places of 32 of them at a time
   uint64_t at = 0;
@@ -916,16 +1007,103 @@ __device__ __forceinline__ void fp4_segment(Fp4Smem<DP>& sm, const Fp4Args<kView
   }
 }
 
-// The same with tiles that the waves share: each has 16 MT of the item's rows and
-// decodes one in four tiles' values for all of them.
+// A wave's part of a cut item of shared tiles: its rows' maxima and sums, then 16 dims of 16 rows at a time, so
+// that a store of the wave is one run of 1 KB.
+struct Fp4Part {
+  float* base;
+  int rows, blocks;
+  __device__ __forceinline__ float* m(int row) const { return base + row; }
+  __device__ __forceinline__ float* l(int row) const { return base + rows + row; }
+  __device__ __forceinline__ f32x4* quad(int row, int d) const {
+    return reinterpret_cast<f32x4*>(base + 2 * rows) + (((row >> 4) * blocks + (d >> 2)) * 16 + (row & 15)) * 4 + (d & 3);
+  }
+};
+
+// The tiles [t_lo, t_hi) that the waves share, in rounds of four: a wave brings one of them to LDS, its
+// values decoded, its keys as they are, these a round earlier, so that a tile's scores are made beside the weights
+// of the one before, over a round's end too.  (2 prompts' 1000 tokens over 16k, 32 heads on 8 of 128: 512 us, 556 with
+// every wave loading all keys itself and a tile's scores ahead of its own weights.)
 template <int DP, int MT, bool kExact, bool kView>
-__device__ __forceinline__ void fp4_segment_shared(Fp4Smem<DP>& sm, const Fp4Args<kView>& a, int b, int rb, int hk, const Fp4Span& sp,
-                                                   int t_from, int t_to, int slot_of_part, Fp4Pace& pace, int done) {
+__device__ __forceinline__ void fp4_rounds_ahead(Fp4Smem<DP, true>& sm, Fp4Wave<DP, MT, kExact, true, kView>& w, const Fp4Span& sp, int b,
+                                           int wave, int lane, int t_lo, int t_hi, Fp4Pace& pace, int done) {
   using Wave = Fp4Wave<DP, MT, kExact, true, kView>;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x) / kWave, lane = fp4_fresh_tid() % kWave;
-  const int r0 = (rb * kF4Waves + wave) * 16 * MT;
-  const int t_lo = fp4_tile_base<kView>(sp) + t_from, t_hi = fp4_tile_base<kView>(sp) + min(t_to, sp.tiles);
-  Wave w(a, sp, b, hk, r0, lane);
+  const int n = t_hi - t_lo;
+  // lane 2 j + h, j < 4: half h of tile i + j (past the last something mapped)
+  const auto places = [&](int i, uint64_t& at, int& slot) {
+    w.lookup(b, fp4_tile<kView>(sp, min(t_lo + i + ((lane >> 1) & 3), t_hi)) * kF4Tile + 16 * (lane & 1), at, slot);
+  };
+  // A round is four tiles: a wave brings one of them to LDS, its values decoded, its keys a round earlier, so that
+  // the first scores of a round are made in the one before.
+  typename Wave::Raw keys, vals, now;
+  uint64_t at[2];  // of the next round and the one after
+  int slot, slot_next[2];
+  places(0, at[0], slot);
+  w.template fetch<true, false>(keys, at[0], slot, 2 * wave);
+  w.template fetch<false, true>(vals, at[0], slot, 2 * wave);
+  places(kF4Waves, at[0], slot_next[0]);
+  places(2 * kF4Waves, at[1], slot_next[1]);
+  w.template unpack_scales<true, false>(keys);
+  w.keep_keys(keys, sm.keys[0][wave], lane);
+  w.template fetch<true, false>(keys, at[0], slot_next[0], 2 * wave);
+  lds_barrier();
+  Fp4Tile<MT> tl;
+  w.take_keys(now, sm.keys[0][0], lane);
+  w.scores(now, tl);
+  float mult = 0.f;
+  // a tile's masks, and its scores under them
+  const auto settle = [&](int i, int j) {
+    const int pos = fp4_tile<kView>(sp, t_lo + i + j) * kF4Tile;
+    tl.slot[0] = now.slot[0] = __builtin_amdgcn_readlane(slot, 2 * j);
+    tl.slot[1] = now.slot[1] = __builtin_amdgcn_readlane(slot, 2 * j + 1);
+    tl.nan_keys = __builtin_amdgcn_readfirstlane(sm.nan_keys[j]);
+    tl.masked = w.uneven(now, pos) || tl.nan_keys != 0;
+    mult = w.settle(tl, pos);
+  };
+  for (int i = 0; i < n; i += kF4Waves) {
+    pace.at(done + i);
+    const int buf = (i / kF4Waves) & 1;
+    {
+      const int pos = fp4_tile<kView>(sp, t_lo + i + wave) * kF4Tile;
+      w.template unpack_scales<false, true>(vals);
+      uint32_t nan_keys = 0;
+      if (w.uneven(vals, pos) || w.any_nan(vals)) nan_keys = w.clean(vals, pos);  // uniform
+      w.values(vals, reinterpret_cast<uint16_t*>(sm.tile[wave]));
+      if (lane == 0) sm.nan_keys[wave] = nan_keys;
+      w.template unpack_scales<true, false>(keys);
+      w.keep_keys(keys, sm.keys[buf ^ 1][wave], lane);
+    }
+    w.template fetch<false, true>(vals, at[0], slot_next[0], 2 * wave);
+    w.template fetch<true, false>(keys, at[1], slot_next[1], 2 * wave);
+    lds_barrier();  // the tiles are there
+    settle(i, 0);
+#pragma unroll
+    for (int j = 0; j < kF4Waves; ++j) {
+      if (i + j < n) {  // uniform
+        // the next tile's scores beside this one's weights
+        typename Wave::Weights p;
+        Fp4Tile<MT> next;
+        w.take_keys(now, j < kF4Waves - 1 ? sm.keys[buf][j + 1] : sm.keys[buf ^ 1][0], lane);
+        w.scores(now, next);
+        w.weigh(tl, mult, p);
+        w.product(p, reinterpret_cast<const uint16_t*>(sm.tile[j]));
+        tl = next;
+        if (j < kF4Waves - 1 && i + j + 1 < n) settle(i, j + 1);
+      }
+    }
+    slot = slot_next[0];
+    at[0] = at[1];
+    slot_next[0] = slot_next[1];
+    places(i + 3 * kF4Waves, at[1], slot_next[1]);
+    lds_barrier();  // the tiles have been read
+  }
+}
+
+// The same where LDS has no room for keys beside two workgroups' values (heads of 256 dims; one workgroup with it: 764 us
+// become 1060 for 2 prompts of 16 heads on 4).
+template <int DP, int MT, bool kExact, bool kView>
+__device__ __forceinline__ void fp4_rounds(Fp4Smem<DP, true>& sm, Fp4Wave<DP, MT, kExact, true, kView>& w, const Fp4Span& sp, int b,
+                                           int wave, int lane, int t_lo, int t_hi, Fp4Pace& pace, int done) {
+  using Wave = Fp4Wave<DP, MT, kExact, true, kView>;
   const int n = t_hi - t_lo;
   // lane 2 j + h, j < 4: half h of tile i + j (past the last something mapped)
   const auto places = [&](int i, uint64_t& at, int& slot) {
@@ -948,7 +1126,7 @@ __device__ __forceinline__ void fp4_segment_shared(Fp4Smem<DP>& sm, const Fp4Arg
       if (lane == 0) sm.nan_keys[wave] = nan_keys;
     }
     places(i + kF4Waves, at_next, slot_next);
-    __syncthreads();  // the tiles are there
+    lds_barrier();  // the tiles are there
 #pragma unroll
     for (int j = 0; j < kF4Waves; ++j) {
       typename Wave::Raw &kr = keys[j & 1], &next = keys[(j + 1) & 1];
@@ -970,7 +1148,24 @@ __device__ __forceinline__ void fp4_segment_shared(Fp4Smem<DP>& sm, const Fp4Arg
     }
     at = at_next;
     slot = slot_next;
-    __syncthreads();  // the tiles have been read
+    lds_barrier();  // the tiles have been read
+  }
+}
+
+// The same with tiles that the waves share: each has 16 MT of the item's rows and
+// decodes one in four tiles' values for all of them.
+template <int DP, int MT, bool kExact, bool kView>
+__device__ __forceinline__ void fp4_segment_shared(Fp4Smem<DP, true>& sm, const Fp4Args<kView>& a, int b, int rb, int hk, const Fp4Span& sp,
+                                                   int t_from, int t_to, int slot_of_part, Fp4Pace& pace, int done) {
+  using Wave = Fp4Wave<DP, MT, kExact, true, kView>;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x) / kWave, lane = fp4_fresh_tid() % kWave;
+  const int r0 = (rb * kF4Waves + wave) * 16 * MT;
+  const int t_lo = fp4_tile_base<kView>(sp) + t_from, t_hi = fp4_tile_base<kView>(sp) + min(t_to, sp.tiles);
+  Wave w(a, sp, b, hk, r0, lane);
+  if constexpr (Fp4Smem<DP, true>::kKeys) {
+    fp4_rounds_ahead(sm, w, sp, b, wave, lane, t_lo, t_hi, pace, done);
+  } else {
+    fp4_rounds(sm, w, sp, b, wave, lane, t_lo, t_hi, pace, done);
   }
   w.drop_blind();
   const int tid = fp4_fresh_tid(), col = tid & 15, grp = (tid >> 4) & 3;
@@ -999,15 +1194,14 @@ __device__ __forceinline__ void fp4_segment_shared(Fp4Smem<DP>& sm, const Fp4Arg
         *reinterpret_cast<u32x2*>(out + d) = u32x2{bf16_pack2(v[0], v[1]), bf16_pack2(v[2], v[3])};
       }
     } else {
-      float* part = a.part + (static_cast<int64_t>(slot_of_part) * kF4Waves + wave) * (16 * MT) * (D + 4) + (16 * mt + col) * (D + 4);
+      const Fp4Part part{a.part + (static_cast<int64_t>(slot_of_part) * kF4Waves + wave) * (16 * MT) * (D + 4), 16 * MT, D / 16};
       if (grp == 0) {
-        part[0] = w.m[mt];
-        part[1] = l;
+        *part.m(16 * mt + col) = w.m[mt];
+        *part.l(16 * mt + col) = l;
       }
 #pragma unroll
       for (int x = 0; x < Wave::kBlocks; ++x) {
-        const int d = 16 * x + 4 * grp;
-        if (kExact || d < D) *reinterpret_cast<f32x4*>(part + 4 + d) = w.acc[mt][x];
+        if (kExact || 16 * x < D) *part.quad(16 * mt + col, 4 * x + grp) = w.acc[mt][x];
       }
     }
   }
@@ -1016,7 +1210,7 @@ __device__ __forceinline__ void fp4_segment_shared(Fp4Smem<DP>& sm, const Fp4Arg
 template <int DP, int MT, bool kExact, bool kShared, bool kView>
 __global__ __launch_bounds__(kF4Threads, fp4_resident(DP, MT)) void k_fp4_attn(Fp4Args<kView> a) {
   constexpr int kRows = 16 * MT * (kShared ? kF4Waves : 1);
-  __shared__ Fp4Smem<DP> sm;
+  __shared__ Fp4Smem<DP, kShared> sm;
   const int tid = threadIdx.x;
   const int items = a.B * a.row_blocks;
   const auto span_of = [&](int item, int& b, int& rb) {
@@ -1153,18 +1347,30 @@ inline int fp4_attn_plan(const skv_fp4_attention_desc* d, const skv_fp4_view* v,
     if (reinterpret_cast<uintptr_t>(v->tree) & 7) return set_error(SKV_EINVAL, "%s: tree must be 8-byte aligned", what);
   }
   p.mt = p.shared ? mt : rows <= 16 || p.dims > 256 ? 1 : 2;
+  // the most tiles that a block of so many rows may see
+  const int64_t capacity = d->cache.bt_stride * d->cache.block_size;
+  const auto tiles_of = [&](int64_t block_rows) {
+    int64_t len = d->max_len > 0 ? std::min(d->max_len, capacity) : capacity;
+    if (d->window > 0) {
+      // the rows' tokens see a window and as many more as they are (in a tree: as there are nodes), and the first ones
+      const int64_t tokens = v && v->tree ? d->n_queries : ceil_div(block_rows, d->n_heads / hkv);
+      len = std::min(len, d->window + tokens + (v && v->first > 0 ? v->first + kF4Tile : 0));
+    }
+    return ceil_div(len, kF4Tile) + 1;
+  };
+  // With a view, few tiles and few rows: a workgroup's latency is the call's, and blocks of 16 rows have the shortest, as
+  // long as the device holds them all at once (trees of 8 nodes, 16 heads on 2 of 128, over 400 tokens: 11.0 us for 14.6 with
+  // 1 sequence, 14.8 for 15.9 with 64; 32 nodes, 64 heads on 8: 11.2 for 22.1 with 1, 13.8 for 22.5 with 4, but 38.3 for
+  // 24.8 with 16, which are 2,048 blocks).
+  if (v && d->splits == 0 && tiles_of(16) <= kF4SmallTiles &&
+      d->cache.batch * ceil_div(rows, 16) * hkv <= static_cast<int64_t>(fp4_resident(p.dims, 1)) * device_cus()) {
+    p.shared = false;
+    p.mt = 1;
+  }
   p.rows = 16 * p.mt * (p.shared ? kF4Waves : 1);
   p.row_blocks = ceil_div(rows, p.rows);
   p.items = d->cache.batch * p.row_blocks;
-  // the most tiles that a row block may see
-  const int64_t capacity = d->cache.bt_stride * d->cache.block_size;
-  int64_t len = d->max_len > 0 ? std::min(d->max_len, capacity) : capacity;
-  if (d->window > 0) {
-    // the rows' tokens see a window and as many more as they are (in a tree: as there are nodes), and the first ones
-    const int64_t tokens = v && v->tree ? d->n_queries : ceil_div(p.rows, d->n_heads / hkv);
-    len = std::min(len, d->window + tokens + (v && v->first > 0 ? v->first + kF4Tile : 0));
-  }
-  const int64_t tiles = ceil_div(len, kF4Tile) + 1, units = std::max<int64_t>(p.items * hkv, 1);
+  const int64_t tiles = tiles_of(p.rows), units = std::max<int64_t>(p.items * hkv, 1);
   p.cut = tiles > kF4SmallTiles || d->splits > 0;
   if (p.items > kF4MaxItems || units > INT32_MAX / (ceil_div(capacity, kF4Tile) + 1 + kF4Lead)) p.cut = false;
   if (units >= (1 << 24)) return set_error(SKV_EINVAL, "%s: too many workgroups", what);

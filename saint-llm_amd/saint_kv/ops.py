@@ -37,6 +37,16 @@ def _require_i32(t: torch.Tensor, name: str, shape: tuple[int, ...] | None = Non
         raise ValueError(f"{name} must have shape {shape}; got {tuple(t.shape)}")
 
 
+def _require_i32_on(device: torch.device, **named: tuple[torch.Tensor | None, tuple[int, ...]]) -> None:
+    """Every (tensor, shape) a contiguous int32 tensor of that shape on ``device`` (or None)."""
+    for name, (t, shape) in named.items():
+        # in one condition: ten tensors' separate checks take about as long as a launch
+        if t is not None and not (isinstance(t, torch.Tensor) and t.dtype is INT32 and t.shape == shape
+                                  and t.device == device and t.is_contiguous()):
+            _require_i32(t, name, shape)
+            raise ValueError(f"{name} is on {t.device}, the others on {device}")
+
+
 def _launch(device: torch.device, name: str, *args) -> None:
     """Call an entry point whose last argument is the stream, with ``device``
     current for the call where it is not."""
@@ -770,10 +780,9 @@ def _tree_shape(parents: torch.Tensor, n_new: torch.Tensor | None) -> tuple[int,
     _require_i32(parents, "parents")
     if parents.dim() != 2 or not 1 <= parents.shape[1] <= MAX_NODES:
         raise ValueError(f"parents must be int32 [batch, 1..{MAX_NODES}]; got {tuple(parents.shape)}")
-    if n_new is not None:
-        _require_i32(n_new, "n_new", tuple(parents.shape[:1]))
-        _same_device(parents, "parents", n_new=n_new)
-    return parents.shape[0], parents.shape[1]
+    batch, nodes = parents.shape
+    _require_i32_on(parents.device, n_new=(n_new, (batch,)))
+    return batch, nodes
 
 
 def draft_tree(parents: torch.Tensor, n_new: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
@@ -785,19 +794,23 @@ def draft_tree(parents: torch.Tensor, n_new: torch.Tensor | None = None) -> tupl
     a step, for all layers); depths: int32 [B, T], a node's rotary position less that of the first new
     token.  Past ``n_new[b]``, and where a parent is not an earlier node, a mask is empty and the depth 0."""
     batch, nodes = _tree_shape(parents, n_new)
-    tree = torch.empty(batch, nodes, -(-nodes // 64), dtype=torch.int64, device=parents.device)
-    depths = torch.empty(batch, nodes, dtype=INT32, device=parents.device)
-    _launch(parents.device, "skv_draft_tree", parents.data_ptr(), _lib.ptr(n_new), batch, nodes, tree.data_ptr(),
+    device = parents.device
+    tree = torch.empty(batch, nodes, -(-nodes // 64), dtype=torch.int64, device=device)
+    depths = torch.empty(batch, nodes, dtype=INT32, device=device)
+    _launch(device, "skv_draft_tree", parents.data_ptr(), _lib.ptr(n_new), batch, nodes, tree.data_ptr(),
             depths.data_ptr())
     return tree, depths
 
 
-def _token_ids(t: torch.Tensor, name: str, shape: tuple[int, ...]) -> _lib.TokenIds:
+def _token_ids(t: torch.Tensor, name: str, shape: tuple[int, ...], device: torch.device) -> _lib.TokenIds:
     """skv_token_ids of t, int32 or int64 of one or two dims and any strides."""
     _require_gpu(t, name)
-    if t.dtype not in (INT32, torch.int64) or tuple(t.shape) != shape:
+    if t.dtype not in (INT32, torch.int64) or t.shape != shape:
         raise ValueError(f"{name} must be int32 or int64 {list(shape)}; got {t.dtype} {list(t.shape)}")
-    return _lib.TokenIds(t.data_ptr(), t.stride(0), t.stride(-1), t.dtype == torch.int64)
+    if t.device != device:
+        raise ValueError(f"{name} is on {t.device}, the others on {device}")
+    strides = t.stride()
+    return _lib.TokenIds(t.data_ptr(), strides[0], strides[-1], t.dtype is torch.int64)
 
 
 def accept_drafts(parents: torch.Tensor, tokens: torch.Tensor, picks: torch.Tensor,
@@ -810,12 +823,12 @@ def accept_drafts(parents: torch.Tensor, tokens: torch.Tensor, picks: torch.Tens
     int32 [B, T], the accepted nodes, then -1; n_keep: int32 [B], their number; next: [B] of picks'
     type, the pick after the last of them (-1 where a tree has no nodes).  ``keep_tokens`` takes path and n_keep."""
     batch, nodes = _tree_shape(parents, n_new)
-    ids, wanted = _token_ids(tokens, "tokens", (batch, nodes)), _token_ids(picks, "picks", (batch, nodes))
-    _same_device(parents, "parents", tokens=tokens, picks=picks)
-    path = torch.empty(batch, nodes, dtype=INT32, device=parents.device)
-    n_keep = torch.empty(batch, dtype=INT32, device=parents.device)
-    following = torch.empty(batch, dtype=picks.dtype, device=parents.device)
-    _launch(parents.device, "skv_accept_drafts", parents.data_ptr(), ctypes.byref(ids), ctypes.byref(wanted),
+    device, shape = parents.device, (batch, nodes)
+    ids, wanted = _token_ids(tokens, "tokens", shape, device), _token_ids(picks, "picks", shape, device)
+    path = torch.empty(batch, nodes, dtype=INT32, device=device)
+    n_keep = torch.empty(batch, dtype=INT32, device=device)
+    following = torch.empty(batch, dtype=picks.dtype, device=device)
+    _launch(device, "skv_accept_drafts", parents.data_ptr(), ctypes.byref(ids), ctypes.byref(wanted),
             _lib.ptr(n_new), batch, nodes, path.data_ptr(), n_keep.data_ptr(), following.data_ptr())
     return path, n_keep, following
 
@@ -831,44 +844,35 @@ def keep_tokens(free_stack: torch.Tensor, free_top: torch.Tensor, block_table: t
     workspace: 16 bytes for each entry of path, of no other call that may run at the same time (None: one is
     allocated for the call).  All-or-nothing: a refusal sets ``status`` and writes nothing else (see
     skv_keep_tokens)."""
-    n_pages = free_stack.numel()
-    _require_i32(free_stack, "free_stack")
-    _require_i32(free_top, "free_top", (1,))
     if not 1 <= len(pools) <= 32:
         raise ValueError(f"keep_tokens takes 1 to 32 pools; got {len(pools)}")
     cache = fp4_cache(pools[0], block_table)
-    batch = block_table.shape[0]
-    shape, bases = pools[0].shape, (ctypes.c_void_p * len(pools))()
-    if shape[0] != n_pages:
-        raise ValueError(f"free_stack is of {n_pages} pages, the pools of {shape[0]}")
+    batch, n_pages, device, shape = cache.batch, cache.n_pages, block_table.device, pools[0].shape
+    bases = (ctypes.c_void_p * len(pools))()
     for i, p in enumerate(pools):
-        _require_gpu(p, f"pools[{i}]")
-        if p.dtype != torch.uint8 or p.shape != shape or not p.is_contiguous():
-            raise ValueError(f"pools[{i}] must be a contiguous uint8 {list(shape)} tensor; got {p.dtype} {list(p.shape)}")
-        if p.device != block_table.device:
-            raise ValueError(f"pools[{i}] is on {p.device}, block_table on {block_table.device}")
+        if not isinstance(p, torch.Tensor) or p.dtype is not torch.uint8 or p.shape != shape or not p.is_contiguous():
+            raise ValueError(f"pools[{i}] must be a contiguous uint8 {list(shape)} tensor")
+        if p.device != device:
+            raise ValueError(f"pools[{i}] is on {p.device}, block_table on {device}")
         bases[i] = p.data_ptr()
-    _require_i32(seq_lens, "seq_lens", (batch,))
     _require_i32(path, "path")
     if path.dim() != 2 or path.shape[0] != batch or not 1 <= path.shape[1] <= MAX_NODES:
         raise ValueError(f"path must be int32 [{batch}, 1..{MAX_NODES}]; got {tuple(path.shape)}")
-    _require_i32(n_keep, "n_keep", (batch,))
-    _require_i32(status, "status", (1,))
-    if refs is not None:
-        _require_i32(refs, "refs", (n_pages,))
+    width, one, each = path.shape[1], (1,), (batch,)
+    _require_i32_on(device, path=(path, path.shape), free_stack=(free_stack, (n_pages,)), free_top=(free_top, one),
+                    seq_lens=(seq_lens, each), n_keep=(n_keep, each), status=(status, one), refs=(refs, (n_pages,)))
     n_ptr, n_uni = _n_new_args(n_new, batch)
-    _same_device(block_table, "block_table", free_stack=free_stack, free_top=free_top, seq_lens=seq_lens, path=path,
-                 n_keep=n_keep, status=status, refs=refs, n_new=n_new if n_ptr is not None else None)
-    need = path.numel() * 16
+    if n_ptr is not None and n_new.device != device:
+        raise ValueError(f"n_new is on {n_new.device}, block_table on {device}")
+    need = batch * width * 16
     if workspace is None:
-        workspace = torch.empty(need, dtype=torch.uint8, device=path.device)
-    elif (workspace.device != path.device or workspace.numel() * workspace.element_size() < need
+        workspace = torch.empty(need, dtype=torch.uint8, device=device)
+    elif (workspace.device != device or workspace.numel() * workspace.element_size() < need
           or not workspace.is_contiguous() or workspace.data_ptr() % 16):
-        raise ValueError(f"workspace must hold {need} contiguous bytes on {path.device}, 16-byte aligned")
-    _launch(block_table.device, "skv_keep_tokens", free_stack.data_ptr(), free_top.data_ptr(), _lib.ptr(refs),
-            ctypes.byref(cache), block_table.data_ptr(), seq_lens.data_ptr(), n_ptr, n_uni, path.data_ptr(),
-            path.shape[1], n_keep.data_ptr(), ctypes.cast(bases, ctypes.c_void_p), len(pools), status.data_ptr(),
-            workspace.data_ptr(), workspace.numel() * workspace.element_size())
+        raise ValueError(f"workspace must hold {need} contiguous bytes on {device}, 16-byte aligned")
+    _launch(device, "skv_keep_tokens", free_stack.data_ptr(), free_top.data_ptr(), _lib.ptr(refs), ctypes.byref(cache),
+            block_table.data_ptr(), seq_lens.data_ptr(), n_ptr, n_uni, path.data_ptr(), width, n_keep.data_ptr(), bases,
+            len(pools), status.data_ptr(), workspace.data_ptr(), need)
 
 
 # ---------------------------------------------------------------------------
@@ -899,17 +903,16 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor | None = None, *, 
     same time (None: one is allocated where the call needs it)."""
     rows, stride, lead = _logit_rows(logits, top)
     vocab, device = logits.shape[-1], logits.device
-    f32 = dict(dtype=torch.float32, device=device)
+    f32 = {"dtype": torch.float32, "device": device}
     ids = None
     if tokens is not None:
-        if tuple(tokens.shape) != lead:
+        if tokens.shape != lead:
             raise ValueError(f"tokens must be int32 or int64 {list(lead)}; got {tokens.dtype} {list(tokens.shape)}")
-        flat = tokens.reshape(-1)
-        ids = _token_ids(flat, "tokens", (rows,))
-        _same_device(logits, "logits", tokens=flat)
+        flat = tokens if len(lead) == 1 else tokens.reshape(-1)
+        ids = _token_ids(flat, "tokens", (rows,), device)
     out = TokenLogprobs(None if tokens is None else torch.empty(lead, **f32), torch.empty(lead, **f32),
                         torch.empty(*lead, top, dtype=INT32, device=device), torch.empty(*lead, top, **f32))
-    need = int(_lib.load().skv_token_logprobs_workspace(rows, vocab, _LOGITS[logits.dtype], top))
+    need = _lib.load().skv_token_logprobs_workspace(rows, vocab, _LOGITS[logits.dtype], top)
     if need < 0:
         _lib.check(_lib.SKV_EINVAL, "skv_token_logprobs_workspace")
     if workspace is not None:
@@ -920,8 +923,7 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor | None = None, *, 
         workspace = torch.empty(need, dtype=torch.uint8, device=device)
     _launch(device, "skv_token_logprobs", logits.data_ptr(), rows, vocab, stride, _LOGITS[logits.dtype],
             None if ids is None else ctypes.byref(ids), top, _lib.ptr(out.logprobs), out.entropy.data_ptr(),
-            out.top_ids.data_ptr(), out.top_logprobs.data_ptr(), _lib.ptr(workspace),
-            0 if workspace is None else workspace.numel() * workspace.element_size())
+            out.top_ids.data_ptr(), out.top_logprobs.data_ptr(), _lib.ptr(workspace), need)
     return out
 
 
@@ -939,12 +941,14 @@ def _logit_rows(logits: torch.Tensor, top: int) -> tuple[int, int, tuple[int, ..
     _require_gpu(logits, "logits")
     if logits.dtype not in _LOGITS or logits.dim() < 1 or logits.shape[-1] < 1:
         raise ValueError(f"logits must be bf16, fp16 or fp32 [..., V]; got {logits.dtype} {tuple(logits.shape)}")
-    lead, vocab = tuple(logits.shape[:-1]), logits.shape[-1]
+    lead, vocab, strides = tuple(logits.shape[:-1]), logits.shape[-1], logits.stride()
     if not 0 <= top <= min(MAX_TOP, vocab):
         raise ValueError(f"top must be in [0, {min(MAX_TOP, vocab)}]; got {top}")
-    if vocab > 1 and logits.stride(-1) != 1:
+    if vocab > 1 and strides[-1] != 1:
         raise ValueError("a row's logits must be contiguous")
-    sizes = [(n, s) for n, s in zip(lead, logits.stride()[:-1]) if n != 1]
+    if len(lead) == 1:
+        return lead[0], strides[0], lead
+    sizes = [(n, s) for n, s in zip(lead, strides[:-1]) if n != 1]
     for (_, outer), (n, inner) in zip(sizes, sizes[1:]):
         if outer != n * inner:
             raise ValueError(f"logits of strides {logits.stride()} have no one stride between their rows")
