@@ -5,31 +5,38 @@
 //
 // One pass over a row: a lane keeps a running m, l and s of the logits that it sees; lanes, waves and (of rows
 // that several workgroups share) segments are joined by exp(m_i - m), under which s_i becomes s_i + l_i (m_i - m).
-// HBM bounds it with many rows (each logit is read once), the vector work close behind: about eight instructions
-// and an exponential a logit.
+// HBM bounds it with many rows (each logit is read once), the vector work close behind: about five instructions
+// and an exponential a logit.  3001 rows of 100,003 fp16 logits, 8 alternatives: 110 us (5.5 TB/s); 256 of 131,072
+// bf16, 20 alternatives: 17 us (4.0 TB/s, the last steps of rows that all end at once); one of 32,000 fp32: 8.5 us.
 //
 // The `top` largest cost next to nothing on the way: a lane notes the maximum of every 64 bytes (4 loads of 16)
 // that it sees, in LDS.  The top-th largest of the lanes' own maxima is a bound that at least `top` logits
 // reach, and little more do (of 256 lanes and 20 wanted about 21); only the noted 64 bytes that reach it are
 // read again and what reaches it in them is sorted, by value and then id, as one 64-bit key.  Where too much
 // does (equal logits throughout, or most of a row -inf), the waves go through the row once more with a list
-// of the best so far each.
+// of the best so far each (256 rows of 131,072 zeros: 46 us).
 #include <algorithm>
+#include <type_traits>
 
 #include "skv_common.h"
 
+// A rounded product and its rest are told apart below: fused operations are those written as such.
+#pragma clang fp contract(off)
+
 namespace skv {
 
-constexpr int kLpThreads = 256;
-constexpr int kLpWaves = kLpThreads / kWave;
-constexpr int kLpVecs = 4;        // 16-byte loads of a lane's chunk
-constexpr int kLpMaxTop = 64;     // a wave's list
-constexpr int kLpMaxChunks = 32;  // of a segment: LDS holds their maxima
-constexpr int kLpList = 256;      // chunks read again
-constexpr int kLpPend = 512;      // logits that reach the bound
+constexpr int kLpSmall = 256, kLpLarge = 1024;  // threads of a workgroup
+constexpr int kLpVecs = 4;     // 16-byte loads of a lane's chunk
+constexpr int kLpMaxTop = 64;  // a wave's list
+constexpr int kLpBins = 256;   // lanes' maxima, or those of four lanes
+constexpr int kLpMine = 2 * kWave;  // a wave's pending keys: 63 and a load's 64
+// Chunks of a segment whose maxima LDS holds.
+constexpr int lp_max_chunks(int threads) { return threads == kLpSmall ? 32 : 8; }
 constexpr float kLpLog2e = 1.4426950408889634f;
 constexpr float kLpLowest = -3.4028234663852886e38f;
-constexpr float kLpGone = -1e4f;  // exp of it is 0; times 0 it is 0, as -inf would not be
+constexpr float kLpLn2 = 0.6931471805599453f;
+constexpr float kLpGone = -1e4f;   // exp of it is 0; times 0 it is 0, as -inf would not be
+constexpr float kLpHuge = 1e37f;  // logits up to it stay finite in the log2 domain
 
 struct LpArgs {
   const uint8_t* x;
@@ -109,40 +116,77 @@ __device__ __forceinline__ float lp_value(uint32_t k) {
 // Larger values first, of equal ones the lower id.
 __device__ __forceinline__ uint64_t lp_key(uint32_t order, uint32_t id) { return static_cast<uint64_t>(order) << 32 | ~id; }
 
-__device__ __forceinline__ uint64_t lp_shfl_xor(uint64_t v, int by) {
-  const uint32_t lo = __shfl_xor(static_cast<int>(v), by), hi = __shfl_xor(static_cast<int>(v >> 32), by);
-  return static_cast<uint64_t>(hi) << 32 | lo;
+// The value of lane ^ kBy, without LDS: within a row of 16 lanes by its permutes (xor 4 is the mirror of 8 lanes,
+// xor 7, and that of 4, xor 3), across rows by swaps.
+template <int kBy>
+__device__ __forceinline__ uint32_t lp_xor(uint32_t v) {
+  const auto dpp = [](auto ctrl, uint32_t x) {
+    return static_cast<uint32_t>(__builtin_amdgcn_mov_dpp(static_cast<int>(x), decltype(ctrl)::value, 0xf, 0xf, true));
+  };
+  if constexpr (kBy == 1) return dpp(std::integral_constant<int, 0xb1>{}, v);   // quad_perm 1 0 3 2
+  if constexpr (kBy == 2) return dpp(std::integral_constant<int, 0x4e>{}, v);   // quad_perm 2 3 0 1
+  if constexpr (kBy == 4) return dpp(std::integral_constant<int, 0x1b>{}, dpp(std::integral_constant<int, 0x141>{}, v));
+  if constexpr (kBy == 8) return dpp(std::integral_constant<int, 0x128>{}, v);  // row_ror 8
+  if constexpr (kBy == 16) {  // rows 0 1 2 3 of the first with those of the second: 0 0 2 2 and 1 1 3 3
+    const auto x = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    return threadIdx.x & 16 ? x[0] : x[1];
+  }
+  if constexpr (kBy == 32) {
+    const auto x = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    return threadIdx.x & 32 ? x[0] : x[1];
+  }
 }
+template <int kBy>
+__device__ __forceinline__ uint64_t lp_xor64(uint64_t v) {
+  return static_cast<uint64_t>(lp_xor<kBy>(static_cast<uint32_t>(v >> 32))) << 32 | lp_xor<kBy>(static_cast<uint32_t>(v));
+}
+// f(x of lane ^ 1), then ^ 2, ^ 4 .. ^ 32.
+template <class F>
+__device__ __forceinline__ void lp_lanes(const F& f) {
+  f(std::integral_constant<int, 1>{});
+  f(std::integral_constant<int, 2>{});
+  f(std::integral_constant<int, 4>{});
+  f(std::integral_constant<int, 8>{});
+  f(std::integral_constant<int, 16>{});
+  f(std::integral_constant<int, 32>{});
+}
+template <int kBy>
+__device__ __forceinline__ float lp_xorf(float v) { return __uint_as_float(lp_xor<kBy>(__float_as_uint(v))); }
 __device__ __forceinline__ uint64_t lp_shfl(uint64_t v, int from) {
   const uint32_t lo = __shfl(static_cast<int>(v), from), hi = __shfl(static_cast<int>(v >> 32), from);
   return static_cast<uint64_t>(hi) << 32 | lo;
 }
 
+// One step of a bitonic sort: of lanes kBy apart the lower one keeps the larger key where `down`.
+template <int kBy>
+__device__ __forceinline__ uint64_t lp_step(uint64_t v, bool down) {
+  const uint64_t o = lp_xor64<kBy>(v);
+  return (o > v) == (down == ((threadIdx.x & kBy) == 0)) ? o : v;
+}
+// Of blocks of kSize keys that rise and then fall (or the other way round) the order asked for.
+template <int kSize>
+__device__ __forceinline__ uint64_t lp_bitonic(uint64_t v, bool down) {
+  if constexpr (kSize >= 64) v = lp_step<32>(v, down);
+  if constexpr (kSize >= 32) v = lp_step<16>(v, down);
+  if constexpr (kSize >= 16) v = lp_step<8>(v, down);
+  if constexpr (kSize >= 8) v = lp_step<4>(v, down);
+  if constexpr (kSize >= 4) v = lp_step<2>(v, down);
+  return lp_step<1>(v, down);
+}
 // A wave's 64 keys, one a lane, in descending order.
 __device__ __forceinline__ uint64_t lp_sort(uint64_t v) {
-  const int lane = threadIdx.x % kWave;
-#pragma unroll
-  for (int size = 2; size <= kWave; size *= 2) {
-#pragma unroll
-    for (int by = size / 2; by > 0; by /= 2) {
-      const uint64_t o = lp_shfl_xor(v, by);
-      const bool larger = ((lane & size) == 0) == ((lane & by) == 0);
-      v = (o > v) == larger ? o : v;
-    }
-  }
-  return v;
+  const int lane = threadIdx.x;
+  v = lp_bitonic<2>(v, (lane & 2) == 0);
+  v = lp_bitonic<4>(v, (lane & 4) == 0);
+  v = lp_bitonic<8>(v, (lane & 8) == 0);
+  v = lp_bitonic<16>(v, (lane & 16) == 0);
+  v = lp_bitonic<32>(v, (lane & 32) == 0);
+  return lp_bitonic<64>(v, true);
 }
 // The 64 largest of two lists in descending order, in that order.
 __device__ __forceinline__ uint64_t lp_merge(uint64_t a, uint64_t b) {
-  const int lane = threadIdx.x % kWave;
-  const uint64_t o = lp_shfl(b, kWave - 1 - lane);
-  uint64_t v = o > a ? o : a;
-#pragma unroll
-  for (int by = kWave / 2; by > 0; by /= 2) {
-    const uint64_t p = lp_shfl_xor(v, by);
-    v = (p > v) == ((lane & by) == 0) ? p : v;
-  }
-  return v;
+  const uint64_t o = lp_shfl(b, kWave - 1 - threadIdx.x % kWave);
+  return lp_bitonic<64>(o > a ? o : a, true);
 }
 
 __device__ __forceinline__ float lp_max(float a, float b) { return __builtin_elementwise_maximum(a, b); }  // a NaN stays
@@ -184,25 +228,30 @@ __device__ __forceinline__ void lp_token(const LpArgs& a, int64_t row, int64_t& 
   logit = Type::value(x[in ? token : 0]);
 }
 
-template <bool kTop>
+template <bool kTop, int kThreads>
 struct LpSmem {
-  float part[kLpWaves][4];
-  uint32_t bins[kTop ? kLpThreads : 1];
+  static constexpr int kWaves = kThreads / kWave;
+  static constexpr int kList = 256;               // chunks read again
+  static constexpr int kPend = kWaves * kLpMine;  // logits that reach the bound
+  float part[kWaves][4];
+  uint32_t bins[kTop ? kLpBins : 1];
   uint32_t bound;
   int n_list, n_pend;
-  int32_t list[kTop ? kLpList : 1];
-  uint64_t pend[kTop ? kLpPend : 1];
+  int32_t list[kTop ? kList : 1];
+  uint64_t pend[kTop ? kPend : 1];
 };
 
-// grid: rows x segments.  A segment is `chunks` times kLpThreads * kLpVecs vectors of the row, which are
+// grid: rows x segments.  A segment is `chunks` times kThreads * kLpVecs vectors of the row, which are
 // counted from the 16-byte boundary at or before its first logit.
-template <int kFormat, bool kTop>
-__global__ __launch_bounds__(kLpThreads) void k_logprobs(LpArgs a) {
+template <int kFormat, bool kTop, int kThreads>
+__global__ __launch_bounds__(kThreads) void k_logprobs(LpArgs a) {
+  using Smem = LpSmem<kTop, kThreads>;
+  constexpr int kWaves = Smem::kWaves;
   using Type = LpType<kFormat>;
   using Elem = typename Type::elem;
   constexpr int kVec = Type::kVec, kElems = kVec * kLpVecs;
-  __shared__ LpSmem<kTop> sm;
-  extern __shared__ float noted[];  // [chunks][kLpThreads]
+  __shared__ Smem sm;
+  extern __shared__ float noted[];  // [chunks][kThreads]
   const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
   const int64_t row = blockIdx.x / a.segments;
   const int seg = blockIdx.x - static_cast<int>(row) * a.segments;
@@ -214,11 +263,13 @@ __global__ __launch_bounds__(kLpThreads) void k_logprobs(LpArgs a) {
   float logit = 0.f;
   if (a.segments == 1 && tid == 0) lp_token<kFormat>(a, row, token, logit);
   if (kTop && tid == 0) sm.n_list = sm.n_pend = 0;
-  const int first = seg * a.chunks * kLpVecs * kLpThreads;  // vector
-  const auto vector_of = [&](int c, int i) { return first + (c * kLpVecs + i) * kLpThreads + tid; };
+  const int first = seg * a.chunks * kLpVecs * kThreads;  // vector
+  // chunks that hold logits: the last may be there for rows that begin off a boundary alone
+  const int chunks = min(a.chunks, ((end + kVec - 1) / kVec - first + kLpVecs * kThreads - 1) / (kLpVecs * kThreads));
+  const auto vector_of = [&](int c, int i) { return first + (c * kLpVecs + i) * kThreads + tid; };
   const auto load = [&](u32x4* r, int c) {
-    const int v0 = first + c * kLpVecs * kLpThreads;
-    if (v0 * kVec >= off && (v0 + kLpVecs * kLpThreads) * kVec <= end) {  // uniform: inside the row
+    const int v0 = first + c * kLpVecs * kThreads;
+    if (v0 * kVec >= off && (v0 + kLpVecs * kThreads) * kVec <= end) {  // uniform: inside the row
 #pragma unroll
       for (int i = 0; i < kLpVecs; ++i) r[i] = ld_stream(reinterpret_cast<const u32x4*>(x0) + vector_of(c, i));
     } else {
@@ -244,71 +295,122 @@ __global__ __launch_bounds__(kLpThreads) void k_logprobs(LpArgs a) {
       }
     }
   };
-  float m = kLpLowest, l = 0.f, s = 0.f, top = -__builtin_huge_valf();
-  const auto fold = [&](const u32x4* r, int c) {
+  // In the log2 domain: l = sum 2^(x log2(e) - c), s = sum of the same times its exponent, c = m log2(e) rounded; of a
+  // product and c the difference is one rounding.
+  float m = -kLpHuge, c = -kLpHuge * kLpLog2e, l = 0.f, s = 0.f, top = -__builtin_huge_valf();
+  const auto fold = [&](const u32x4* r, int k) {
     float x[kElems];
 #pragma unroll
     for (int i = 0; i < kLpVecs; ++i) Type::unpack(r[i], x + i * kVec);
-    float cm = x[0];
+    float most = x[0], least = x[0];
 #pragma unroll
-    for (int i = 1; i < kElems; ++i) cm = lp_max(cm, x[i]);
-    if (kTop) noted[c * kLpThreads + tid] = cm;
-    top = lp_max(top, cm);
-    lp_rebase(m, l, s, lp_max(m, cm));
-    float lk[4] = {0.f, 0.f, 0.f, 0.f}, sk[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int i = 0; i < kElems; ++i) {
-      const float d = fmaxf(x[i] - m, kLpGone), e = __builtin_amdgcn_exp2f(d * kLpLog2e);
-      lk[i & 3] += e;
-      sk[i & 3] = __builtin_fmaf(e, d, sk[i & 3]);
+    for (int i = 1; i < kElems; ++i) {
+      most = lp_max(most, x[i]);
+      least = fminf(least, x[i]);
     }
+    if (kTop) noted[k * kThreads + tid] = most;
+    top = lp_max(top, most);
+    m = fminf(fmaxf(m, most), kLpHuge);
+    const float up = m * kLpLog2e, by = c - up, f = __builtin_amdgcn_exp2f(by);
+    s = f * __builtin_fmaf(l, by, s);
+    l *= f;
+    c = up;
+    float lk[4] = {0.f, 0.f, 0.f, 0.f}, sk[4] = {0.f, 0.f, 0.f, 0.f};
+    const auto sum = [&](auto clamped) {
+#pragma unroll
+      for (int i = 0; i < kElems; ++i) {
+        float d = __builtin_fmaf(x[i], kLpLog2e, -c);
+        if constexpr (decltype(clamped)::value) d = fmaxf(d, kLpGone);
+        const float e = __builtin_amdgcn_exp2f(d);
+        lk[i & 3] += e;
+        sk[i & 3] = __builtin_fmaf(e, d, sk[i & 3]);
+      }
+    };
+    // an exponent of -inf has to go before it meets its weight of 0: where a lane of the wave has one
+    if (__ballot(!(least >= -kLpHuge))) sum(std::true_type{}); else sum(std::false_type{});
     l += (lk[0] + lk[1]) + (lk[2] + lk[3]);
     s += (sk[0] + sk[1]) + (sk[2] + sk[3]);
   };
   u32x4 r0[kLpVecs], r1[kLpVecs];
-  load(r0, 0);
-  int c = 0;
-  for (; c + 1 < a.chunks; c += 2) {
-    load(r1, c + 1);
-    fold(r0, c);
-    if (c + 2 < a.chunks) load(r0, c + 2);
-    fold(r1, c + 1);
+  if (chunks > 0) load(r0, 0);
+  int at = 0;
+  for (; at + 1 < chunks; at += 2) {
+    load(r1, at + 1);
+    fold(r0, at);
+    if (at + 2 < chunks) load(r0, at + 2);
+    fold(r1, at + 1);
   }
-  if (c < a.chunks) fold(r0, c);
-  // join the lanes, then the waves
+  if (at < chunks) fold(r0, at);
+  // join the lanes, then the waves; and back to m itself: c = m log2(e) - r
   float wm = m, wtop = top;
-#pragma unroll
-  for (int by = 1; by < kWave; by *= 2) {
-    wm = lp_max(wm, __shfl_xor(wm, by));
-    wtop = lp_max(wtop, __shfl_xor(wtop, by));
+  lp_lanes([&](auto by) {
+    wm = fmaxf(wm, lp_xorf<decltype(by)::value>(wm));
+    wtop = lp_max(wtop, lp_xorf<decltype(by)::value>(wtop));
+  });
+  {
+    const float up = wm * kLpLog2e, r = __builtin_fmaf(wm, kLpLog2e, -up), by = c - up, f = __builtin_amdgcn_exp2f(by - r);
+    s = f * __builtin_fmaf(l, by - r, s) * kLpLn2;
+    l *= f;
+    m = wm;
   }
-  lp_rebase(m, l, s, wm);
+  lp_lanes([&](auto by) {
+    l += lp_xorf<decltype(by)::value>(l);
+    s += lp_xorf<decltype(by)::value>(s);
+  });
+  if (__builtin_fabsf(wtop) > kLpHuge && __builtin_fabsf(wtop) < __builtin_huge_valf()) {  // uniform in the wave
+    // too large for that: once more by differences
+    m = kLpLowest;
+    l = s = 0.f;
+    for (int k = 0; k < chunks; ++k) {
+      load(r0, k);
+      float x[kElems];
 #pragma unroll
-  for (int by = 1; by < kWave; by *= 2) {
-    l += __shfl_xor(l, by);
-    s += __shfl_xor(s, by);
+      for (int i = 0; i < kLpVecs; ++i) Type::unpack(r0[i], x + i * kVec);
+#pragma unroll
+      for (int i = 0; i < kElems; ++i) {
+        const float d = fmaxf(x[i] - wtop, kLpGone), e = __builtin_amdgcn_exp2f(d * kLpLog2e);
+        l += e;
+        s = __builtin_fmaf(e, d, s);
+      }
+    }
+    wm = wtop;
+    lp_lanes([&](auto by) {
+      l += lp_xorf<decltype(by)::value>(l);
+      s += lp_xorf<decltype(by)::value>(s);
+    });
   }
   if (lane == 0) {
     sm.part[wave][0] = wtop;
-    sm.part[wave][1] = wm;
+    sm.part[wave][1] = wtop == -__builtin_huge_valf() ? kLpLowest : wm;  // (nothing but -inf: below all others)
     sm.part[wave][2] = l;
     sm.part[wave][3] = s;
   }
-  if (kTop) sm.bins[tid] = lp_order(top);
+  if constexpr (kTop) {
+    uint32_t bin = lp_order(top);
+    if constexpr (kThreads > kLpBins) {  // of four lanes
+      static_assert(kThreads == 4 * kLpBins, "a bin is a lane's or four lanes'");
+      bin = max(bin, lp_xor<1>(bin));
+      bin = max(bin, lp_xor<2>(bin));
+      if ((tid & 3) == 0) sm.bins[tid >> 2] = bin;
+    } else {
+      sm.bins[tid] = bin;
+    }
+  }
   __syncthreads();
   uint64_t best = 0;
   if constexpr (kTop) {
     // the bound: the largest that `top` bins reach
     if (wave == 0) {
-      uint32_t b[kLpWaves], t = 0;
+      constexpr int kOf = kLpBins / kWave;
+      uint32_t b[kOf], t = 0;
 #pragma unroll
-      for (int i = 0; i < kLpWaves; ++i) b[i] = sm.bins[i * kWave + lane];
+      for (int i = 0; i < kOf; ++i) b[i] = sm.bins[i * kWave + lane];
 #pragma unroll
       for (int bit = 31; bit >= Type::kLowBit; --bit) {
         const uint32_t up = t | 1u << bit;
         int n = 0;
 #pragma unroll
-        for (int i = 0; i < kLpWaves; ++i) n += __popcll(__ballot(b[i] >= up));
+        for (int i = 0; i < kOf; ++i) n += __popcll(__ballot(b[i] >= up));
         if (n >= a.top) t = up;
       }
       if (lane == 0) sm.bound = t;
@@ -316,41 +418,40 @@ __global__ __launch_bounds__(kLpThreads) void k_logprobs(LpArgs a) {
     __syncthreads();
     const uint32_t bound = sm.bound;
     if (lp_order(top) >= bound) {
-      for (int k = 0; k < a.chunks; ++k) {
-        if (lp_order(noted[k * kLpThreads + tid]) >= bound) {
+      for (int k = 0; k < chunks; ++k) {
+        if (lp_order(noted[k * kThreads + tid]) >= bound) {
           const int at = atomicAdd(&sm.n_list, 1);
-          if (at < kLpList) sm.list[at] = k * kLpThreads + tid;
+          if (at < Smem::kList) sm.list[at] = k * kThreads + tid;
         }
       }
     }
     __syncthreads();
     const int listed = sm.n_list;
-    if (listed <= kLpList) {  // uniform
-      for (int i = tid / kElems; i < listed; i += kLpThreads / kElems) {
-        const int at = sm.list[i], k = at / kLpThreads, t = at % kLpThreads, e = tid % kElems;
-        const int id = (first + (k * kLpVecs + e / kVec) * kLpThreads + t) * kVec + e % kVec - off;
+    if (listed <= Smem::kList) {  // uniform
+      for (int i = tid / kElems; i < listed; i += kThreads / kElems) {
+        const int at = sm.list[i], k = at / kThreads, t = at % kThreads, e = tid % kElems;
+        const int id = (first + (k * kLpVecs + e / kVec) * kThreads + t) * kVec + e % kVec - off;
         if (id < 0 || id >= V) continue;
         const uint32_t order = lp_order(Type::value(reinterpret_cast<const Elem*>(base)[id]));
         if (order >= bound) {
           const int p = atomicAdd(&sm.n_pend, 1);
-          if (p < kLpPend) sm.pend[p] = lp_key(order, id);
+          if (p < Smem::kPend) sm.pend[p] = lp_key(order, id);
         }
       }
     }
     __syncthreads();
     const int pending = sm.n_pend;
-    if (listed <= kLpList && pending <= kLpPend) {  // uniform
+    if (listed <= Smem::kList && pending <= Smem::kPend) {  // uniform
       if (wave == 0) {
         best = lp_sort(lane < pending ? sm.pend[lane] : 0);
         for (int p = kWave; p < pending; p += kWave) best = lp_merge(best, lp_sort(p + lane < pending ? sm.pend[p + lane] : 0));
       }
     } else {
-      // a quarter of the segment to a wave, in the order of the ids, and a list of the best so far
+      // a part of the segment to each wave, in the order of the ids, and a list of the best so far
       __syncthreads();  // pend has been counted
-      constexpr int kAhead = 16;
-      uint64_t* mine = sm.pend + wave * (kLpPend / kLpWaves);
-      static_assert(kLpPend / kLpWaves >= 2 * kWave, "a wave's pending keys: 63 and a load's 64");
-      const int span = a.chunks * kLpVecs * kLpThreads * kVec / kLpWaves;
+      constexpr int kAhead = 8;
+      uint64_t* mine = sm.pend + wave * kLpMine;
+      const int span = max(chunks, 0) * kLpVecs * kThreads * kVec / kWaves;
       const int lo = max(first * kVec + wave * span - off, 0), hi = min(first * kVec + (wave + 1) * span - off, V);
       uint64_t least = 0;  // the top-th of the list
       int n = 0;
@@ -384,7 +485,7 @@ __global__ __launch_bounds__(kLpThreads) void k_logprobs(LpArgs a) {
       __syncthreads();
       if (wave == 0) {
 #pragma unroll
-        for (int w = 1; w < kLpWaves; ++w) best = lp_merge(best, sm.pend[w * kWave + lane]);
+        for (int w = 1; w < kWaves; ++w) best = lp_merge(best, sm.pend[w * kWave + lane]);
       }
     }
   }
@@ -392,13 +493,13 @@ __global__ __launch_bounds__(kLpThreads) void k_logprobs(LpArgs a) {
   top = -__builtin_huge_valf();
   m = kLpLowest;
 #pragma unroll
-  for (int w = 0; w < kLpWaves; ++w) {
+  for (int w = 0; w < kWaves; ++w) {
     top = lp_max(top, sm.part[w][0]);
     m = lp_max(m, sm.part[w][1]);
   }
   l = s = 0.f;
 #pragma unroll
-  for (int w = 0; w < kLpWaves; ++w) {
+  for (int w = 0; w < kWaves; ++w) {
     float pm = sm.part[w][1], pl = sm.part[w][2], ps = sm.part[w][3];
     lp_rebase(pm, pl, ps, m);
     l += pl;
@@ -412,9 +513,9 @@ __global__ __launch_bounds__(kLpThreads) void k_logprobs(LpArgs a) {
 
 // grid: rows.  Segments' states and lists, a wave every fourth of them.
 template <int kFormat>
-__global__ __launch_bounds__(kLpThreads) void k_logprobs_join(LpArgs a) {
-  __shared__ float parts[kLpWaves][4];
-  __shared__ uint64_t lists[kLpWaves][kWave];
+__global__ __launch_bounds__(kLpSmall) void k_logprobs_join(LpArgs a) {
+  __shared__ float parts[(kLpSmall / kWave)][4];
+  __shared__ uint64_t lists[(kLpSmall / kWave)][kWave];
   const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
   const int64_t row = blockIdx.x;
   int64_t token = -1;
@@ -424,7 +525,7 @@ __global__ __launch_bounds__(kLpThreads) void k_logprobs_join(LpArgs a) {
   const uint8_t* part = a.parts + row * a.segments * size;
   // a lane's segments
   float top = -__builtin_huge_valf(), m = kLpLowest, l = 0.f, s = 0.f;
-  for (int i = tid; i < a.segments; i += kLpThreads) {
+  for (int i = tid; i < a.segments; i += kLpSmall) {
     LpPart p = *reinterpret_cast<const LpPart*>(part + i * size);
     top = lp_max(top, p.top);
     const float to = lp_max(m, p.m);
@@ -434,17 +535,15 @@ __global__ __launch_bounds__(kLpThreads) void k_logprobs_join(LpArgs a) {
     s += p.s;
   }
   float wm = m, wtop = top;
-#pragma unroll
-  for (int by = 1; by < kWave; by *= 2) {
-    wm = lp_max(wm, __shfl_xor(wm, by));
-    wtop = lp_max(wtop, __shfl_xor(wtop, by));
-  }
+  lp_lanes([&](auto by) {
+    wm = lp_max(wm, lp_xorf<decltype(by)::value>(wm));
+    wtop = lp_max(wtop, lp_xorf<decltype(by)::value>(wtop));
+  });
   lp_rebase(m, l, s, wm);
-#pragma unroll
-  for (int by = 1; by < kWave; by *= 2) {
-    l += __shfl_xor(l, by);
-    s += __shfl_xor(s, by);
-  }
+  lp_lanes([&](auto by) {
+    l += lp_xorf<decltype(by)::value>(l);
+    s += lp_xorf<decltype(by)::value>(s);
+  });
   if (lane == 0) {
     parts[wave][0] = wtop;
     parts[wave][1] = wm;
@@ -453,7 +552,7 @@ __global__ __launch_bounds__(kLpThreads) void k_logprobs_join(LpArgs a) {
   }
   uint64_t best = 0;
   if (a.top > 0) {
-    for (int i = wave; i < a.segments; i += kLpWaves) {
+    for (int i = wave; i < a.segments; i += (kLpSmall / kWave)) {
       const uint64_t key = lane < a.top ? reinterpret_cast<const uint64_t*>(part + i * size + sizeof(LpPart))[lane] : 0;
       best = lp_merge(best, key);
     }
@@ -463,18 +562,18 @@ __global__ __launch_bounds__(kLpThreads) void k_logprobs_join(LpArgs a) {
   if (wave != 0) return;
   if (a.top > 0) {
 #pragma unroll
-    for (int w = 1; w < kLpWaves; ++w) best = lp_merge(best, lists[w][lane]);
+    for (int w = 1; w < (kLpSmall / kWave); ++w) best = lp_merge(best, lists[w][lane]);
   }
   top = -__builtin_huge_valf();
   m = kLpLowest;
 #pragma unroll
-  for (int w = 0; w < kLpWaves; ++w) {
+  for (int w = 0; w < (kLpSmall / kWave); ++w) {
     top = lp_max(top, parts[w][0]);
     m = lp_max(m, parts[w][1]);
   }
   l = s = 0.f;
 #pragma unroll
-  for (int w = 0; w < kLpWaves; ++w) {
+  for (int w = 0; w < (kLpSmall / kWave); ++w) {
     float pm = parts[w][1], pl = parts[w][2], ps = parts[w][3];
     lp_rebase(pm, pl, ps, m);
     l += pl;
@@ -484,7 +583,7 @@ __global__ __launch_bounds__(kLpThreads) void k_logprobs_join(LpArgs a) {
 }
 
 struct LpPlan {
-  int elem, vec;
+  int elem, vec, threads;
   int64_t chunks, segments;  // of a segment; of a row
   int64_t ws_bytes;
 };
@@ -499,27 +598,47 @@ int lp_plan(int64_t rows, int64_t vocab, int32_t format, int64_t top, LpPlan& p)
   }
   p.elem = format == SKV_LOGITS_F32 ? 4 : 2;
   p.vec = 16 / p.elem;
+  // A workgroup of 256 threads for each row where that makes four for a compute unit, else one of 1024, which has as
+  // much in flight; a long row of few goes to several of these, in segments of four chunks or more, that a second launch
+  // joins.  RULE_MEASURED
+  const int64_t cus = device_cus();
   // chunks of a row that begins anywhere between 16-byte boundaries
-  const int64_t chunks = ceil_div(ceil_div(vocab + p.vec - 1, p.vec), kLpVecs * kLpThreads);
-  const int64_t wanted = std::min<int64_t>(chunks, ceil_div(4 * device_cus(), std::max<int64_t>(rows, 1)));
-  p.chunks = std::min<int64_t>(kLpMaxChunks, ceil_div(chunks, wanted));
+  const auto chunks_of = [&](int threads) { return ceil_div(ceil_div(vocab + p.vec - 1, p.vec), kLpVecs * threads); };
+  // Rows for every compute unit four times over: a workgroup of 256 threads each.  Fewer are cut into segments for as
+  // many workgroups, which a second launch joins; but for no more rows than compute units one workgroup of 1024 threads,
+  // which has as much in flight as four, does with one launch what is not too long for it (us, bf16, 20 alternatives):
+  //   1, 64, 256 rows of 32,000    7.6, 8.3, 9.0 for 9.9, 10.5, 14.1      384 rows  15.6 for 16.0, 768  24.5 for 26.7, 1024  32.4 for 21.2
+  //   1, 64, 256 rows of 131,072   13.6, 13.6, 19.1 for 11.2, 15.0, 24.8
+  //   1, 64, 256 rows of 262,144   24.3, 26.3, 51.4 for 12.9, 17.8, 38.3
+  // and rows that 256 threads see at once need no more (64 rows of 5,000: 9.2 for 7.3).
+  const bool wide = rows <= cus && chunks_of(kLpSmall) > 1 &&
+                    (chunks_of(kLpLarge) <= 3 || (chunks_of(kLpLarge) <= 5 && 4 * rows >= cus));
+  p.threads = wide ? kLpLarge : kLpSmall;
+  const int64_t chunks = chunks_of(p.threads);
+  const int64_t wanted = wide ? 1 : std::min<int64_t>(chunks, ceil_div(4 * cus, std::max<int64_t>(rows, 1)));
+  p.chunks = std::min<int64_t>(lp_max_chunks(p.threads), ceil_div(chunks, wanted));
   p.segments = ceil_div(chunks, p.chunks);
   if (rows * p.segments >= (int64_t{1} << 31)) return set_error(SKV_EINVAL, "%s: too many rows of so many logits", what);
   p.ws_bytes = p.segments > 1 ? rows * p.segments * (static_cast<int64_t>(sizeof(LpPart)) + 8 * top) : 0;
   return SKV_OK;
 }
 
-template <int kFormat>
-int lp_launch(const LpArgs& a, hipStream_t s, const char* what) {
+template <int kFormat, int kThreads>
+void lp_launch_rows(const LpArgs& a, hipStream_t s) {
   const dim3 grid(static_cast<unsigned>(static_cast<int64_t>(a.rows) * a.segments));
   if (a.top > 0) {
-    hipLaunchKernelGGL((k_logprobs<kFormat, true>), grid, dim3(kLpThreads), a.chunks * kLpThreads * 4, s, a);
+    hipLaunchKernelGGL((k_logprobs<kFormat, true, kThreads>), grid, dim3(kThreads), a.chunks * kThreads * 4, s, a);
   } else {
-    hipLaunchKernelGGL((k_logprobs<kFormat, false>), grid, dim3(kLpThreads), 0, s, a);
+    hipLaunchKernelGGL((k_logprobs<kFormat, false, kThreads>), grid, dim3(kThreads), 0, s, a);
   }
+}
+
+template <int kFormat>
+int lp_launch(const LpArgs& a, int threads, hipStream_t s, const char* what) {
+  if (threads == kLpSmall) lp_launch_rows<kFormat, kLpSmall>(a, s); else lp_launch_rows<kFormat, kLpLarge>(a, s);
   if (const int rc = check_launch(what)) return rc;
   if (a.segments == 1) return SKV_OK;
-  hipLaunchKernelGGL((k_logprobs_join<kFormat>), dim3(static_cast<unsigned>(a.rows)), dim3(kLpThreads), 0, s, a);
+  hipLaunchKernelGGL((k_logprobs_join<kFormat>), dim3(static_cast<unsigned>(a.rows)), dim3(kLpSmall), 0, s, a);
   return check_launch(what);
 }
 
@@ -566,7 +685,7 @@ extern "C" int skv_token_logprobs(const void* logits, int64_t rows, int64_t voca
   a.top_logprobs = top_logprobs;
   a.parts = static_cast<uint8_t*>(workspace);
   hipStream_t s = static_cast<hipStream_t>(stream);
-  if (format == SKV_LOGITS_BF16) return lp_launch<SKV_LOGITS_BF16>(a, s, what);
-  if (format == SKV_LOGITS_F16) return lp_launch<SKV_LOGITS_F16>(a, s, what);
-  return lp_launch<SKV_LOGITS_F32>(a, s, what);
+  if (format == SKV_LOGITS_BF16) return lp_launch<SKV_LOGITS_BF16>(a, p.threads, s, what);
+  if (format == SKV_LOGITS_F16) return lp_launch<SKV_LOGITS_F16>(a, p.threads, s, what);
+  return lp_launch<SKV_LOGITS_F32>(a, p.threads, s, what);
 }

@@ -166,7 +166,7 @@ def test_tokens_outside_the_vocabulary(dev) -> None:
 def test_refusals(dev) -> None:
     from saint_kv import ops
 
-    x, t = inputs(dev, 2, 40000, "bf16", seed=1)
+    x, t = inputs(dev, 2, 400000, "bf16", seed=1)  # in segments, so with a workspace
     for bad in (dict(logits=x.double()), dict(logits=x.t()), dict(logits=x[:, :0], tokens=None), dict(tokens=t[:1]),
                 dict(tokens=t.float()), dict(top=-1), dict(top=65), dict(logits=x[:, :3], top=4),
                 dict(workspace=torch.zeros(8, device=dev), top=4)):

@@ -158,9 +158,9 @@ def test_bad_logits_are_refused() -> None:
                        (dict(top=65), "top"), (dict(top=101), "top"), (dict(vocab=4, top=5), "top"), (dict(logits=None), "NULL"),
                        (dict(h=None), "NULL"), (dict(lp=None), "NULL"), (dict(ti=None), "NULL"), (dict(tl=None), "NULL"),
                        (dict(logits=FAKE + 1), "aligned"), (dict(logits=FAKE + 2, fmt=2), "aligned"), (dict(stride=-1), "row_stride"),
-                       (dict(tokens=_lib.TokenIds(None, 0, 1, 0, 0)), "NULL"), (dict(rows=1, vocab=100000), "workspace"),
-                       (dict(rows=1, vocab=100000, ws=FAKE, n=8), "workspace"),
-                       (dict(rows=1, vocab=100000, ws=FAKE + 8, n=1 << 20), "workspace")):
+                       (dict(tokens=_lib.TokenIds(None, 0, 1, 0, 0)), "NULL"), (dict(rows=1, vocab=1 << 22), "workspace"),
+                       (dict(rows=1, vocab=1 << 22, ws=FAKE, n=8), "workspace"),
+                       (dict(rows=1, vocab=1 << 22, ws=FAKE + 8, n=1 << 20), "workspace")):
         _refused(call(**over), text)
     assert call(rows=0) == 0
     assert lib.skv_token_logprobs_workspace(1 << 16, 100, 0, 5) == 0  # rows enough for the device
