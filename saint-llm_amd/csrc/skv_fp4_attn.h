@@ -1251,8 +1251,17 @@ __global__ __launch_bounds__(kF4Threads, fp4_resident(DP, MT)) void k_fp4_attn(F
     total = uniform(total);
     int groups = fp4_groups(a, total);
     const int units = items * a.Hkv;
+    // The workgroups that the chip's time is counted in: as many as run; with a view, whose items are often of one
+    // length, and two or more for each compute unit, which keep the memory busy, as many as the items put there (64
+    // windows of 4k, 64 heads on 8 of 128: 59 us uncut with 512 of the 768 workgroups that fit, 69 cut for all; of 64 dims 42
+    // and 48).
+    int slots = groups;
+    if constexpr (kView) {
+      const int cus = a.max_groups / fp4_resident(DP, MT);
+      if (units >= 2 * cus) slots = (units + cus - 1) / cus * cus;
+    }
     const bool whole = a.small == kF4SmallTiles && units <= groups &&
-                       static_cast<int64_t>(uniform(sm.longest)) * groups * (kF4Idle - 1) <= static_cast<int64_t>(total) * kF4Idle;
+                       static_cast<int64_t>(uniform(sm.longest)) * slots * (kF4Idle - 1) <= static_cast<int64_t>(total) * kF4Idle;
     if (g == 0) {
       for (int i = tid; i <= items; i += kF4Threads) a.sched[i] = sm.pre[i];
       if (tid == 0) a.sched[items + 1] = whole ? INT32_MAX : a.small;
