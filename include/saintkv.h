@@ -579,8 +579,8 @@ int skv_accept_drafts(const int32_t* parents, const skv_token_ids* tokens, const
 
 /* Of the n_new[b] newest tokens of sequence b (n_new NULL: n_new_uniform) the
  * n_keep[b] ones path[b][0] < path[b][1] < ... stay, as its newest: in every
- * pool (skv_fp4_cache pages of the same geometry, cache->pool and
- * ->block_table unused) their keys' and values' rows move together behind the
+ * pool (skv_fp4_cache pages of the same geometry, none of them twice;
+ * cache->pool and ->block_table unused) their keys' and values' rows move together behind the
  * tokens before, seq_lens[b] shrinks by n_new[b] - n_keep[b], and pages
  * without a token return to the free stack (sequences ascending, a sequence's
  * last page first), their table entries becoming -1.  n_keep 0 drops all of the

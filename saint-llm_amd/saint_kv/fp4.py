@@ -332,6 +332,8 @@ class Fp4TokenCache:
             raise RuntimeError(f"the tokens reserved last have not been appended to layers {sorted(missing)}")
         if self._shared:
             raise RuntimeError("the tokens reserved last are a fork's, too: they lie in shared pages")
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("keep reads back how many tokens stayed; a graph records ops.keep_tokens")
         n_new = torch.as_tensor(self._host_new.astype(np.int32), device=self.device)  # none of a released sequence
         ops.keep_tokens(self.free_stack, self.free_top, self.block_table, self.seq_lens, n_new, path, n_keep, self.pool,
                         self._status_word(), refs=self.refs)

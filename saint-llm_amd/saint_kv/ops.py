@@ -855,6 +855,8 @@ def keep_tokens(free_stack: torch.Tensor, free_top: torch.Tensor, block_table: t
         if p.device != device:
             raise ValueError(f"pools[{i}] is on {p.device}, block_table on {device}")
         bases[i] = p.data_ptr()
+    if len(set(bases)) != len(pools):
+        raise ValueError("a pool is given twice")
     _require_i32(path, "path")
     if path.dim() != 2 or path.shape[0] != batch or not 1 <= path.shape[1] <= MAX_NODES:
         raise ValueError(f"path must be int32 [{batch}, 1..{MAX_NODES}]; got {tuple(path.shape)}")

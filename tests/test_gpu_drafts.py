@@ -208,7 +208,7 @@ def test_refusals_on_the_host(dev) -> None:
     ok = dict(free_stack=stack, free_top=top, block_table=bt, seq_lens=lens, n_new=0, path=parents, n_keep=n, pools=[pool],
               status=torch.zeros(1, **i32))
     ops.keep_tokens(**ok)
-    for bad in (dict(pools=[]), dict(pools=[pool] * 33), dict(pools=[pool, pool[:3]]), dict(pools=[pool.int()]), dict(n_new=-1),
+    for bad in (dict(pools=[]), dict(pools=[pool] * 33), dict(pools=[pool, pool]), dict(pools=[pool, pool[:3]]), dict(pools=[pool.int()]), dict(n_new=-1),
                 dict(free_stack=torch.zeros(5, **i32)), dict(path=parents[:1]), dict(path=torch.zeros(2, 0, **i32)),
                 dict(path=torch.zeros(2, 1025, **i32)), dict(n_keep=n.long()), dict(refs=torch.zeros(3, **i32)),
                 dict(workspace=torch.zeros(15, dtype=torch.uint8, device=dev)), dict(seq_lens=lens[:1])):
@@ -356,3 +356,38 @@ def test_keeps_of_a_cache_that_forks(dev) -> None:
     assert int(cache.free_top.item()) == cache.host_free
     shared_pages.check(cache.refs.cpu().numpy(), cache.free_stack.cpu().numpy(), cache.host_free,
                        cache.block_table.cpu().numpy(), cache.seq_lens.cpu().numpy(), 16)
+
+
+def test_a_captured_keep_of_a_cache_is_refused(dev) -> None:
+    """It reads back how many tokens stayed; nothing is recorded, and the cache is as it was."""
+    from saint_kv import Fp4TokenCache
+
+    cache = Fp4TokenCache(1, 1, 64, 1, 32, block_size=16, device=dev)
+    cache.reserve(8)
+    cache.append(0, torch.zeros(1, 8, 1, 32, dtype=torch.bfloat16, device=dev), torch.zeros(1, 8, 1, 32, dtype=torch.bfloat16, device=dev))
+    path, n_keep = torch.zeros(1, 4, dtype=torch.int32, device=dev), torch.ones(1, dtype=torch.int32, device=dev)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        with pytest.raises(RuntimeError, match="keep"):
+            cache.keep(path, n_keep)
+        path.zero_()
+    graph.replay()
+    assert cache.keep(path, n_keep).tolist() == [1] and cache.host_lens.tolist() == [1]
+
+
+def test_mixed_ids_and_trees_on_another_stream(dev) -> None:
+    """int32 tokens with int64 picks, on a stream of the caller's."""
+    from saint_kv import ops
+
+    rng = np.random.default_rng(9)
+    parents, tokens, picks = trees(rng, 5, 40), rng.integers(0, 2, (5, 40)).astype(np.int32), rng.integers(0, 2, (5, 40))
+    want = drafts.accept(parents, tokens, picks, np.full(5, 40))
+    stream = torch.cuda.Stream(device=dev)
+    stream.wait_stream(torch.cuda.current_stream(dev))
+    with torch.cuda.stream(stream):
+        got = ops.accept_drafts(*(torch.as_tensor(x, device=dev) for x in (parents, tokens, picks)))
+        tree, _ = ops.draft_tree(torch.as_tensor(parents, device=dev))
+    stream.synchronize()
+    assert all(np.array_equal(g.cpu().numpy(), w) for g, w in zip(got, want)) and got[2].dtype == torch.int64
+    assert np.array_equal(tree.cpu().numpy(), ora.pack_masks(ora.tree_masks(parents, np.full(5, 40))))

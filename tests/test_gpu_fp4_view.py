@@ -334,3 +334,67 @@ def test_far_pages(dev) -> None:
     ids = torch.unique(bt).long()
     small = torch.searchsorted(ids, bt.long()).to(torch.int32)
     check(got, q, pool[ids], small, lens, seen=seen, window=90, first=3)
+
+
+@pytest.mark.parametrize("t,heads,kv,dim,sink", [(70, 16, 2, 96, True), (70, 16, 2, 128, False), (40, 16, 2, 256, True), (90, 16, 2, 64, False)])
+def test_many_rows_in_parts(dev, t, heads, kv, dim, sink) -> None:
+    """Cut items of shared tiles with so many rows that a workgroup joins an item's blocks; a NaN block among the old tokens."""
+    from saint_kv import fp4_attention, ops
+
+    lens = [1400, 300, 5, 700]
+    pool, bt, lens_t = make(dev, lens, 16, kv, dim, seed=dim, spare=60)
+    x = torch.randn(4, 1, kv, dim, device=dev).to(torch.bfloat16)
+    y = x.clone()
+    y[1, 0, 1, 3] = float("inf")
+    at, one = torch.zeros(4, dtype=torch.int32, device=dev), torch.zeros(4, dtype=torch.int32, device=dev)
+    at[1], one[1] = 40, 1
+    ops.fp4_quant_append(pool, bt, at, x, y, one)
+    q = torch.randn(4, t, heads, dim, generator=torch.Generator(device=dev).manual_seed(1), device=dev).to(torch.bfloat16)
+    kw = dict(sink=torch.linspace(-3, 3, heads, device=dev) if sink else None)
+    seen = masks(4, t, [t] * 4, seed=3)
+    got = fp4_attention(q, pool, bt, lens_t, tree=to_words(seen, dev), **kw)
+    check(got, q, pool, bt, lens_t, seen=seen, **kw)
+    assert torch.isnan(got[1]).any() and not torch.isnan(got[0]).any() and (got[2] == 0).all()
+    check(fp4_attention(q, pool, bt, lens_t, window=600, first=20, **kw), q, pool, bt, lens_t, window=600, first=20, **kw)
+
+
+def test_calls_on_two_streams_at_once(dev) -> None:
+    from saint_kv import fp4_attention
+
+    pool, bt, lens = make(dev, [3000, 900], 64, 2, 128, seed=6, spare=20)
+    tree = to_words(masks(2, 6, [6, 6], seed=1), dev)
+    calls = [(torch.randn(2, 6, 8, 128, device=dev).to(torch.bfloat16), dict(tree=tree)),
+             (torch.randn(2, 1, 8, 128, device=dev).to(torch.bfloat16), dict(window=2000, first=100)),
+             (torch.randn(2, 6, 64, 128, device=dev).to(torch.bfloat16), dict(tree=tree, window=900, first=5))]
+    want = [fp4_attention(q, pool, bt, lens, **kw) for q, kw in calls]
+    streams = [torch.cuda.Stream(device=dev) for _ in calls]
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(5):
+        for stream, (q, kw) in zip(streams, calls):
+            with torch.cuda.stream(stream):
+                got.append(fp4_attention(q, pool, bt, lens, **kw))
+    torch.cuda.synchronize()
+    assert all(torch.equal(g, want[i % 3]) for i, g in enumerate(got))
+
+
+@pytest.mark.parametrize("seed", range(12))
+def test_random_views(dev, seed) -> None:
+    """Shapes, windows, trees and lengths at random, small enough for the oracle."""
+    from saint_kv import fp4_attention
+
+    rng = np.random.default_rng(100 + seed)
+    batch, kv, g = int(rng.integers(1, 5)), int(rng.integers(1, 4)), int(rng.integers(1, 9))
+    dim, block = int(rng.choice([32, 64, 96, 128, 192, 256, 384, 512])), int(rng.choice([16, 48, 64]))
+    t = int(rng.choice([1, 3, 17, 40, 66]))
+    lens = rng.integers(0, 400, batch)
+    n_new = rng.integers(0, t + 1, batch).astype(np.int32)
+    pool, bt, lens_t = make(dev, lens, block, kv, dim, seed=seed)
+    q = torch.randn(batch, t, kv * g, dim, generator=torch.Generator(device=dev).manual_seed(seed), device=dev).to(torch.bfloat16)
+    kw = dict(window=int(rng.integers(1, 200)) if rng.random() < 0.7 else None, first=int(rng.integers(0, 80)),
+              n_new=torch.as_tensor(n_new, device=dev) if rng.random() < 0.6 else None, softcap=20.0 if rng.random() < 0.3 else None,
+              sink=torch.randn(kv * g, device=dev) if rng.random() < 0.5 else None)
+    seen = masks(batch, t, n_new if kw["n_new"] is not None else [t] * batch, seed)
+    more = dict(max_len=int(rng.choice([0, 50, 400])), splits=int(rng.choice([0, 0, 2])))
+    check(fp4_attention(q, pool, bt, lens_t, tree=to_words(seen, dev), **kw, **more), q, pool, bt, lens_t, seen=seen, **kw)
+    check(fp4_attention(q, pool, bt, lens_t, **kw, **more), q, pool, bt, lens_t, **kw)

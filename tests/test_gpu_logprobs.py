@@ -215,3 +215,39 @@ def test_captured_calls_replay(dev) -> None:
         for _, f, out in graphs:
             assert all(torch.equal(a, b) for a, b in zip(out, f()))
         assert graphs[0][2][-2].tolist() == [6, 3]
+
+
+def test_calls_on_two_streams_at_once(dev) -> None:
+    from saint_kv import ops
+
+    cases = [(inputs(dev, 3, 300007, "bf16", seed=1), 20), (inputs(dev, 200, 32000, "fp32", seed=2), 64), (inputs(dev, 1500, 3000, "fp16", seed=3), 5)]
+    want = [ops.token_logprobs(x, t, top=top) for (x, t), top in cases]
+    streams = [torch.cuda.Stream(device=dev) for _ in cases]
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(5):
+        for stream, ((x, t), top) in zip(streams, cases):
+            with torch.cuda.stream(stream):
+                got.append(ops.token_logprobs(x, t, top=top))
+    torch.cuda.synchronize()
+    for i, g in enumerate(got):
+        assert all(torch.equal(a, b) for a, b in zip(g, want[i % 3]))
+
+
+@pytest.mark.parametrize("kind", ["bf16", "fp32"])
+def test_huge_logits_among_others(dev, kind) -> None:
+    """Logits past 1e37 in a wave, a segment or a row of their own, above, below and beside ordinary ones."""
+    from saint_kv import ops
+
+    for vocab in (3000, 70001, 300007):
+        x, t = inputs(dev, 8, vocab, kind, seed=vocab)
+        x[0, 17] = 2e38
+        x[1, ::3] = -2e38
+        x[2, : vocab // 2] = -3e38
+        x[3] = 1e38
+        x[4] = -1e38
+        x[4, vocab - 1] = -0.99e38
+        x[5, 1:] = -3e38
+        x[6, vocab // 2:] = 3e38
+        x[7] = x[7].abs() * 1e37
+        check(ops.token_logprobs(x, t, top=6), x, t, 6)
