@@ -53,6 +53,20 @@
 
 namespace skv {
 
+// The first workgroup of an item's head, and how many have a piece of it.
+struct Fp4Pieces {
+  int first, n;
+};
+__device__ __forceinline__ Fp4Pieces fp4_pieces(const Fp4AttnArgs& a, int items, int item, int hk) {
+  const int total = a.sched[items], p0 = a.sched[item], n = (a.sched[item + 1] - p0) / a.Hkv, small = a.sched[items + 1];
+  if (small < 0) return {p0 + hk * n, n};  // counted in pieces, a workgroup each
+  if (n - a.lead <= small) return {0, 1};
+  const int groups = fp4_groups(a, total);
+  const int x0 = p0 + hk * n;
+  const int w0 = fp4_owner(x0 + min(fp4_early(a), n - 1), total, groups);
+  return {w0, fp4_owner(x0 + n - 1, total, groups) - w0 + 1};
+}
+
 // Joins the pieces of a cut item's row: the pieces' weights, then the weighted sum
 // of their outputs with D / 4 threads to a piece, as many pieces at a time as the
 // row's kThreads threads have room for.  (256 threads a row where there are few rows,
@@ -64,11 +78,7 @@ __global__ __launch_bounds__(kF4Threads) void k_fp4_attn_join(Fp4AttnArgs a, int
   const int items = a.B * a.row_blocks;
   const int item = blockIdx.x / a.Hkv, hk = blockIdx.x - item * a.Hkv;
   const int b = item / a.row_blocks, rb = item - b * a.row_blocks;
-  const int total = a.sched[items], p0 = a.sched[item], n = (a.sched[item + 1] - p0) / a.Hkv;
-  if (n - a.lead <= a.sched[items + 1]) return;  // uniform
-  const int groups = fp4_groups(a, total);
-  const int x0 = p0 + hk * n;
-  const int w0 = fp4_owner(x0 + min(fp4_early(a), n - 1), total, groups), pieces = fp4_owner(x0 + n - 1, total, groups) - w0 + 1;
+  const auto [w0, pieces] = fp4_pieces(a, items, item, hk);
   if (pieces == 1) return;  // uniform
   const int tid = threadIdx.x % kThreads, mine = threadIdx.x / kThreads, lane = threadIdx.x % kWave;
   const int64_t pitch = a.D + 4;
@@ -154,11 +164,7 @@ __global__ __launch_bounds__(kF4Threads) void k_fp4_attn_join_blocks(Fp4AttnArgs
   const int items = a.B * a.row_blocks;
   const int item = blockIdx.x / a.Hkv, hk = blockIdx.x - item * a.Hkv;
   const int b = item / a.row_blocks, rb = item - b * a.row_blocks;
-  const int total = a.sched[items], p0 = a.sched[item], n = (a.sched[item + 1] - p0) / a.Hkv;
-  if (n - a.lead <= a.sched[items + 1]) return;  // uniform
-  const int groups = fp4_groups(a, total);
-  const int x0 = p0 + hk * n;
-  const int w0 = fp4_owner(x0 + min(fp4_early(a), n - 1), total, groups), pieces = fp4_owner(x0 + n - 1, total, groups) - w0 + 1;
+  const auto [w0, pieces] = fp4_pieces(a, items, item, hk);
   if (pieces == 1) return;  // uniform
   const int wave = threadIdx.x / kWave, col = threadIdx.x % kWave >> 2, grp = threadIdx.x & 3;
   const int wave_rows = rows_per_block / kF4Waves, per_row = a.D / 16;

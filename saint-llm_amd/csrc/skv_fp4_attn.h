@@ -1223,6 +1223,9 @@ __global__ __launch_bounds__(kF4Threads, fp4_resident(DP, MT)) void k_fp4_attn(F
   const bool each = a.max_groups == 0;  // none is cut, a workgroup each
   const int g = blockIdx.x;
   int x = g, end = g + 1, total = 0, b, rb;
+  // with a view: the piece of an item that a workgroup has where it has one alone
+  bool alone = false;
+  int own_item = 0, own_head = 0, own_piece = 0, own_pieces = 1;
   const auto item_of = [&](int u) {  // u < total: pre[item] <= u < pre[item + 1]; the wave looks in 64 places at a time
     const int lane = tid % kWave, step = (items + kWave - 1) / kWave;
     const auto last_of = [&](int first, int by, int n) {  // of pre[first + by i] <= u, i < n
@@ -1262,12 +1265,41 @@ __global__ __launch_bounds__(kF4Threads, fp4_resident(DP, MT)) void k_fp4_attn(F
     }
     const bool whole = a.small == kF4SmallTiles && units <= groups &&
                        static_cast<int64_t>(uniform(sm.longest)) * slots * (kF4Idle - 1) <= static_cast<int64_t>(total) * kF4Idle;
+    // With a view and fewer items than half of the workgroups, an item is cut into pieces of its own instead, one to a
+    // workgroup: a run over an item's end would pay for a segment's start and end twice (5 trees of 25 nodes, 8 heads on 1 of
+    // 512, over 1.2k tokens: 35 us for 85; 20 of 8 nodes, 16 on 4 of 32, over 2.2k: 31 for 44).
+    if constexpr (kView) alone = a.lead == 0 && a.small == kF4SmallTiles && !whole;  // uniform
+    if (alone) {
+      // of about run tiles, no more pieces than workgroups: sum ceil(n / run) <= total / run + units
+      const int room = max(a.max_groups - units, 1), run = max((total + room - 1) / room, kF4RunTiles);
+      total = 0;
+      for (int base = 0; base < items; base += kF4Threads) {
+        const int item = base + tid;
+        const int n = item < items ? (sm.pre[item + 1] - sm.pre[item]) / a.Hkv : 0;
+        __syncthreads();  // before they are written over
+        int tot;
+        const int ex = block_exclusive_scan((n + run - 1) / run * a.Hkv, sm.scan, &tot);
+        if (item < items) sm.pre[item] = total + ex;
+        total += tot;
+      }
+      if (tid == 0) sm.pre[items] = total;
+      __syncthreads();
+      total = uniform(total);
+      groups = total;
+    }
     if (g == 0) {
       for (int i = tid; i <= items; i += kF4Threads) a.sched[i] = sm.pre[i];
-      if (tid == 0) a.sched[items + 1] = whole ? INT32_MAX : a.small;
+      if (tid == 0) a.sched[items + 1] = whole ? INT32_MAX : alone ? -1 : a.small;
     }
     if (whole) groups = units;
     if (g >= groups) return;  // uniform
+    if (alone) {
+      own_item = uniform(item_of(g));
+      own_pieces = uniform((sm.pre[own_item + 1] - sm.pre[own_item]) / a.Hkv);
+      const int in = g - uniform(sm.pre[own_item]);
+      own_head = in / own_pieces;
+      own_piece = in - own_head * own_pieces;
+    }
     // a run's end inside a small item moves to one of the item's
     const auto run_start = [&](int i) {
       if (whole) return i == units ? total : sm.pre[i / a.Hkv] + i % a.Hkv * ((sm.pre[i / a.Hkv + 1] - sm.pre[i / a.Hkv]) / a.Hkv);
@@ -1278,19 +1310,25 @@ __global__ __launch_bounds__(kF4Threads, fp4_resident(DP, MT)) void k_fp4_attn(F
       if (n - a.lead <= a.small) return 2 * over < n ? u - over : u - over + n;
       return over <= fp4_early(a) ? u - over : u;
     };
-    x = uniform(run_start(g));
-    end = uniform(run_start(g + 1));
+    if (alone) {
+      const int n = span_of(own_item, b, rb).units();
+      x = n * own_piece / own_pieces;
+      end = n * (own_piece + 1) / own_pieces;
+    } else {
+      x = uniform(run_start(g));
+      end = uniform(run_start(g + 1));
+    }
   }
   Fp4Pace pace{0, 0, 0};
   if (!each) pace.start(end - x);  // in a grid of more than the device holds the oldest may go first
   const int x0 = x;
   while (x < end) {
-    const int item = each ? x / a.Hkv : uniform(item_of(x));
+    const int item = each ? x / a.Hkv : alone ? own_item : uniform(item_of(x));
     const Fp4Span sp = span_of(item, b, rb);
     const int lead = each ? 0 : a.lead, n = sp.units() + lead;
-    const int in = each ? 0 : x - uniform(sm.pre[item]);
-    const int hk = each ? x - item * a.Hkv : in / n;
-    const int x1 = each ? 0 : in - hk * n, x2 = each ? n : min(n, x1 + end - x);
+    const int in = each || alone ? 0 : x - uniform(sm.pre[item]);
+    const int hk = each ? x - item * a.Hkv : alone ? own_head : in / n;
+    const int x1 = each ? 0 : alone ? x : in - hk * n, x2 = each ? n : min(n, x1 + end - x);
     const int from = max(x1 - lead, 0), to = x2 - lead;
     const int part = x1 == 0 && x2 == n ? -1 : x1 == 0 ? 2 * g + 1 : 2 * g;
     if constexpr (kShared) {
