@@ -588,8 +588,8 @@ int skv_accept_drafts(const int32_t* parents, const skv_token_ids* tokens, const
  * where a count or a path is not as said, a page is not mapped, or one that is
  * written or cut is shared (SKV_STATUS_BADARG), or the stack would overflow
  * (SKV_STATUS_STACK), nothing is written but *status (not NULL) and the
- * workspace.  path: int32, rows of path_stride <= 1024; batch <= 4096, up to 32
- * pools.  Calls that share a workspace must not overlap. */
+ * workspace.  path: int32, rows of path_stride <= 1024; batch <= 4096, a table of
+ * less than 2^31 entries, up to 32 pools.  Calls that share a workspace must not overlap. */
 int64_t skv_keep_tokens_workspace(int64_t batch, int64_t path_stride);
 int skv_keep_tokens(int32_t* free_stack, int32_t* free_top, const int32_t* refs, const skv_fp4_cache* cache,
                     int32_t* block_table, int32_t* seq_lens, const int32_t* n_new, int32_t n_new_uniform,
@@ -606,8 +606,8 @@ int skv_keep_tokens(int32_t* free_stack, int32_t* free_top, const int32_t* refs,
  *     descending order, of equal ones the lowest id first, a NaN before all
  * in fp32 (int32 ids).  Logits of -inf have probability 0; a row whose largest
  * logit is infinite or a NaN has NaN for all of its numbers.  tokens: rows ids with
- * tok_stride (seq_stride unused), or NULL: logprobs is not written.  The bytes that
- * a call needs: skv_token_logprobs_workspace (-1: bad sizes). */
+ * tok_stride (seq_stride unused), or NULL: logprobs is not written.  Fewer than 2^24
+ * rows, vocab <= 2^24.  The bytes that a call needs: skv_token_logprobs_workspace (-1: bad sizes). */
 #define SKV_LOGITS_BF16 0
 #define SKV_LOGITS_F16 1
 #define SKV_LOGITS_F32 2

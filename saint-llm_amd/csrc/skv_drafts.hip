@@ -365,6 +365,7 @@ extern "C" int skv_keep_tokens(int32_t* free_stack, int32_t* free_top, const int
     if (const int rc = fp4_check_cache(&c, what)) return rc;
     kp.base[q] = static_cast<uint8_t*>(pools[q]);
   }
+  if (c.batch * c.bt_stride > INT32_MAX) return set_error(SKV_EINVAL, "%s: block_table has more than 2^31 - 1 entries", what);
   if (!n_new && n_new_uniform < 0) return set_error(SKV_EINVAL, "%s: n_new_uniform must be >= 0", what);
   if (c.batch == 0) return SKV_OK;
   if (!free_stack || !free_top || !block_table || !seq_lens || !path || !n_keep || !status) {

@@ -311,8 +311,8 @@ __global__ __launch_bounds__(kThreads) void k_logprobs(LpArgs a) {
     if (kTop) noted[k * kThreads + tid] = most;
     top = lp_max(top, most);
     m = fminf(fmaxf(m, most), kLpHuge);
-    const float up = m * kLpLog2e, by = c - up, f = __builtin_amdgcn_exp2f(by);
-    s = f * __builtin_fmaf(l, by, s);
+    const float up = m * kLpLog2e, by = fmaxf(c - up, kLpGone), f = __builtin_amdgcn_exp2f(by);
+    s = f * __builtin_fmaf(l, by, s);  // finite before it meets a weight of 0
     l *= f;
     c = up;
     float lk[4] = {0.f, 0.f, 0.f, 0.f}, sk[4] = {0.f, 0.f, 0.f, 0.f};
@@ -348,8 +348,9 @@ __global__ __launch_bounds__(kThreads) void k_logprobs(LpArgs a) {
     wtop = lp_max(wtop, lp_xorf<decltype(by)::value>(wtop));
   });
   {
-    const float up = wm * kLpLog2e, r = __builtin_fmaf(wm, kLpLog2e, -up), by = c - up, f = __builtin_amdgcn_exp2f(by - r);
-    s = f * __builtin_fmaf(l, by - r, s) * kLpLn2;
+    const float up = wm * kLpLog2e, r = __builtin_fmaf(wm, kLpLog2e, -up);
+    const float by = fmaxf((c - up) - r, kLpGone), f = __builtin_amdgcn_exp2f(by);
+    s = f * __builtin_fmaf(l, by, s) * kLpLn2;
     l *= f;
     m = wm;
   }
@@ -598,9 +599,6 @@ int lp_plan(int64_t rows, int64_t vocab, int32_t format, int64_t top, LpPlan& p)
   }
   p.elem = format == SKV_LOGITS_F32 ? 4 : 2;
   p.vec = 16 / p.elem;
-  // A workgroup of 256 threads for each row where that makes four for a compute unit, else one of 1024, which has as
-  // much in flight; a long row of few goes to several of these, in segments of four chunks or more, that a second launch
-  // joins.  RULE_MEASURED
   const int64_t cus = device_cus();
   // chunks of a row that begins anywhere between 16-byte boundaries
   const auto chunks_of = [&](int threads) { return ceil_div(ceil_div(vocab + p.vec - 1, p.vec), kLpVecs * threads); };
@@ -618,7 +616,7 @@ int lp_plan(int64_t rows, int64_t vocab, int32_t format, int64_t top, LpPlan& p)
   const int64_t wanted = wide ? 1 : std::min<int64_t>(chunks, ceil_div(4 * cus, std::max<int64_t>(rows, 1)));
   p.chunks = std::min<int64_t>(lp_max_chunks(p.threads), ceil_div(chunks, wanted));
   p.segments = ceil_div(chunks, p.chunks);
-  if (rows * p.segments >= (int64_t{1} << 31)) return set_error(SKV_EINVAL, "%s: too many rows of so many logits", what);
+  if (rows * p.segments * p.threads >= (int64_t{1} << 32)) return set_error(SKV_EINVAL, "%s: too many rows of so many logits", what);
   p.ws_bytes = p.segments > 1 ? rows * p.segments * (static_cast<int64_t>(sizeof(LpPart)) + 8 * top) : 0;
   return SKV_OK;
 }

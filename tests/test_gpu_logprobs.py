@@ -251,3 +251,18 @@ def test_huge_logits_among_others(dev, kind) -> None:
         x[6, vocab // 2:] = 3e38
         x[7] = x[7].abs() * 1e37
         check(ops.token_logprobs(x, t, top=6), x, t, 6)
+
+
+@pytest.mark.parametrize("mask", [-1e30, -1e34, -1e35, -1e36, -5e36, -9.9e36, -1.1e37])
+@pytest.mark.parametrize("kind", ["bf16", "fp32"])
+def test_masks_far_below_the_rest(dev, kind, mask) -> None:
+    """Lanes and waves that see nothing but a finite mask, many times over: their sum times the way up to the maximum
+    passes fp32, and counts for nothing."""
+    from saint_kv import ops
+
+    for rows, vocab in ((2, 32000), (1, 262145), (700, 32000), (700, 3001)):
+        x, t = inputs(dev, rows, vocab, kind, seed=rows)
+        x[:, 9:vocab - 1] = mask
+        x[0] = mask
+        x[-1, :40] = mask
+        check(ops.token_logprobs(x, t, top=5), x, t, 5)

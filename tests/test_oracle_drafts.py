@@ -165,3 +165,21 @@ def test_bad_logits_are_refused() -> None:
     assert call(rows=0) == 0
     assert lib.skv_token_logprobs_workspace(1 << 16, 100, 0, 5) == 0  # rows enough for the device
     assert lib.skv_token_logprobs_workspace(1, 1 << 20, 0, 5) > 0 and lib.skv_token_logprobs_workspace(1, 0, 0, 5) == -1
+
+
+def test_sizes_past_a_launch_are_refused() -> None:
+    """2^32 work-items, and a table whose pages a 32-bit count could not number."""
+    from saint_kv import _lib
+
+    lib = _lib.load()
+    ids = _lib.TokenIds(FAKE, 0, 1, 1, 0)
+    most = (1 << 24) - 1  # rows of a workgroup of 256 each
+    assert lib.skv_token_logprobs_workspace(most, 8, 0, 2) == 0 and lib.skv_token_logprobs_workspace(most + 1, 8, 0, 2) == -1
+    _refused(lib.skv_token_logprobs(FAKE, most + 1, 8, 8, 0, ctypes.byref(ids), 2, FAKE, FAKE, FAKE, FAKE, None, 0, None),
+             "too many rows")
+    c = _lib.Fp4Cache(pool=None, block_size=16, n_pages=8, n_kv_heads=2, head_dim=128, block_table=None, bt_stride=1 << 20,
+                      batch=2048)
+    pools = (ctypes.c_void_p * 1)(FAKE)
+    rc = lib.skv_keep_tokens(FAKE, FAKE, None, ctypes.byref(c), FAKE, FAKE, None, 4, FAKE, 4, FAKE,
+                             ctypes.cast(pools, ctypes.c_void_p), 1, FAKE, FAKE, 1 << 20, None)
+    _refused(rc, "block_table")
