@@ -36,7 +36,8 @@ constexpr float kLpLog2e = 1.4426950408889634f;
 constexpr float kLpLowest = -3.4028234663852886e38f;
 constexpr float kLpLn2 = 0.6931471805599453f;
 constexpr float kLpGone = -1e4f;   // exp of it is 0; times 0 it is 0, as -inf would not be
-constexpr float kLpHuge = 1e37f;  // logits up to it stay finite in the log2 domain
+constexpr float kLpFar = 1e37f;       // logits up to it stay finite in the log2 domain
+constexpr float kLpHuge = 67108864.f;  // maxima up to it are less than 2^3 from their rounding there: weights up to 2^3
 
 struct LpArgs {
   const uint8_t* x;
@@ -296,7 +297,8 @@ __global__ __launch_bounds__(kThreads) void k_logprobs(LpArgs a) {
     }
   };
   // In the log2 domain: l = sum 2^(x log2(e) - c), s = sum of the same times its exponent, c = m log2(e) rounded; of a
-  // product and c the difference is one rounding.
+  // product and c the difference is one rounding.  m stays within kLpHuge: a lane that sees less has weights near 0, and
+  // waves whose maximum is past it (c's rounding would be) go through their logits again below.
   float m = -kLpHuge, c = -kLpHuge * kLpLog2e, l = 0.f, s = 0.f, top = -__builtin_huge_valf();
   const auto fold = [&](const u32x4* r, int k) {
     float x[kElems];
@@ -327,7 +329,7 @@ __global__ __launch_bounds__(kThreads) void k_logprobs(LpArgs a) {
       }
     };
     // an exponent of -inf has to go before it meets its weight of 0: where a lane of the wave has one
-    if (__ballot(!(least >= -kLpHuge))) sum(std::true_type{}); else sum(std::false_type{});
+    if (__ballot(!(least >= -kLpFar))) sum(std::true_type{}); else sum(std::false_type{});
     l += (lk[0] + lk[1]) + (lk[2] + lk[3]);
     s += (sk[0] + sk[1]) + (sk[2] + sk[3]);
   };

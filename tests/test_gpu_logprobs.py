@@ -253,7 +253,24 @@ def test_huge_logits_among_others(dev, kind) -> None:
         check(ops.token_logprobs(x, t, top=6), x, t, 6)
 
 
-@pytest.mark.parametrize("mask", [-1e30, -1e34, -1e35, -1e36, -5e36, -9.9e36, -1.1e37])
+@pytest.mark.parametrize("scale", [1e5, 1e7, 6e7, 1e8, 1e9, 1e12, 1e20, 1e30, 1e36])
+@pytest.mark.parametrize("kind", ["bf16", "fp32"])
+def test_logits_of_any_size(dev, kind, scale) -> None:
+    """All of a row's logits large, of both signs, of one, close together, and some lanes' alone."""
+    from saint_kv import ops
+
+    for rows, vocab in ((5, 32000), (700, 3001)):
+        x, t = inputs(dev, rows, vocab, "fp32", seed=rows)
+        x = x * scale
+        x[1].abs_()
+        x[2] = -x[2].abs()
+        x[3] = scale * (1 + 2.0 ** -20 * torch.arange(vocab, device=dev) / vocab)
+        x[4, 300:] = 0.01
+        x = x.to(TYPES[kind])
+        check(ops.token_logprobs(x, t, top=5), x, t, 5)
+
+
+@pytest.mark.parametrize("mask", [-1e4, -1e7, -1e9, -1e20, -1e30, -1e34, -1e35, -1e36, -5e36, -9.9e36, -1.1e37])
 @pytest.mark.parametrize("kind", ["bf16", "fp32"])
 def test_masks_far_below_the_rest(dev, kind, mask) -> None:
     """Lanes and waves that see nothing but a finite mask, many times over: their sum times the way up to the maximum
