@@ -651,8 +651,8 @@ struct Fp4Wave {
   }
 
   // Whether a row may not see a key of the tile at `pos`, or a key's values are NaN somewhere.
-  __device__ __forceinline__ bool uneven(const Raw& r, int pos) const {
-    return pos < sp.all_lo || pos + kF4Tile > sp.all_hi || (r.slot[0] | r.slot[1]) < 0;
+  __device__ __forceinline__ bool uneven(const int (&slot)[2], int pos) const {
+    return pos < sp.all_lo || pos + kF4Tile > sp.all_hi || (slot[0] | slot[1]) < 0;
   }
   __device__ __forceinline__ bool any_nan(const Raw& r) const {
     bool nan = false;
@@ -711,6 +711,14 @@ struct Fp4Wave {
     }
   }
 
+  // Chunk far + near + i of row r (near + i % 8 < 8).  A swizzle is within eight chunks, so that those eight apart have one
+  // address; waves with tiles of their own, which are short of registers, take it so (64 windows of 4k, 64 heads on 8
+  // of 128: 55 us, 60 with an address for each; heads of 512 dims 54 and 56; the shared tiles' 205 and 200).
+  __device__ __forceinline__ static int chunk(int r, int far, int near, int i) {
+    if constexpr (kShared && DP <= 256) return fp4_chunk(r, far + near + i);
+    return far + (i & ~7) + fp4_chunk(r, near + (i & 7));
+  }
+
   // 32 keys' values to LDS.
   __device__ __forceinline__ void values(const Raw& r, uint16_t* vt) const {
 #pragma unroll
@@ -718,7 +726,7 @@ struct Fp4Wave {
       uint16_t* dst = vt + (16 * h + col) * DP;
 #pragma unroll
       for (int w = 0; w < kWords; ++w) {
-        *reinterpret_cast<u32x4*>(dst + 8 * fp4_chunk(col, grp * kWords + w)) =
+        *reinterpret_cast<u32x4*>(dst + 8 * chunk(col, grp * kWords & ~7, grp * kWords & 7, w)) =
             fp4_decode8(r.v[h][w], fp4_scale(r.vs[h][w / 4 < kScales ? w / 4 : 0]));
       }
     }
@@ -833,7 +841,7 @@ struct Fp4Wave {
     const uint16_t* v0 = vt + vr * DP + 4 * (col & 1);
 #pragma unroll
     for (int x = 0; x < kBlocks; ++x) {
-      const uint16_t* src = v0 + 8 * fp4_chunk(vr, 2 * x + ((col & 3) >> 1));
+      const uint16_t* src = v0 + 8 * chunk(vr, 0, (col & 3) >> 1, 2 * x);
       const u32x2 lo2 = fp4_read_tr(src), hi2 = fp4_read_tr(src + 16 * DP);
       const u32x4 v = u32x4{lo2[0], lo2[1], hi2[0], hi2[1]};
 #pragma unroll
@@ -920,7 +928,7 @@ __device__ __forceinline__ void fp4_segment(Fp4Smem<DP, false>& sm, const Fp4Arg
     Fp4Tile<MT> tl;
     tl.slot[0] = raw.slot[0];
     tl.slot[1] = raw.slot[1];
-    tl.masked = w.uneven(raw, pos) || w.any_nan(raw);
+    tl.masked = w.uneven(raw.slot, pos) || w.any_nan(raw);
     tl.nan_keys = 0;
     if (tl.masked) tl.nan_keys = w.clean(raw, pos);  // uniform
     w.scores(raw, tl);
@@ -1053,10 +1061,10 @@ __device__ __forceinline__ void fp4_rounds_ahead(Fp4Smem<DP, true>& sm, Fp4Wave<
   // a tile's masks, and its scores under them
   const auto settle = [&](int i, int j) {
     const int pos = fp4_tile<kView>(sp, t_lo + i + j) * kF4Tile;
-    tl.slot[0] = now.slot[0] = __builtin_amdgcn_readlane(slot, 2 * j);
-    tl.slot[1] = now.slot[1] = __builtin_amdgcn_readlane(slot, 2 * j + 1);
+    tl.slot[0] = __builtin_amdgcn_readlane(slot, 2 * j);
+    tl.slot[1] = __builtin_amdgcn_readlane(slot, 2 * j + 1);
     tl.nan_keys = __builtin_amdgcn_readfirstlane(sm.nan_keys[j]);
-    tl.masked = w.uneven(now, pos) || tl.nan_keys != 0;
+    tl.masked = w.uneven(tl.slot, pos) || tl.nan_keys != 0;
     mult = w.settle(tl, pos);
   };
   for (int i = 0; i < n; i += kF4Waves) {
@@ -1066,7 +1074,7 @@ __device__ __forceinline__ void fp4_rounds_ahead(Fp4Smem<DP, true>& sm, Fp4Wave<
       const int pos = fp4_tile<kView>(sp, t_lo + i + wave) * kF4Tile;
       w.template unpack_scales<false, true>(vals);
       uint32_t nan_keys = 0;
-      if (w.uneven(vals, pos) || w.any_nan(vals)) nan_keys = w.clean(vals, pos);  // uniform
+      if (w.uneven(vals.slot, pos) || w.any_nan(vals)) nan_keys = w.clean(vals, pos);  // uniform
       w.values(vals, reinterpret_cast<uint16_t*>(sm.tile[wave]));
       if (lane == 0) sm.nan_keys[wave] = nan_keys;
       w.template unpack_scales<true, false>(keys);
@@ -1121,7 +1129,7 @@ __device__ __forceinline__ void fp4_rounds(Fp4Smem<DP, true>& sm, Fp4Wave<DP, MT
       const int pos = fp4_tile<kView>(sp, t_lo + i + wave) * kF4Tile;
       w.template unpack_scales<false, true>(vals);
       uint32_t nan_keys = 0;
-      if (w.uneven(vals, pos) || w.any_nan(vals)) nan_keys = w.clean(vals, pos);  // uniform
+      if (w.uneven(vals.slot, pos) || w.any_nan(vals)) nan_keys = w.clean(vals, pos);  // uniform
       w.values(vals, reinterpret_cast<uint16_t*>(sm.tile[wave]));
       if (lane == 0) sm.nan_keys[wave] = nan_keys;
     }
@@ -1141,13 +1149,85 @@ __device__ __forceinline__ void fp4_rounds(Fp4Smem<DP, true>& sm, Fp4Wave<DP, MT
       tl.slot[0] = kr.slot[0];
       tl.slot[1] = kr.slot[1];
       tl.nan_keys = __builtin_amdgcn_readfirstlane(sm.nan_keys[j]);
-      tl.masked = w.uneven(kr, pos) || tl.nan_keys != 0;
+      tl.masked = w.uneven(kr.slot, pos) || tl.nan_keys != 0;
       w.template unpack_scales<true, false>(kr);
       w.scores(kr, tl);
       if (i + j < n) w.output(tl, pos, reinterpret_cast<const uint16_t*>(sm.tile[j]));  // uniform
     }
     at = at_next;
     slot = slot_next;
+    lds_barrier();  // the tiles have been read
+  }
+}
+
+// The same with every wave loading all keys itself (heads of 512 dims: one workgroup on a compute unit, whose LDS the
+// values fill).  A tile's keys take their registers from the ones before once these have been multiplied.  (6 trees of 99 nodes,
+// 16 heads on one, in windows of 128: 43 us a call, 54 with a tile's scores ahead of its own weights, and 54 with tiles of each
+// wave's own; 9 chunks of 401 tokens, 8 heads on one, over 4k: 585, 661 and 787.  Two waves on a SIMD hide more of each other's
+// waits without it: 2 prompts of 16 heads on 4 of 256 dims 835 us with it and 754.)
+template <int DP, int MT, bool kExact, bool kView>
+__device__ __forceinline__ void fp4_rounds_wide(Fp4Smem<DP, true>& sm, Fp4Wave<DP, MT, kExact, true, kView>& w, const Fp4Span& sp, int b,
+                                           int wave, int lane, int t_lo, int t_hi, Fp4Pace& pace, int done) {
+  using Wave = Fp4Wave<DP, MT, kExact, true, kView>;
+  const int n = t_hi - t_lo;
+  // lane 2 j + h, j < 4: half h of tile i + j (past the last something mapped)
+  const auto places = [&](int i, uint64_t& at, int& slot) {
+    w.lookup(b, fp4_tile<kView>(sp, min(t_lo + i + ((lane >> 1) & 3), t_hi)) * kF4Tile + 16 * (lane & 1), at, slot);
+  };
+  typename Wave::Raw keys, vals;
+  uint64_t at, at_next;
+  int slot, slot_next;
+  places(0, at, slot);
+  w.template fetch<true, false>(keys, at, slot, 0);
+  w.template fetch<false, true>(vals, at, slot, 2 * wave);
+  places(kF4Waves, at_next, slot_next);
+  Fp4Tile<MT> tl;
+  w.scores(keys, tl);
+  w.template fetch<true, false>(keys, at, slot, 2);
+  float mult = 0.f;
+  // a tile's masks, and its scores under them
+  const auto settle = [&](int i, int j) {
+    const int pos = fp4_tile<kView>(sp, t_lo + i + j) * kF4Tile;
+    tl.slot[0] = __builtin_amdgcn_readlane(slot, 2 * j);
+    tl.slot[1] = __builtin_amdgcn_readlane(slot, 2 * j + 1);
+    tl.nan_keys = __builtin_amdgcn_readfirstlane(sm.nan_keys[j]);
+    tl.masked = w.uneven(tl.slot, pos) || tl.nan_keys != 0;
+    mult = w.settle(tl, pos);
+  };
+  for (int i = 0; i < n; i += kF4Waves) {
+    pace.at(done + i);
+    {
+      const int pos = fp4_tile<kView>(sp, t_lo + i + wave) * kF4Tile;
+      w.template unpack_scales<false, true>(vals);
+      uint32_t nan_keys = 0;
+      if (w.uneven(vals.slot, pos) || w.any_nan(vals)) nan_keys = w.clean(vals, pos);  // uniform
+      w.values(vals, reinterpret_cast<uint16_t*>(sm.tile[wave]));
+      if (lane == 0) sm.nan_keys[wave] = nan_keys;
+    }
+    lds_barrier();  // the tiles are there
+    settle(i, 0);
+#pragma unroll
+    for (int j = 0; j < kF4Waves; ++j) {
+      if (i + j < n) {  // uniform
+        // the next tile's scores beside this one's weights, the keys of the one after on their way
+        typename Wave::Weights p;
+        Fp4Tile<MT> next;
+        w.scores(keys, next);
+        if (j < kF4Waves - 2) {
+          w.template fetch<true, false>(keys, at, slot, 2 * (j + 2));
+        } else {
+          w.template fetch<true, false>(keys, at_next, slot_next, 2 * (j + 2 - kF4Waves));
+        }
+        if (j == 1) w.template fetch<false, true>(vals, at_next, slot_next, 2 * wave);
+        w.weigh(tl, mult, p);
+        w.product(p, reinterpret_cast<const uint16_t*>(sm.tile[j]));
+        tl = next;
+        if (j < kF4Waves - 1 && i + j + 1 < n) settle(i, j + 1);
+      }
+    }
+    at = at_next;
+    slot = slot_next;
+    places(i + 2 * kF4Waves, at_next, slot_next);
     lds_barrier();  // the tiles have been read
   }
 }
@@ -1164,6 +1244,8 @@ __device__ __forceinline__ void fp4_segment_shared(Fp4Smem<DP, true>& sm, const 
   Wave w(a, sp, b, hk, r0, lane);
   if constexpr (Fp4Smem<DP, true>::kKeys) {
     fp4_rounds_ahead(sm, w, sp, b, wave, lane, t_lo, t_hi, pace, done);
+  } else if constexpr (DP > 256) {
+    fp4_rounds_wide(sm, w, sp, b, wave, lane, t_lo, t_hi, pace, done);
   } else {
     fp4_rounds(sm, w, sp, b, wave, lane, t_lo, t_hi, pace, done);
   }
@@ -1381,10 +1463,14 @@ inline int fp4_attn_plan(const skv_fp4_attention_desc* d, const skv_fp4_view* v,
   // more than half of the rows of such a workgroup are there: 16 sequences of 32k on one
   // head of 128 dims take 56 us shared and 48 apart with 64 rows, 56 and 71 with 65 (another row
   // block), 53 and 36 with 32; of 64 dims 44 and 42 with 64 rows, 45 either way with 65, 49 and 60 with
-  // 128; of 256 dims 68 and 65 with 32 rows, 68 and 101 with 33.  Heads of 512 dims stay apart (16
-  // sequences of 4k: 57 us with 33 rows and 53 with 64, shared 61 and 64; their registers spill).
+  // 128; of 256 dims 68 and 65 with 32 rows, 68 and 101 with 33.  Heads of up to 512 dims stay apart, but with a view
+  // those of 512 where a sixteenth of the compute units get such a workgroup, as a cut into more pieces is more to join (us
+  // shared and apart: 300 windows of 128, 33 rows 56 and 70, 64 rows 63 and 91; 16 of 4k 48 and 46, 51 and 58; 8 windows of 9k, 64
+  // rows 53 and 57; one of 100k 90 and 68).  The sizes between spill registers (40 trees of 9 nodes, 32 heads on 2 of 288 dims,
+  // over 8k: 720 and 650).
   const int mt = fp4_shared_mt(p.dims);
-  p.shared = p.dims <= 256 && rows > 16 * mt * kF4Waves / 2;
+  p.shared = rows > 16 * mt * kF4Waves / 2 &&
+             (p.dims <= 256 || (v && D == 512 && 16 * d->cache.batch * hkv * ceil_div(rows, 16 * mt * kF4Waves) >= device_cus()));
   if (v) {
     if (v->first < 0 || v->first > (1 << 24)) return set_error(SKV_EINVAL, "%s: first must be in [0, 2^24]", what);
     if (v->tree && (d->n_queries > kF4MaxNodes || v->tree_words != ceil_div(d->n_queries, 64))) {
@@ -1436,8 +1522,10 @@ template <int DP, bool kExact, bool kView>
 void launch_rows(const Fp4Args<kView>& a, const Fp4AttnPlan& p, hipStream_t s) {
   const dim3 grid(static_cast<unsigned>(a.max_groups > 0 ? a.max_groups : static_cast<int64_t>(a.B) * a.row_blocks * a.Hkv));
   const auto go = [&](auto* kernel) { hipLaunchKernelGGL(kernel, grid, dim3(kF4Threads), 0, s, a); };
-  if constexpr (DP <= 256) {
+  if constexpr (DP <= 256 || (kExact && kView)) {
     if (p.shared) return go(&k_fp4_attn<DP, fp4_shared_mt(DP), kExact, true, kView>);
+  }
+  if constexpr (DP <= 256) {
     if (p.mt == 2) return go(&k_fp4_attn<DP, 2, kExact, false, kView>);
   }
   go(&k_fp4_attn<DP, 1, kExact, false, kView>);

@@ -398,3 +398,29 @@ def test_random_views(dev, seed) -> None:
     more = dict(max_len=int(rng.choice([0, 50, 400])), splits=int(rng.choice([0, 0, 2])))
     check(fp4_attention(q, pool, bt, lens_t, tree=to_words(seen, dev), **kw, **more), q, pool, bt, lens_t, seen=seen, **kw)
     check(fp4_attention(q, pool, bt, lens_t, **kw, **more), q, pool, bt, lens_t, **kw)
+
+
+@pytest.mark.parametrize("lens,n_new,t,heads,kv,block,window,first,sink,softcap", [
+    ([1500, 700, 33, 0, 40], [40, 33, 33, 0, 1], 40, 16, 1, 16, None, 0, False, None),
+    ([1500, 700, 45, 0, 39], None, 40, 16, 1, 64, 200, 70, True, 30.0),
+    ([130, 64, 65, 31, 32, 1, 100, 99], None, 1, 80, 2, 16, None, 0, True, None),  # 40 rows a head
+    ([300] * 17, None, 3, 11, 1, 16, 100, 4, False, None),  # 33 rows
+    ([5000, 4000], None, 66, 16, 2, 64, None, 0, False, 5.0)])
+def test_wide_heads_whose_waves_share_tiles(dev, lens, n_new, t, heads, kv, block, window, first, sink, softcap) -> None:
+    from saint_kv import fp4_attention
+
+    pool, bt, lens_t = make(dev, lens, block, kv, 512, seed=t)
+    g = torch.Generator(device=dev).manual_seed(t)
+    q = torch.randn(len(lens), t, heads, 512, generator=g, device=dev).to(torch.bfloat16)
+    seen = masks(len(lens), t, n_new or [t] * len(lens), seed=t)
+    counts = None if n_new is None else torch.tensor(n_new, dtype=torch.int32, device=dev)
+    kw = dict(window=window, softcap=softcap, sink=torch.randn(heads, generator=g, device=dev) if sink else None,
+              n_new=counts, first=first)
+    for tree, of in ((to_words(seen, dev), seen), (None, None)):
+        if tree is None and not first:
+            continue
+        extra = {} if of is None else {"seen": of}
+        for splits in (0, 1, 3):
+            got = fp4_attention(q, pool, bt, lens_t, splits=splits, tree=tree, **kw)
+            check(got, q, pool, bt, lens_t, **extra, **kw)
+            assert torch.equal(got, fp4_attention(q, pool, bt, lens_t, splits=splits, tree=tree, **kw))
