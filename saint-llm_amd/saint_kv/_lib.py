@@ -232,8 +232,9 @@ def check(rc: int, what: str) -> None:
 
 
 def call(name: str, *args) -> None:
-    fn = getattr(load(), name)
-    check(fn(*args), name)
+    rc = getattr(_lib or load(), name)(*args)
+    if rc != SKV_OK:
+        check(rc, name)
 
 
 def stream_handle(device: torch.device | None = None) -> int:

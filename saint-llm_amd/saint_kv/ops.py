@@ -39,10 +39,11 @@ def _require_i32(t: torch.Tensor, name: str, shape: tuple[int, ...] | None = Non
 
 def _require_i32_on(device: torch.device, **named: tuple[torch.Tensor | None, tuple[int, ...]]) -> None:
     """Every (tensor, shape) a contiguous int32 tensor of that shape on ``device`` (or None)."""
+    index = device.index
     for name, (t, shape) in named.items():
         # in one condition: ten tensors' separate checks take about as long as a launch
         if t is not None and not (isinstance(t, torch.Tensor) and t.dtype is INT32 and t.shape == shape
-                                  and t.device == device and t.is_contiguous()):
+                                  and t.get_device() == index and t.is_contiguous()):
             _require_i32(t, name, shape)
             raise ValueError(f"{name} is on {t.device}, the others on {device}")
 
@@ -701,17 +702,17 @@ def fp4_cache(pool: torch.Tensor, block_table: torch.Tensor) -> _lib.Fp4Cache:
     _require_i32(block_table, "block_table")
     if block_table.dim() != 2:
         raise ValueError("block_table must be 2D [batch, max_pages]")
-    if block_table.device != pool.device:
+    if block_table.get_device() != pool.get_device():
         raise ValueError(f"block_table is on {block_table.device}, pool on {pool.device}")
     batch, bt_stride = block_table.shape
     return _lib.Fp4Cache(pool.data_ptr(), bs, n_pages, heads, row // 17 * 16, block_table.data_ptr(), bt_stride, batch)
 
 
 def _same_device(t: torch.Tensor, name: str, **others: torch.Tensor | None) -> None:
-    device = t.device
+    index = t.get_device()
     for other, x in others.items():
-        if x is not None and x.device != device:
-            raise ValueError(f"{other} is on {x.device}, {name} on {device}")
+        if x is not None and x.get_device() != index:
+            raise ValueError(f"{other} is on {x.device}, {name} on {t.device}")
 
 
 def _fp4_rows(t: torch.Tensor, name: str, like: tuple[int, int, int], dtypes: tuple[torch.dtype, ...]) -> _lib.Fp4Rows:
@@ -796,7 +797,7 @@ def draft_tree(parents: torch.Tensor, n_new: torch.Tensor | None = None) -> tupl
     batch, nodes = _tree_shape(parents, n_new)
     device = parents.device
     tree = torch.empty(batch, nodes, -(-nodes // 64), dtype=torch.int64, device=device)
-    depths = torch.empty(batch, nodes, dtype=INT32, device=device)
+    depths = parents.new_empty(batch, nodes)
     _launch(device, "skv_draft_tree", parents.data_ptr(), _lib.ptr(n_new), batch, nodes, tree.data_ptr(),
             depths.data_ptr())
     return tree, depths
@@ -807,7 +808,7 @@ def _token_ids(t: torch.Tensor, name: str, shape: tuple[int, ...], device: torch
     _require_gpu(t, name)
     if t.dtype not in (INT32, torch.int64) or t.shape != shape:
         raise ValueError(f"{name} must be int32 or int64 {list(shape)}; got {t.dtype} {list(t.shape)}")
-    if t.device != device:
+    if t.get_device() != device.index:
         raise ValueError(f"{name} is on {t.device}, the others on {device}")
     strides = t.stride()
     return _lib.TokenIds(t.data_ptr(), strides[0], strides[-1], t.dtype is torch.int64)
@@ -825,9 +826,7 @@ def accept_drafts(parents: torch.Tensor, tokens: torch.Tensor, picks: torch.Tens
     batch, nodes = _tree_shape(parents, n_new)
     device, shape = parents.device, (batch, nodes)
     ids, wanted = _token_ids(tokens, "tokens", shape, device), _token_ids(picks, "picks", shape, device)
-    path = torch.empty(batch, nodes, dtype=INT32, device=device)
-    n_keep = torch.empty(batch, dtype=INT32, device=device)
-    following = torch.empty(batch, dtype=picks.dtype, device=device)
+    path, n_keep, following = parents.new_empty(batch, nodes), parents.new_empty(batch), picks.new_empty(batch)
     _launch(device, "skv_accept_drafts", parents.data_ptr(), ctypes.byref(ids), ctypes.byref(wanted),
             _lib.ptr(n_new), batch, nodes, path.data_ptr(), n_keep.data_ptr(), following.data_ptr())
     return path, n_keep, following
@@ -849,7 +848,8 @@ def keep_tokens(free_stack: torch.Tensor, free_top: torch.Tensor, block_table: t
     cache = fp4_cache(pools[0], block_table)
     batch, n_pages, device, shape = cache.batch, cache.n_pages, block_table.device, pools[0].shape
     bases = (ctypes.c_void_p * len(pools))()
-    for i, p in enumerate(pools):
+    bases[0] = cache.pool
+    for i, p in enumerate(pools[1:], 1):  # the first has been checked
         if not isinstance(p, torch.Tensor) or p.dtype is not torch.uint8 or p.shape != shape or not p.is_contiguous():
             raise ValueError(f"pools[{i}] must be a contiguous uint8 {list(shape)} tensor")
         if p.device != device:
@@ -857,14 +857,15 @@ def keep_tokens(free_stack: torch.Tensor, free_top: torch.Tensor, block_table: t
         bases[i] = p.data_ptr()
     if len(set(bases)) != len(pools):
         raise ValueError("a pool is given twice")
-    _require_i32(path, "path")
-    if path.dim() != 2 or path.shape[0] != batch or not 1 <= path.shape[1] <= MAX_NODES:
+    width = path.shape[1] if isinstance(path, torch.Tensor) and path.dim() == 2 else 0
+    if not 1 <= width <= MAX_NODES:
+        _require_i32(path, "path")
         raise ValueError(f"path must be int32 [{batch}, 1..{MAX_NODES}]; got {tuple(path.shape)}")
-    width, one, each = path.shape[1], (1,), (batch,)
-    _require_i32_on(device, path=(path, path.shape), free_stack=(free_stack, (n_pages,)), free_top=(free_top, one),
+    one, each = (1,), (batch,)
+    _require_i32_on(device, path=(path, (batch, width)), free_stack=(free_stack, (n_pages,)), free_top=(free_top, one),
                     seq_lens=(seq_lens, each), n_keep=(n_keep, each), status=(status, one), refs=(refs, (n_pages,)))
     n_ptr, n_uni = _n_new_args(n_new, batch)
-    if n_ptr is not None and n_new.device != device:
+    if n_ptr is not None and n_new.get_device() != device.index:
         raise ValueError(f"n_new is on {n_new.device}, block_table on {device}")
     need = batch * width * 16
     if workspace is None:
@@ -906,13 +907,14 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor | None = None, *, 
     rows, stride, lead = _logit_rows(logits, top)
     vocab, device = logits.shape[-1], logits.device
     f32 = {"dtype": torch.float32, "device": device}
+    sizes = lead or ((),)  # sizes one by one take torch half the time that a tuple does
     ids = None
     if tokens is not None:
         if tokens.shape != lead:
             raise ValueError(f"tokens must be int32 or int64 {list(lead)}; got {tokens.dtype} {list(tokens.shape)}")
         flat = tokens if len(lead) == 1 else tokens.reshape(-1)
         ids = _token_ids(flat, "tokens", (rows,), device)
-    out = TokenLogprobs(None if tokens is None else torch.empty(lead, **f32), torch.empty(lead, **f32),
+    out = TokenLogprobs(None if tokens is None else torch.empty(*sizes, **f32), torch.empty(*sizes, **f32),
                         torch.empty(*lead, top, dtype=INT32, device=device), torch.empty(*lead, top, **f32))
     need = _lib.load().skv_token_logprobs_workspace(rows, vocab, _LOGITS[logits.dtype], top)
     if need < 0:
