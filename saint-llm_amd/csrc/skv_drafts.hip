@@ -8,8 +8,8 @@
 //   keep   : the tokens path[0] < path[1] < ... of the newest n become the newest k of them: path[i]'s row, in every
 //            layer's pages, moves to row i of the n, the length is cut behind row k - 1 and the pages behind it go
 //            on the free stack.
-// All of it is the latency of a few dependent reads; MI355X: 3 us for masks and paths of 64 trees of 64 nodes each,
-// and what the rows cost to move (below).
+// All of it is the latency of a few dependent reads; MI355X: 64 trees of up to 64 nodes take 4.2 us for their masks, 5.3
+// for their paths, 8.7 for the plan of what is kept and 6.3 to move its rows in 8 layers (8 heads of 128 dims).
 #include <algorithm>
 
 #include "skv_fp4.h"

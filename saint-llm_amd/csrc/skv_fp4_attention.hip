@@ -39,12 +39,12 @@
 //
 // Measured, us a call (both launches) in a graph of several, with the time of the bytes
 // at 6.1 TB/s (or of the products at 1.4 PFLOP/s, an 8192^3 library product's rate):
-//   64 sequences of 1k - 32k, 64 heads on 8 of 128 dims                    139 (117)
-//   4 of 256k - 1M, 4 tokens, 16 heads on 4 of 64                          91 (74)
-//   16 of 64k, 64 heads on 1 of 128                                        79 (25, products)
-//   2 prompts' 1000 tokens over 16k, 32 heads on 8 of 128                  508 (367, products)
-//   1 prompt's 512 tokens over 200k, the same heads                        1690 (1200, products)
-//   32 windows of 128, 64 heads on 1 of 512                                21 (1)
+//   64 sequences of 1k - 32k, 64 heads on 8 of 128 dims                    131 (117)
+//   4 of 256k - 1M, 4 tokens, 16 heads on 4 of 64                          93 (74)
+//   16 of 64k, 64 heads on 1 of 128                                        78 (25, products)
+//   2 prompts' 1000 tokens over 16k, 32 heads on 8 of 128                  510 (367, products)
+//   1 prompt's 512 tokens over 200k, the same heads                        1567 (1200, products)
+//   32 windows of 128, 64 heads on 1 of 512                                20 (1)
 // and dropped: two row groups of two waves with half the tiles each for 33 - 64 rows (68 ->
 // 74 us for the 64k sequences, before their weights had rests: a tile's latency is then seen by
 // all four waves); the next tile's scores ahead of a tile's weights (1%); a prologue that loads

@@ -127,8 +127,8 @@ __device__ __forceinline__ int fp4_tile_base(const Fp4Span& s) { return kView ? 
 constexpr int kF4RunTiles = 8;
 constexpr int kF4SmallTiles = 16;
 // What a segment costs beside its tiles, in tiles: the first loads' latencies and the
-// waves' join.  A step of 64 sequences of 1k - 32k, 8 K/V heads: 165 us without it, with 12 tiles
-// 144 and with 20 139 us; the other cases of skv_fp4_attention.hip stay within 1%.  Counted where
+// waves' join.  A step of 64 sequences of 1k - 32k, 8 K/V heads: 156 us without it, with 12 tiles
+// 135 and with 20 131 us; the other cases of skv_fp4_attention.hip stay within 1%.  Counted where
 // there are about as many items as workgroups or more; a run that would begin in this
 // lead or just past it begins with the item.
 constexpr int kF4Lead = 20;
@@ -269,17 +269,17 @@ struct Fp4Wave {
   static constexpr bool kPacked = kExact && DP <= 128;
   // A weight's bf16 rounding, 2^-9 of it on average over few keys as over many, is as
   // large an error as the output's own.  Waves with tiles of their own carry its rest
-  // into a second product, 139 us for a step of 64 sequences and 138 without (64 rows on one
-  // head 79 and 67); where the products bound the time (a prompt's chunk 557, with rests 705 us)
-  // the rounded weight stands.
+  // into a second product, 131 us for a step of 64 sequences and 129 without (64 rows on one
+  // head 78 and 66, trees of 7 nodes over 256k - 1M 154 and 128); where the products bound the time (a
+  // prompt's chunk 510, with rests 709 us) the rounded weight stands.
   static constexpr bool kRest = !kShared;
   // Waves of the same rows split a wide query's steps among them (a step is about 1,100 instructions;
-  // 32 windows of 128, 64 rows of 512 dims: 21 us a call, 23 with every wave splitting all four steps).
+  // 32 windows of 128, 64 rows of 512 dims: 20 us a call, 23 with every wave splitting all four steps).
   static constexpr bool kSplit = !kShared && kSteps > 1;
   static constexpr int kSplitWords = 17 * kWave;
   static constexpr bool kTwo = DP * MT <= 256;  // two tiles in flight; wider ones have registers for one
-  // A page is read by one workgroup, or by two: nontemporal loads (a step of 64 sequences 139 us,
-  // 156 with plain ones; 4 of 256k - 1M 91 and 103; 64 rows on one head, read twice, 79 either way).
+  // A page is read by one workgroup, or by two: nontemporal loads (a step of 64 sequences 131 us,
+  // 151 with plain ones; 4 of 256k - 1M 94 and 103; 64 rows on one head, read twice, 78 either way).
   static constexpr bool kOnce = !kShared && DP * MT <= 256;
 
   const Fp4Args<kView>& a;

@@ -70,8 +70,8 @@ def fp4_attention(q: torch.Tensor, pool: torch.Tensor, block_table: torch.Tensor
     sequence b's newest, token t at position seq_lens - n_new + t, and later ones
     get 0 (a count past T is T).  pool, block_table: as ``ops.fp4_quant_append`` wrote them; seq_lens:
     int32 [B].  window: only the newest ``window`` positions up to itself (None:
-    all); first: the sequence's first positions that stay visible behind a window; sink: fp32 [H] or None; softcap: c*tanh(s/c) of the scores, or None;
-    scale: of the scores (None: 1/sqrt(D)).  A token that sees nothing gets 0.
+    all); first: the sequence's first positions that stay visible behind a window; sink: fp32 [H]
+    or None; softcap: c*tanh(s/c) of the scores, or None; scale: of the scores (None: 1/sqrt(D)).  A token that sees nothing gets 0.
     tree: int64 [B, T, ceil(T / 64)], T <= 1024, where the new tokens are a drafted tree
     (``ops.draft_tree`` makes it): bit j of token t's words says that it sees new token
     j <= t.  ``window`` and ``first`` then count in a token's history, the positions before the
@@ -82,7 +82,8 @@ def fp4_attention(q: torch.Tensor, pool: torch.Tensor, block_table: torch.Tensor
     instead of as many as the device holds (0).  Up to 64 query rows of a K/V head
     (its query heads times the query tokens; 32 of 129 to 256 dims, any number of
     more dims) the softmax's weights keep 16 bits for the product with the values,
-    beyond them 8, as the output has.
+    beyond them 8, as the output has.  With ``first`` or ``tree`` those of many rows over
+    at most 512 positions may keep 16, those of more than 32 rows of 512 dims 8.
     workspace: a tensor of at least ``fp4_attention_workspace`` bytes, of no other
     call that may run at the same time (None: one is allocated for the call)."""
     d, out = _desc(q, pool, block_table, seq_lens, n_new, window, sink, softcap, scale, max_len, splits, out)
