@@ -248,7 +248,7 @@ struct Fp4Smem {
   int pre[kF4MaxItems + 1];
   int scan[17];
   int longest;
-  // of shared tiles the keys' codes and scale bytes, as the lanes hold them: this round's and the next one's
+  // of shared tiles the keys' codes and scale bytes, as the lanes hold them: of four tiles and of the next four
   static constexpr bool kKeys = kShared && DP <= 128;
   alignas(16) uint32_t keys[2][kKeys ? kF4Waves : 1][2][kKeys ? (Fp4Raw<DP>::kKeyWords + Fp4Raw<DP>::kScales) * kWave : 4];
 };
