@@ -391,3 +391,32 @@ def test_mixed_ids_and_trees_on_another_stream(dev) -> None:
     stream.synchronize()
     assert all(np.array_equal(g.cpu().numpy(), w) for g, w in zip(got, want)) and got[2].dtype == torch.int64
     assert np.array_equal(tree.cpu().numpy(), ora.pack_masks(ora.tree_masks(parents, np.full(5, 40))))
+
+
+def test_far_pages(dev) -> None:
+    """Pages whose bytes lie past 2^32."""
+    from saint_kv import ops
+
+    n_pages, block, heads, dim = 65000, 64, 8, 128
+    pool = ops.fp4_pool(n_pages, block, heads, dim, dev)
+    assert pool.numel() > 2 ** 32
+    used = np.array([64999, 3, 64001, 62500], dtype=np.int64)
+    at = torch.as_tensor(used, device=dev)
+    rng = np.random.default_rng(8)
+    small = rng.integers(0, 256, (4, block, heads, dim * 17 // 16), dtype=np.uint8)
+    pool[at] = torch.as_tensor(small, device=dev)
+    lens, n_new = np.array([130, 64], dtype=np.int32), np.array([90, 60], dtype=np.int32)
+    path, n_keep = paths(rng, n_new, 90)
+    where = np.array([[0, 1, 2], [3, -1, -1]], dtype=np.int32)
+    bt = torch.as_tensor(np.where(where < 0, -1, used[where]).astype(np.int32), device=dev)
+    stack, top = torch.zeros(n_pages, dtype=torch.int32, device=dev), torch.zeros(1, dtype=torch.int32, device=dev)
+    status, lens_t = torch.full((1,), 7, dtype=torch.int32, device=dev), torch.as_tensor(lens, device=dev)
+    ops.keep_tokens(stack, top, bt, lens_t, torch.as_tensor(n_new, device=dev), torch.as_tensor(path, device=dev),
+                    torch.as_tensor(n_keep, device=dev), [pool], status)
+    free = np.zeros(4, dtype=np.int32)
+    count, ok = drafts.keep(free, 0, where, lens, n_new, path, n_keep, [small])
+    assert int(status.item()) == ok == 0 and int(top.item()) == count
+    assert np.array_equal(pool[at].cpu().numpy(), small)
+    assert np.array_equal(lens_t.cpu().numpy(), lens)
+    assert np.array_equal(stack[:count].cpu().numpy(), used[free[:count]])
+    assert np.array_equal(bt.cpu().numpy(), np.where(where < 0, -1, used[where]))

@@ -283,3 +283,18 @@ def test_masks_far_below_the_rest(dev, kind, mask) -> None:
         x[0] = mask
         x[-1, :40] = mask
         check(ops.token_logprobs(x, t, top=5), x, t, 5)
+
+
+@pytest.mark.parametrize("rows,vocab", [(5, 5001), (3, 200003), (1100, 700)])
+def test_far_rows(dev, rows, vocab) -> None:
+    """Rows whose bytes lie past 2^32."""
+    from saint_kv import ops
+
+    stride = (3 << 30) // rows // 8 * 8 + 3
+    buffer = torch.empty(stride * rows, dtype=torch.bfloat16, device=dev)
+    assert stride * (rows - 1) * 2 > 2 ** 32
+    far = buffer.view(rows, stride)[:, :vocab]
+    x, t = inputs(dev, rows, vocab, "bf16", seed=vocab)
+    far.copy_(x)
+    got = ops.token_logprobs(far, t, top=7)
+    check(got, x, t, 7)
