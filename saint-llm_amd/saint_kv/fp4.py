@@ -336,15 +336,18 @@ class Fp4TokenCache:
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError("keep reads back how many tokens stayed; a graph records ops.keep_tokens")
         n_new = torch.as_tensor(self._host_new.astype(np.int32), device=self.device)  # none of a released sequence
+        word = self._status_word()
         ops.keep_tokens(self.free_stack, self.free_top, self.block_table, self.seq_lens, n_new, path, n_keep, self.pool,
-                        self._status_word(), refs=self.refs)
+                        word, refs=self.refs)
         kept = n_keep.clone()
-        counts = kept.cpu().numpy().astype(np.int64)
+        counts = torch.cat((kept, word)).cpu().numpy().astype(np.int64)
+        counts, refused = counts[:-1], counts[-1]
+        if not refused:  # an earlier refusal, raised below, leaves what stayed in order
+            bs, before = self.block_size, self.host_lens
+            self.host_lens = before - self._host_new + counts
+            self.host_free += int(((before + bs - 1) // bs - (self.host_lens + bs - 1) // bs).sum())
+            self._n_new, self._host_new, self._most_new = kept, counts, int(counts.max())
         self.check_status()
-        bs, before = self.block_size, self.host_lens
-        self.host_lens = before - self._host_new + counts
-        self.host_free += int(((before + bs - 1) // bs - (self.host_lens + bs - 1) // bs).sum())
-        self._n_new, self._host_new, self._most_new = kept, counts, int(counts.max())
         return counts
 
     def check_status(self) -> None:

@@ -420,3 +420,25 @@ def test_far_pages(dev) -> None:
     assert np.array_equal(lens_t.cpu().numpy(), lens)
     assert np.array_equal(stack[:count].cpu().numpy(), used[free[:count]])
     assert np.array_equal(bt.cpu().numpy(), np.where(where < 0, -1, used[where]))
+
+
+def test_an_earlier_refusal_leaves_what_stayed_in_order(dev) -> None:
+    """It is raised by the keep, whose tokens have moved: the next keep counts from these; a keep's own refusal moves none."""
+    from saint_kv import Fp4TokenCache
+
+    cache = Fp4TokenCache(1, 2, 64, 1, 32, block_size=16, device=dev)
+    rows = torch.randn(2, 9, 1, 32, generator=torch.Generator(device=dev).manual_seed(0), device=dev).to(torch.bfloat16)
+    cache.reserve(9)
+    cache.append(0, rows, rows)
+    cache.status.fill_(4)  # as a launch before may have left it
+    path = torch.tensor([[0, 2, 5, -1], [1, -1, -1, -1]], dtype=torch.int32, device=dev)
+    with pytest.raises(RuntimeError, match="refused"):
+        cache.keep(path, torch.tensor([3, 1], dtype=torch.int32, device=dev))
+    assert cache.host_lens.tolist() == [3, 1] == cache.seq_lens.tolist()
+    with pytest.raises(RuntimeError, match="refused"):  # one of a sequence's single token twice
+        cache.keep(path, torch.tensor([3, 2], dtype=torch.int32, device=dev))
+    assert cache.host_lens.tolist() == [3, 1] == cache.seq_lens.tolist()
+    path = torch.tensor([[1, 2], [0, -1]], dtype=torch.int32, device=dev)
+    assert cache.keep(path, torch.tensor([2, 1], dtype=torch.int32, device=dev)).tolist() == [2, 1]
+    assert cache.host_lens.tolist() == [2, 1] == cache.seq_lens.tolist()
+    assert int(cache.free_top.item()) == cache.host_free
