@@ -65,6 +65,7 @@ def to_words(seen: np.ndarray, dev) -> torch.Tensor:
 
 
 def check(got, q, pool, bt, lens, **kw):
+    """One output, or several of the same call."""
     qn, pn, btn, ln = q.cpu().double().numpy(), pool.cpu().numpy(), bt.cpu().numpy(), lens.cpu().numpy()
     kw = {n: x.cpu().numpy() if isinstance(x, torch.Tensor) else x for n, x in kw.items()}
     want = ora.view_attention(qn, pn, btn, ln, **kw)
@@ -73,11 +74,12 @@ def check(got, q, pool, bt, lens, **kw):
     half = p.block * p.dim // 2
     p.flat[:, :, half:2 * half] &= 0x77  # |v|: the signs of the values' codes cleared
     a = ora.view_attention(qn, mag, btn, ln, **kw)
-    g = got.detach().cpu().double().numpy().reshape(want.shape)
-    assert np.array_equal(np.isnan(g), np.isnan(want))
-    off = np.abs(g - want) - (2.0 ** -8 * np.abs(want) + 1.25 * 2.0 ** -8 * a)
-    off[np.isnan(want)] = -1
-    assert (off <= 0).all(), f"worst {off.max()} at {np.unravel_index(off.argmax(), off.shape)}"
+    for i, one in enumerate(got if isinstance(got, list) else [got]):
+        g = one.detach().cpu().double().numpy().reshape(want.shape)
+        assert np.array_equal(np.isnan(g), np.isnan(want))
+        off = np.abs(g - want) - (2.0 ** -8 * np.abs(want) + 1.25 * 2.0 ** -8 * a)
+        off[np.isnan(want)] = -1
+        assert (off <= 0).all(), f"output {i}: worst {off.max()} at {np.unravel_index(off.argmax(), off.shape)}"
 
 
 TREES = [
@@ -116,10 +118,10 @@ def test_trees(dev, lens, n_new, t, heads, kv, dim, block, window, first, sink, 
     kw = dict(window=window, softcap=softcap, sink=torch.randn(heads, generator=g, device=dev) if sink else None,
               n_new=n_new, first=first)
     tree = to_words(seen, dev)
-    for splits in (0, 1, 3):
-        got = fp4_attention(q, pool, bt, lens_t, splits=splits, tree=tree, **kw)
-        assert got.dtype == torch.bfloat16 and got.shape == q.shape
-        check(got, q, pool, bt, lens_t, seen=seen, **kw)
+    every = [fp4_attention(q, pool, bt, lens_t, splits=splits, tree=tree, **kw) for splits in (0, 1, 3)]
+    got = every[-1]
+    assert got.dtype == torch.bfloat16 and got.shape == q.shape
+    check(every, q, pool, bt, lens_t, seen=seen, **kw)
     if t == 1:
         assert torch.equal(fp4_attention(q[:, 0], pool, bt, lens_t, splits=3, tree=tree, **kw), got[:, 0])
 
@@ -151,9 +153,9 @@ def test_first_tokens(dev, lens, n_new, t, heads, kv, dim, block, window, first,
     n_new = None if n_new is None else torch.tensor(n_new, dtype=torch.int32, device=dev)
     kw = dict(window=window, softcap=softcap, sink=torch.randn(heads, generator=g, device=dev) if sink else None,
               n_new=n_new, first=first)
-    for splits in (0, 1, 3):
-        got = fp4_attention(q, pool, bt, lens_t, splits=splits, **kw)
-        check(got, q, pool, bt, lens_t, **kw)
+    every = [fp4_attention(q, pool, bt, lens_t, splits=splits, **kw) for splits in (0, 1, 3)]
+    got = every[-1]
+    check(every, q, pool, bt, lens_t, **kw)
     if t == 1:
         assert torch.equal(fp4_attention(q[:, 0], pool, bt, lens_t, splits=3, **kw), got[:, 0])
 
@@ -405,7 +407,7 @@ def test_random_views(dev, seed) -> None:
     ([1500, 700, 45, 0, 39], None, 40, 16, 1, 64, 200, 70, True, 30.0),
     ([130, 64, 65, 31, 32, 1, 100, 99], None, 1, 80, 2, 16, None, 0, True, None),  # 40 rows a head
     ([300] * 17, None, 3, 11, 1, 16, 100, 4, False, None),  # 33 rows
-    ([5000, 4000], None, 66, 16, 2, 64, None, 0, False, 5.0)])
+    ([1900, 1300], None, 66, 16, 2, 64, None, 0, False, 5.0)])
 def test_wide_heads_whose_waves_share_tiles(dev, lens, n_new, t, heads, kv, block, window, first, sink, softcap) -> None:
     from saint_kv import fp4_attention
 
@@ -420,7 +422,7 @@ def test_wide_heads_whose_waves_share_tiles(dev, lens, n_new, t, heads, kv, bloc
         if tree is None and not first:
             continue
         extra = {} if of is None else {"seen": of}
-        for splits in (0, 1, 3):
-            got = fp4_attention(q, pool, bt, lens_t, splits=splits, tree=tree, **kw)
-            check(got, q, pool, bt, lens_t, **extra, **kw)
+        every = [fp4_attention(q, pool, bt, lens_t, splits=splits, tree=tree, **kw) for splits in (0, 1, 3)]
+        check(every, q, pool, bt, lens_t, **extra, **kw)
+        for splits, got in zip((0, 1, 3), every):
             assert torch.equal(got, fp4_attention(q, pool, bt, lens_t, splits=splits, tree=tree, **kw))

@@ -27,7 +27,8 @@ U = 2.0 ** -24
 TYPES = {"bf16": torch.bfloat16, "fp16": torch.float16, "fp32": torch.float32}
 
 
-def check(got, x: torch.Tensor, tokens: torch.Tensor | None, top: int) -> None:
+def check(got, x: torch.Tensor, tokens: torch.Tensor | None, top: int, times: int = 1) -> None:
+    """Of rows that each came ``times`` times, one after another."""
     x = x.float().cpu().double().numpy().reshape(-1, x.shape[-1])
     t = np.full(x.shape[0], -1) if tokens is None else tokens.cpu().numpy().reshape(-1)
     with np.errstate(invalid="ignore", over="ignore", divide="ignore"):
@@ -39,6 +40,7 @@ def check(got, x: torch.Tensor, tokens: torch.Tensor | None, top: int) -> None:
         norm = np.log(total)
         dz = np.where(e > 0, d, 0.0)
         mean, square = (e * dz).sum(-1) / total, (e * dz * dz).sum(-1) / total
+    lp, h, ids, best, norm, mean, square = (np.repeat(a, times, 0) for a in (lp, h, ids, best, norm, mean, square))
     assert np.array_equal(got.top_ids.cpu().numpy().reshape(ids.shape), ids)
 
     def near(g, want, bound):
@@ -132,7 +134,7 @@ def test_special_rows(dev, kind, vocab) -> None:
     for top in (0, 1, 20, 64):
         check(ops.token_logprobs(x, t, top=top), x, t, top)
         many = x.repeat_interleave(60, 0)  # a workgroup a row
-        check(ops.token_logprobs(many, t.repeat_interleave(60), top=top), x.repeat_interleave(60, 0), t.repeat_interleave(60), top)
+        check(ops.token_logprobs(many, t.repeat_interleave(60), top=top), x, t, top, times=60)
 
 
 @pytest.mark.parametrize("kind", TYPES)
