@@ -1424,6 +1424,9 @@ __global__ __launch_bounds__(kF4Threads, fp4_resident(DP, MT)) void k_fp4_attn(F
 }
 
 constexpr int kF4MaxNodes = 1024;
+// What cutting and joining costs in the tiles of a workgroup's own time, of heads up to 128 dims on tiles of each wave's
+// own and of others; and the longest items (in tiles) that a window leaves whole for it (see fp4_attn_plan).
+constexpr int kF4JoinTiles = 48, kF4JoinTilesWide = 24, kF4UncutTiles = 128;
 
 struct Fp4AttnPlan {
   int dims, mt;  // padded dims, row tiles of a wave
@@ -1506,6 +1509,17 @@ inline int fp4_attn_plan(const skv_fp4_attention_desc* d, const skv_fp4_view* v,
   const int64_t tiles = tiles_of(p.rows), units = std::max<int64_t>(p.items * hkv, 1);
   p.cut = tiles > kF4SmallTiles || d->splits > 0;
   if (p.items > kF4MaxItems || units > INT32_MAX / (ceil_div(capacity, kF4Tile) + 1 + kF4Lead)) p.cut = false;
+  // With a view, the items of a window are at most a few tiles long.  They stay whole, a workgroup each, dealt out as others
+  // end, where the workgroups that the last round leaves idle lose less than runs, parts and the join cost (us whole and
+  // cut, sequences far longer than the window and, second, of anything from 64 tokens to two windows; 64 heads on 8 of 128,
+  // windows of 1k, one token: 64 of them 20 and 25, 20 and 34; 16 of them 14.5 and 22, 15 and 20; chunks of 1000 tokens, 32 heads:
+  // one 42 and 57, three 86 and 110, of windows of 2k two 90 and 93).  Past these numbers they lose (a chunk of 500 tokens
+  // in windows of 2k: 66 and 51; 64 tokens of 16 heads on 1 of 512, windows of 1k: 40 and 34).
+  if (v && p.cut && d->window > 0 && d->splits == 0 && tiles <= kF4UncutTiles) {
+    const int64_t slots = static_cast<int64_t>(fp4_resident(p.dims, p.mt)) * device_cus();
+    const int64_t idle = ceil_div(units, slots) * slots - units;
+    if (idle * tiles <= (p.shared || p.dims > 128 ? kF4JoinTilesWide : kF4JoinTiles) * slots) p.cut = false;
+  }
   if (units >= (1 << 24)) return set_error(SKV_EINVAL, "%s: too many workgroups", what);
   if (p.cut && d->splits > ((1 << 24) - 1) / units) {  // before it is multiplied: the product could wrap
     return set_error(SKV_EINVAL, "%s: splits must leave fewer than 2^24 runs; got %lld of %lld rows and heads", what,
