@@ -1339,7 +1339,7 @@ __global__ __launch_bounds__(kF4Threads, fp4_resident(DP, MT)) void k_fp4_attn(F
     // The workgroups that the chip's time is counted in: as many as run; with a view, whose items are often of one
     // length, and two or more for each compute unit, which keep the memory busy, as many as the items put there (64
     // windows of 4k, 64 heads on 8 of 128: 59 us uncut with 512 of the 768 workgroups that fit, 69 cut for all; of 64 dims 42
-    // and 48).
+    // and 48, before the plan itself left such windows whole).
     int slots = groups;
     if constexpr (kView) {
       const int cus = a.max_groups / fp4_resident(DP, MT);
@@ -1426,7 +1426,7 @@ __global__ __launch_bounds__(kF4Threads, fp4_resident(DP, MT)) void k_fp4_attn(F
 constexpr int kF4MaxNodes = 1024;
 // What cutting and joining costs in the tiles of a workgroup's own time, of heads up to 128 dims on tiles of each wave's
 // own and of others; and the longest items (in tiles) that a window leaves whole for it (see fp4_attn_plan).
-constexpr int kF4JoinTiles = 48, kF4JoinTilesWide = 24, kF4UncutTiles = 128;
+constexpr int kF4JoinTiles = 48, kF4JoinTilesWide = 24, kF4UncutTiles = 160;
 
 struct Fp4AttnPlan {
   int dims, mt;  // padded dims, row tiles of a wave
@@ -1513,8 +1513,9 @@ inline int fp4_attn_plan(const skv_fp4_attention_desc* d, const skv_fp4_view* v,
   // end, where the workgroups that the last round leaves idle lose less than runs, parts and the join cost (us whole and
   // cut, sequences far longer than the window and, second, of anything from 64 tokens to two windows; 64 heads on 8 of 128,
   // windows of 1k, one token: 64 of them 20 and 25, 20 and 34; 16 of them 14.5 and 22, 15 and 20; chunks of 1000 tokens, 32 heads:
-  // one 42 and 57, three 86 and 110, of windows of 2k two 90 and 93).  Past these numbers they lose (a chunk of 500 tokens
-  // in windows of 2k: 66 and 51; 64 tokens of 16 heads on 1 of 512, windows of 1k: 40 and 34).
+  // one 42 and 57, three 86 and 110, of windows of 2k two 90 and 93; 90 windows of 4k 74 and 79, 63 and 74).  Past these numbers
+  // they lose (a chunk of 500 tokens in windows of 2k: 66 and 51; 64 tokens of 16 heads on 1 of 512, windows of 1k: 40 and 34;
+  // windows of 8k, 220 of 4 tokens, 16 heads on 4 of 64: 110 and 120, but 102 and 98).
   if (v && p.cut && d->window > 0 && d->splits == 0 && tiles <= kF4UncutTiles) {
     const int64_t slots = static_cast<int64_t>(fp4_resident(p.dims, p.mt)) * device_cus();
     const int64_t idle = ceil_div(units, slots) * slots - units;
