@@ -249,7 +249,8 @@ class Fp4TokenCache:
         # that of one whose refusal nobody has read
         self._words = torch.zeros(STATUS_WORDS, **i32)
         self._word_views = list(self._words.split(1))
-        self._word, self._refusals = 0, torch.zeros(STATUS_WORDS, **i32)
+        # the word of the last reservation stays its own until the next: word 0 until the first
+        self._word, self._reserved, self._refusals = 1, 0, torch.zeros(STATUS_WORDS, **i32)
         self.host_lens, self.host_free = np.zeros(batch, dtype=np.int64), self.n_pages
         self._n_new: int | torch.Tensor = 0
         self._host_new = np.zeros(batch, dtype=np.int64)  # each sequence's tokens reserved last
@@ -274,17 +275,20 @@ class Fp4TokenCache:
         self._take_pages(need)
         self._n_new = int(n_new) if np.ndim(n_new) == 0 else torch.as_tensor(counts.astype(np.int32),
                                                                             device=self.device)
-        ops.reserve(self.free_stack, self.free_top, self.block_table, self.seq_lens, self._n_new, self.block_size,
-                    self._status_word())
+        word = self._status_word()
+        self._reserved = self._word - 1
+        ops.reserve(self.free_stack, self.free_top, self.block_table, self.seq_lens, self._n_new, self.block_size, word)
         self.host_lens = self.host_lens + counts
         self._host_new, self._most_new = counts.copy(), int(counts.max())
         self._shared = self._padded = False
         self._unwritten = set(range(len(self.pool))) if counts.any() else set()
 
     def _status_word(self) -> torch.Tensor:
+        if self._word == self._reserved:
+            self._word += 1
         if self._word == STATUS_WORDS:  # all used: what they hold is kept aside
             self._refusals.bitwise_or_(self._words)
-            self._word = 0
+            self._word = int(self._reserved == 0)
         self._word += 1
         return self._word_views[self._word - 1]
 
@@ -327,7 +331,8 @@ class Fp4TokenCache:
         """Of each sequence's tokens reserved last only ``path[b, :n_keep[b]]`` stay (int32 [B, P] and [B], as
         ``ops.accept_drafts`` gives them): the others leave the lengths and every layer, and
         pages behind return to the free list.  They are the tokens reserved last from then on.  Reads back, and returns,
-        how many stayed; raises if a layer still has to append them, or a fork shares them."""
+        how many stayed; raises if a layer still has to append them, a fork shares them, or the device refused their
+        reservation or these counts (nothing is written then)."""
         missing = self._unwritten - self._recorded
         if missing:
             raise RuntimeError(f"the tokens reserved last have not been appended to layers {sorted(missing)}")
@@ -336,31 +341,44 @@ class Fp4TokenCache:
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError("keep reads back how many tokens stayed; a graph records ops.keep_tokens")
         n_new = torch.as_tensor(self._host_new.astype(np.int32), device=self.device)  # none of a released sequence
+        # where the device refused the reservation its newest tokens are older ones: counts of -1 are refused, too
+        n_new = torch.where(self._word_views[self._reserved] == 0, n_new, -1)
         word = self._status_word()
+        at = self.batch + self._word - 1
         ops.keep_tokens(self.free_stack, self.free_top, self.block_table, self.seq_lens, n_new, path, n_keep, self.pool,
                         word, refs=self.refs)
         kept = n_keep.clone()
-        counts = torch.cat((kept, word)).cpu().numpy().astype(np.int64)
-        counts, refused = counts[:-1], counts[-1]
-        if not refused:  # an earlier refusal, raised below, leaves what stayed in order
+        report = torch.cat((kept, self._words, self._refusals, self.status)).cpu().numpy()
+        counts = report[:self.batch].astype(np.int64)
+        if not report[at]:  # another call's refusal, raised below, leaves what stayed in order
             bs, before = self.block_size, self.host_lens
             self.host_lens = before - self._host_new + counts
             self.host_free += int(((before + bs - 1) // bs - (self.host_lens + bs - 1) // bs).sum())
             self._n_new, self._host_new, self._most_new = kept, counts, int(counts.max())
-        self.check_status()
+        self._raise_refusals(report[self.batch:])
         return counts
 
     def check_status(self) -> None:
         """Synchronise and raise if the device refused a reservation, fork or release
         since the last check, as it does where the tables were changed behind the
-        host's back (it wrote nothing; the host's counts are read back)."""
-        bits = int(np.bitwise_or.reduce(torch.cat((self._refusals, self._words, self.status)).cpu().numpy()))
-        if bits:
-            for t in (self._refusals, self._words, self.status):
-                t.zero_()
-            self.host_lens = self.seq_lens.cpu().numpy().astype(np.int64)
-            self.host_free = int(self.free_top.item())
-            raise RuntimeError(f"Fp4TokenCache reservation, fork or release refused, or a keep (status bits {bits})")
+        host's back (it wrote nothing; the host's counts are read back).  Where that can
+        be, check before an append: after a refused reservation the newest tokens, which it
+        writes, are older ones."""
+        self._raise_refusals(torch.cat((self._words, self._refusals, self.status)).cpu().numpy())
+
+    def _raise_refusals(self, words: np.ndarray) -> None:
+        """``words``: ``_words`` and the others, as read back."""
+        bits = int(np.bitwise_or.reduce(words))
+        if not bits:
+            return
+        for t in (self._refusals, self._words, self.status):
+            t.zero_()
+        self.host_lens = self.seq_lens.cpu().numpy().astype(np.int64)
+        self.host_free = int(self.free_top.item())
+        if words[self._reserved]:  # no tokens were reserved: there are none to append or keep
+            self._n_new, self._host_new, self._most_new = 0, np.zeros(self.batch, dtype=np.int64), 0
+            self._unwritten = set()
+        raise RuntimeError(f"Fp4TokenCache reservation, fork or release refused, or a keep (status bits {bits})")
 
     # ------------------------------------------------------ forks, eviction --
     def fork(self, src: list[int], dst: list[int]) -> None:

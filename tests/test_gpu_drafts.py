@@ -442,3 +442,74 @@ def test_an_earlier_refusal_leaves_what_stayed_in_order(dev) -> None:
     assert cache.keep(path, torch.tensor([2, 1], dtype=torch.int32, device=dev)).tolist() == [2, 1]
     assert cache.host_lens.tolist() == [2, 1] == cache.seq_lens.tolist()
     assert int(cache.free_top.item()) == cache.host_free
+
+
+def books_of(cache):
+    return [x.clone() for x in (cache.seq_lens, cache.block_table, cache.free_stack, cache.free_top, cache.refs, *cache.pool)]
+
+
+@pytest.mark.parametrize("noticed", [False, True])
+@pytest.mark.parametrize("counts", [30, np.array([30, 0, 20])])
+def test_tokens_of_a_refused_reservation_are_not_kept(dev, counts, noticed) -> None:
+    """The device refuses a reservation (its free pages were taken behind the host's back): a keep raises and leaves the
+    committed tokens, also once the refusal has been raised, and after more status words than there are."""
+    from saint_kv import Fp4TokenCache
+
+    rng = np.random.default_rng(6)
+    cache = Fp4TokenCache(2, 3, 256, 1, 32, block_size=16, device=dev)
+
+    def append(n):
+        cache.reserve(n)
+        t = int(np.max(n))
+        for i in range(2):
+            cache.append(i, rows_of(dev, rng, 3, t, 1, 32), rows_of(dev, rng, 3, t, 1, 32))
+
+    append(np.array([40, 35, 64]))
+    path = torch.tensor([[0, 2, 5], [0, -1, -1], [1, 2, -1]], dtype=torch.int32, device=dev)
+    n_keep = torch.tensor([3, 0, 2] if isinstance(counts, np.ndarray) else [3, 1, 2], dtype=torch.int32, device=dev)
+    free = cache.free_top.clone()
+    cache.free_top.zero_()
+    append(counts)
+    before = books_of(cache)
+    if noticed:
+        with pytest.raises(RuntimeError, match="refused"):
+            cache.check_status()
+    else:
+        for _ in range(200):  # of other calls
+            cache._status_word()
+    for _ in range(2):
+        with pytest.raises(RuntimeError, match="refused"):
+            cache.keep(path, n_keep)
+        assert all(torch.equal(x, y) for x, y in zip(books_of(cache), before))
+        assert cache.host_lens.tolist() == [40, 35, 64] and cache.host_free == 0
+    # nothing of the refused one is left: none of its tokens can be kept or must be appended
+    assert cache.keep(path, torch.zeros_like(n_keep)).tolist() == [0, 0, 0]
+    assert all(torch.equal(x, y) for x, y in zip(books_of(cache), before))
+    cache.free_top.copy_(free)
+    cache.host_free = int(free.item())
+    append(np.array([6, 3, 4]))
+    assert cache.keep(path, n_keep).tolist() == n_keep.tolist()
+    assert cache.host_lens.tolist() == (np.array([40, 35, 64]) + n_keep.cpu().numpy()).tolist() == cache.seq_lens.tolist()
+    assert int(cache.free_top.item()) == cache.host_free
+
+
+def test_a_reservation_after_a_refused_one_is_kept(dev) -> None:
+    """An earlier refusal that nobody has read is raised; the tokens reserved since have moved, and count."""
+    from saint_kv import Fp4TokenCache
+
+    cache = Fp4TokenCache(1, 2, 256, 1, 32, block_size=16, device=dev)
+    rows = rows_of(dev, np.random.default_rng(0), 2, 40, 1, 32)
+    cache.reserve(40)
+    cache.append(0, rows, rows)
+    free = cache.free_top.clone()
+    cache.free_top.zero_()
+    cache.reserve(30)  # refused
+    cache.free_top.copy_(free)
+    cache.reserve(5)
+    cache.append(0, rows, rows)
+    path = torch.tensor([[0, 3], [2, -1]], dtype=torch.int32, device=dev)
+    with pytest.raises(RuntimeError, match="refused"):
+        cache.keep(path, torch.tensor([2, 1], dtype=torch.int32, device=dev))
+    assert cache.host_lens.tolist() == [42, 41] == cache.seq_lens.tolist()
+    assert cache.keep(path[:, :1] * 0, torch.ones(2, dtype=torch.int32, device=dev)).tolist() == [1, 1]
+    assert cache.host_lens.tolist() == [41, 41] and int(cache.free_top.item()) == cache.host_free
