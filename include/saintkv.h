@@ -530,7 +530,8 @@ int skv_fp4_attention(const skv_fp4_attention_desc* desc, void* workspace, int64
  * drafted tree).  It sees the history's last `window` positions (0: all of it)
  * and its first `first` ones.  A token with an empty mask sees nothing and gets
  * 0, and so do all of a sequence that is shorter than its new tokens, with a
- * tree.  n_queries <= 1024 with a tree.  The reference's first tokens
+ * tree.  n_queries <= 1024 with a tree.  Without a tree a call that has no window, or
+ * no first tokens, is skv_fp4_attention's.  The reference's first tokens
  * (model.py:267-276) fall out of its window layers' sight (swa.py:119-125); its
  * drafted tokens are a chain (eagle3.py). */
 typedef struct skv_fp4_view {

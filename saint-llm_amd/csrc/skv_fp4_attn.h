@@ -1438,6 +1438,17 @@ struct Fp4AttnPlan {
   int64_t sched_bytes, ws_bytes;
 };
 
+inline int fp4_check_view(const skv_fp4_attention_desc* d, const skv_fp4_view* v) {
+  const char* what = "skv_fp4_attention";
+  if (v->first < 0 || v->first > (1 << 24)) return set_error(SKV_EINVAL, "%s: first must be in [0, 2^24]", what);
+  if (v->tree && (d->n_queries > kF4MaxNodes || v->tree_words != ceil_div(d->n_queries, 64))) {
+    return set_error(SKV_EINVAL, "%s: a tree has at most %d nodes and a word for every 64; got %lld nodes and %lld words", what,
+                     kF4MaxNodes, (long long)d->n_queries, (long long)v->tree_words);
+  }
+  if (reinterpret_cast<uintptr_t>(v->tree) & 7) return set_error(SKV_EINVAL, "%s: tree must be 8-byte aligned", what);
+  return SKV_OK;
+}
+
 inline int fp4_attn_plan(const skv_fp4_attention_desc* d, const skv_fp4_view* v, Fp4AttnPlan& p) {
   const char* what = "skv_fp4_attention";
   if (!d) return set_error(SKV_EINVAL, "%s: NULL descriptor", what);
@@ -1475,12 +1486,7 @@ inline int fp4_attn_plan(const skv_fp4_attention_desc* d, const skv_fp4_view* v,
   p.shared = rows > 16 * mt * kF4Waves / 2 &&
              (p.dims <= 256 || (v && D == 512 && 16 * d->cache.batch * hkv * ceil_div(rows, 16 * mt * kF4Waves) >= device_cus()));
   if (v) {
-    if (v->first < 0 || v->first > (1 << 24)) return set_error(SKV_EINVAL, "%s: first must be in [0, 2^24]", what);
-    if (v->tree && (d->n_queries > kF4MaxNodes || v->tree_words != ceil_div(d->n_queries, 64))) {
-      return set_error(SKV_EINVAL, "%s: a tree has at most %d nodes and a word for every 64; got %lld nodes and %lld words", what,
-                       kF4MaxNodes, (long long)d->n_queries, (long long)v->tree_words);
-    }
-    if (reinterpret_cast<uintptr_t>(v->tree) & 7) return set_error(SKV_EINVAL, "%s: tree must be 8-byte aligned", what);
+    if (const int rc = fp4_check_view(d, v)) return rc;
   }
   p.mt = p.shared ? mt : rows <= 16 || p.dims > 256 ? 1 : 2;
   // the most tiles that a block of so many rows may see

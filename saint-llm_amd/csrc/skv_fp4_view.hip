@@ -23,10 +23,21 @@
 //   a tree of 8 nodes over 400 tokens, one token in a window of 128                  10, 9
 #include "skv_fp4_attn.h"
 
+namespace skv {
+
+// Whether v adds nothing to the plain call: without a tree, where no window hides the first tokens.  It is that call then,
+// to the bit and in its precision.
+inline bool fp4_plain(const skv_fp4_attention_desc* d, const skv_fp4_view* v) {
+  return d && !v->tree && (d->window == 0 || v->first == 0);
+}
+
+}  // namespace skv
+
 using namespace skv;
 
 extern "C" int64_t skv_fp4_attention_view_workspace(const skv_fp4_attention_desc* d, const skv_fp4_view* v) {
   if (!v) return set_error(SKV_EINVAL, "skv_fp4_attention_view: NULL view"), -1;
+  if (fp4_plain(d, v)) return fp4_check_view(d, v) == SKV_OK ? skv_fp4_attention_workspace(d) : -1;
   Fp4AttnPlan p;
   return fp4_attn_plan(d, v, p) == SKV_OK ? p.ws_bytes : -1;
 }
@@ -34,5 +45,9 @@ extern "C" int64_t skv_fp4_attention_view_workspace(const skv_fp4_attention_desc
 extern "C" int skv_fp4_attention_view(const skv_fp4_attention_desc* d, const skv_fp4_view* v, void* workspace, int64_t ws_bytes,
                                       void* stream) {
   if (!v) return set_error(SKV_EINVAL, "skv_fp4_attention_view: NULL view");
+  if (fp4_plain(d, v)) {
+    const int rc = fp4_check_view(d, v);
+    return rc ? rc : skv_fp4_attention(d, workspace, ws_bytes, stream);
+  }
   return fp4_attn_call<true>(d, v, workspace, ws_bytes, stream);
 }

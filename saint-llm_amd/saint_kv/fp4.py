@@ -70,7 +70,8 @@ def fp4_attention(q: torch.Tensor, pool: torch.Tensor, block_table: torch.Tensor
     sequence b's newest, token t at position seq_lens - n_new + t, and later ones
     get 0 (a count past T is T).  pool, block_table: as ``ops.fp4_quant_append`` wrote them; seq_lens:
     int32 [B].  window: only the newest ``window`` positions up to itself (None:
-    all); first: the sequence's first positions that stay visible behind a window; sink: fp32 [H]
+    all); first: the sequence's first positions that stay visible behind a window (without
+    one they are anyway); sink: fp32 [H]
     or None; softcap: c*tanh(s/c) of the scores, or None; scale: of the scores (None: 1/sqrt(D)).  A token that sees nothing gets 0.
     tree: int64 [B, T, ceil(T / 64)], T <= 1024, where the new tokens are a drafted tree
     (``ops.draft_tree`` makes it): bit j of token t's words says that it sees new token

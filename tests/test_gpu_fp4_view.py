@@ -426,3 +426,19 @@ def test_wide_heads_whose_waves_share_tiles(dev, lens, n_new, t, heads, kv, bloc
         check(every, q, pool, bt, lens_t, **extra, **kw)
         for splits, got in zip((0, 1, 3), every):
             assert torch.equal(got, fp4_attention(q, pool, bt, lens_t, splits=splits, tree=tree, **kw))
+
+
+@pytest.mark.parametrize("lens,t,heads,kv,dim", [([333], 8, 16, 2, 128), ([300] * 17, 3, 11, 1, 512), ([1500, 700], 40, 16, 1, 512),
+                                                 ([200, 90, 41, 12], 5, 12, 3, 224), ([900, 0, 5], 1, 8, 1, 64)])
+def test_first_tokens_without_a_window_are_no_view(dev, lens, t, heads, kv, dim) -> None:
+    """Every position is seen with them and without: the plain call, to the bit, and its workspace."""
+    from saint_kv import fp4_attention
+    from saint_kv.fp4 import fp4_attention_workspace
+
+    pool, bt, lens_t = make(dev, lens, 16, kv, dim, seed=2)
+    q = torch.randn(len(lens), t, heads, dim, generator=torch.Generator(device=dev).manual_seed(1), device=dev).to(torch.bfloat16)
+    for splits in (0, 3):
+        got = fp4_attention(q, pool, bt, lens_t, first=4, splits=splits)
+        assert torch.equal(got, fp4_attention(q, pool, bt, lens_t, splits=splits))
+        need = [fp4_attention_workspace(q, pool, bt, first=first, splits=splits) for first in (0, 4)]
+        assert need[0] == need[1]
