@@ -271,8 +271,10 @@ struct Fp4Wave {
   // large an error as the output's own.  Waves with tiles of their own carry its rest
   // into a second product, 131 us for a step of 64 sequences and 129 without (64 rows on one
   // head 78 and 66, trees of 7 nodes over 256k - 1M 154 and 128); where the products bound the time (a
-  // prompt's chunk 510, with rests 709 us) the rounded weight stands.
-  static constexpr bool kRest = !kShared;
+  // prompt's chunk 510, with rests 709 us) the rounded weight stands.  Heads of more than 256 dims keep the rests where
+  // a view's tiles are shared, too, as the plain call, which shares none, keeps them (6 trees of 99 nodes, 16 heads on 1
+  // of 512, in windows of 128: 46 us, 44 without; over 8k 420 and 386).
+  static constexpr bool kRest = !kShared || DP > 256;
   // Waves of the same rows split a wide query's steps among them (a step is about 1,100 instructions;
   // 32 windows of 128, 64 rows of 512 dims: 20 us a call, 23 with every wave splitting all four steps).
   static constexpr bool kSplit = !kShared && kSteps > 1;
@@ -1162,9 +1164,9 @@ __device__ __forceinline__ void fp4_rounds(Fp4Smem<DP, true>& sm, Fp4Wave<DP, MT
 
 // The same with every wave loading all keys itself (heads of 512 dims: one workgroup on a compute unit, whose LDS the
 // values fill).  A tile's keys take their registers from the ones before once these have been multiplied.  (6 trees of 99 nodes,
-// 16 heads on one, in windows of 128: 43 us a call, 54 with a tile's scores ahead of its own weights, and 54 with tiles of each
-// wave's own; 9 chunks of 401 tokens, 8 heads on one, over 4k: 585, 661 and 787.  Two waves on a SIMD hide more of each other's
-// waits without it: 2 prompts of 16 heads on 4 of 256 dims 835 us with it and 754.)
+// 16 heads on one, in windows of 128: 46 us a call, 53 with tiles of each wave's own; 9 trees of 401 nodes, 8 heads on one,
+// over 4k: 632 and 799.  A tile's scores ahead of its own weights, both without the weights' rests: 54 us for 43, 661 for 585.
+// Two waves on a SIMD hide more of each other's waits without it: 2 prompts of 16 heads on 4 of 256 dims 835 us with it and 754.)
 template <int DP, int MT, bool kExact, bool kView>
 __device__ __forceinline__ void fp4_rounds_wide(Fp4Smem<DP, true>& sm, Fp4Wave<DP, MT, kExact, true, kView>& w, const Fp4Span& sp, int b,
                                            int wave, int lane, int t_lo, int t_hi, Fp4Pace& pace, int done) {
@@ -1479,9 +1481,9 @@ inline int fp4_attn_plan(const skv_fp4_attention_desc* d, const skv_fp4_view* v,
   // block), 53 and 36 with 32; of 64 dims 44 and 42 with 64 rows, 45 either way with 65, 49 and 60 with
   // 128; of 256 dims 68 and 65 with 32 rows, 68 and 101 with 33.  Heads of up to 512 dims stay apart, but with a view
   // those of 512 where a sixteenth of the compute units get such a workgroup, as a cut into more pieces is more to join (us
-  // shared and apart: 300 windows of 128, 33 rows 56 and 70, 64 rows 63 and 91; 16 of 4k 48 and 46, 51 and 58; 8 windows of 9k, 64
-  // rows 53 and 57; one of 100k 90 and 68).  The sizes between spill registers (40 trees of 9 nodes, 32 heads on 2 of 288 dims,
-  // over 8k: 720 and 650).
+  // shared and apart: 300 windows of 128, 33 rows 58 and 70, 64 rows 64 and 91; 16 of 4k 50 and 46, 53 and 59; 8 windows of 9k, 64
+  // rows 55 and 57; one of 100k 94 and 68).  The sizes between spill registers (40 trees of 9 nodes, 32 heads on 2 of 288 dims,
+  // over 8k: 720, without the weights' rests, and 650).
   const int mt = fp4_shared_mt(p.dims);
   p.shared = rows > 16 * mt * kF4Waves / 2 &&
              (p.dims <= 256 || (v && D == 512 && 16 * d->cache.batch * hkv * ceil_div(rows, 16 * mt * kF4Waves) >= device_cus()));

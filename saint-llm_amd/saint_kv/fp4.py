@@ -84,7 +84,7 @@ def fp4_attention(q: torch.Tensor, pool: torch.Tensor, block_table: torch.Tensor
     (its query heads times the query tokens; 32 of 129 to 256 dims, any number of
     more dims) the softmax's weights keep 16 bits for the product with the values,
     beyond them 8, as the output has.  With ``first`` or ``tree`` those of many rows over
-    at most 512 positions may keep 16, those of more than 32 rows of 512 dims 8.
+    at most 512 positions may keep 16.
     workspace: a tensor of at least ``fp4_attention_workspace`` bytes, of no other
     call that may run at the same time (None: one is allocated for the call)."""
     d, out = _desc(q, pool, block_table, seq_lens, n_new, window, sink, softcap, scale, max_len, splits, out)

@@ -76,3 +76,37 @@ def test_small_outputs_of_large_values(dev, t, heads, kv, dim, sink) -> None:
         got = fp4_attention(q, pool, bt, lens_t, splits=splits, **kw).double().cpu().numpy()
         off = np.abs(got - want) - bound(want, a)
         assert (off <= 0).all(), (splits, off.max(), (off > 0).mean())
+
+
+# views whose rows stay few, and those of 512 dims of any number of rows: 33 of 17 sequences and 200 of four in tiles that waves share
+@pytest.mark.gpu
+@pytest.mark.parametrize("lens,t,heads,kv,dim", [([80, 41, 2, 66], 1, 64, 1, 64), ([80, 41, 2, 66], 4, 32, 2, 128), ([80, 41, 2, 66], 1, 32, 1, 256),
+                                                 ([80, 41, 2, 66], 2, 20, 1, 384), ([80, 41, 2, 66], 1, 64, 1, 512),
+                                                 ([80, 41, 5, 66] * 4 + [80], 3, 11, 1, 512), ([80, 41, 33, 66] * 4 + [70], 2, 48, 2, 512),
+                                                 ([160, 100, 133, 101], 100, 2, 1, 512)])
+@pytest.mark.parametrize("window,first", [(None, 0), (50, 3)])
+def test_small_outputs_of_large_values_with_a_view(dev, lens, t, heads, kv, dim, window, first) -> None:
+    """As above; a chain given as a tree, and without a tree the window behind first tokens."""
+    from saint_kv import fp4_attention, ops
+
+    batch, longest = len(lens), max(lens)
+    pool, bt, lens_t = make(dev, lens, 16, kv, dim, seed=dim)
+    g = torch.Generator(device=dev).manual_seed(heads)
+    k, v = (torch.randn(batch, longest, kv, dim, generator=g, device=dev) for _ in range(2))
+    v[:, 1::2] = -v[:, 0::2]
+    ops.fp4_quant_append(pool, bt, lens_t, k, v, lens_t)
+    q = torch.randn(batch, t, heads, dim, generator=g, device=dev).to(torch.bfloat16)
+    chain = np.broadcast_to(np.tri(t, dtype=bool), (batch, t, t))
+    tree = torch.as_tensor(ora.pack_masks(chain), device=dev)
+    kw = dict(scale=SCALE, window=window, first=first)
+    qn, pn, btn, ln = q.cpu().double().numpy(), pool.cpu().numpy(), bt.cpu().numpy(), lens_t.cpu().numpy()
+    want = [ora.view_attention(qn, pn, btn, ln, seen=seen, **kw) for seen in (chain, None)]
+    p = ora.Pages(pn)
+    half = p.block * p.dim // 2
+    p.flat[:, :, half:2 * half] &= 0x77
+    a = [ora.view_attention(qn, pn, btn, ln, seen=seen, **kw) for seen in (chain, None)]
+    for splits in (0, 1, 3):
+        for i, masks in enumerate((tree, None)):
+            got = fp4_attention(q, pool, bt, lens_t, splits=splits, tree=masks, **kw).double().cpu().numpy()
+            off = np.abs(got - want[i]) - bound(want[i], a[i])
+            assert (off <= 0).all(), (splits, i, off.max(), (off > 0).mean())
