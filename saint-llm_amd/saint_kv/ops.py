@@ -952,6 +952,8 @@ def _logit_rows(logits: torch.Tensor, top: int) -> tuple[int, int, tuple[int, ..
         raise ValueError("a row's logits must be contiguous")
     if len(lead) == 1:
         return lead[0], strides[0], lead
+    if 0 in lead:  # whose strides say nothing
+        return 0, vocab, lead
     sizes = [(n, s) for n, s in zip(lead, strides[:-1]) if n != 1]
     for (_, outer), (n, inner) in zip(sizes, sizes[1:]):
         if outer != n * inner:

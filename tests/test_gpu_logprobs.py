@@ -300,3 +300,14 @@ def test_far_rows(dev, rows, vocab) -> None:
     far.copy_(x)
     got = ops.token_logprobs(far, t, top=7)
     check(got, x, t, 7)
+
+
+@pytest.mark.parametrize("lead", [(0,), (5, 0), (0, 5), (3, 0, 2), (1, 0)])
+def test_no_rows(dev, lead) -> None:
+    """A dimension of no rows anywhere: outputs of as many."""
+    from saint_kv import ops
+
+    x = torch.zeros(*lead, 50, dtype=torch.bfloat16, device=dev)
+    got = ops.token_logprobs(x, torch.zeros(lead, dtype=torch.int64, device=dev), top=4)
+    assert got.logprobs.shape == got.entropy.shape == lead and got.top_ids.shape == got.top_logprobs.shape == (*lead, 4)
+    assert ops.token_logprobs_workspace(x, 4) == 0
