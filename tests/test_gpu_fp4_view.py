@@ -442,3 +442,51 @@ def test_first_tokens_without_a_window_are_no_view(dev, lens, t, heads, kv, dim)
         assert torch.equal(got, fp4_attention(q, pool, bt, lens_t, splits=splits))
         need = [fp4_attention_workspace(q, pool, bt, first=first, splits=splits) for first in (0, 4)]
         assert need[0] == need[1]
+
+
+def some(keep, q, pool, bt, lens, seen):
+    """Of a large batch the sequences of a sample: what check takes of them, their pages alone."""
+    ids, small = torch.unique(bt[keep].clamp_min(0).long(), return_inverse=True)
+    table = torch.where(bt[keep] < 0, -1, small.to(torch.int32))
+    return q[keep], pool[ids], table, lens[keep], seen[keep.cpu().numpy()]
+
+
+@pytest.mark.parametrize("batch", [100, 300])
+def test_pieces_of_many_sequences(dev, batch) -> None:
+    """More items than a workgroup counts in one turn, or than a wave looks through at once, each in pieces of its own."""
+    from saint_kv import fp4_attention
+
+    rng = np.random.default_rng(batch)
+    lens = rng.integers(600, 1500, batch)
+    lens[[0, 7, batch // 2, batch - 1]] = [0, 2, 33, 0]
+    pool, bt, lens_t = make(dev, lens, 64, 1, 64, seed=1)
+    q = torch.randn(batch, 2, 2, 64, generator=torch.Generator(device=dev).manual_seed(1), device=dev).to(torch.bfloat16)
+    seen = masks(batch, 2, [2] * batch, seed=4)
+    got = fp4_attention(q, pool, bt, lens_t, tree=to_words(seen, dev))
+    assert torch.equal(got, fp4_attention(q, pool, bt, lens_t, tree=to_words(seen, dev)))
+    keep = torch.unique(torch.cat((torch.tensor([0, 1, 7, 63, 64, batch // 2, batch - 2, batch - 1]),
+                                   torch.as_tensor(rng.integers(0, batch, 24))))).to(dev)
+    q, pool, bt, lens_t, seen = some(keep, q, pool, bt, lens_t, seen)
+    check(got[keep], q, pool, bt, lens_t, seen=seen)
+
+
+@pytest.mark.parametrize("lens,t,heads,kv,dim,window,first", [
+    ([2600, 1800, 1700, 1000, 33, 0] + [2500] * 58, 1, 8, 8, 128, 1600, 4),  # 51 tiles
+    ([5200, 4900, 4700, 3000] + [5000] * 92, 1, 8, 8, 64, 4700, 70),  # 152
+    ([2400, 2300, 900], 512, 32, 32, 128, 1700, 40), ([3500, 3000, 1000] + [2900] * 21, 64, 16, 8, 256, 2700, 1)])
+def test_windows_left_whole(dev, lens, t, heads, kv, dim, window, first) -> None:
+    """Windows of 49 to 160 tiles that are not cut: no workspace, one launch."""
+    from saint_kv import fp4_attention
+    from saint_kv.fp4 import fp4_attention_workspace
+
+    batch = len(lens)
+    pool, bt, lens_t = make(dev, lens, 64, kv, dim, seed=t)
+    q = torch.randn(batch, t, heads, dim, generator=torch.Generator(device=dev).manual_seed(1), device=dev).to(torch.bfloat16)
+    assert fp4_attention_workspace(q, pool, bt, window=window, first=first) == 0
+    got = fp4_attention(q, pool, bt, lens_t, window=window, first=first)
+    keep = torch.arange(min(batch, 4 if t == 1 else 3), device=dev)
+    step = max(1, t // 3)  # rows of a chunk: its newest, and others down to its oldest
+    rows = torch.arange(t - 1, -1, -step).flip(0)
+    q, pool, bt, lens_t, _ = some(keep, q, pool, bt, lens_t, np.zeros((batch, 1, 1)))
+    for r in rows.tolist():  # as the newest of a sequence that ends with it
+        check(got[keep, r:r + 1], q[:, r:r + 1], pool, bt, lens_t - (t - 1 - r), window=window, first=first)
