@@ -259,6 +259,7 @@ class Fp4TokenCache:
         self._unwritten: set[int] = set()  # layers that these have not been appended to
         self._recorded: set[int] = set()  # layers that a graph appends to
         self._shared = False  # some of these lie in shared pages
+        self._ended = False  # a sequence was released since: it has none of them
         self._compact_ws = torch.zeros(3 * self.n_pages, **i32)
         self._compact_info = torch.zeros(2, **i32)
 
@@ -281,7 +282,7 @@ class Fp4TokenCache:
         ops.reserve(self.free_stack, self.free_top, self.block_table, self.seq_lens, self._n_new, self.block_size, word)
         self.host_lens = self.host_lens + counts
         self._host_new, self._most_new = counts.copy(), int(counts.max())
-        self._shared = self._padded = False
+        self._shared = self._padded = self._ended = False
         self._unwritten = set(range(len(self.pool))) if counts.any() else set()
 
     def _status_word(self) -> torch.Tensor:
@@ -341,9 +342,15 @@ class Fp4TokenCache:
             raise RuntimeError("the tokens reserved last are a fork's, too: they lie in shared pages")
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError("keep reads back how many tokens stayed; a graph records ops.keep_tokens")
-        n_new = torch.as_tensor(self._host_new.astype(np.int32), device=self.device)  # none of a released sequence
-        # where the device refused the reservation its newest tokens are older ones: counts of -1 are refused, too
-        n_new = torch.where(self._word_views[self._reserved] == 0, n_new, -1)
+        if self._ended:  # none of a released sequence
+            n_new = torch.as_tensor(self._host_new.astype(np.int32), device=self.device)
+        elif isinstance(self._n_new, int):
+            n_new = torch.full((self.batch,), self._n_new, dtype=torch.int32, device=self.device)
+        else:
+            n_new = self._n_new
+        # where the device refused the reservation (a status of bits up to 16) its newest tokens are older ones: counts, of up
+        # to 2^24, that become negative are refused, too
+        n_new = torch.sub(n_new, self._word_views[self._reserved], alpha=1 << 25)
         word = self._status_word()
         at = self.batch + self._word - 1
         ops.keep_tokens(self.free_stack, self.free_top, self.block_table, self.seq_lens, n_new, path, n_keep, self.pool,
@@ -355,7 +362,7 @@ class Fp4TokenCache:
             bs, before = self.block_size, self.host_lens
             self.host_lens = before - self._host_new + counts
             self.host_free += int(((before + bs - 1) // bs - (self.host_lens + bs - 1) // bs).sum())
-            self._n_new, self._host_new, self._most_new = kept, counts, int(counts.max())
+            self._n_new, self._host_new, self._most_new, self._ended = kept, counts, int(counts.max()), False
         self._raise_refusals(report[self.batch:])
         return counts
 
@@ -378,7 +385,7 @@ class Fp4TokenCache:
         self.host_free = int(self.free_top.item())
         if words[self._reserved]:  # no tokens were reserved: there are none to append or keep
             self._n_new, self._host_new, self._most_new = 0, np.zeros(self.batch, dtype=np.int64), 0
-            self._unwritten = set()
+            self._unwritten, self._ended = set(), False
         raise RuntimeError(f"Fp4TokenCache reservation, fork or release refused, or a keep (status bits {bits})")
 
     # ------------------------------------------------------ forks, eviction --
@@ -416,6 +423,7 @@ class Fp4TokenCache:
                     torch.as_tensor(mask.astype(np.uint8), device=self.device), self.block_size, self._status_word(),
                     refs=self.refs)
         self._host_new[mask] = 0
+        self._ended |= bool(mask.any())
         self.check_status()
         self.host_lens[mask] = 0
         self.host_free = int(self.free_top.item())

@@ -513,3 +513,26 @@ def test_a_reservation_after_a_refused_one_is_kept(dev) -> None:
     assert cache.host_lens.tolist() == [42, 41] == cache.seq_lens.tolist()
     assert cache.keep(path[:, :1] * 0, torch.ones(2, dtype=torch.int32, device=dev)).tolist() == [1, 1]
     assert cache.host_lens.tolist() == [41, 41] and int(cache.free_top.item()) == cache.host_free
+
+
+@pytest.mark.parametrize("counts", [6, np.array([6, 4, 0])])
+def test_a_keep_after_a_release(dev, counts) -> None:
+    """A released sequence has no newest tokens, whether all had as many or each its own."""
+    from saint_kv import Fp4TokenCache
+
+    rng = np.random.default_rng(7)
+    cache = Fp4TokenCache(1, 3, 128, 1, 32, block_size=16, device=dev)
+    for n in (np.array([20, 30, 16]), counts):
+        cache.reserve(n)
+        t = int(np.max(n))
+        cache.append(0, rows_of(dev, rng, 3, t, 1, 32), rows_of(dev, rng, 3, t, 1, 32))
+    cache.release(np.array([True, False, False]))
+    third = 0 if isinstance(counts, np.ndarray) else 1
+    path = torch.tensor([[-1, -1], [1, 3], [5, -1]], dtype=torch.int32, device=dev)
+    with pytest.raises(RuntimeError, match="refused"):
+        cache.keep(path * 0, torch.tensor([1, 2, third], dtype=torch.int32, device=dev))
+    for n_keep in ([0, 2, third], [0, 1, 0]):  # and of those that stayed
+        assert cache.keep(path, torch.tensor(n_keep, dtype=torch.int32, device=dev)).tolist() == n_keep
+        path = path * 0
+    assert cache.host_lens.tolist() == [0, 31, 16] == cache.seq_lens.tolist()
+    assert int(cache.free_top.item()) == cache.host_free
