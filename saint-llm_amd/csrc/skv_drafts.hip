@@ -8,8 +8,9 @@
 //   keep   : the tokens path[0] < path[1] < ... of the newest n become the newest k of them: path[i]'s row, in every
 //            layer's pages, moves to row i of the n, the length is cut behind row k - 1 and the pages behind it go
 //            on the free stack.
-// All of it is the latency of a few dependent reads; MI355X: 64 trees of up to 64 nodes take 4.2 us for their masks, 5.3
-// for their paths, 8.7 for the plan of what is kept and 6.3 to move its rows in 8 layers (8 heads of 128 dims).
+// All of it is the latency of a few dependent reads; MI355X: 64 trees of up to 64 nodes take 4.2 us for their masks, 5.5
+// for their paths (320 nodes accepted), 8.4 for the plan of what is kept and 6.0 to move its rows (184 in each of 8 layers, 8
+// heads of 128 dims); with longer paths (618 accepted, 482 moved, onto each other's places) 8.0, 8.5 and 8.7.
 #include <algorithm>
 
 #include "skv_fp4.h"

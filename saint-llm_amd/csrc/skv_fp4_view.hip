@@ -15,12 +15,12 @@
 // in the tiles that all see, and cleared at the end.
 //
 // Measured, us a call in a graph of several, with the time of the bytes at 6.1 TB/s or of the products at 1.4 PFLOP/s:
-//   trees of up to 32 nodes of 32 sequences of 1k - 16k, 64 heads on 8 of 128 dims   205 (99, products)
-//   trees of up to 7 nodes of 4 of 256k - 1M, 16 heads on 4 of 64                    144 (88)
-//   trees of up to 99 nodes of 6, windows of 128, 16 heads on 1 of 512               45 (3, products)
-//   64 windows of 4k behind 4 first tokens, 64 heads on 8 of 128                     54 (44)
+//   trees of up to 32 nodes of 32 sequences of 1k - 16k, 64 heads on 8 of 128 dims   204 (99, products)
+//   trees of up to 7 nodes of 4 of 256k - 1M, 16 heads on 4 of 64                    147 (143 - 153; 88)
+//   trees of up to 99 nodes of 6, windows of 128, 16 heads on 1 of 512               46 (3, products)
+//   64 windows of 4k behind 4 first tokens, 64 heads on 8 of 128                     50 - 56 (44)
 //   2 prompts' 1000 tokens, windows of 2k behind 64, 32 heads on 8 of 128            90 (49, products)
-//   a tree of 8 nodes over 400 tokens, one token in a window of 128                  10, 9
+//   a tree of 8 nodes over 341 tokens, one token in a window of 128                  9.5, 7.9
 #include "skv_fp4_attn.h"
 
 namespace skv {

@@ -6,8 +6,9 @@
 // One pass over a row: a lane keeps a running m, l and s of the logits that it sees; lanes, waves and (of rows
 // that several workgroups share) segments are joined by exp(m_i - m), under which s_i becomes s_i + l_i (m_i - m).
 // HBM bounds it with many rows (each logit is read once), the vector work close behind: about five instructions
-// and an exponential a logit.  3001 rows of 100,003 fp16 logits, 8 alternatives: 110 us (5.5 TB/s); 256 of 131,072
-// bf16, 20 alternatives: 17 us (4.0 TB/s, the last steps of rows that all end at once); one of 32,000 fp32: 8.5 us.
+// and an exponential a logit.  A launch over 3001 rows of 100,003 logits, 8 alternatives: 113 us of fp16 (5.3 TB/s, some
+// rows half -inf), 191 of fp32 (6.3 TB/s); over 256 of 131,072 bf16, 20 alternatives: 17 - 19 us (3.5 - 4 TB/s, the last steps
+// of rows that all end at once); one of 32,000 fp32 in a graph of several: 8.5 us.
 //
 // The `top` largest cost next to nothing on the way: a lane notes the maximum of every 64 bytes (4 loads of 16)
 // that it sees, in LDS.  The top-th largest of the lanes' own maxima is a bound that at least `top` logits
@@ -37,7 +38,8 @@ constexpr float kLpLowest = -3.4028234663852886e38f;
 constexpr float kLpLn2 = 0.6931471805599453f;
 constexpr float kLpGone = -1e4f;   // exp of it is 0; times 0 it is 0, as -inf would not be
 constexpr float kLpFar = 1e37f;       // logits up to it stay finite in the log2 domain
-constexpr float kLpHuge = 67108864.f;  // maxima up to it are less than 2^3 from their rounding there: weights up to 2^3
+// Of maxima up to it the product with log2(e) is rounded by at most 4 (a step is 8 there): weights up to 2^4.
+constexpr float kLpHuge = 67108864.f;
 
 struct LpArgs {
   const uint8_t* x;
