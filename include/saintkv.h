@@ -590,7 +590,8 @@ int skv_accept_drafts(const int32_t* parents, const skv_token_ids* tokens, const
  * written or cut is shared (SKV_STATUS_BADARG), or the stack would overflow
  * (SKV_STATUS_STACK), nothing is written but *status (not NULL) and the
  * workspace.  path: int32, rows of path_stride <= 1024; batch <= 4096, a table of
- * less than 2^31 entries, up to 32 pools.  Calls that share a workspace must not overlap. */
+ * less than 2^31 entries, up to 32 pools.  Calls that share a workspace or a status word must not
+ * overlap. */
 int64_t skv_keep_tokens_workspace(int64_t batch, int64_t path_stride);
 int skv_keep_tokens(int32_t* free_stack, int32_t* free_top, const int32_t* refs, const skv_fp4_cache* cache,
                     int32_t* block_table, int32_t* seq_lens, const int32_t* n_new, int32_t n_new_uniform,
